@@ -1,0 +1,1212 @@
+// Attention on the gfx950 matrix cores: prompts (g16_attention) and single tokens over a cache whose
+// requests share a prefix (g16_attention_decode). The formulas and arguments stand in g16.h.
+//
+// Structure, for one key head and a tile of its query rows (row r of a sequence is token r / group,
+// query head r % group: the query heads that share a key head share its tiles, too):
+//   * Scores are computed transposed, S^T = K Q^T, in 32x32 blocks: a lane of the accumulator then holds
+//     16 keys of ONE query row (lanes l and l + 32 the other half's), so a row's maximum and sum need one
+//     exchange across the two halves, the running maximum, sum and rescale factor are one register each,
+//     and the output is accumulated transposed as well, O^T += V^T P^T, each lane still on its own row.
+//   * The weights P leave the score accumulator in exactly the order in which the next product wants
+//     them: its 16-deep step s takes keys 16 s + 4 h + {0..3} and 16 s + 8 + 4 h + {0..3} from lane half h,
+//     which are registers 8 s .. 8 s + 7 of the block. No weight moves between lanes. V^T comes from
+//     row-major V in LDS in that order through the transposing reads (fp16) or plain dword reads (fp32).
+//   * One pass over the keys with a running maximum. A maximum only moves when a row's new one is more
+//     than 2^kLag above it (the weights grow to at most 2^(kShift + kLag), far inside fp16), which after
+//     the first tiles spares almost every rescale of O. Weights are computed 2^kShift above their value,
+//     which keeps those far below the maximum out of fp16's subnormals.
+//   * fp32 inputs run the same code on v_mfma_f32_32x32x2_f32, eight of them where fp16 has one 32x32x16:
+//     the lanes' eight values per step are the same, only their order along the sum differs.
+//   * Keys arrive by DMA into LDS with the row swizzles of Tile. A tile that ends past its sequence is cut
+//     off by the buffer descriptor's range, which writes zeros: no value from behind a sequence's end
+//     reaches a product.
+// Two shapes of workgroup, both of 4 wavefronts:
+//   * rows: 128 query rows, 32 per wavefront, all on the same keys, two tiles in LDS, one barrier a tile.
+//   * keys: 32 query rows, every wavefront on its own tiles of 32 keys, joined at the end; for few rows,
+//     where the time is that of reading the keys.
+// With too few tiles to fill the card, the keys are split over workgroups as well, which leave (O, maximum,
+// sum) in the workspace; a second launch joins them in split order (no atomics: repeated calls agree).
+#include "g16_common.hpp"
+
+namespace g16 {
+namespace {
+
+typedef float float8v __attribute__((ext_vector_type(8)));
+typedef float float2v __attribute__((ext_vector_type(2)));
+
+constexpr float kShift = 8.f, kLag = 7.f;
+constexpr float kLog2e = 1.44269504088896341f;
+constexpr int kRowTile = 128, kKeyTile = 32;  // query rows of the two workgroup shapes
+constexpr int kThreads = 256;
+
+__device__ __attribute__((aligned(16))) const uint32_t g_zero_row[G16_ATTENTION_MAX_D] = {};
+
+template <typename T>
+struct Vec8 {
+  using V = half8;
+};
+template <>
+struct Vec8<float> {
+  using V = float8v;
+};
+
+__device__ inline float16v mma(half8 a, half8 b, float16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ inline float16v mma(float8v a, float8v b, float16v c) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+  return c;
+}
+
+// The value of the lane 32 away.
+__device__ inline float other_half(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
+}
+
+template <typename P>
+__device__ inline P* uniform(P* p) {
+  const uint64_t v = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32));
+  return reinterpret_cast<P*>((static_cast<uint64_t>(hi) << 32) | lo);
+}
+__device__ inline int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+struct Params {
+  const char *q, *k, *v, *sk, *sv;
+  char* out;
+  const int32_t *q_off, *k_off, *visible, *lengths, *pages;
+  const float* slopes;
+  float* part;
+  int64_t q_seq, q_tok, q_head, k_seq, k_head, v_seq, v_head, sk_head, sv_head;  // bytes
+  uint32_t k_tok, v_tok, sk_tok, sv_tok;                                        // bytes
+  int seqs, q_len, k_len, hq, hkv, group, d, shared, causal;
+  int page, max_pages, num_pages;
+  int tiles, splits;              // prompts: row tiles (an upper bound where packed), key splits
+  int stiles, ssplits, osplits;   // single tokens: row tiles and splits of the shared keys, splits of the own
+  int otiles;                     // ... and row tiles of 32 of one request's `group` rows
+  float scale, softcap;
+};
+
+// One run of keys: the shared ones, or a sequence's own.
+struct Keys {
+  const char *k, *v;      // first key's row of this head
+  uint32_t k_tok, v_tok;  // bytes between rows
+  int len, pos0;          // keys; position of the first
+};
+struct KeyRuns {
+  Keys shared, own;
+  // (in scalar registers: the DMA's descriptors are made of them)
+  __device__ Keys run(bool second) const {
+    return Keys{uniform(second ? own.k : shared.k), uniform(second ? own.v : shared.v),
+                static_cast<uint32_t>(uniform(static_cast<int>(second ? own.k_tok : shared.k_tok))),
+                static_cast<uint32_t>(uniform(static_cast<int>(second ? own.v_tok : shared.v_tok))),
+                uniform(second ? own.len : shared.len), uniform(second ? own.pos0 : shared.pos0)};
+  }
+};
+
+// ---- tiles in LDS -------------------------------------------------------------------------------
+// BN rows (keys) of DP values, 16-byte chunk c of row r at chunk position c ^ swizzle(r). K is read a
+// row per lane (16 lanes cover 16 rows at one chunk: their positions differ in a 256-byte bank period);
+// V in runs along a row, 4 rows and 64 bytes (fp16, transposing reads) or rows r and r + 4 and 128 bytes
+// (fp32) at a time, which the swizzle puts on different banks.
+template <typename T, int DP, int BN>
+struct Tile {
+  static constexpr int ROWB = DP * sizeof(T), RC = ROWB / 16, RPI = 64 / RC;
+  static constexpr int BYTES = BN * ROWB, NI = BYTES / 1024;  // 1 KB DMA instructions
+  using V8 = typename Vec8<T>::V;
+  __device__ static int swz_k(int row) { return RC == 8 ? (row >> 1) & 7 : row & 15; }
+  __device__ static int swz_v(int row) {
+    if constexpr (sizeof(T) == 4) return ((row >> 2) & 1) << 3;
+    else if constexpr (RC == 8) return (((row >> 1) & 1) << 2) | (((row >> 3) & 1) << 1);
+    else return (row & 3) << 2;
+  }
+  // K rows 32 kb + lane % 32 of the tile, values 16 ks + 8 (lane / 32) .. +7
+  __device__ static V8 k_frag(const char* lds, int kb, int ks, int lane) {
+    const int row = 32 * kb + (lane & 31), h = lane >> 5;
+    const char* at = lds + row * ROWB;
+    if constexpr (sizeof(T) == 2) {
+      return *reinterpret_cast<const half8*>(at + (((2 * ks + h) ^ swz_k(row)) << 4));
+    } else {
+      const float4v a = *reinterpret_cast<const float4v*>(at + (((4 * ks + 2 * h) ^ swz_k(row)) << 4));
+      const float4v b = *reinterpret_cast<const float4v*>(at + (((4 * ks + 2 * h + 1) ^ swz_k(row)) << 4));
+      return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  }
+  // V^T row (value) 32 db + lane % 32, keys 16 ks + 4 h + {0..3} and 16 ks + 8 + 4 h + {0..3}
+  __device__ static V8 v_frag(const char* lds, int ks, int db, int lane) {
+    const int h = lane >> 5;
+    if constexpr (sizeof(T) == 2) {
+      const int q = lane & 15;
+      half4 part[2];
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const int row = 16 * ks + 8 * g + 4 * h + (q >> 2);
+        const int chunk = 4 * db + 2 * ((lane >> 4) & 1) + ((q & 3) >> 1);
+        const uint32_t at = lds_base(lds) + row * ROWB + ((chunk ^ swz_v(row)) << 4) + (q & 1) * 8;
+        part[g] = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds4_at(at)));
+      }
+      return __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
+    } else {
+      float8v r;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int row = 16 * ks + 8 * (j >> 2) + 4 * h + (j & 3);
+        const int chunk = 8 * db + ((lane & 31) >> 2);
+        r[j] = *reinterpret_cast<const float*>(lds + row * ROWB + ((chunk ^ swz_v(row)) << 4) + (lane & 3) * 4);
+      }
+      return r;
+    }
+  }
+};
+
+// The byte offsets of a wavefront's DMA instructions first .. first + N - 1 within a tile of rows `tok`
+// bytes apart: lane i's chunk of instruction n goes to LDS byte 1024 n + 16 i.
+template <typename TL, int N, bool IS_V>
+__device__ inline void dma_offsets(uint32_t (&off)[N], int first, int lane, uint32_t tok, int row_bytes) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const int row = (first + n) * TL::RPI + lane / TL::RC;
+    const int c = (lane % TL::RC) ^ (IS_V ? TL::swz_v(row) : TL::swz_k(row));
+    off[n] = c * 16 < row_bytes ? static_cast<uint32_t>(row) * tok + c * 16 : kOob;
+  }
+}
+template <int N>
+__device__ inline void dma_rows(const char* base, uint32_t tok, int rows, const uint32_t (&off)[N], uint32_t lds) {
+  const __amdgpu_buffer_rsrc_t r =
+      __builtin_amdgcn_make_buffer_rsrc(uniform(const_cast<char*>(base)), 0, uniform(static_cast<int>(tok * static_cast<uint32_t>(rows))),
+                                        kRawBufferDword3);
+#pragma unroll
+  for (int n = 0; n < N; ++n) dma16(r, lds + n * 1024, off[n]);
+}
+// The same from any address, for rows that lie in pages.
+__device__ inline void dma16_from(const char* at, uint32_t lds_addr) {
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off"
+               :
+               : "s"(__builtin_amdgcn_readfirstlane(lds_addr)), "v"(at)
+               : "memory", "m0");
+}
+
+// ---- one lane's query row ------------------------------------------------------------------------
+struct Row {
+  const char* q;  // NULL: no such row
+  char* out;
+  int pos, limit;  // position; last position it sees (INT_MAX: every key)
+  float slope;     // slope * log2(e)
+};
+
+// Scores (products q.k) -> t = log2(e) * f(scale * s) - slope * distance, for keys pos0 + {0 .. } of a
+// block whose lane half h holds keys 8 (r / 4) + 4 h + r % 4 in register r.
+struct Scoring {
+  float c;         // scale * log2(e)
+  float cap, inv;  // softcap * log2(e); 2 log2(e) scale / softcap
+  bool capped, biased;
+};
+
+__device__ inline Scoring scoring(const Params& p) {
+  Scoring s;
+  s.c = p.scale * kLog2e;
+  s.capped = p.softcap != 0.f;
+  s.biased = p.slopes != nullptr;
+  s.cap = p.softcap * kLog2e;
+  s.inv = s.capped ? p.scale / p.softcap : 0.f;
+  return s;
+}
+
+// tanh to fp32's last bits near 0, where a cap leaves most scores (an odd polynomial fitted by least
+// squares to (tanh(y) / y - 1) / y^2 on [0, 0.625], largest relative error 4e-9), and 1 - 2 / (e^2y + 1)
+// past it. fp16 inputs need no more than the second form's absolute error of 1e-7.
+template <typename T>
+__device__ inline float tanh_of(float y) {
+  const float e = __builtin_amdgcn_exp2f(y * (2.f * kLog2e));
+  const float big = 1.f - 2.f * __builtin_amdgcn_rcpf(e + 1.f);
+  if constexpr (sizeof(T) == 2) {
+    return big;
+  } else {
+    const float u = y * y;
+    float r = fmaf(u, -0.00571705f, 0.02065059f);
+    r = fmaf(u, r, -0.0537435f);
+    r = fmaf(u, r, 0.13331491f);
+    r = fmaf(u, r, -0.33333284f);
+    r = fmaf(y * u, r, y);
+    return fabsf(y) < 0.625f ? r : big;
+  }
+}
+
+template <typename T>
+__device__ inline float score_of(const Scoring& s, float x, float slope, float distance) {
+  float t = s.capped ? s.cap * tanh_of<T>(x * s.inv) : x * s.c;
+  return s.biased ? fmaf(-slope, fabsf(distance), t) : t;
+}
+
+// ---- the running softmax and product of 32 rows in one wavefront ---------------------------------
+template <typename T, int DP>
+struct Wave {
+  using V8 = typename Vec8<T>::V;
+  V8 q[DP / 16];
+  float16v o[DP / 32];
+  float m, l;  // the reference maximum (log2 units) and this lane's part of the sum of weights
+
+  __device__ void start(const Row& row, int d, int lane) {
+    const int h = lane >> 5;
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks) {
+      const int at = 16 * ks + 8 * h;
+      V8 v = {};
+      if (row.q != nullptr && at < d) v = *reinterpret_cast<const V8*>(row.q + at * sizeof(T));
+      q[ks] = v;
+    }
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i) o[i] = float16v{};
+    m = -__builtin_huge_valf();
+    l = 0.f;
+  }
+
+  // S^T of the tile's NB blocks of 32 keys
+  template <int NB, typename TL>
+  __device__ void products(const char* kt, float16v (&s)[NB], int lane) const {
+#pragma unroll
+    for (int kb = 0; kb < NB; ++kb) {
+      s[kb] = float16v{};
+#pragma unroll
+      for (int ks = 0; ks < DP / 16; ++ks) s[kb] = mma(TL::k_frag(kt, kb, ks, lane), q[ks], s[kb]);
+    }
+  }
+
+  // The weights of the tile's keys: positions pos0 .., `left` of them in the sequence.
+  template <int NB>
+  __device__ void weights(float16v (&s)[NB], const Scoring& sc, const Row& row, int pos0, int left, int last_seen, int lane) {
+    const int h4 = (lane >> 5) * 4;
+    float c = sc.c;
+    if (sc.capped || !(c > 0.f)) {
+#pragma unroll
+      for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[kb][r] = sc.capped ? sc.cap * tanh_of<T>(s[kb][r] * sc.inv) : s[kb][r] * c;
+      c = 1.f;
+    }
+    if (sc.biased) {
+      const float at = static_cast<float>(row.pos - pos0 - h4);
+#pragma unroll
+      for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float e = static_cast<float>(32 * kb + 8 * (r >> 2) + (r & 3));
+          s[kb][r] = fmaf(-row.slope, fabsf(at - e), s[kb][r] * c);
+        }
+      c = 1.f;
+    }
+    if (left < 32 * NB || last_seen < pos0 + 32 * NB - 1) {
+      const int lim = min(left - 1, row.limit - pos0) - h4;
+#pragma unroll
+      for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          if (32 * kb + 8 * (r >> 2) + (r & 3) > lim) s[kb][r] = -__builtin_huge_valf();
+        }
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[kb][r]);
+    top = fmaxf(top, other_half(top)) * c;
+    // (-inf times c stays -inf: c > 0.) A lane whose maximum moves takes the whole wavefront along.
+    if (__any(top > m + kLag)) {
+      const float next = fmaxf(m, top);
+      const float f = next == m ? 1.f : __builtin_amdgcn_exp2f(m - next);
+      m = next;
+      l *= f;
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[i][r] *= f;
+    }
+    // a row that has seen no key yet (m = -inf): every score is -inf, every weight 0
+    const float ref = (m == -__builtin_huge_valf() ? 0.f : m) - kShift;
+    float sum = 0.f;
+#pragma unroll
+    for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float w = __builtin_amdgcn_exp2f(fmaf(s[kb][r], c, -ref));
+        s[kb][r] = w;
+        sum += w;
+      }
+    l += sum;
+  }
+
+  // O^T += V^T P^T
+  template <int NB, typename TL>
+  __device__ void add(const char* vt, const float16v (&s)[NB], int lane) {
+#pragma unroll
+    for (int ks = 0; ks < 2 * NB; ++ks) {
+      V8 w;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = static_cast<T>(s[ks >> 1][8 * (ks & 1) + j]);
+#pragma unroll
+      for (int db = 0; db < DP / 32; ++db) o[db] = mma(TL::v_frag(vt, ks, db, lane), w, o[db]);
+    }
+  }
+};
+
+// Where a tile's rows go: the output, or a slot of the workspace with rows x DP sums, then the rows'
+// reference maxima and sums of weights (and a gap, so that every slot starts on 16 bytes).
+__host__ __device__ constexpr size_t slot_floats(int rows, int dp) { return static_cast<size_t>(rows) * (dp + 4); }
+struct Slot {
+  float* at;  // NULL: the output
+  int rows;
+};
+template <int DP>
+__device__ inline float* slot_m(const Slot& s) { return s.at + static_cast<size_t>(s.rows) * DP; }
+
+template <typename T, int N>
+__device__ inline void store_out(char* out, int d0, const float (&v)[N]) {
+  if constexpr (sizeof(T) == 2) {
+    if constexpr (N == 4) {
+      const half4 h = {static_cast<_Float16>(v[0]), static_cast<_Float16>(v[1]), static_cast<_Float16>(v[2]), static_cast<_Float16>(v[3])};
+      *reinterpret_cast<half4*>(out + d0 * 2) = h;
+    } else {
+      half8 h;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) h[i] = static_cast<_Float16>(v[i]);
+      *reinterpret_cast<half8*>(out + d0 * 2) = h;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) *reinterpret_cast<float4v*>(out + (d0 + i) * 4) = float4v{v[i], v[i + 1], v[i + 2], v[i + 3]};
+  }
+}
+
+// One row again, key by key, for rows whose sums are not finite: an infinity or NaN behind a key that
+// the row does not see, times that key's weight 0, may be the reason. Only the keys that it sees are
+// read here. The whole wavefront works on the row.
+template <typename T, int DP>
+__device__ __attribute__((noinline)) void careful_row(const char* q, char* out, int pos, int limit, float slope, const Scoring sc,
+                                                      const KeyRuns runs, int from0, int to0, int from1, int to1, int d,
+                                                      float* part, float* part_m, float* part_l) {
+  const int lane = threadIdx.x & 63;
+  const T* qv = reinterpret_cast<const T*>(q);
+  auto score = [&](const Keys& s, int j) {
+    const T* kr = reinterpret_cast<const T*>(s.k + static_cast<size_t>(j) * s.k_tok);
+    float x = 0.f;
+    for (int i = 0; i < d; ++i) x = fmaf(to_f(qv[i]), to_f(kr[i]), x);
+    return score_of<T>(sc, x, slope, static_cast<float>(pos - s.pos0 - j));
+  };
+  float top = -__builtin_huge_valf();
+  for (int g = 0; g < 2; ++g) {
+    const Keys& s = g ? runs.own : runs.shared;
+    const int end = min(g ? to1 : to0, s.len);
+    for (int j = (g ? from1 : from0) + lane; j < end && s.pos0 + j <= limit; j += kWave) top = fmaxf(top, score(s, j));
+  }
+  for (int i = 1; i < kWave; i *= 2) top = fmaxf(top, __shfl_xor(top, i));
+  const float ref = (top == -__builtin_huge_valf() ? 0.f : top) - kShift;
+  float l = 0.f, o[DP / 64] = {};
+  for (int g = 0; g < 2; ++g) {
+    const Keys& s = g ? runs.own : runs.shared;
+    const int end = min(min(g ? to1 : to0, s.len), limit < s.pos0 ? 0 : limit - s.pos0 + 1);
+    for (int j0 = g ? from1 : from0; j0 < end; j0 += kWave) {
+      const float w = j0 + lane < end ? __builtin_amdgcn_exp2f(score(s, j0 + lane) - ref) : 0.f;
+      l += w;
+      for (int i = 0; i < min(kWave, end - j0); ++i) {
+        const float wi = __shfl(w, i);
+        const T* vr = reinterpret_cast<const T*>(s.v + static_cast<size_t>(j0 + i) * s.v_tok);
+#pragma unroll
+        for (int e = 0; e < DP / 64; ++e)
+          if (lane + 64 * e < d) o[e] = fmaf(to_f(static_cast<T>(wi)), to_f(vr[lane + 64 * e]), o[e]);
+      }
+    }
+  }
+  for (int i = 1; i < kWave; i *= 2) l += __shfl_xor(l, i);
+#pragma unroll
+  for (int e = 0; e < DP / 64; ++e) {
+    const int at = lane + 64 * e;
+    if (part != nullptr) part[at] = at < d ? o[e] : 0.f;
+    else if (at < d) reinterpret_cast<T*>(out)[at] = static_cast<T>(l > 0.f || l != l ? o[e] / l : 0.f);
+  }
+  if (part != nullptr && lane == 0) {
+    *part_m = top;
+    *part_l = l;
+  }
+}
+
+// 1 / l, with 0 for a row that saw no key (a NaN stays one)
+__device__ inline float inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
+
+// ---- workgroup of 128 rows ---------------------------------------------------------------------------
+// Wavefront w holds rows 32 w .. 32 w + 31. last_seen: a position up to which every valid row of this
+// wavefront sees; wave_limit: the last position that any of them sees.
+template <typename T, int DP>
+__device__ void rows_workgroup(const Params& p, char* lds, const Row& row, const KeyRuns& runs, int n0, int tbeg, int tend,
+                               int last_seen, int wave_limit, const Slot& slot) {
+  constexpr int BN = sizeof(T) == 2 ? 64 : 32, NB = BN / 32;
+  using TL = Tile<T, DP, BN>;
+  constexpr int NIW = TL::NI / 4;  // DMA instructions of a wavefront per tile and operand
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+  const uint32_t base = lds_base(lds);
+  const Scoring sc = scoring(p);
+  uint32_t koff[NIW], voff[NIW];
+  int at_seg = -1;
+  Keys cur = {};  // the run that the offsets are for
+  auto issue = [&](int t, int buf) {
+    const int g = t < n0 ? 0 : 1, j0 = (t - (g ? n0 : 0)) * BN;
+    if (g != at_seg) {
+      at_seg = g;
+      cur = runs.run(g != 0);
+      dma_offsets<TL, NIW, false>(koff, wave * NIW, lane, cur.k_tok, p.d * static_cast<int>(sizeof(T)));
+      dma_offsets<TL, NIW, true>(voff, wave * NIW, lane, cur.v_tok, p.d * static_cast<int>(sizeof(T)));
+    }
+    const int rows = min(BN, cur.len - j0);
+    const uint32_t to = base + buf * 2 * TL::BYTES + wave * NIW * 1024;
+    dma_rows<NIW>(cur.k + static_cast<size_t>(j0) * cur.k_tok, cur.k_tok, rows, koff, to);
+    dma_rows<NIW>(cur.v + static_cast<size_t>(j0) * cur.v_tok, cur.v_tok, rows, voff, to + TL::BYTES);
+  };
+  Wave<T, DP> w;
+  if (tbeg < tend) issue(tbeg, 0);
+  w.start(row, p.d, lane);
+  for (int t = tbeg; t < tend; ++t) {
+    const int buf = (t - tbeg) & 1;
+    wait_dma_le<0>();
+    phase_barrier();  // tile t has arrived for every wavefront, and every one is done with tile t - 1
+    if (t + 1 < tend) issue(t + 1, buf ^ 1);
+    const int g = t < n0 ? 0 : 1, j0 = (t - (g ? n0 : 0)) * BN;
+    const int pos0 = (g ? runs.own.pos0 : runs.shared.pos0) + j0, left = (g ? runs.own.len : runs.shared.len) - j0;
+    if (pos0 > wave_limit) continue;
+    const char* kt = lds + buf * 2 * TL::BYTES;
+    float16v s[NB];
+    w.template products<NB, TL>(kt, s, lane);
+    w.template weights<NB>(s, sc, row, pos0, left, last_seen, lane);
+    w.template add<NB, TL>(kt + TL::BYTES, s, lane);
+  }
+  const float l = w.l + other_half(w.l);
+  const int h = lane >> 5, r = wave * 32 + (lane & 31);
+  float bad = 0.f;
+  if (slot.at != nullptr) {
+    float* o = slot.at + static_cast<size_t>(r) * DP;
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float16v& a = w.o[db];
+        *reinterpret_cast<float4v*>(o + 32 * db + 8 * q + 4 * h) = float4v{a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]};
+      }
+    if (h == 0) {
+      slot_m<DP>(slot)[r] = w.m;
+      slot_m<DP>(slot)[slot.rows + r] = l;
+    }
+  } else if (row.out != nullptr) {
+    const float inv = inverse(l);
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int d0 = 32 * db + 8 * q + 4 * h;
+        const float v[4] = {w.o[db][4 * q] * inv, w.o[db][4 * q + 1] * inv, w.o[db][4 * q + 2] * inv, w.o[db][4 * q + 3] * inv};
+        if (d0 < p.d) store_out<T, 4>(row.out, d0, v);
+      }
+  }
+  if (!p.causal) return;
+#pragma unroll
+  for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) bad = fmaf(w.o[db][i], 0.f, bad);
+  const uint64_t which = __ballot(bad != 0.f && row.q != nullptr);
+  uint32_t rows = static_cast<uint32_t>(which) | static_cast<uint32_t>(which >> 32);
+  if (__builtin_expect(rows != 0u, 0)) {
+    __builtin_amdgcn_s_waitcnt(0);  // the rows' first results are stored before their second ones
+    while (rows) {
+      const int i = __builtin_ctz(rows);
+      rows &= rows - 1;
+      const int rr = wave * 32 + i;
+      float* pm = slot.at == nullptr ? nullptr : slot_m<DP>(slot) + rr;
+      careful_row<T, DP>(reinterpret_cast<const char*>(__shfl(reinterpret_cast<unsigned long long>(row.q), i)),
+                         reinterpret_cast<char*>(__shfl(reinterpret_cast<unsigned long long>(row.out), i)), __shfl(row.pos, i),
+                         __shfl(row.limit, i), __shfl(row.slope, i), sc, runs, min(tbeg, n0) * BN, min(tend, n0) * BN,
+                         max(tbeg - n0, 0) * BN, max(tend - n0, 0) * BN, p.d,
+                         slot.at == nullptr ? nullptr : slot.at + static_cast<size_t>(rr) * DP, pm,
+                         pm == nullptr ? nullptr : pm + slot.rows);
+    }
+  }
+}
+
+// ---- workgroup of 32 rows, every wavefront on its own keys -------------------------------------------
+// Wavefront w takes tiles tbeg + w, tbeg + w + 4, .. of 32 keys, K and V each in one buffer of its own: the
+// next K is on its way from the moment the scores are computed, the next V from that of the products.
+// PAGED: the own keys lie in pages (prow: the lane's page row base; see decode_kernel).
+struct Pages {
+  const int32_t* table;  // this sequence's pages; NULL: its keys lie in a row
+  int page, num_pages;
+  int64_t k_seq, v_seq;
+};
+template <typename T, int DP, bool PAGED>
+__device__ void keys_workgroup(const Params& p, char* lds, float* joint, const Row& row, const KeyRuns& runs, const Pages& pages,
+                               int n0, int tbeg, int tend, int last_seen, const Slot& slot) {
+  constexpr int BN = 32;
+  using TL = Tile<T, DP, BN>;
+  constexpr int NI = TL::NI;
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+  char* mine = lds + wave * 2 * TL::BYTES;
+  const uint32_t kl = lds_base(mine), vl = kl + TL::BYTES;
+  const Scoring sc = scoring(p);
+  const int row_bytes = p.d * static_cast<int>(sizeof(T));
+  uint32_t koff[NI], voff[NI];
+  int at_seg = -1;
+  Keys cur = {};  // the run that the offsets are for
+  auto where = [&](int t, int& g, int& j0) {
+    g = t < n0 ? 0 : 1;
+    j0 = (t - (g ? n0 : 0)) * BN;
+  };
+  // PAGED: the page of this lane's key (lane % 32) of tile t, loaded a tile ahead
+  auto page_of = [&](int t) {
+    if (!PAGED || t >= tend || pages.table == nullptr) return 0;
+    const int j = (t - n0) * BN + (lane & 31);
+    return t >= n0 && j < runs.own.len ? pages.table[j / pages.page] : 0;
+  };
+  auto dma_paged = [&](int j0, int pg, bool is_v, uint32_t to) {
+    const int j = j0 + (lane & 31);
+    const char* at = nullptr;
+    if (j < runs.own.len && static_cast<unsigned>(pg) < static_cast<unsigned>(pages.num_pages))
+      at = (is_v ? runs.own.v : runs.own.k) + pg * (is_v ? pages.v_seq : pages.k_seq) +
+           static_cast<int64_t>(j % pages.page) * (is_v ? runs.own.v_tok : runs.own.k_tok);
+    const uint64_t a = reinterpret_cast<uint64_t>(at);
+    const uint32_t lo = static_cast<uint32_t>(a), hi = static_cast<uint32_t>(a >> 32);
+#pragma unroll
+    for (int n = 0; n < NI; ++n) {
+      const int r = n * TL::RPI + lane / TL::RC;
+      const int c = (lane % TL::RC) ^ (is_v ? TL::swz_v(r) : TL::swz_k(r));
+      const uint64_t b = (static_cast<uint64_t>(static_cast<uint32_t>(__shfl(static_cast<int>(hi), r))) << 32) |
+                         static_cast<uint32_t>(__shfl(static_cast<int>(lo), r));
+      const char* from = b != 0 && c * 16 < row_bytes ? reinterpret_cast<const char*>(b) + c * 16
+                                                      : reinterpret_cast<const char*>(g_zero_row);
+      dma16_from(from, to + n * 1024);
+    }
+  };
+  auto issue = [&](int t, int pg, bool is_v) {
+    int g, j0;
+    where(t, g, j0);
+    if (PAGED && g == 1 && pages.table != nullptr) {
+      dma_paged(j0, pg, is_v, is_v ? vl : kl);
+      return;
+    }
+    if (g != at_seg) {
+      at_seg = g;
+      cur = runs.run(g != 0);
+      dma_offsets<TL, NI, false>(koff, 0, lane, cur.k_tok, row_bytes);
+      dma_offsets<TL, NI, true>(voff, 0, lane, cur.v_tok, row_bytes);
+    }
+    const int rows = min(BN, cur.len - j0);
+    if (is_v) dma_rows<NI>(cur.v + static_cast<size_t>(j0) * cur.v_tok, cur.v_tok, rows, voff, vl);
+    else dma_rows<NI>(cur.k + static_cast<size_t>(j0) * cur.k_tok, cur.k_tok, rows, koff, kl);
+  };
+  Wave<T, DP> w;
+  int t = tbeg + wave;
+  int pg = page_of(t);
+  if (t < tend) {
+    issue(t, pg, false);
+    issue(t, pg, true);
+  }
+  int pg_next = page_of(t + 4);
+  w.start(row, p.d, lane);
+  // (the rows' loads are done before the loop, so its waits count DMA only)
+  __builtin_amdgcn_s_waitcnt(0);
+  for (; t < tend; t += 4) {
+    int g, j0;
+    where(t, g, j0);
+    const bool more = t + 4 < tend;
+    float16v s[1];
+    // K has arrived: only V's instructions may be in flight (younger page loads only make it wait longer)
+    wait_dma_le<NI>();
+    w.template products<1, TL>(mine, s, lane);
+    // the K buffer has been read (the products' operands are in registers) before the next K overwrites it
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (more) issue(t + 4, pg_next, false);
+    w.template weights<1>(s, sc, row, (g ? runs.own.pos0 : runs.shared.pos0) + j0, (g ? runs.own.len : runs.shared.len) - j0, last_seen, lane);
+    if (more) wait_dma_le<NI>();
+    else wait_dma_le<0>();
+    w.template add<1, TL>(mine + TL::BYTES, s, lane);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (more) issue(t + 4, pg_next, true);
+    pg_next = page_of(t + 8);
+  }
+  // ---- join the four wavefronts: sums [wave][value][row] in LDS, then 8 threads a row ----
+  const float l = w.l + other_half(w.l);
+  const int h = lane >> 5, r = lane & 31;
+  __syncthreads();
+  float* so = reinterpret_cast<float*>(lds);
+#pragma unroll
+  for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) so[(wave * DP + 32 * db + 8 * (i >> 2) + 4 * h + (i & 3)) * 32 + r] = w.o[db][i];
+  if (h == 0) {
+    joint[wave * 32 + r] = w.m;
+    joint[128 + wave * 32 + r] = l;
+  }
+  if (tid == 0) joint[256] = 0.f;
+  __syncthreads();
+  float top = -__builtin_huge_valf();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) top = fmaxf(top, joint[i * 32 + r]);
+  float f[4], total = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float mi = joint[i * 32 + r];
+    f[i] = mi == top ? 1.f : __builtin_amdgcn_exp2f(mi - top);
+    total += f[i] * joint[128 + i * 32 + r];
+  }
+  constexpr int DT = DP / 8;  // values a thread: d0 .. d0 + DT - 1
+  const int d0 = (tid >> 5) * DT;
+  const float inv = slot.at != nullptr ? 1.f : inverse(total);
+  float bad = 0.f;
+  const bool stored = slot.at != nullptr ? r < slot.rows : row.out != nullptr;
+#pragma unroll
+  for (int c = 0; c < DT; c += 8) {
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float x = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x = fmaf(f[i], so[(i * DP + d0 + c + e) * 32 + r], x);
+      v[e] = x * inv;
+      bad = fmaf(x, 0.f, bad);
+    }
+    if (stored && slot.at != nullptr) {
+      float* o = slot.at + static_cast<size_t>(r) * DP + d0 + c;
+      *reinterpret_cast<float4v*>(o) = float4v{v[0], v[1], v[2], v[3]};
+      *reinterpret_cast<float4v*>(o + 4) = float4v{v[4], v[5], v[6], v[7]};
+    } else if (stored && d0 + c < p.d) {
+      store_out<T, 8>(row.out, d0 + c, v);
+    }
+  }
+  if (slot.at != nullptr && tid < 32 && r < slot.rows) {
+    slot_m<DP>(slot)[r] = top;
+    slot_m<DP>(slot)[slot.rows + r] = total;
+  }
+  if constexpr (!PAGED) {
+    if (!p.causal) return;
+    uint32_t* flags = reinterpret_cast<uint32_t*>(joint + 256);
+    const uint64_t which = __ballot(bad != 0.f && row.q != nullptr);
+    const uint32_t some = static_cast<uint32_t>(which) | static_cast<uint32_t>(which >> 32);
+    if (lane == 0 && some) atomicOr(flags, some);
+    __builtin_amdgcn_s_waitcnt(0);  // the rows' first results are stored before their second ones
+    __syncthreads();
+    uint32_t rows = *flags;
+    if (__builtin_expect(rows != 0u, 0)) {
+      for (int k = 0; rows; ++k) {
+        const int i = __builtin_ctz(rows);
+        rows &= rows - 1;
+        if ((k & 3) != wave) continue;
+        float* pm = slot.at == nullptr ? nullptr : slot_m<DP>(slot) + i;
+        careful_row<T, DP>(reinterpret_cast<const char*>(__shfl(reinterpret_cast<unsigned long long>(row.q), i)),
+                           reinterpret_cast<char*>(__shfl(reinterpret_cast<unsigned long long>(row.out), i)), __shfl(row.pos, i),
+                           __shfl(row.limit, i), __shfl(row.slope, i), sc, runs, min(tbeg, n0) * BN, min(tend, n0) * BN,
+                         max(tbeg - n0, 0) * BN, max(tend - n0, 0) * BN, p.d,
+                           slot.at == nullptr ? nullptr : slot.at + static_cast<size_t>(i) * DP, pm,
+                           pm == nullptr ? nullptr : pm + slot.rows);
+      }
+    }
+  }
+}
+
+template <typename T, int DP>
+constexpr int rows_lds() {
+  return 4 * Tile<T, DP, sizeof(T) == 2 ? 64 : 32>::BYTES;
+}
+template <typename T, int DP>
+constexpr int keys_lds() {
+  return 8 * Tile<T, DP, 32>::BYTES > 4 * DP * 32 * 4 ? 8 * Tile<T, DP, 32>::BYTES : 4 * DP * 32 * 4;
+}
+constexpr int cmax(int a, int b) { return a > b ? a : b; }
+
+// ---- prompts -------------------------------------------------------------------------------------------
+// Row tile t of all sequences' tiles of `rt` rows: its sequence and where that sequence's rows and keys
+// are. Packed sequences: every wavefront counts the tiles of 64 sequences at a time. false: past the end.
+struct Where {
+  int seq, tile, lq, lk;
+  int64_t q0, k0;  // first row, first key (packed)
+};
+__device__ inline bool find_tile(const Params& p, int t, int rt, Where& w) {
+  if (p.q_off == nullptr) {
+    // equal sequences: the last tiles first (under a causal mask they have the most keys)
+    w.lq = p.q_len;
+    w.lk = p.k_len;
+    const int each = ceil_div(p.q_len * p.group, rt);
+    w.seq = t % p.seqs;
+    w.tile = each - 1 - t / p.seqs;
+    w.q0 = w.k0 = 0;
+    return w.tile >= 0;
+  }
+  const int lane = threadIdx.x & 63;
+  for (int b0 = 0; b0 < p.seqs; b0 += kWave) {
+    const int b = b0 + lane;
+    int q0 = 0, lq = 0;
+    if (b < p.seqs) {
+      q0 = min(max(p.q_off[b], 0), p.q_len);
+      lq = max(min(p.q_off[b + 1], p.q_len) - q0, 0);
+    }
+    const int n = static_cast<int>((static_cast<int64_t>(lq) * p.group + rt - 1) / rt);
+    int upto = n;
+#pragma unroll
+    for (int i = 1; i < kWave; i *= 2) {
+      const int x = __shfl_up(upto, i);
+      if (lane >= i) upto += x;
+    }
+    const uint64_t hit = __ballot(t < upto);
+    if (hit != 0) {
+      const int l = __builtin_ctzll(hit);
+      w.seq = b0 + l;
+      w.lq = __shfl(lq, l);
+      w.q0 = __shfl(q0, l);
+      w.tile = __shfl(upto, l) - 1 - t;  // the sequence's last tile first
+      const int ka = min(max(p.k_off[w.seq], 0), p.k_len);
+      w.lk = max(min(p.k_off[w.seq + 1], p.k_len) - ka, 0);
+      w.k0 = ka;
+      w.seq = uniform(w.seq);
+      w.lq = uniform(w.lq);
+      w.lk = uniform(w.lk);
+      w.tile = uniform(w.tile);
+      w.q0 = uniform(static_cast<int>(w.q0));
+      w.k0 = uniform(static_cast<int>(w.k0));
+      return true;
+    }
+    t -= __shfl(upto, kWave - 1);
+  }
+  return false;
+}
+
+// A row of the sequence `w`.
+__device__ inline Row prompt_row(const Params& p, const Where& w, int kv, int r, int size) {
+  Row row;
+  const int tok = r / p.group, head = kv * p.group + r % p.group;
+  const bool ok = tok < w.lq;
+  const int64_t at = (p.q_off == nullptr ? static_cast<int64_t>(w.seq) * p.q_len : w.q0) + tok;
+  row.q = ok ? p.q + (p.q_off == nullptr ? w.seq * p.q_seq : w.q0 * p.q_tok) + tok * p.q_tok + head * p.q_head : nullptr;
+  row.out = ok ? p.out + (at * p.hq + head) * p.d * size : nullptr;
+  row.pos = p.shared + w.lk - w.lq + tok;
+  row.limit = p.causal ? max(row.pos, p.visible != nullptr ? p.visible[w.seq] - 1 : -1) : 0x7fffffff;
+  row.slope = p.slopes != nullptr && ok ? p.slopes[head] * kLog2e : 0.f;
+  return row;
+}
+
+template <typename T, int DP, bool KEYS>
+__global__ __launch_bounds__(kThreads, 2) void prompt_kernel(Params p) {
+  constexpr int RT = KEYS ? kKeyTile : kRowTile, BN = KEYS ? 32 : (sizeof(T) == 2 ? 64 : 32);
+  __shared__ __attribute__((aligned(1024))) char lds[KEYS ? keys_lds<T, DP>() : rows_lds<T, DP>()];
+  __shared__ float joint[KEYS ? 257 : 1];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  int lin = blockIdx.x;
+  const int kv = lin % p.hkv;
+  lin /= p.hkv;
+  const int split = lin % p.splits, t = lin / p.splits;
+  Where w;
+  if (!find_tile(p, t, RT, w)) return;
+  const int r0 = w.tile * RT, first = r0 + (KEYS ? 0 : 32 * wave);
+  const Row row = prompt_row(p, w, kv, first + (lane & 31), sizeof(T));
+  const KeyRuns runs = {
+      {p.sk + kv * p.sk_head, p.sv + kv * p.sv_head, p.sk_tok, p.sv_tok, p.shared, 0},
+      {p.k + (p.k_off == nullptr ? w.seq * p.k_seq : w.k0 * p.k_tok) + kv * p.k_head,
+       p.v + (p.k_off == nullptr ? w.seq * p.v_seq : w.k0 * p.v_tok) + kv * p.v_head, p.k_tok, p.v_tok, w.lk, p.shared}};
+  // the keys that some row of the tile sees
+  int seen = 0x7fffffff, last_seen = 0x7fffffff, wave_limit = 0x7fffffff;
+  if (p.causal) {
+    const int vis = p.visible != nullptr ? uniform(p.visible[w.seq]) - 1 : -1;
+    const int pos0 = p.shared + w.lk - w.lq;
+    const int last_tok = min(r0 + RT - 1, w.lq * p.group - 1) / p.group;
+    seen = max(pos0 + last_tok, vis);
+    last_seen = max(pos0 + first / p.group, vis);
+    wave_limit = max(pos0 + min(first + 31, w.lq * p.group - 1) / p.group, vis);
+    if (first >= w.lq * p.group) wave_limit = -1;  // no such rows
+  }
+  const int end0 = min(p.shared, seen < 0 ? 0 : (seen == 0x7fffffff ? seen : seen + 1));
+  const int end1 = min(w.lk, seen < p.shared ? 0 : (seen == 0x7fffffff ? seen : seen + 1 - p.shared));
+  const int n0 = ceil_div(end0, BN), n = n0 + ceil_div(end1, BN);
+  const int tbeg = static_cast<int>(static_cast<int64_t>(n) * split / p.splits);
+  const int tend = static_cast<int>(static_cast<int64_t>(n) * (split + 1) / p.splits);
+  Slot slot = {nullptr, RT};
+  if (p.splits > 1) slot.at = p.part + static_cast<size_t>(blockIdx.x) * slot_floats(RT, DP);
+  if constexpr (KEYS) {
+    keys_workgroup<T, DP, false>(p, lds, joint, row, runs, Pages{}, n0, tbeg, tend, last_seen, slot);
+  } else {
+    rows_workgroup<T, DP>(p, lds, row, runs, n0, tbeg, tend, last_seen, wave_limit, slot);
+  }
+}
+
+// One row from its partial sums: `of(i)` gives part i's sums, reference maximum and sum of weights. A
+// wavefront a row, DP / 64 values a lane.
+template <typename T, int DP, typename F>
+__device__ inline void join_row(char* out, int d, int parts, const F& of) {
+  const int lane = threadIdx.x & 63;
+  constexpr int N = DP / 64;
+  float top = -__builtin_huge_valf(), l = 0.f, o[N] = {};
+  for (int i = lane; i < parts; i += kWave) {
+    const float *s, *m;
+    int rows;
+    of(i, s, m, rows);
+    top = fmaxf(top, *m);
+  }
+#pragma unroll
+  for (int i = 1; i < kWave; i *= 2) top = fmaxf(top, __shfl_xor(top, i));
+#pragma unroll 4
+  for (int i = 0; i < parts; ++i) {
+    const float *s, *m;
+    int rows;
+    of(i, s, m, rows);
+    const float f = *m == top ? 1.f : __builtin_amdgcn_exp2f(*m - top);
+    l = fmaf(f, m[rows], l);
+#pragma unroll
+    for (int e = 0; e < N; ++e) o[e] = fmaf(f, s[lane * N + e], o[e]);
+  }
+  const float inv = inverse(l);
+#pragma unroll
+  for (int e = 0; e < N; ++e)
+    if (lane * N + e < d) reinterpret_cast<T*>(out)[lane * N + e] = static_cast<T>(o[e] * inv);
+}
+
+constexpr int kJoinRows = 8;  // rows of a workgroup of the joining kernels: two a wavefront
+
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads) void prompt_join_kernel(Params p, int rt) {
+  const int per = rt / kJoinRows, wave = uniform(threadIdx.x >> 6);
+  const int chunk = blockIdx.x % per, lin = blockIdx.x / per;
+  const int kv = lin % p.hkv, t = lin / p.hkv;
+  Where w;
+  if (!find_tile(p, t, rt, w)) return;
+  for (int i = 0; i < kJoinRows / 4; ++i) {
+    const int r = chunk * kJoinRows + i * 4 + wave;
+    const int tok = (w.tile * rt + r) / p.group, head = kv * p.group + (w.tile * rt + r) % p.group;
+    if (tok >= w.lq) break;
+    const int64_t at = (p.q_off == nullptr ? static_cast<int64_t>(w.seq) * p.q_len : w.q0) + tok;
+    join_row<T, DP>(p.out + (at * p.hq + head) * p.d * static_cast<int>(sizeof(T)), p.d, p.splits,
+                    [&](int s, const float*& o, const float*& m, int& rows) {
+                      const float* slot = p.part + (static_cast<size_t>(t * p.splits + s) * p.hkv + kv) * slot_floats(rt, DP);
+                      o = slot + static_cast<size_t>(r) * DP;
+                      m = slot + static_cast<size_t>(rt) * DP + r;
+                      rows = rt;
+                    });
+  }
+}
+
+// ---- single tokens -------------------------------------------------------------------------------------
+// Workgroups [0, stiles * ssplits * hkv): the shared keys, for the rows (request, query head) of all
+// requests at once, `srows` of them a tile. Then [.., + seqs * otiles * osplits * hkv): the requests' own
+// keys, 32 rows a tile. Slots in the same order. One split of one kind alone writes the output itself.
+__host__ __device__ inline int own_rows(int group) { return group < kKeyTile ? group : kKeyTile; }
+
+template <typename T, int DP, bool SKEYS>
+__global__ __launch_bounds__(kThreads, 2) void decode_kernel(Params p) {
+  constexpr int SRT = SKEYS ? kKeyTile : kRowTile, SBN = SKEYS ? 32 : (sizeof(T) == 2 ? 64 : 32);
+  __shared__ __attribute__((aligned(1024))) char lds[SKEYS ? keys_lds<T, DP>() : cmax(keys_lds<T, DP>(), rows_lds<T, DP>())];
+  __shared__ float joint[257];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int nshared = p.stiles * p.ssplits * p.hkv;
+  const int parts = p.ssplits * (p.stiles > 0) + p.osplits;
+  auto row_of = [&](int b, int head, bool ok) {
+    Row row;
+    row.q = ok ? p.q + b * p.q_seq + head * p.q_head : nullptr;
+    row.out = ok ? p.out + (static_cast<int64_t>(b) * p.hq + head) * p.d * static_cast<int>(sizeof(T)) : nullptr;
+    const int len = ok ? min(max(p.lengths[b], 0), p.k_len) : 0;
+    row.pos = p.shared + len - 1;
+    row.limit = 0x7fffffff;
+    row.slope = ok && p.slopes != nullptr ? p.slopes[head] * kLog2e : 0.f;
+    return row;
+  };
+  if (static_cast<int>(blockIdx.x) < nshared) {
+    int lin = blockIdx.x;
+    const int kv = lin % p.hkv;
+    lin /= p.hkv;
+    const int split = lin % p.ssplits, t = lin / p.ssplits;
+    const int r = t * SRT + (SKEYS ? 0 : 32 * wave) + (lane & 31);
+    const int b = r / p.group;
+    const Row row = row_of(b, kv * p.group + r % p.group, b < p.seqs);
+    const KeyRuns runs = {{p.sk + kv * p.sk_head, p.sv + kv * p.sv_head, p.sk_tok, p.sv_tok, p.shared, 0}, {}};
+    const int n = ceil_div(p.shared, SBN);
+    const int tbeg = static_cast<int>(static_cast<int64_t>(n) * split / p.ssplits);
+    const int tend = static_cast<int>(static_cast<int64_t>(n) * (split + 1) / p.ssplits);
+    Slot slot = {p.part + static_cast<size_t>(blockIdx.x) * slot_floats(SRT, DP), SRT};
+    if constexpr (SKEYS) {
+      keys_workgroup<T, DP, false>(p, lds, joint, row, runs, Pages{}, n, tbeg, tend, 0x7fffffff, slot);
+    } else {
+      const bool some = t * SRT + 32 * wave < p.seqs * p.group;  // a wavefront without rows computes nothing
+      rows_workgroup<T, DP>(p, lds, row, runs, n, tbeg, tend, 0x7fffffff, some ? 0x7fffffff : -1, slot);
+    }
+    return;
+  }
+  int lin = blockIdx.x - nshared;
+  const int own = lin;
+  const int kv = lin % p.hkv;
+  lin /= p.hkv;
+  const int split = lin % p.osplits;
+  lin /= p.osplits;
+  const int rt = lin % p.otiles, b = lin / p.otiles;
+  const int orows = own_rows(p.group), r = rt * kKeyTile + (lane & 31);
+  const Row row = row_of(b, kv * p.group + r, r < p.group);
+  const int len = uniform(min(max(p.lengths[b], 0), p.k_len));
+  KeyRuns runs = {{}, {p.k + kv * p.k_head, p.v + kv * p.v_head, p.k_tok, p.v_tok, len, p.shared}};
+  const Pages pages = {p.pages == nullptr ? nullptr : p.pages + static_cast<size_t>(b) * p.max_pages, p.page, p.num_pages, p.k_seq, p.v_seq};
+  if (p.pages == nullptr) {
+    runs.own.k += b * p.k_seq;
+    runs.own.v += b * p.v_seq;
+  }
+  const int n = ceil_div(len, 32);
+  const int tbeg = static_cast<int>(static_cast<int64_t>(n) * split / p.osplits);
+  const int tend = static_cast<int>(static_cast<int64_t>(n) * (split + 1) / p.osplits);
+  Slot slot = {nullptr, orows};
+  if (parts > 1) slot.at = p.part + static_cast<size_t>(nshared) * slot_floats(SRT, DP) + static_cast<size_t>(own) * slot_floats(orows, DP);
+  keys_workgroup<T, DP, true>(p, lds, joint, row, runs, pages, 0, tbeg, tend, 0x7fffffff, slot);
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads) void decode_join_kernel(Params p, int srt) {
+  const int row = uniform(static_cast<int>(blockIdx.x) * 4 + static_cast<int>(threadIdx.x >> 6));
+  if (row >= p.seqs * p.hq) return;
+  const int b = row / p.hq, head = row % p.hq, kv = head / p.group, g = head % p.group;
+  const int ns = p.stiles > 0 ? p.ssplits : 0, orows = own_rows(p.group);
+  const size_t nshared = static_cast<size_t>(p.stiles) * p.ssplits * p.hkv;
+  const int sr = b * p.group + g;
+  join_row<T, DP>(p.out + static_cast<int64_t>(row) * p.d * static_cast<int>(sizeof(T)), p.d, ns + p.osplits,
+                  [&](int i, const float*& o, const float*& m, int& rows) {
+                    const float* slot;
+                    int r;
+                    if (i < ns) {
+                      slot = p.part + (static_cast<size_t>((sr / srt) * p.ssplits + i) * p.hkv + kv) * slot_floats(srt, DP);
+                      r = sr % srt;
+                      rows = srt;
+                    } else {
+                      const size_t at = ((static_cast<size_t>(b) * p.otiles + g / kKeyTile) * p.osplits + (i - ns)) * p.hkv + kv;
+                      slot = p.part + nshared * slot_floats(srt, DP) + at * slot_floats(orows, DP);
+                      r = g % kKeyTile;
+                      rows = orows;
+                    }
+                    o = slot + static_cast<size_t>(r) * DP;
+                    m = slot + static_cast<size_t>(rows) * DP + r;
+                  });
+}
+
+// ---- host ------------------------------------------------------------------------------------------------
+
+// (what the Python binding packs)
+static_assert(sizeof(g16_attention_args) == 12 * 8 + 13 * 8 + 16 * 4 + 16, "no padding");
+
+int cus_of(const g16_attention_args& a) {
+  if (a.num_cus > 0) return a.num_cus;
+  int dev = 0, n = 0;
+  if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess) return 256;
+  return n > 0 ? n : 256;
+}
+
+// What both entry points check; the strides of operands without elements are not looked at.
+int check(const g16_attention_args& a, bool decode) {
+  const int size = a.is_f32 ? 4 : 2;
+  if (a.is_f32 != 0 && a.is_f32 != 1) return G16_E_DTYPE;
+  if (a.seqs < 0 || a.q_len < 0 || a.k_len < 0 || a.hq < 0 || a.hkv < 0 || a.shared < 0 || a.d <= 0 || a.d % 8 != 0 ||
+      a.d > G16_ATTENTION_MAX_D)
+    return G16_E_SHAPE;
+  if (a.seqs == 0 || a.hq == 0 || (!decode && a.q_len == 0)) return G16_OK;
+  if (a.hkv == 0 || a.hq % a.hkv != 0 || !(a.softcap >= 0.f) || !(a.scale == a.scale)) return G16_E_SHAPE;
+  if (static_cast<int64_t>(a.shared) + a.k_len > (1 << 30) || static_cast<int64_t>(a.q_len) * a.hq > (1LL << 31) - 1 ||
+      static_cast<int64_t>(a.seqs) * a.hq > (1LL << 31) - 1)
+    return G16_E_SHAPE;
+  if (a.q == nullptr || a.out == nullptr) return G16_E_NULL;
+  auto row = [&](int64_t token, int64_t head, bool longest) {
+    const int64_t t = token * size, h = head * size;
+    return t % 16 == 0 && h % 16 == 0 && (!longest || (token >= a.d && t < G16_ATTENTION_MAX_STRIDE));
+  };
+  if (!aligned16(a.q) || !aligned16(a.out) || !row(decode ? 0 : a.q_token, a.q_head, false) || a.q_seq * size % 16 != 0) return G16_E_ALIGN;
+  const bool own = decode ? a.k_len > 0 : a.k_len > 0;
+  if (own) {
+    if (a.k == nullptr || a.v == nullptr) return G16_E_NULL;
+    if (!aligned16(a.k) || !aligned16(a.v) || a.k_seq * size % 16 != 0 || a.v_seq * size % 16 != 0) return G16_E_ALIGN;
+    if (!row(a.k_token, a.k_head, true) || !row(a.v_token, a.v_head, true)) return G16_E_SHAPE;
+  }
+  if (a.shared > 0) {
+    if (a.shared_k == nullptr || a.shared_v == nullptr) return G16_E_NULL;
+    if (!aligned16(a.shared_k) || !aligned16(a.shared_v)) return G16_E_ALIGN;
+    if (!row(a.shared_k_token, a.shared_k_head, true) || !row(a.shared_v_token, a.shared_v_head, true)) return G16_E_SHAPE;
+  }
+  if (decode) {
+    if (a.lengths == nullptr) return G16_E_NULL;
+    if (a.page < 0 || a.max_pages < 0 || a.num_pages < 0) return G16_E_SHAPE;
+    if (a.pages != nullptr && (a.page <= 0 || static_cast<int64_t>(a.page) * a.max_pages < a.k_len)) return G16_E_SHAPE;
+  } else if ((a.q_offsets == nullptr) != (a.k_offsets == nullptr)) {
+    return G16_E_NULL;
+  }
+  return G16_OK;
+}
+
+Params params(const g16_attention_args& a) {
+  const int64_t size = a.is_f32 ? 4 : 2;
+  Params p = {};
+  p.q = static_cast<const char*>(a.q);
+  p.k = static_cast<const char*>(a.k);
+  p.v = static_cast<const char*>(a.v);
+  p.sk = static_cast<const char*>(a.shared_k);
+  p.sv = static_cast<const char*>(a.shared_v);
+  p.out = static_cast<char*>(a.out);
+  p.q_off = a.q_offsets;
+  p.k_off = a.k_offsets;
+  p.visible = a.visible;
+  p.lengths = a.lengths;
+  p.pages = a.pages;
+  p.slopes = a.slopes;
+  p.part = static_cast<float*>(a.workspace);
+  p.q_seq = a.q_seq * size;
+  p.q_tok = a.q_token * size;
+  p.q_head = a.q_head * size;
+  p.k_seq = a.k_seq * size;
+  p.k_head = a.k_head * size;
+  p.v_seq = a.v_seq * size;
+  p.v_head = a.v_head * size;
+  p.sk_head = a.shared_k_head * size;
+  p.sv_head = a.shared_v_head * size;
+  p.k_tok = static_cast<uint32_t>(a.k_token * size);
+  p.v_tok = static_cast<uint32_t>(a.v_token * size);
+  p.sk_tok = static_cast<uint32_t>(a.shared_k_token * size);
+  p.sv_tok = static_cast<uint32_t>(a.shared_v_token * size);
+  p.seqs = a.seqs;
+  p.q_len = a.q_len;
+  p.k_len = a.k_len;
+  p.hq = a.hq;
+  p.hkv = a.hkv;
+  p.group = a.hq / a.hkv;
+  p.d = a.d;
+  p.shared = a.shared;
+  p.causal = a.causal != 0;
+  p.page = a.page;
+  p.max_pages = a.max_pages;
+  p.num_pages = a.num_pages;
+  p.scale = a.scale;
+  p.softcap = a.softcap;
+  return p;
+}
+
+// Splits of `tiles` key tiles so that `items` workgroups become about two a CU, with at least `least` tiles
+// a split.
+int splits_for(int64_t items, int64_t tiles, int cus, int least) {
+  if (items <= 0 || tiles <= 0) return 1;
+  int64_t s = (2 * cus + items - 1) / items;
+  if (s > tiles / least) s = tiles / least;
+  return s < 1 ? 1 : static_cast<int>(s > 256 ? 256 : s);
+}
+
+struct PromptPlan {
+  bool keys;
+  int rt, tiles, splits;
+  size_t bytes;
+};
+PromptPlan plan_prompt(const g16_attention_args& a) {
+  PromptPlan r = {};
+  const int group = a.hq / a.hkv, dp = a.d <= 64 ? 64 : 128;
+  const int64_t rows = a.q_offsets == nullptr ? static_cast<int64_t>(a.q_len) * group : static_cast<int64_t>(a.q_len) * group / a.seqs;
+  r.keys = rows <= 64;
+  r.rt = r.keys ? kKeyTile : kRowTile;
+  const int64_t tiles = a.q_offsets == nullptr ? (rows + r.rt - 1) / r.rt * a.seqs
+                                               : static_cast<int64_t>(a.q_len) * group / r.rt + a.seqs;
+  r.tiles = static_cast<int>(tiles);
+  const int bn = r.keys || a.is_f32 ? 32 : 64;
+  // keys of an average sequence (packed lengths are known on the device only)
+  const int64_t keys = a.shared + (a.q_offsets == nullptr ? a.k_len : a.k_len / a.seqs);
+  const int64_t busy = a.q_offsets == nullptr ? tiles : (rows + r.rt - 1) / r.rt * a.seqs;
+  r.splits = splits_for(busy * a.hkv, (keys + bn - 1) / bn, cus_of(a), r.keys ? 16 : 4);
+  if (r.splits > 1) r.bytes = static_cast<size_t>(r.tiles) * r.splits * a.hkv * slot_floats(r.rt, dp) * sizeof(float);
+  return r;
+}
+
+struct DecodePlan {
+  bool skeys;
+  int stiles, ssplits, otiles, osplits;
+  size_t bytes;
+};
+DecodePlan plan_decode(const g16_attention_args& a) {
+  DecodePlan r = {};
+  const int group = a.hq / a.hkv, dp = a.d <= 64 ? 64 : 128, cus = cus_of(a);
+  const int64_t rows = static_cast<int64_t>(a.seqs) * group;
+  r.skeys = rows <= kKeyTile;
+  const int srt = r.skeys ? kKeyTile : kRowTile, sbn = r.skeys || a.is_f32 ? 32 : 64;
+  r.stiles = a.shared > 0 ? static_cast<int>((rows + srt - 1) / srt) : 0;
+  r.ssplits = splits_for(static_cast<int64_t>(r.stiles) * a.hkv, (a.shared + sbn - 1) / sbn, cus, r.skeys ? 16 : 4);
+  r.otiles = (group + kKeyTile - 1) / kKeyTile;
+  r.osplits = splits_for(static_cast<int64_t>(a.seqs) * r.otiles * a.hkv, (a.k_len + 31) / 32, cus, 16);
+  if (r.stiles > 0 || r.osplits > 1) {
+    r.bytes = (static_cast<size_t>(r.stiles) * r.ssplits * a.hkv * slot_floats(srt, dp) +
+               static_cast<size_t>(a.seqs) * r.otiles * r.osplits * a.hkv * slot_floats(own_rows(group), dp)) * sizeof(float);
+  }
+  return r;
+}
+
+template <typename T, int DP>
+int run_prompt(const Params& p, const PromptPlan& plan, hipStream_t stream) {
+  const dim3 grid(static_cast<unsigned>(plan.tiles) * plan.splits * p.hkv);
+  int rc = plan.keys ? launch(prompt_kernel<T, DP, true>, grid, dim3(kThreads), stream, p)
+                     : launch(prompt_kernel<T, DP, false>, grid, dim3(kThreads), stream, p);
+  if (rc == 0 && plan.splits > 1)
+    rc = launch(prompt_join_kernel<T, DP>, dim3(static_cast<unsigned>(plan.tiles) * p.hkv * (plan.rt / kJoinRows)), dim3(kThreads), stream, p,
+                plan.rt);
+  return rc;
+}
+template <typename T, int DP>
+int run_decode(const Params& p, const DecodePlan& plan, hipStream_t stream) {
+  const dim3 grid((static_cast<unsigned>(p.stiles) * p.ssplits + static_cast<unsigned>(p.seqs) * p.otiles * p.osplits) * p.hkv);
+  int rc = plan.skeys ? launch(decode_kernel<T, DP, true>, grid, dim3(kThreads), stream, p)
+                      : launch(decode_kernel<T, DP, false>, grid, dim3(kThreads), stream, p);
+  if (rc == 0 && plan.bytes > 0)
+    rc = launch(decode_join_kernel<T, DP>, dim3(static_cast<unsigned>((static_cast<int64_t>(p.seqs) * p.hq + 3) / 4)), dim3(kThreads), stream, p,
+                plan.skeys ? kKeyTile : kRowTile);
+  return rc;
+}
+
+bool fits_grid(int64_t workgroups) { return workgroups <= (1LL << 24) - 1; }  // 2^32 threads a launch
+
+}  // namespace
+}  // namespace g16
+
+using namespace g16;
+
+extern "C" size_t g16_attention_workspace_bytes(const g16_attention_args* args) {
+  if (args == nullptr || check(*args, false) != G16_OK || args->seqs == 0 || args->hq == 0 || args->q_len == 0) return 0;
+  return plan_prompt(*args).bytes;
+}
+
+extern "C" int g16_attention(const g16_attention_args* args, void* stream) {
+  if (args == nullptr) return G16_E_NULL;
+  const g16_attention_args& a = *args;
+  const int st = check(a, false);
+  if (st != G16_OK || a.seqs == 0 || a.hq == 0 || a.q_len == 0) return st;
+  const PromptPlan plan = plan_prompt(a);
+  if (plan.bytes > 0 && (a.workspace == nullptr || static_cast<size_t>(a.workspace_bytes) < plan.bytes)) return G16_E_WORKSPACE;
+  if (!aligned16(a.workspace)) return G16_E_ALIGN;
+  if (!fits_grid(static_cast<int64_t>(plan.tiles) * plan.splits * a.hkv) ||
+      !fits_grid(static_cast<int64_t>(plan.tiles) * a.hkv * (plan.rt / kJoinRows)))
+    return G16_E_SHAPE;
+  Params p = params(a);
+  p.tiles = plan.tiles;
+  p.splits = plan.splits;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (a.is_f32) return a.d <= 64 ? run_prompt<float, 64>(p, plan, s) : run_prompt<float, 128>(p, plan, s);
+  return a.d <= 64 ? run_prompt<_Float16, 64>(p, plan, s) : run_prompt<_Float16, 128>(p, plan, s);
+}
+
+extern "C" size_t g16_attention_decode_workspace_bytes(const g16_attention_args* args) {
+  if (args == nullptr || check(*args, true) != G16_OK || args->seqs == 0 || args->hq == 0) return 0;
+  return plan_decode(*args).bytes;
+}
+
+extern "C" int g16_attention_decode(const g16_attention_args* args, void* stream) {
+  if (args == nullptr) return G16_E_NULL;
+  const g16_attention_args& a = *args;
+  const int st = check(a, true);
+  if (st != G16_OK || a.seqs == 0 || a.hq == 0) return st;
+  const DecodePlan plan = plan_decode(a);
+  if (plan.bytes > 0 && (a.workspace == nullptr || static_cast<size_t>(a.workspace_bytes) < plan.bytes)) return G16_E_WORKSPACE;
+  if (!aligned16(a.workspace)) return G16_E_ALIGN;
+  if (!fits_grid((static_cast<int64_t>(plan.stiles) * plan.ssplits + static_cast<int64_t>(a.seqs) * plan.otiles * plan.osplits) * a.hkv) ||
+      !fits_grid((static_cast<int64_t>(a.seqs) * a.hq + 3) / 4))
+    return G16_E_SHAPE;
+  Params p = params(a);
+  p.causal = 0;
+  p.stiles = plan.stiles;
+  p.ssplits = plan.ssplits;
+  p.otiles = plan.otiles;
+  p.osplits = plan.osplits;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (a.is_f32) return a.d <= 64 ? run_decode<float, 64>(p, plan, s) : run_decode<float, 128>(p, plan, s);
+  return a.d <= 64 ? run_decode<_Float16, 64>(p, plan, s) : run_decode<_Float16, 128>(p, plan, s);
+}

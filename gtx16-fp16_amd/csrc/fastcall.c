@@ -13,6 +13,7 @@
 #include <Python.h>
 #include <stddef.h>
 #include <stdint.h>
+#include <string.h>
 
 typedef int (*skinny_fn)(const void*, const void*, void*, const void*, int, int, int, int, void*, size_t, void*,
                          size_t, void*);
@@ -179,6 +180,56 @@ static PyObject* fast_mm_t_gemm(PyObject* self, PyObject* const* args, Py_ssize_
   return PyLong_FromLong(st);
 }
 
+/* Entry points that take one struct of arguments whose last two fields are the workspace and its size:
+ * `head` holds the fields before them. */
+typedef size_t (*args_size_fn)(const void*);
+typedef int (*args_call_fn)(const void*, void*);
+enum { kMaxArgs = 512 };
+typedef struct {
+  void* workspace;
+  int64_t workspace_bytes;
+} args_tail;
+
+static int join_args(PyObject* head, void* ws, size_t ws_bytes, unsigned char* out) {
+  char* data;
+  Py_ssize_t n;
+  if (PyBytes_AsStringAndSize(head, &data, &n)) return -1;
+  if (n % 8 != 0 || n > (Py_ssize_t)(kMaxArgs - sizeof(args_tail))) {
+    PyErr_SetString(PyExc_ValueError, "argument struct of an unexpected size");
+    return -1;
+  }
+  const args_tail tail = {ws, (int64_t)ws_bytes};
+  memcpy(out, data, (size_t)n);
+  memcpy(out + n, &tail, sizeof(tail));
+  return 0;
+}
+
+/* args_size(fn_addr, head) -> size_t fn(const args*) */
+static PyObject* fast_args_size(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  void* fn;
+  _Alignas(16) unsigned char buf[kMaxArgs];
+  if (check_nargs("args_size", nargs, 2) || as_ptr(args[0], &fn) || check_bound(fn) || join_args(args[1], NULL, 0, buf))
+    return NULL;
+  return PyLong_FromSize_t(((args_size_fn)fn)(buf));
+}
+
+/* args_call(fn_addr, head, workspace, workspace_bytes, stream) -> status of int fn(const args*, stream) */
+static PyObject* fast_args_call(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  void *fn, *ws, *stream;
+  size_t ws_bytes;
+  int st;
+  _Alignas(16) unsigned char buf[kMaxArgs];
+  if (check_nargs("args_call", nargs, 5) || as_ptr(args[0], &fn) || check_bound(fn) || as_ptr(args[2], &ws) ||
+      as_size(args[3], &ws_bytes) || as_ptr(args[4], &stream) || join_args(args[1], ws, ws_bytes, buf))
+    return NULL;
+  Py_BEGIN_ALLOW_THREADS
+  st = ((args_call_fn)fn)(buf, stream);
+  Py_END_ALLOW_THREADS
+  return PyLong_FromLong(st);
+}
+
 static PyMethodDef fast_methods[] = {
     {"bind", (PyCFunction)(void (*)(void))fast_bind, METH_FASTCALL,
      "bind(skinny_f32in_addr, mm_t_gemm_addr, skinny_strips_f32in_addr, skinny_addr, skinny_strips_addr)"},
@@ -192,6 +243,10 @@ static PyMethodDef fast_methods[] = {
      "g16_skinny_f32in with fast argument parsing; returns its status"},
     {"mm_t_gemm", (PyCFunction)(void (*)(void))fast_mm_t_gemm, METH_FASTCALL,
      "g16_mm_t_gemm with fast argument parsing; returns its status"},
+    {"args_size", (PyCFunction)(void (*)(void))fast_args_size, METH_FASTCALL,
+     "a *_workspace_bytes entry point, by address, on a struct of arguments; returns its size"},
+    {"args_call", (PyCFunction)(void (*)(void))fast_args_call, METH_FASTCALL,
+     "an entry point, by address, on a struct of arguments; returns its status"},
     {NULL, NULL, 0, NULL},
 };
 

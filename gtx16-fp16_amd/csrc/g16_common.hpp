@@ -123,6 +123,53 @@ __device__ inline void reset_counter(uint32_t* counter) {
   if (threadIdx.x == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
+// ---- LDS: DMA into it, transposing reads, barriers ----
+
+constexpr uint32_t kOob = 0x80000000u;  // buffer offset past every descriptor's range: reads 0
+
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(3))) short4v lds_short4v;
+
+// LDS byte address -> LDS address-space pointer (the transpose-read builtin takes one).
+__device__ inline lds_short4v* lds4_at(uint32_t addr) { return reinterpret_cast<lds_short4v*>(static_cast<uintptr_t>(addr)); }
+
+// 16-byte DMA global -> LDS: lane i's chunk at buffer offset `off` lands at LDS byte lds + 16 i.
+// Issued as inline asm so the compiler's wait-counter bookkeeping does not see an LDS write it
+// cannot tell apart from the stage being read (it would wait for the DMA before every LDS
+// read); the kernel waits for its DMA explicitly (vmcnt 0) before the barrier that publishes a
+// stage. Vector memory returns in order, so the compiler's own vmcnt waits stay correct (they can
+// only wait longer) with these loads in flight. M0 (the LDS base of the DMA) is set and consumed
+// inside the same statement; clang warns that m0 is reserved, but these kernels contain no other
+// reader of M0 (no LDS-direct, GWS or message instructions): in the generated assembly every
+// `s_mov_b32 m0` is one of these statements, immediately followed by its DMA.
+// `lds_addr` is the LDS byte address (see lds_base) of the 1 KB the instruction fills.
+__device__ inline void dma16(__amdgpu_buffer_rsrc_t rsrc, uint32_t lds_addr, uint32_t off) {
+  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :
+               : "s"(__builtin_amdgcn_readfirstlane(lds_addr)), "v"(off), "s"(rsrc)
+               : "memory", "m0");
+}
+
+// LDS byte address of a __shared__ object, taken once per kernel: converting a generic pointer to
+// the LDS address space costs a 64-bit add and a null test, too much to repeat for every DMA
+// instruction of a loop that issues few other instructions.
+__device__ inline uint32_t lds_base(const void* p) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void*)p));
+}
+
+// s_waitcnt vmcnt(N) with expcnt/lgkmcnt left alone: waits until at most N of this wavefront's
+// vector-memory operations (here: the DMA of younger stages) are still in flight.
+template <int N>
+__device__ inline void wait_dma_le() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// Workgroup barrier without the counter waits __syncthreads() adds: the caller has already waited
+// for exactly the memory operations the next phase depends on. The memory clobber keeps the
+// compiler from moving LDS accesses across it.
+__device__ inline void phase_barrier() { asm volatile("s_barrier" ::: "memory"); }
+
 // Tile-packed operand layout of the 256x256 GEMM (activations from the rowscale cast, weights from
 // g16_pack_weight). An operand with R rows (rows = M for activations, N for the transposed
 // weight) and K columns is stored as blocks of kPackRows rows x kPackK columns; block (t, ks) is at

@@ -92,39 +92,6 @@ constexpr int kSplitAlign = 64;  // split-K slices start on a multiple of every 
 // vs 7.2); at K = 1024 four slices win (64 x 1024^2 7.7 -> 7.1).
 constexpr int kMinSplitK = 1024;
 constexpr float kHalfMax = 65504.f;  // largest finite fp16
-constexpr uint32_t kOob = 0x80000000u;  // buffer offset past every descriptor's range: reads 0
-
-typedef short short4v __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) void lds_void;
-typedef __attribute__((address_space(3))) short4v lds_short4v;
-
-// LDS byte address -> LDS address-space pointer (the transpose-read builtin takes one).
-__device__ inline lds_short4v* lds4_at(uint32_t addr) { return reinterpret_cast<lds_short4v*>(static_cast<uintptr_t>(addr)); }
-
-// 16-byte DMA global -> LDS: lane i's chunk at buffer offset `off` lands at LDS byte lds + 16 i.
-// Issued as inline asm so the compiler's wait-counter bookkeeping does not see an LDS write it
-// cannot tell apart from the stage being read (it would wait for the DMA before every LDS
-// read); the kernel waits for its DMA explicitly (vmcnt 0) before the barrier that publishes a
-// stage. Vector memory returns in order, so the compiler's own vmcnt waits stay correct (they can
-// only wait longer) with these loads in flight. M0 (the LDS base of the DMA) is set and consumed
-// inside the same statement; clang warns that m0 is reserved, but these kernels contain no other
-// reader of M0 (no LDS-direct, GWS or message instructions): in the generated assembly every
-// `s_mov_b32 m0` is one of these statements, immediately followed by its DMA.
-// `lds_addr` is the LDS byte address (see lds_base) of the 1 KB the instruction fills.
-__device__ inline void dma16(__amdgpu_buffer_rsrc_t rsrc, uint32_t lds_addr, uint32_t off) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-               :
-               : "s"(__builtin_amdgcn_readfirstlane(lds_addr)), "v"(off), "s"(rsrc)
-               : "memory", "m0");
-}
-
-// LDS byte address of a __shared__ object, taken once per kernel: converting a generic pointer to
-// the LDS address space costs a 64-bit add and a null test, too much to repeat for every DMA
-// instruction of a loop that issues few other instructions.
-__device__ inline uint32_t lds_base(const void* p) {
-  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void*)p));
-}
-
 template <int BM_, int BN_, int BK_, int WGM_, int WGN_, int NSTAGE_, bool MF16_ = false>
 struct TileCfg {
   static constexpr int BM = BM_, BN = BN_, BK = BK_, WGM = WGM_, WGN = WGN_, NSTAGE = NSTAGE_;
@@ -194,12 +161,6 @@ using Cfg64 = TileCfg<64, 128, 64, 1, 4, 4>;
 using Cfg32 = TileCfg<32, 128, 64, 1, 4, 4>;
 using Cfg64x64 = TileCfg<64, 64, 64, 2, 2, 4>;  // 64 KB: the square 4-wavefront tile
 
-// s_waitcnt vmcnt(N) with expcnt/lgkmcnt left alone: waits until at most N of this wavefront's
-// vector-memory operations (here: the DMA of younger stages) are still in flight.
-template <int N>
-__device__ inline void wait_dma_le() {
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-}
 // s_waitcnt immediate for vmcnt(0) alone (expcnt 7, lgkmcnt 15 leave those counters alone), for
 // __builtin_amdgcn_s_waitcnt, whose waits the compiler's own wait tracking takes into account.
 constexpr int kWaitVmcnt0 = 0x0f70;
@@ -247,11 +208,6 @@ __device__ inline uint32_t arrive_add_coherent(uint32_t* counter, uint32_t add) 
 // row (direct); each slice adds its own bit once, so the fields never carry into each other.
 constexpr int kSpecShift = 8;
 constexpr int kSpecMaxSplit = 32 - kSpecShift;
-
-// Workgroup barrier without the counter waits __syncthreads() adds: the caller has already waited
-// for exactly the memory operations the next phase depends on. The memory clobber keeps the
-// compiler from moving LDS accesses across it.
-__device__ inline void phase_barrier() { asm volatile("s_barrier" ::: "memory"); }
 
 // Largest |x| of m and 4 values, a NaN among them kept: the cast of direct A takes it over several rows
 // of a lane at once, and v_max_f32 and v_max3_f32, which drop a quiet NaN, lose the maximum itself to a

@@ -6,6 +6,7 @@
 
 Same exports and version as the reference package (src/gtx16_fp16/__init__.py:7-11).
 """
+from .attn import attention, attention_decode
 from .linear import FastLinear, patch
 from .ops import is_affected, matmul, mm_t, supported
 

@@ -16,7 +16,7 @@ from pathlib import Path
 import torch  # noqa: F401  (loads torch's HIP runtime before libg16.so)
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libg16.so"
-ABI_VERSION = 16
+ABI_VERSION = 17
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
@@ -68,6 +68,10 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "g16_skinny": (_I, [_P, _I, _P, _P, _I, _P, _I, _I, _I, _I, _P, _SZ, _P, _SZ, _P]),
     "g16_skinny_strips": (_I, [_P, _I, _P, _P, _I, _P, _I, _I, _I, _P]),
     "g16_skinny_strips_route": (_I, [_I, _I, _I, _I]),
+    "g16_attention_workspace_bytes": (_SZ, [_P]),
+    "g16_attention": (_I, [_P, _P]),
+    "g16_attention_decode_workspace_bytes": (_SZ, [_P]),
+    "g16_attention_decode": (_I, [_P, _P]),
     "g16_gemm_clock": (_I, [_P, _P]),
     "g16_peak_flops_per_lane_iter": (ctypes.c_double, [_I]),
     "g16_peak_run": (_I, [_I, _I, _I, _P, _P]),
@@ -104,6 +108,11 @@ def load(path: Path | str | None = None) -> ctypes.CDLL:
         if path is None:
             _lib = lib
         return lib
+
+
+def address(name: str) -> int:
+    """Address of the library's entry point ``name``, for ``fast().args_size`` and ``fast().args_call``."""
+    return ctypes.cast(getattr(load(), name), ctypes.c_void_p).value
 
 
 _fast = None

@@ -47,7 +47,7 @@
 extern "C" {
 #endif
 
-#define G16_ABI_VERSION 16
+#define G16_ABI_VERSION 17
 
 /* Status codes (negative: rejected by the library before any launch). */
 #define G16_OK 0
@@ -354,6 +354,52 @@ int g16_peak_run_clocked(int kind, int blocks, int iters, float* out, unsigned l
 int g16_stream_read(const void* buf, size_t bytes, int blocks, float* out, void* stream);
 int g16_peak_mfma_data(int blocks, int iters, const uint16_t* operands, int ngroups, float* out,
                        unsigned long long* clocks, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Attention of packed prompts (g16_attention) and of one token per request over a cache
+ * (g16_attention_decode). For query row i at position p_i and the keys j at positions p_j that it sees,
+ *     s_ij = f(scale * q_i . k_j),  f(x) = softcap * tanh(x / softcap) (softcap 0: x),
+ *     s_ij -= slopes[head] * |p_i - p_j|                               (slopes NULL: nothing),
+ *     out_i = sum_j softmax_j(s_ij) v_j,
+ * zeros where a row sees no key. Query head h reads key head h / (hq / hkv). Types: fp16 or fp32 (is_f32),
+ * head dimension d a multiple of 8 up to G16_ATTENTION_MAX_D; scores, softmax and sums in fp32 (fp16
+ * weights are rounded to fp16 for their product with v).
+ *   The keys of a sequence are `shared` common ones (positions 0 ..), then its own (positions shared ..).
+ * g16_attention: its query rows stand at the end of its own keys, row t of lq at position
+ * shared + lk - lq + t. q_offsets and k_offsets (int32, seqs + 1 values) give the sequences' runs in
+ * packed q and k, v (q_len, k_len: rows of the packed tensors); without them sequence b starts at
+ * b * q_seq, b * k_seq, b * v_seq and has q_len rows and k_len keys. causal: a row sees p_j <= p_i and p_j <
+ * visible[b] (NULL: none); else every key of its sequence. Values behind keys that a row does not see
+ * do not reach it, infinities and NaN included.
+ * g16_attention_decode: one row per sequence, q and out [seqs, hq, d], at position shared + lengths[b] - 1; its
+ * own keys are the first lengths[b] (held to 0 .. its capacity) of its cache: rows of pages of `page` keys,
+ * pages[b * max_pages + i] the i-th (a page outside 0 .. num_pages - 1 reads as zeros; page stride k_seq,
+ * v_seq), or, with pages NULL, the `page` keys at b * k_seq. Values past a length do not reach any row.
+ *   Strides are in elements, multiples of 16 bytes, d elements contiguous; a token's stride is at least d
+ * and below G16_ATTENTION_MAX_STRIDE bytes. out is contiguous ([rows, hq, d]). workspace: at least
+ * *_workspace_bytes() for the same arguments, 16-byte aligned, no initialisation (NULL where that is 0).
+ * One launch, two where the keys are split over workgroups. Offsets outside the tensors are held to them.
+ */
+#define G16_ATTENTION_MAX_D 128
+#define G16_ATTENTION_MAX_STRIDE (1 << 24)
+typedef struct {
+  const void *q, *k, *v, *shared_k, *shared_v;
+  void* out;
+  const int32_t *q_offsets, *k_offsets, *visible, *lengths, *pages;
+  const float* slopes;
+  int64_t q_seq, q_token, q_head, k_seq, k_token, k_head, v_seq, v_token, v_head;
+  int64_t shared_k_token, shared_k_head, shared_v_token, shared_v_head;
+  int32_t seqs, q_len, k_len, hq, hkv, d, shared, causal;
+  int32_t page, max_pages, num_pages, is_f32, num_cus;
+  float scale, softcap;
+  int32_t reserved; /* 0 */
+  void* workspace;
+  int64_t workspace_bytes;
+} g16_attention_args;
+size_t g16_attention_workspace_bytes(const g16_attention_args* args);
+int g16_attention(const g16_attention_args* args, void* stream);
+size_t g16_attention_decode_workspace_bytes(const g16_attention_args* args);
+int g16_attention_decode(const g16_attention_args* args, void* stream);
 
 #ifdef __cplusplus
 }
