@@ -8,6 +8,7 @@ Same exports and version as the reference package (src/gtx16_fp16/__init__.py:7-
 """
 from .attn import attention, attention_decode
 from .linear import FastLinear, patch
+from .lora import lora_mm_t
 from .ops import is_affected, matmul, mm_t, supported
 
 __all__ = ["FastLinear", "patch", "is_affected", "matmul", "mm_t", "supported"]

@@ -72,6 +72,9 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "g16_attention": (_I, [_P, _P]),
     "g16_attention_decode_workspace_bytes": (_SZ, [_P]),
     "g16_attention_decode": (_I, [_P, _P]),
+    "g16_lora_workspace_bytes": (_SZ, [_P]),
+    "g16_lora_shrink": (_I, [_P, _P]),
+    "g16_lora_expand": (_I, [_P, _P]),
     "g16_gemm_clock": (_I, [_P, _P]),
     "g16_peak_flops_per_lane_iter": (ctypes.c_double, [_I]),
     "g16_peak_run": (_I, [_I, _I, _I, _P, _P]),

@@ -401,6 +401,31 @@ int g16_attention(const g16_attention_args* args, void* stream);
 size_t g16_attention_decode_workspace_bytes(const g16_attention_args* args);
 int g16_attention_decode(const g16_attention_args* args, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Low-rank adapters beside a shared projection: with y [M,N] (fp32) the projection's result,
+ *     out[m,:] = y[m,:] + scale[a] * (x[m,:] @ down[a]^T) @ up[a]^T,   a = index[m],
+ * x [M,K] fp32 or fp16, down [adapters,rank,K] and up [adapters,N,rank] fp16, scale [adapters] fp32 (NULL: 1),
+ * out [M,N] fp32 (y itself, too) or fp16. A row whose index is negative or not below `adapters` has no
+ * adapter: out is y there. K, N and rank multiples of 8, rank up to G16_LORA_MAX_RANK; all contiguous, 16-byte
+ * aligned. g16_lora_shrink leaves scale * x @ down^T in the workspace (fp32), g16_lora_expand does the
+ * rest: two launches, between which the projection may run. Both take the same arguments and a workspace of
+ * g16_lora_workspace_bytes(). Sums are fp32, and nothing is rounded before the output.
+ */
+#define G16_LORA_MAX_RANK 128
+typedef struct {
+  const void* x;
+  const uint16_t *down, *up;
+  const int32_t* index;
+  const float *scale, *y;
+  void* out;
+  int32_t M, K, N, rank, adapters, x_is_f32, out_is_f16, num_cus;
+  void* workspace;
+  int64_t workspace_bytes;
+} g16_lora_args;
+size_t g16_lora_workspace_bytes(const g16_lora_args* args);
+int g16_lora_shrink(const g16_lora_args* args, void* stream);
+int g16_lora_expand(const g16_lora_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,194 @@
+"""GPU tests of ``lora_mm_t`` against the formula in 64 bits.
+
+Bounds: the output is rounded once to its type (2^-11 or 2^-24); sums over K and over the rank are fp32 (random
+roundings: 4 sqrt(n) 2^-24 of the sum of magnitudes); past 8 rows the shared product rounds fp32 activations
+to fp16 (2^-11 of each, at most 2^-11 of the sum of |x w|), as ``mm_t`` says; the adapters' part rounds nothing.
+"""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import gtx16_fp16 as g
+from gtx16_fp16 import ops
+
+pytestmark = pytest.mark.gpu
+
+F16, F32 = torch.float16, torch.float32
+
+
+def make(M, K, N, r, n, dtype=F16, seed=0, bias=True, scale=True):
+    gen = torch.Generator().manual_seed(seed)
+    rand = lambda *s, by=1.0: by * torch.randn(*s, generator=gen)  # noqa: E731
+    return dict(x=rand(M, K).to(dtype), w=rand(K, N, by=0.05).half(), down=rand(n, r, K, by=K ** -0.5 if K else 1.0).half(),
+                up=rand(n, N, r, by=0.2).half(), index=torch.randint(-1, max(n, 1), (M,), generator=gen, dtype=torch.int32),
+                bias=rand(N) if bias else None, scale=0.5 + torch.rand(n, generator=gen) if scale else None)
+
+
+def reference(c, out):
+    x, w = c["x"].double(), c["w"].double()
+    K = x.shape[1]
+    y, size = x @ w, x.abs() @ w.abs()
+    err = (4 * K ** 0.5 * 2.0 ** -24 + (2.0 ** -11 if c["x"].dtype == F32 and x.shape[0] > 8 else 0.0)) * size
+    if c["bias"] is not None:
+        y = y + c["bias"].double()
+    for a in range(c["down"].shape[0]):
+        rows = (c["index"] == a).nonzero().flatten()
+        if rows.numel():
+            s = 1.0 if c["scale"] is None else float(c["scale"][a])
+            d, u = c["down"][a].double(), c["up"][a].double()
+            y[rows] += s * ((x[rows] @ d.T) @ u.T)
+            low = s * (x[rows].abs() @ d.abs().T) @ u.abs().T
+            err[rows] += 4 * (K ** 0.5 + d.shape[0] ** 0.5 + 2) * 2.0 ** -24 * low
+    # (the last additions: the shared result, the bias and the adapters' part in fp32)
+    u = 2.0 ** -11 if out == F16 else 2.0 ** -24
+    return y, err + (u + 2 * 2.0 ** -24) * y.abs() + 2 * 2.0 ** -24 * size + (2.0 ** -25 if out == F16 else 1e-37)
+
+
+def run(dev, c, out=F16):
+    put = lambda t: None if t is None else t.to(dev)  # noqa: E731
+    return g.lora_mm_t(put(c["x"]), put(c["w"]), put(c["down"]), put(c["up"]), put(c["index"]), scale=put(c["scale"]), bias=put(c["bias"]),
+                       out_dtype=out)
+
+
+def check(dev, c, out=F16):
+    y = run(dev, c, out)
+    assert y.dtype == out and y.is_contiguous()
+    ref, tol = reference(c, out)
+    over = ((y.double().cpu() - ref).abs() / tol).max().item() if ref.numel() else 0.0
+    assert over <= 1.0, f"{over:.3g} times the bound"
+    return y
+
+
+@pytest.mark.parametrize("M", [1, 2, 7, 8, 9, 15, 16, 17, 64, 130, 600])
+@pytest.mark.parametrize("x,out", [(F16, F16), (F16, F32), (F32, F32), (F32, F16)])
+def test_rows_and_types(cuda, M, x, out):
+    check(cuda, make(M, 512, 384, 16, 5, x, seed=M), out)
+
+
+@pytest.mark.parametrize("r", [8, 16, 24, 32, 40, 64, 72, 128])
+@pytest.mark.parametrize("M", [3, 50, 300])
+@pytest.mark.parametrize("x", [F16, F32])
+def test_ranks(cuda, r, M, x):
+    check(cuda, make(M, 264, 520, r, 4, x, seed=r))
+
+
+@pytest.mark.parametrize("K,N", [(8, 8), (8, 4096), (4096, 8), (40, 72), (1000, 1048), (5000, 264)])
+@pytest.mark.parametrize("M", [1, 33])
+def test_odd_sizes(cuda, K, N, M):
+    check(cuda, make(M, K, N, 8, 3, seed=K + N))
+    check(cuda, make(M, K, N, 32, 3, F32, seed=K + N), F32)
+
+
+@pytest.mark.parametrize("M,n", [(48, 48), (200, 64), (5000, 3)])
+def test_every_row_its_own_adapter_or_long_runs(cuda, M, n):
+    c = make(M, 256, 256, 16, n, seed=M)
+    if n == 48:
+        c["index"] = torch.randperm(48, dtype=torch.int32)
+    elif n == 3:
+        c["index"] = (torch.arange(M) // 1700).to(torch.int32)
+    check(cuda, c)
+
+
+def test_rows_without_an_adapter_equal_the_shared_product(cuda):
+    c = make(100, 256, 512, 16, 4)
+    c["index"][:] = -1
+    c["index"][[3, 40]] = torch.tensor([4, 1 << 30], dtype=torch.int32)  # past the last adapter
+    y = run(cuda, c, F32)
+    assert torch.equal(y, ops.mm_t(c["x"].to(cuda), c["w"].to(cuda), c["bias"].to(cuda), F32))
+    check(cuda, c, F16)
+
+
+@pytest.mark.parametrize("n,r", [(0, 16), (3, 0)])
+@pytest.mark.parametrize("out", [F16, F32])
+def test_no_adapters(cuda, n, r, out):
+    c = make(20, 64, 64, r, n)
+    y = run(cuda, c, out)
+    assert torch.equal(y, ops.mm_t(c["x"].to(cuda), c["w"].to(cuda), c["bias"].to(cuda), F32).to(out))
+
+
+def test_empty_sizes(cuda):
+    assert run(cuda, make(0, 64, 64, 8, 2)).shape == (0, 64)
+    c = make(5, 0, 64, 8, 2)
+    assert torch.equal(run(cuda, c, F32).cpu(), c["bias"].expand(5, 64))
+
+
+def test_without_scale_and_bias(cuda):
+    check(cuda, make(70, 256, 264, 24, 3, bias=False, scale=False))
+
+
+def test_large_activations_keep_the_adapters_exact(cuda):
+    # rows far past fp16's range: low-rank sums of 1e6 and more
+    c = make(40, 256, 256, 16, 3, F32)
+    c["x"][7] *= 1e6
+    check(cuda, c, F32)
+
+
+def test_infinite_and_nan_activations_stay_in_their_rows(cuda):
+    for M in (5, 40, 600):
+        c = make(M, 256, 264, 16, 3, F32)
+        c["index"][:] = torch.arange(M, dtype=torch.int32) % 3
+        ref, tol = reference(c, F32)
+        c["x"][1, 5], c["x"][2, 9] = float("inf"), float("nan")
+        y = run(cuda, c, F32).cpu().double()
+        keep = [i for i in range(M) if i not in (1, 2)]
+        assert ((y - ref).abs() / tol)[keep].max() <= 1.0
+        assert not torch.isfinite(y[1:3]).any()
+
+
+def test_views_are_copied(cuda):
+    c = make(30, 128, 128, 8, 2)
+    want = run(cuda, c)
+    put = lambda t: t.to(cuda)  # noqa: E731
+    wide = torch.zeros(30, 256, dtype=F16, device=cuda)
+    wide[:, 3:131] = put(c["x"])
+    down = put(c["down"]).transpose(1, 2).contiguous().transpose(1, 2)
+    up = put(c["up"]).transpose(1, 2).contiguous().transpose(1, 2)
+    idx = put(c["index"]).repeat_interleave(2)[::2]
+    y = g.lora_mm_t(wide[:, 3:131], put(c["w"]), down, up, idx, scale=put(c["scale"]), bias=put(c["bias"]), out_dtype=F16)
+    assert torch.equal(y, want)
+
+
+def test_repeated_calls_streams_and_graphs(cuda):
+    for M in (4, 40, 700):
+        c = {k: None if v is None else v.to(cuda) for k, v in make(M, 512, 512, 16, 6).items()}
+        call = lambda: g.lora_mm_t(c["x"], c["w"], c["down"], c["up"], c["index"], scale=c["scale"], bias=c["bias"], out_dtype=F16)  # noqa: E731,B023
+        want = call()
+        assert all(torch.equal(call(), want) for _ in range(4))
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(s):
+            y = call()
+            with torch.cuda.graph(graph, stream=s):
+                z = call()
+        torch.cuda.current_stream().wait_stream(s)
+        assert torch.equal(y, want)
+        for _ in range(3):
+            z.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(z, want)
+            assert torch.equal(call(), want)
+
+
+def test_refusals(cuda):
+    c = {k: v.to(cuda) for k, v in make(20, 64, 64, 8, 2).items()}
+
+    def call(**changes):
+        d = dict(c, out=F16, **{})
+        d.update(changes)
+        return g.lora_mm_t(d["x"], d["w"], d["down"], d["up"], d["index"], scale=d["scale"], bias=d["bias"], out_dtype=d["out"])
+
+    call()
+    for changes in (dict(x=c["x"].bfloat16()), dict(x=c["x"].cpu()), dict(x=c["x"][0]), dict(w=c["w"].float()), dict(w=c["w"][:32]),
+                    dict(down=c["down"].float()), dict(down=c["down"][:1]), dict(down=c["down"][:, :, :32]), dict(up=c["up"][:, :, :4]),
+                    dict(up=c["up"].transpose(1, 2)), dict(down=c["down"][:, :4], up=c["up"][:, :, :4]), dict(up=c["up"].cpu()),
+                    dict(down=c["down"].repeat(1, 17, 1), up=c["up"].repeat(1, 1, 17)), dict(index=c["index"].long()),
+                    dict(index=c["index"][:3]), dict(index=c["index"].cpu()), dict(scale=c["scale"].half()), dict(scale=c["scale"][:1]),
+                    dict(bias=c["bias"][:3]), dict(out=torch.bfloat16)):
+        with pytest.raises(ValueError):
+            call(**changes)
+            pytest.fail(f"{list(changes)} was taken")
+    with pytest.raises(RuntimeError, match="no_grad"):
+        call(x=c["x"].clone().requires_grad_())
