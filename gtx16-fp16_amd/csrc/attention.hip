@@ -85,7 +85,8 @@ struct Params {
   int tiles, splits;              // prompts: row tiles (an upper bound where packed), key splits
   int stiles, ssplits, osplits;   // single tokens: row tiles and splits of the shared keys, splits of the own
   int otiles;                     // ... and row tiles of 32 of one request's `group` rows
-  float scale, softcap;
+  float scale, softcap;  // scale > 0, with its sign (0 for 0) in `sign`, which the queries take on
+  float sign;
 };
 
 // One run of keys: the shared ones, or a sequence's own.
@@ -105,6 +106,11 @@ struct KeyRuns {
   }
 };
 
+template <typename V>
+__device__ inline const __attribute__((address_space(3))) V* lds_at(uint32_t addr) {
+  return reinterpret_cast<const __attribute__((address_space(3))) V*>(static_cast<uintptr_t>(addr));
+}
+
 // ---- tiles in LDS -------------------------------------------------------------------------------
 // BN rows (keys) of DP values, 16-byte chunk c of row r at chunk position c ^ swizzle(r). K is read a
 // row per lane (16 lanes cover 16 rows at one chunk: their positions differ in a 256-byte bank period);
@@ -121,40 +127,46 @@ struct Tile {
     else if constexpr (RC == 8) return (((row >> 1) & 1) << 2) | (((row >> 3) & 1) << 1);
     else return (row & 3) << 2;
   }
+  // Within a row the swizzle and a step's chunks only touch different bits, so a lane's place in the tile
+  // is one address per tile, and a step's an exclusive or and an immediate away from it.
   // K rows 32 kb + lane % 32 of the tile, values 16 ks + 8 (lane / 32) .. +7
-  __device__ static V8 k_frag(const char* lds, int kb, int ks, int lane) {
-    const int row = 32 * kb + (lane & 31), h = lane >> 5;
-    const char* at = lds + row * ROWB;
+  __device__ static uint32_t k_lane(int lane) {
+    const int row = lane & 31, h = lane >> 5;
+    return row * ROWB + (((sizeof(T) == 2 ? h : 2 * h) ^ swz_k(row)) << 4);
+  }
+  __device__ static V8 k_frag(uint32_t at, int kb, int ks) {
     if constexpr (sizeof(T) == 2) {
-      return *reinterpret_cast<const half8*>(at + (((2 * ks + h) ^ swz_k(row)) << 4));
+      return *lds_at<half8>((at ^ (ks * 32)) + kb * 32 * ROWB);
     } else {
-      const float4v a = *reinterpret_cast<const float4v*>(at + (((4 * ks + 2 * h) ^ swz_k(row)) << 4));
-      const float4v b = *reinterpret_cast<const float4v*>(at + (((4 * ks + 2 * h + 1) ^ swz_k(row)) << 4));
+      const float4v a = *lds_at<float4v>((at ^ (ks * 64)) + kb * 32 * ROWB);
+      const float4v b = *lds_at<float4v>((at ^ (ks * 64 + 16)) + kb * 32 * ROWB);
       return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
     }
   }
   // V^T row (value) 32 db + lane % 32, keys 16 ks + 4 h + {0..3} and 16 ks + 8 + 4 h + {0..3}
-  __device__ static V8 v_frag(const char* lds, int ks, int db, int lane) {
-    const int h = lane >> 5;
+  __device__ static uint32_t v_lane(int lane) {
+    const int h = lane >> 5, q = lane & 15;
     if constexpr (sizeof(T) == 2) {
-      const int q = lane & 15;
+      const int row = 4 * h + (q >> 2), chunk = 2 * ((lane >> 4) & 1) + ((q & 3) >> 1);
+      return row * ROWB + ((chunk ^ swz_v(row)) << 4) + (q & 1) * 8;
+    } else {
+      const int row = 4 * h, chunk = (lane & 31) >> 2;
+      return row * ROWB + ((chunk ^ swz_v(row)) << 4) + (lane & 3) * 4;
+    }
+  }
+  __device__ static V8 v_frag(uint32_t at, int ks, int db) {
+    if constexpr (sizeof(T) == 2) {
       half4 part[2];
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
-        const int row = 16 * ks + 8 * g + 4 * h + (q >> 2);
-        const int chunk = 4 * db + 2 * ((lane >> 4) & 1) + ((q & 3) >> 1);
-        const uint32_t at = lds_base(lds) + row * ROWB + ((chunk ^ swz_v(row)) << 4) + (q & 1) * 8;
-        part[g] = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds4_at(at)));
+        const uint32_t x = at ^ (db * 64 + (swz_v(8 * g) << 4));
+        part[g] = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds4_at(x + (16 * ks + 8 * g) * ROWB)));
       }
       return __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
     } else {
       float8v r;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int row = 16 * ks + 8 * (j >> 2) + 4 * h + (j & 3);
-        const int chunk = 8 * db + ((lane & 31) >> 2);
-        r[j] = *reinterpret_cast<const float*>(lds + row * ROWB + ((chunk ^ swz_v(row)) << 4) + (lane & 3) * 4);
-      }
+      for (int j = 0; j < 8; ++j) r[j] = *lds_at<float>((at ^ (db * 128)) + (16 * ks + 8 * (j >> 2) + (j & 3)) * ROWB);
       return r;
     }
   }
@@ -199,7 +211,8 @@ struct Row {
 // block whose lane half h holds keys 8 (r / 4) + 4 h + r % 4 in register r.
 struct Scoring {
   float c;         // scale * log2(e)
-  float cap, inv;  // softcap * log2(e); 2 log2(e) scale / softcap
+  float cap;       // softcap * log2(e)
+  float inv, inv2; // scale / softcap, and that times 2 log2(e)
   bool capped, biased;
 };
 
@@ -210,6 +223,7 @@ __device__ inline Scoring scoring(const Params& p) {
   s.biased = p.slopes != nullptr;
   s.cap = p.softcap * kLog2e;
   s.inv = s.capped ? p.scale / p.softcap : 0.f;
+  s.inv2 = s.inv * (2.f * kLog2e);
   return s;
 }
 
@@ -247,14 +261,14 @@ struct Wave {
   float16v o[DP / 32];
   float m, l;  // the reference maximum (log2 units) and this lane's part of the sum of weights
 
-  __device__ void start(const Row& row, int d, int lane) {
+  __device__ void start(const Row& row, float sign, int d, int lane) {
     const int h = lane >> 5;
 #pragma unroll
     for (int ks = 0; ks < DP / 16; ++ks) {
       const int at = 16 * ks + 8 * h;
       V8 v = {};
       if (row.q != nullptr && at < d) v = *reinterpret_cast<const V8*>(row.q + at * sizeof(T));
-      q[ks] = v;
+      q[ks] = sign == 1.f ? v : v * static_cast<T>(sign);
     }
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i) o[i] = float16v{};
@@ -262,14 +276,21 @@ struct Wave {
     l = 0.f;
   }
 
+  // Keeps the sums whole up to here: taken apart for the stores below, they would be copied in every
+  // pass of the loop before.
+  __device__ void settle() {
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i) asm volatile("" : "+v"(o[i]));
+  }
+
   // S^T of the tile's NB blocks of 32 keys
   template <int NB, typename TL>
-  __device__ void products(const char* kt, float16v (&s)[NB], int lane) const {
+  __device__ void products(uint32_t kt, float16v (&s)[NB]) const {
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb) {
       s[kb] = float16v{};
 #pragma unroll
-      for (int ks = 0; ks < DP / 16; ++ks) s[kb] = mma(TL::k_frag(kt, kb, ks, lane), q[ks], s[kb]);
+      for (int ks = 0; ks < DP / 16; ++ks) s[kb] = mma(TL::k_frag(kt, kb, ks), q[ks], s[kb]);
     }
   }
 
@@ -277,13 +298,24 @@ struct Wave {
   template <int NB>
   __device__ void weights(float16v (&s)[NB], const Scoring& sc, const Row& row, int pos0, int left, int last_seen, int lane) {
     const int h4 = (lane >> 5) * 4;
-    float c = sc.c;
-    if (sc.capped || !(c > 0.f)) {
+    // t = s * c + off
+    float c = sc.c, off = 0.f;
+    if (sc.capped) {
+      if constexpr (sizeof(T) == 2) {
+        // tanh(y) = 1 - 2 / (e^2y + 1): s becomes -1 / (e^2y + 1), and the rest of it joins c and off
 #pragma unroll
-      for (int kb = 0; kb < NB; ++kb)
+        for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[kb][r] = sc.capped ? sc.cap * tanh_of<T>(s[kb][r] * sc.inv) : s[kb][r] * c;
-      c = 1.f;
+          for (int r = 0; r < 16; ++r) s[kb][r] = __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(s[kb][r] * sc.inv2));
+        c = 2.f * sc.cap;
+        off = sc.cap;
+      } else {
+#pragma unroll
+        for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[kb][r] = tanh_of<T>(s[kb][r] * sc.inv);
+        c = sc.cap;
+      }
     }
     if (sc.biased) {
       const float at = static_cast<float>(row.pos - pos0 - h4);
@@ -292,9 +324,10 @@ struct Wave {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const float e = static_cast<float>(32 * kb + 8 * (r >> 2) + (r & 3));
-          s[kb][r] = fmaf(-row.slope, fabsf(at - e), s[kb][r] * c);
+          s[kb][r] = fmaf(-row.slope, fabsf(at - e), fmaf(s[kb][r], c, off));
         }
       c = 1.f;
+      off = 0.f;
     }
     if (left < 32 * NB || last_seen < pos0 + 32 * NB - 1) {
       const int lim = min(left - 1, row.limit - pos0) - h4;
@@ -310,7 +343,7 @@ struct Wave {
     for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[kb][r]);
-    top = fmaxf(top, other_half(top)) * c;
+    top = fmaf(fmaxf(top, other_half(top)), c, off);
     // (-inf times c stays -inf: c > 0.) A lane whose maximum moves takes the whole wavefront along.
     if (__any(top > m + kLag)) {
       const float next = fmaxf(m, top);
@@ -323,7 +356,7 @@ struct Wave {
         for (int r = 0; r < 16; ++r) o[i][r] *= f;
     }
     // a row that has seen no key yet (m = -inf): every score is -inf, every weight 0
-    const float ref = (m == -__builtin_huge_valf() ? 0.f : m) - kShift;
+    const float ref = (m == -__builtin_huge_valf() ? 0.f : m) - kShift - off;
     float sum = 0.f;
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb)
@@ -338,14 +371,14 @@ struct Wave {
 
   // O^T += V^T P^T
   template <int NB, typename TL>
-  __device__ void add(const char* vt, const float16v (&s)[NB], int lane) {
+  __device__ void add(uint32_t vt, const float16v (&s)[NB]) {
 #pragma unroll
     for (int ks = 0; ks < 2 * NB; ++ks) {
       V8 w;
 #pragma unroll
       for (int j = 0; j < 8; ++j) w[j] = static_cast<T>(s[ks >> 1][8 * (ks & 1) + j]);
 #pragma unroll
-      for (int db = 0; db < DP / 32; ++db) o[db] = mma(TL::v_frag(vt, ks, db, lane), w, o[db]);
+      for (int db = 0; db < DP / 32; ++db) o[db] = mma(TL::v_frag(vt, ks, db), w, o[db]);
     }
   }
 };
@@ -382,7 +415,7 @@ __device__ inline void store_out(char* out, int d0, const float (&v)[N]) {
 // the row does not see, times that key's weight 0, may be the reason. Only the keys that it sees are
 // read here. The whole wavefront works on the row.
 template <typename T, int DP>
-__device__ __attribute__((noinline)) void careful_row(const char* q, char* out, int pos, int limit, float slope, const Scoring sc,
+__device__ __attribute__((noinline)) void careful_row(const char* q, float sign, char* out, int pos, int limit, float slope, const Scoring sc,
                                                       const KeyRuns runs, int from0, int to0, int from1, int to1, int d,
                                                       float* part, float* part_m, float* part_l) {
   const int lane = threadIdx.x & 63;
@@ -390,7 +423,7 @@ __device__ __attribute__((noinline)) void careful_row(const char* q, char* out, 
   auto score = [&](const Keys& s, int j) {
     const T* kr = reinterpret_cast<const T*>(s.k + static_cast<size_t>(j) * s.k_tok);
     float x = 0.f;
-    for (int i = 0; i < d; ++i) x = fmaf(to_f(qv[i]), to_f(kr[i]), x);
+    for (int i = 0; i < d; ++i) x = fmaf(to_f(qv[i]) * sign, to_f(kr[i]), x);
     return score_of<T>(sc, x, slope, static_cast<float>(pos - s.pos0 - j));
   };
   float top = -__builtin_huge_valf();
@@ -446,38 +479,49 @@ __device__ void rows_workgroup(const Params& p, char* lds, const Row& row, const
   const uint32_t base = lds_base(lds);
   const Scoring sc = scoring(p);
   uint32_t koff[NIW], voff[NIW];
-  int at_seg = -1;
-  Keys cur = {};  // the run that the offsets are for
+  Keys at = {};  // the run, from the next tile to load on
+  int pos0 = 0, left = 0, next_pos0, next_left;
   auto issue = [&](int t, int buf) {
-    const int g = t < n0 ? 0 : 1, j0 = (t - (g ? n0 : 0)) * BN;
-    if (g != at_seg) {
-      at_seg = g;
-      cur = runs.run(g != 0);
-      dma_offsets<TL, NIW, false>(koff, wave * NIW, lane, cur.k_tok, p.d * static_cast<int>(sizeof(T)));
-      dma_offsets<TL, NIW, true>(voff, wave * NIW, lane, cur.v_tok, p.d * static_cast<int>(sizeof(T)));
+    if (t == tbeg || t == n0) {  // a run begins
+      at = runs.run(t >= n0);
+      const int j0 = (t - (t >= n0 ? n0 : 0)) * BN;
+      at.k += static_cast<size_t>(j0) * at.k_tok;
+      at.v += static_cast<size_t>(j0) * at.v_tok;
+      at.pos0 += j0;
+      at.len -= j0;
+      dma_offsets<TL, NIW, false>(koff, wave * NIW, lane, at.k_tok, p.d * static_cast<int>(sizeof(T)));
+      dma_offsets<TL, NIW, true>(voff, wave * NIW, lane, at.v_tok, p.d * static_cast<int>(sizeof(T)));
     }
-    const int rows = min(BN, cur.len - j0);
+    const int rows = min(BN, at.len);
     const uint32_t to = base + buf * 2 * TL::BYTES + wave * NIW * 1024;
-    dma_rows<NIW>(cur.k + static_cast<size_t>(j0) * cur.k_tok, cur.k_tok, rows, koff, to);
-    dma_rows<NIW>(cur.v + static_cast<size_t>(j0) * cur.v_tok, cur.v_tok, rows, voff, to + TL::BYTES);
+    dma_rows<NIW>(at.k, at.k_tok, rows, koff, to);
+    dma_rows<NIW>(at.v, at.v_tok, rows, voff, to + TL::BYTES);
+    next_pos0 = at.pos0;
+    next_left = at.len;
+    at.k += static_cast<size_t>(BN) * at.k_tok;
+    at.v += static_cast<size_t>(BN) * at.v_tok;
+    at.pos0 += BN;
+    at.len -= BN;
   };
   Wave<T, DP> w;
   if (tbeg < tend) issue(tbeg, 0);
-  w.start(row, p.d, lane);
+  w.start(row, p.sign, p.d, lane);
+  const uint32_t klane = base + TL::k_lane(lane), vlane = base + TL::BYTES + TL::v_lane(lane);
   for (int t = tbeg; t < tend; ++t) {
-    const int buf = (t - tbeg) & 1;
+    const uint32_t buf = static_cast<uint32_t>((t - tbeg) & 1);
     wait_dma_le<0>();
     phase_barrier();  // tile t has arrived for every wavefront, and every one is done with tile t - 1
+    pos0 = next_pos0;
+    left = next_left;
     if (t + 1 < tend) issue(t + 1, buf ^ 1);
-    const int g = t < n0 ? 0 : 1, j0 = (t - (g ? n0 : 0)) * BN;
-    const int pos0 = (g ? runs.own.pos0 : runs.shared.pos0) + j0, left = (g ? runs.own.len : runs.shared.len) - j0;
-    if (pos0 > wave_limit) continue;
-    const char* kt = lds + buf * 2 * TL::BYTES;
-    float16v s[NB];
-    w.template products<NB, TL>(kt, s, lane);
-    w.template weights<NB>(s, sc, row, pos0, left, last_seen, lane);
-    w.template add<NB, TL>(kt + TL::BYTES, s, lane);
+    if (pos0 <= wave_limit) {
+      float16v s[NB];
+      w.template products<NB, TL>(klane + buf * 2 * TL::BYTES, s);
+      w.template weights<NB>(s, sc, row, pos0, left, last_seen, lane);
+      w.template add<NB, TL>(vlane + buf * 2 * TL::BYTES, s);
+    }
   }
+  w.settle();
   const float l = w.l + other_half(w.l);
   const int h = lane >> 5, r = wave * 32 + (lane & 31);
   float bad = 0.f;
@@ -519,7 +563,7 @@ __device__ void rows_workgroup(const Params& p, char* lds, const Row& row, const
       rows &= rows - 1;
       const int rr = wave * 32 + i;
       float* pm = slot.at == nullptr ? nullptr : slot_m<DP>(slot) + rr;
-      careful_row<T, DP>(reinterpret_cast<const char*>(__shfl(reinterpret_cast<unsigned long long>(row.q), i)),
+      careful_row<T, DP>(reinterpret_cast<const char*>(__shfl(reinterpret_cast<unsigned long long>(row.q), i)), p.sign,
                          reinterpret_cast<char*>(__shfl(reinterpret_cast<unsigned long long>(row.out), i)), __shfl(row.pos, i),
                          __shfl(row.limit, i), __shfl(row.slope, i), sc, runs, min(tbeg, n0) * BN, min(tend, n0) * BN,
                          max(tbeg - n0, 0) * BN, max(tend - n0, 0) * BN, p.d,
@@ -598,6 +642,7 @@ __device__ void keys_workgroup(const Params& p, char* lds, float* joint, const R
     if (is_v) dma_rows<NI>(cur.v + static_cast<size_t>(j0) * cur.v_tok, cur.v_tok, rows, voff, vl);
     else dma_rows<NI>(cur.k + static_cast<size_t>(j0) * cur.k_tok, cur.k_tok, rows, koff, kl);
   };
+  const uint32_t klane = kl + TL::k_lane(lane), vlane = vl + TL::v_lane(lane);
   Wave<T, DP> w;
   int t = tbeg + wave;
   int pg = page_of(t);
@@ -606,7 +651,7 @@ __device__ void keys_workgroup(const Params& p, char* lds, float* joint, const R
     issue(t, pg, true);
   }
   int pg_next = page_of(t + 4);
-  w.start(row, p.d, lane);
+  w.start(row, p.sign, p.d, lane);
   // (the rows' loads are done before the loop, so its waits count DMA only)
   __builtin_amdgcn_s_waitcnt(0);
   for (; t < tend; t += 4) {
@@ -616,18 +661,19 @@ __device__ void keys_workgroup(const Params& p, char* lds, float* joint, const R
     float16v s[1];
     // K has arrived: only V's instructions may be in flight (younger page loads only make it wait longer)
     wait_dma_le<NI>();
-    w.template products<1, TL>(mine, s, lane);
+    w.template products<1, TL>(klane, s);
     // the K buffer has been read (the products' operands are in registers) before the next K overwrites it
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if (more) issue(t + 4, pg_next, false);
     w.template weights<1>(s, sc, row, (g ? runs.own.pos0 : runs.shared.pos0) + j0, (g ? runs.own.len : runs.shared.len) - j0, last_seen, lane);
     if (more) wait_dma_le<NI>();
     else wait_dma_le<0>();
-    w.template add<1, TL>(mine + TL::BYTES, s, lane);
+    w.template add<1, TL>(vlane, s);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if (more) issue(t + 4, pg_next, true);
     pg_next = page_of(t + 8);
   }
+  w.settle();
   // ---- join the four wavefronts: sums [wave][value][row] in LDS, then 8 threads a row ----
   const float l = w.l + other_half(w.l);
   const int h = lane >> 5, r = lane & 31;
@@ -696,7 +742,7 @@ __device__ void keys_workgroup(const Params& p, char* lds, float* joint, const R
         rows &= rows - 1;
         if ((k & 3) != wave) continue;
         float* pm = slot.at == nullptr ? nullptr : slot_m<DP>(slot) + i;
-        careful_row<T, DP>(reinterpret_cast<const char*>(__shfl(reinterpret_cast<unsigned long long>(row.q), i)),
+        careful_row<T, DP>(reinterpret_cast<const char*>(__shfl(reinterpret_cast<unsigned long long>(row.q), i)), p.sign,
                            reinterpret_cast<char*>(__shfl(reinterpret_cast<unsigned long long>(row.out), i)), __shfl(row.pos, i),
                            __shfl(row.limit, i), __shfl(row.slope, i), sc, runs, min(tbeg, n0) * BN, min(tend, n0) * BN,
                          max(tbeg - n0, 0) * BN, max(tend - n0, 0) * BN, p.d,
@@ -1073,7 +1119,8 @@ Params params(const g16_attention_args& a) {
   p.page = a.page;
   p.max_pages = a.max_pages;
   p.num_pages = a.num_pages;
-  p.scale = a.scale;
+  p.scale = a.scale > 0.f ? a.scale : (a.scale < 0.f ? -a.scale : 1.f);
+  p.sign = a.scale > 0.f ? 1.f : (a.scale < 0.f ? -1.f : 0.f);
   p.softcap = a.softcap;
   return p;
 }
