@@ -36,6 +36,7 @@ typedef float float2v __attribute__((ext_vector_type(2)));
 
 constexpr float kShift = 8.f, kLag = 7.f;
 constexpr float kLog2e = 1.44269504088896341f;
+constexpr float kPlainCap = 256.f;  // largest tanh cap that fp16 inputs take the plain form for (tanh_of)
 constexpr int kRowTile = 128, kKeyTile = 32;  // query rows of the two workgroup shapes
 constexpr int kThreads = 256;
 
@@ -83,8 +84,9 @@ struct Params {
   int seqs, q_len, k_len, hq, hkv, group, d, shared, causal;
   int page, max_pages, num_pages;
   int tiles, splits;              // prompts: row tiles (an upper bound where packed), key splits
-  int stiles, ssplits, osplits;   // single tokens: row tiles and splits of the shared keys, splits of the own
-  int otiles;                     // ... and row tiles of 32 of one request's `group` rows
+  int stiles, ssplits;            // single tokens: row tiles and splits of the shared keys
+  int otiles, oitems, least;      // ... row tiles of a request's `group` rows; parts of the own keys, of all
+                                  // requests together: about `oitems`, of at least `least` tiles (0: one each)
   float scale, softcap;  // scale > 0, with its sign (0 for 0) in `sign`, which the queries take on
   float sign;
 };
@@ -213,13 +215,14 @@ struct Scoring {
   float c;         // scale * log2(e)
   float cap;       // softcap * log2(e)
   float inv, inv2; // scale / softcap, and that times 2 log2(e)
-  bool capped, biased;
+  bool capped, fine, biased;  // fine: the cap needs tanh's relative precision near 0 (below)
 };
 
 __device__ inline Scoring scoring(const Params& p) {
   Scoring s;
   s.c = p.scale * kLog2e;
   s.capped = p.softcap != 0.f;
+  s.fine = p.softcap > kPlainCap;
   s.biased = p.slopes != nullptr;
   s.cap = p.softcap * kLog2e;
   s.inv = s.capped ? p.scale / p.softcap : 0.f;
@@ -229,27 +232,22 @@ __device__ inline Scoring scoring(const Params& p) {
 
 // tanh to fp32's last bits near 0, where a cap leaves most scores (an odd polynomial fitted by least
 // squares to (tanh(y) / y - 1) / y^2 on [0, 0.625], largest relative error 4e-9), and 1 - 2 / (e^2y + 1)
-// past it. fp16 inputs need no more than the second form's absolute error of 1e-7.
-template <typename T>
+// past it. With fp16 inputs and a cap up to kPlainCap the second form's absolute error, 1e-7 of the cap, is
+// enough throughout.
 __device__ inline float tanh_of(float y) {
   const float e = __builtin_amdgcn_exp2f(y * (2.f * kLog2e));
   const float big = 1.f - 2.f * __builtin_amdgcn_rcpf(e + 1.f);
-  if constexpr (sizeof(T) == 2) {
-    return big;
-  } else {
-    const float u = y * y;
-    float r = fmaf(u, -0.00571705f, 0.02065059f);
-    r = fmaf(u, r, -0.0537435f);
-    r = fmaf(u, r, 0.13331491f);
-    r = fmaf(u, r, -0.33333284f);
-    r = fmaf(y * u, r, y);
-    return fabsf(y) < 0.625f ? r : big;
-  }
+  const float u = y * y;
+  float r = fmaf(u, -0.00571705f, 0.02065059f);
+  r = fmaf(u, r, -0.0537435f);
+  r = fmaf(u, r, 0.13331491f);
+  r = fmaf(u, r, -0.33333284f);
+  r = fmaf(y * u, r, y);
+  return fabsf(y) < 0.625f ? r : big;
 }
 
-template <typename T>
 __device__ inline float score_of(const Scoring& s, float x, float slope, float distance) {
-  float t = s.capped ? s.cap * tanh_of<T>(x * s.inv) : x * s.c;
+  const float t = s.capped ? s.cap * tanh_of(x * s.inv) : x * s.c;
   return s.biased ? fmaf(-slope, fabsf(distance), t) : t;
 }
 
@@ -301,7 +299,7 @@ struct Wave {
     // t = s * c + off
     float c = sc.c, off = 0.f;
     if (sc.capped) {
-      if constexpr (sizeof(T) == 2) {
+      if (sizeof(T) == 2 && !sc.fine) {
         // tanh(y) = 1 - 2 / (e^2y + 1): s becomes -1 / (e^2y + 1), and the rest of it joins c and off
 #pragma unroll
         for (int kb = 0; kb < NB; ++kb)
@@ -313,7 +311,7 @@ struct Wave {
 #pragma unroll
         for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[kb][r] = tanh_of<T>(s[kb][r] * sc.inv);
+          for (int r = 0; r < 16; ++r) s[kb][r] = tanh_of(s[kb][r] * sc.inv);
         c = sc.cap;
       }
     }
@@ -424,7 +422,7 @@ __device__ __attribute__((noinline)) void careful_row(const char* q, float sign,
     const T* kr = reinterpret_cast<const T*>(s.k + static_cast<size_t>(j) * s.k_tok);
     float x = 0.f;
     for (int i = 0; i < d; ++i) x = fmaf(to_f(qv[i]) * sign, to_f(kr[i]), x);
-    return score_of<T>(sc, x, slope, static_cast<float>(pos - s.pos0 - j));
+    return score_of(sc, x, slope, static_cast<float>(pos - s.pos0 - j));
   };
   float top = -__builtin_huge_valf();
   for (int g = 0; g < 2; ++g) {
@@ -574,9 +572,12 @@ __device__ void rows_workgroup(const Params& p, char* lds, const Row& row, const
 }
 
 // ---- workgroup of 32 rows, every wavefront on its own keys -------------------------------------------
-// Wavefront w takes tiles tbeg + w, tbeg + w + 4, .. of 32 keys, K and V each in one buffer of its own: the
-// next K is on its way from the moment the scores are computed, the next V from that of the products.
-// PAGED: the own keys lie in pages (prow: the lane's page row base; see decode_kernel).
+// Wavefront w takes tiles tbeg + w, tbeg + w + 4, .. of 32 keys. K and V have one buffer each: the next K is on
+// its way from the moment the scores are computed, the next V from that of the products, and a second
+// workgroup on the CU fills the gaps (64 requests of up to 4096 keys, 8 key heads: 3.92 TB/s either way with
+// two buffers each and one workgroup; 16 of up to 6000: 3.6, and 2.9 so).
+// PAGED: the own keys may lie in pages. Of 16 keys or a multiple, as they mostly are, a page holds whole
+// half tiles, whose pages are scalar loads a tile ahead; other sizes look up every key's page by itself.
 struct Pages {
   const int32_t* table;  // this sequence's pages; NULL: its keys lie in a row
   int page, num_pages;
@@ -589,29 +590,62 @@ __device__ void keys_workgroup(const Params& p, char* lds, float* joint, const R
   using TL = Tile<T, DP, BN>;
   constexpr int NI = TL::NI;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
-  char* mine = lds + wave * 2 * TL::BYTES;
-  const uint32_t kl = lds_base(mine), vl = kl + TL::BYTES;
+  const uint32_t kl = lds_base(lds) + wave * (2 * TL::BYTES);  // K, then V
   const Scoring sc = scoring(p);
   const int row_bytes = p.d * static_cast<int>(sizeof(T));
+  const bool paged = PAGED && pages.table != nullptr, whole = paged && pages.page % 16 == 0;
   uint32_t koff[NI], voff[NI];
-  int at_seg = -1;
-  Keys cur = {};  // the run that the offsets are for
-  auto where = [&](int t, int& g, int& j0) {
-    g = t < n0 ? 0 : 1;
-    j0 = (t - (g ? n0 : 0)) * BN;
+  bool second = tbeg >= n0;  // the run that the offsets are for
+  Keys cur = runs.run(second);
+  auto offsets = [&]() {
+    dma_offsets<TL, NI, false>(koff, 0, lane, cur.k_tok, row_bytes);
+    dma_offsets<TL, NI, true>(voff, 0, lane, cur.v_tok, row_bytes);
   };
-  // PAGED: the page of this lane's key (lane % 32) of tile t, loaded a tile ahead
+  offsets();
+  // whole: the pages of a tile's two halves; else the page of this lane's key (lane % 32), in .x
+  struct Ids {
+    int x, y;
+  };
   auto page_of = [&](int t) {
-    if (!PAGED || t >= tend || pages.table == nullptr) return 0;
-    const int j = (t - n0) * BN + (lane & 31);
-    return t >= n0 && j < runs.own.len ? pages.table[j / pages.page] : 0;
+    Ids ids = {0, 0};
+    if (!paged || t >= tend) return ids;
+    const int j0 = (t - n0) * BN;
+    if (whole) {
+      // (constant address space: the table is only read, so these become scalar loads, which the waits for
+      // the tiles do not count)
+      auto* table = reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(reinterpret_cast<uint64_t>(pages.table));
+      ids.x = table[j0 / pages.page];
+      if (j0 + 16 < runs.own.len) ids.y = table[(j0 + 16) / pages.page];
+    } else if (j0 + (lane & 31) < runs.own.len) {
+      ids.x = pages.table[(j0 + (lane & 31)) / pages.page];
+    }
+    return ids;
   };
-  auto dma_paged = [&](int j0, int pg, bool is_v, uint32_t to) {
+  auto dma_halves = [&](int j0, const Ids& ids, bool is_v, uint32_t to) {
+    const char* base = is_v ? cur.v : cur.k;
+    const uint32_t tok = is_v ? cur.v_tok : cur.k_tok;
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const int pg = g ? ids.y : ids.x, j = j0 + 16 * g;
+      const bool known = static_cast<unsigned>(pg) < static_cast<unsigned>(pages.num_pages);
+      const int rows = known ? max(0, min(16, cur.len - j)) : 0;
+      const char* at = base + (known ? pg * (is_v ? pages.v_seq : pages.k_seq) + static_cast<int64_t>(j % pages.page) * tok : 0);
+      const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(uniform(const_cast<char*>(at)), 0,
+                                                                         uniform(static_cast<int>(tok * static_cast<uint32_t>(rows))), kRawBufferDword3);
+#pragma unroll
+      for (int n = 0; n < NI / 2; ++n) {
+        const uint32_t off = is_v ? voff[g * (NI / 2) + n] : koff[g * (NI / 2) + n];
+        // (an out-of-range offset stays one: less than 2^30 is taken off)
+        dma16(r, to + (g * (NI / 2) + n) * 1024, off - 16 * g * tok);
+      }
+    }
+  };
+  auto dma_each = [&](int j0, int pg, bool is_v, uint32_t to) {
     const int j = j0 + (lane & 31);
     const char* at = nullptr;
-    if (j < runs.own.len && static_cast<unsigned>(pg) < static_cast<unsigned>(pages.num_pages))
-      at = (is_v ? runs.own.v : runs.own.k) + pg * (is_v ? pages.v_seq : pages.k_seq) +
-           static_cast<int64_t>(j % pages.page) * (is_v ? runs.own.v_tok : runs.own.k_tok);
+    if (j < cur.len && static_cast<unsigned>(pg) < static_cast<unsigned>(pages.num_pages))
+      at = (is_v ? cur.v : cur.k) + pg * (is_v ? pages.v_seq : pages.k_seq) +
+           static_cast<int64_t>(j % pages.page) * (is_v ? cur.v_tok : cur.k_tok);
     const uint64_t a = reinterpret_cast<uint64_t>(at);
     const uint32_t lo = static_cast<uint32_t>(a), hi = static_cast<uint32_t>(a >> 32);
 #pragma unroll
@@ -625,53 +659,55 @@ __device__ void keys_workgroup(const Params& p, char* lds, float* joint, const R
       dma16_from(from, to + n * 1024);
     }
   };
-  auto issue = [&](int t, int pg, bool is_v) {
-    int g, j0;
-    where(t, g, j0);
-    if (PAGED && g == 1 && pages.table != nullptr) {
-      dma_paged(j0, pg, is_v, is_v ? vl : kl);
-      return;
+  auto issue = [&](int t, const Ids& ids, bool is_v) {
+    const uint32_t to = kl + (is_v ? TL::BYTES : 0);
+    if (!second && t >= n0) {
+      second = true;
+      cur = runs.run(true);
+      offsets();
     }
-    if (g != at_seg) {
-      at_seg = g;
-      cur = runs.run(g != 0);
-      dma_offsets<TL, NI, false>(koff, 0, lane, cur.k_tok, row_bytes);
-      dma_offsets<TL, NI, true>(voff, 0, lane, cur.v_tok, row_bytes);
+    const int j0 = (t - (second ? n0 : 0)) * BN;
+    if (whole) {
+      dma_halves(j0, ids, is_v, to);
+    } else if (paged) {
+      dma_each(j0, ids.x, is_v, to);
+    } else {
+      const int rows = min(BN, cur.len - j0);
+      if (is_v) dma_rows<NI>(cur.v + static_cast<size_t>(j0) * cur.v_tok, cur.v_tok, rows, voff, to);
+      else dma_rows<NI>(cur.k + static_cast<size_t>(j0) * cur.k_tok, cur.k_tok, rows, koff, to);
     }
-    const int rows = min(BN, cur.len - j0);
-    if (is_v) dma_rows<NI>(cur.v + static_cast<size_t>(j0) * cur.v_tok, cur.v_tok, rows, voff, vl);
-    else dma_rows<NI>(cur.k + static_cast<size_t>(j0) * cur.k_tok, cur.k_tok, rows, koff, kl);
   };
-  const uint32_t klane = kl + TL::k_lane(lane), vlane = vl + TL::v_lane(lane);
+  const uint32_t klane = kl + TL::k_lane(lane), vlane = kl + TL::BYTES + TL::v_lane(lane);
   Wave<T, DP> w;
   int t = tbeg + wave;
-  int pg = page_of(t);
   if (t < tend) {
-    issue(t, pg, false);
-    issue(t, pg, true);
+    const Ids ids = page_of(t);
+    issue(t, ids, false);
+    issue(t, ids, true);
   }
-  int pg_next = page_of(t + 4);
+  Ids next = page_of(t + 4);
   w.start(row, p.sign, p.d, lane);
-  // (the rows' loads are done before the loop, so its waits count DMA only)
+  // The rows' loads are done before the loop: its waits count DMA only, and the compiler, which does not
+  // know of that, would wait for all of it before it first uses the rows.
   __builtin_amdgcn_s_waitcnt(0);
   for (; t < tend; t += 4) {
-    int g, j0;
-    where(t, g, j0);
-    const bool more = t + 4 < tend;
+    const bool more = t + 4 < tend, own = t >= n0;
+    const int j0 = (t - (own ? n0 : 0)) * BN;
+    const int pos0 = (own ? runs.own.pos0 : runs.shared.pos0) + j0, left = (own ? runs.own.len : runs.shared.len) - j0;
     float16v s[1];
-    // K has arrived: only V's instructions may be in flight (younger page loads only make it wait longer)
+    // Waits for K, then for V: only the instructions issued after it may be in flight (others among them only
+    // make it wait longer).
     wait_dma_le<NI>();
     w.template products<1, TL>(klane, s);
-    // the K buffer has been read (the products' operands are in registers) before the next K overwrites it
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (more) issue(t + 4, pg_next, false);
-    w.template weights<1>(s, sc, row, (g ? runs.own.pos0 : runs.shared.pos0) + j0, (g ? runs.own.len : runs.shared.len) - j0, last_seen, lane);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K has been read before the next K overwrites it
+    if (more) issue(t + 4, next, false);
+    w.template weights<1>(s, sc, row, pos0, left, last_seen, lane);
     if (more) wait_dma_le<NI>();
     else wait_dma_le<0>();
     w.template add<1, TL>(vlane, s);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (more) issue(t + 4, pg_next, true);
-    pg_next = page_of(t + 8);
+    if (more) issue(t + 4, next, true);
+    next = page_of(t + 8);
   }
   w.settle();
   // ---- join the four wavefronts: sums [wave][value][row] in LDS, then 8 threads a row ----
@@ -757,11 +793,11 @@ template <typename T, int DP>
 constexpr int rows_lds() {
   return 4 * Tile<T, DP, sizeof(T) == 2 ? 64 : 32>::BYTES;
 }
+constexpr int cmax(int a, int b) { return a > b ? a : b; }
 template <typename T, int DP>
 constexpr int keys_lds() {
-  return 8 * Tile<T, DP, 32>::BYTES > 4 * DP * 32 * 4 ? 8 * Tile<T, DP, 32>::BYTES : 4 * DP * 32 * 4;
+  return cmax(8 * Tile<T, DP, 32>::BYTES, 4 * DP * 32 * 4);  // (the second: joining the wavefronts)
 }
-constexpr int cmax(int a, int b) { return a > b ? a : b; }
 
 // ---- prompts -------------------------------------------------------------------------------------------
 // Row tile t of all sequences' tiles of `rt` rows: its sequence and where that sequence's rows and keys
@@ -784,10 +820,13 @@ __device__ inline bool find_tile(const Params& p, int t, int rt, Where& w) {
   const int lane = threadIdx.x & 63;
   for (int b0 = 0; b0 < p.seqs; b0 += kWave) {
     const int b = b0 + lane;
-    int q0 = 0, lq = 0;
-    if (b < p.seqs) {
-      q0 = min(max(p.q_off[b], 0), p.q_len);
-      lq = max(min(p.q_off[b + 1], p.q_len) - q0, 0);
+    int q0 = 0, lq = 0, k0 = 0, lk = 0;
+    if (b < p.seqs) {  // (all four loads together: one round trip before the keys)
+      const int qa = p.q_off[b], qb = p.q_off[b + 1], ka = p.k_off[b], kb = p.k_off[b + 1];
+      q0 = min(max(qa, 0), p.q_len);
+      lq = max(min(qb, p.q_len) - q0, 0);
+      k0 = min(max(ka, 0), p.k_len);
+      lk = max(min(kb, p.k_len) - k0, 0);
     }
     const int n = static_cast<int>((static_cast<int64_t>(lq) * p.group + rt - 1) / rt);
     int upto = n;
@@ -800,21 +839,14 @@ __device__ inline bool find_tile(const Params& p, int t, int rt, Where& w) {
     if (hit != 0) {
       const int l = __builtin_ctzll(hit);
       w.seq = b0 + l;
-      w.lq = __shfl(lq, l);
-      w.q0 = __shfl(q0, l);
-      w.tile = __shfl(upto, l) - 1 - t;  // the sequence's last tile first
-      const int ka = min(max(p.k_off[w.seq], 0), p.k_len);
-      w.lk = max(min(p.k_off[w.seq + 1], p.k_len) - ka, 0);
-      w.k0 = ka;
-      w.seq = uniform(w.seq);
-      w.lq = uniform(w.lq);
-      w.lk = uniform(w.lk);
-      w.tile = uniform(w.tile);
-      w.q0 = uniform(static_cast<int>(w.q0));
-      w.k0 = uniform(static_cast<int>(w.k0));
+      w.lq = __builtin_amdgcn_readlane(lq, l);
+      w.lk = __builtin_amdgcn_readlane(lk, l);
+      w.q0 = __builtin_amdgcn_readlane(q0, l);
+      w.k0 = __builtin_amdgcn_readlane(k0, l);
+      w.tile = __builtin_amdgcn_readlane(upto, l) - 1 - t;  // the sequence's last tile first
       return true;
     }
-    t -= __shfl(upto, kWave - 1);
+    t -= __builtin_amdgcn_readlane(upto, kWave - 1);
   }
   return false;
 }
@@ -828,7 +860,7 @@ __device__ inline Row prompt_row(const Params& p, const Where& w, int kv, int r,
   row.q = ok ? p.q + (p.q_off == nullptr ? w.seq * p.q_seq : w.q0 * p.q_tok) + tok * p.q_tok + head * p.q_head : nullptr;
   row.out = ok ? p.out + (at * p.hq + head) * p.d * size : nullptr;
   row.pos = p.shared + w.lk - w.lq + tok;
-  row.limit = p.causal ? max(row.pos, p.visible != nullptr ? p.visible[w.seq] - 1 : -1) : 0x7fffffff;
+  row.limit = p.causal ? max(row.pos, p.visible != nullptr ? max(p.visible[w.seq], 0) - 1 : -1) : 0x7fffffff;
   row.slope = p.slopes != nullptr && ok ? p.slopes[head] * kLog2e : 0.f;
   return row;
 }
@@ -854,14 +886,14 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_kernel(Params p) {
   // the keys that some row of the tile sees
   int seen = 0x7fffffff, last_seen = 0x7fffffff, wave_limit = 0x7fffffff;
   if (p.causal) {
-    const int vis = p.visible != nullptr ? uniform(p.visible[w.seq]) - 1 : -1;
+    const int vis = p.visible != nullptr ? max(uniform(p.visible[w.seq]), 0) - 1 : -1;
     const int pos0 = p.shared + w.lk - w.lq;
     const int last_tok = min(r0 + RT - 1, w.lq * p.group - 1) / p.group;
     seen = max(pos0 + last_tok, vis);
     last_seen = max(pos0 + first / p.group, vis);
     wave_limit = max(pos0 + min(first + 31, w.lq * p.group - 1) / p.group, vis);
-    if (first >= w.lq * p.group) wave_limit = -1;  // no such rows
   }
+  if (first >= w.lq * p.group) wave_limit = -1;  // no such rows
   const int end0 = min(p.shared, seen < 0 ? 0 : (seen == 0x7fffffff ? seen : seen + 1));
   const int end1 = min(w.lk, seen < p.shared ? 0 : (seen == 0x7fffffff ? seen : seen + 1 - p.shared));
   const int n0 = ceil_div(end0, BN), n = n0 + ceil_div(end1, BN);
@@ -876,35 +908,67 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_kernel(Params p) {
   }
 }
 
-// One row from its partial sums: `of(i)` gives part i's sums, reference maximum and sum of weights. A
-// wavefront a row, DP / 64 values a lane.
+// One row from its partial sums: `of(i)` gives part i's sums, reference maximum and, `rows` floats behind it,
+// sum of weights. A wavefront a row: a lane holds 4 values of every kP-th part, whose weight the lane of
+// that number has. The sums' loads do not wait for the weights.
 template <typename T, int DP, typename F>
 __device__ inline void join_row(char* out, int d, int parts, const F& of) {
-  const int lane = threadIdx.x & 63;
-  constexpr int N = DP / 64;
-  float top = -__builtin_huge_valf(), l = 0.f, o[N] = {};
-  for (int i = lane; i < parts; i += kWave) {
-    const float *s, *m;
-    int rows;
+  constexpr int L = DP / 4, kP = kWave / L, kB = 8;  // lanes of a part, parts at a time, loads at a time
+  const int lane = threadIdx.x & 63, d0 = (lane % L) * 4, mine = lane / L;
+  const float *s, *m;
+  int rows;
+  float top = -__builtin_huge_valf(), first_m = top, first_l = 0.f;
+  if (lane < parts) {
+    of(lane, s, m, rows);
+    first_m = *m;
+    first_l = m[rows];
+  }
+  float4v v[kB];
+  auto load = [&](int b) {
+#pragma unroll
+    for (int i = 0; i < kB; ++i) {
+      of(min(b + i * kP + mine, parts - 1), s, m, rows);
+      v[i] = *reinterpret_cast<const float4v*>(s + d0);
+    }
+  };
+  load(0);
+  top = first_m;
+  for (int i = lane + kWave; i < parts; i += kWave) {
     of(i, s, m, rows);
     top = fmaxf(top, *m);
   }
 #pragma unroll
   for (int i = 1; i < kWave; i *= 2) top = fmaxf(top, __shfl_xor(top, i));
-#pragma unroll 4
-  for (int i = 0; i < parts; ++i) {
-    const float *s, *m;
-    int rows;
-    of(i, s, m, rows);
-    const float f = *m == top ? 1.f : __builtin_amdgcn_exp2f(*m - top);
-    l = fmaf(f, m[rows], l);
+  float l = 0.f, f = 0.f;  // f: the weight of part (64 n + lane)
+  float4v o = {};
+  for (int b = 0; b < parts; b += kB * kP) {
+    if (b % kWave == 0) {
+      float pm = first_m, pl = first_l;
+      if (b > 0 && b + lane < parts) {
+        of(b + lane, s, m, rows);
+        pm = *m;
+        pl = m[rows];
+      }
+      f = b + lane >= parts ? 0.f : (pm == top ? 1.f : __builtin_amdgcn_exp2f(pm - top));
+      l = fmaf(f, b + lane < parts ? pl : 0.f, l);
+    }
+    if (b > 0) load(b);
 #pragma unroll
-    for (int e = 0; e < N; ++e) o[e] = fmaf(f, s[lane * N + e], o[e]);
+    for (int i = 0; i < kB; ++i) {
+      const int part = b + i * kP + mine;
+      const float fi = __shfl(f, part & (kWave - 1));
+      if (part < parts) o += fi * v[i];
+    }
   }
-  const float inv = inverse(l);
 #pragma unroll
-  for (int e = 0; e < N; ++e)
-    if (lane * N + e < d) reinterpret_cast<T*>(out)[lane * N + e] = static_cast<T>(o[e] * inv);
+  for (int i = 1; i < kWave; i *= 2) l += __shfl_xor(l, i);
+#pragma unroll
+  for (int i = L; i < kWave; i *= 2)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], i);
+  const float inv = inverse(l);
+  const float r[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+  if (lane < L && d0 < d) store_out<T, 4>(out, d0, r);
 }
 
 constexpr int kJoinRows = 8;  // rows of a workgroup of the joining kernels: two a wavefront
@@ -933,9 +997,57 @@ __global__ __launch_bounds__(kThreads) void prompt_join_kernel(Params p, int rt)
 
 // ---- single tokens -------------------------------------------------------------------------------------
 // Workgroups [0, stiles * ssplits * hkv): the shared keys, for the rows (request, query head) of all
-// requests at once, `srows` of them a tile. Then [.., + seqs * otiles * osplits * hkv): the requests' own
-// keys, 32 rows a tile. Slots in the same order. One split of one kind alone writes the output itself.
+// requests at once. Then the requests' own keys, 32 rows a tile, in parts of about equal length over all
+// requests: the device knows their lengths, so every wavefront adds them up and finds its part (see Part).
+// Slots in the same order. A request's only part writes the output itself.
 __host__ __device__ inline int own_rows(int group) { return group < kKeyTile ? group : kKeyTile; }
+
+struct Part {
+  int seq, len, split, splits;  // the request and its length; which of its parts this is, and of how many
+  int first;                    // number of the request's first part
+};
+__device__ inline int length_of(const Params& p, int b) { return min(max(p.lengths[b], 0), p.k_len); }
+
+// Tiles of 32 keys a part gets: the requests' tiles over the parts that there should be.
+__device__ inline int part_tiles(const Params& p) {
+  const int lane = threadIdx.x & 63;
+  int64_t total = 0;
+  for (int b = lane; b < p.seqs; b += kWave) total += ceil_div(length_of(p, b), 32);
+#pragma unroll
+  for (int i = 1; i < kWave; i *= 2) total += __shfl_xor(static_cast<long long>(total), i);
+  return max(p.least, uniform(static_cast<int>((total + p.oitems - 1) / p.oitems)));
+}
+// Part `item` of all (by_item), or the first part of request `item`. false: past the last one.
+__device__ inline bool find_part(const Params& p, int item, bool by_item, Part& r) {
+  if (p.least == 0) {
+    r = Part{item, item < p.seqs ? uniform(length_of(p, item)) : 0, 0, 1, item};
+    return item < p.seqs;
+  }
+  const int lane = threadIdx.x & 63, chunk = part_tiles(p);
+  int before = 0;
+  for (int b0 = 0; b0 < p.seqs; b0 += kWave) {
+    const int b = b0 + lane, len = b < p.seqs ? length_of(p, b) : 0;
+    const int n = b < p.seqs ? max(1, ceil_div(ceil_div(len, 32), chunk)) : 0;
+    int upto = n;
+#pragma unroll
+    for (int i = 1; i < kWave; i *= 2) {
+      const int x = __shfl_up(upto, i);
+      if (lane >= i) upto += x;
+    }
+    const uint64_t hit = __ballot(by_item ? item < before + upto : b == item);
+    if (hit != 0) {
+      const int l = __builtin_ctzll(hit);
+      r.seq = b0 + l;
+      r.len = __builtin_amdgcn_readlane(len, l);
+      r.splits = __builtin_amdgcn_readlane(n, l);
+      r.first = before + __builtin_amdgcn_readlane(upto, l) - r.splits;
+      r.split = by_item ? item - r.first : 0;
+      return true;
+    }
+    before += __builtin_amdgcn_readlane(upto, kWave - 1);
+  }
+  return false;
+}
 
 template <typename T, int DP, bool SKEYS>
 __global__ __launch_bounds__(kThreads, 2) void decode_kernel(Params p) {
@@ -944,12 +1056,11 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(Params p) {
   __shared__ float joint[257];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int nshared = p.stiles * p.ssplits * p.hkv;
-  const int parts = p.ssplits * (p.stiles > 0) + p.osplits;
   auto row_of = [&](int b, int head, bool ok) {
     Row row;
     row.q = ok ? p.q + b * p.q_seq + head * p.q_head : nullptr;
     row.out = ok ? p.out + (static_cast<int64_t>(b) * p.hq + head) * p.d * static_cast<int>(sizeof(T)) : nullptr;
-    const int len = ok ? min(max(p.lengths[b], 0), p.k_len) : 0;
+    const int len = ok ? length_of(p, b) : 0;
     row.pos = p.shared + len - 1;
     row.limit = 0x7fffffff;
     row.slope = ok && p.slopes != nullptr ? p.slopes[head] * kLog2e : 0.f;
@@ -959,7 +1070,8 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(Params p) {
     int lin = blockIdx.x;
     const int kv = lin % p.hkv;
     lin /= p.hkv;
-    const int split = lin % p.ssplits, t = lin / p.ssplits;
+    // (a split's row tiles next to each other: they read the same keys)
+    const int t = lin % p.stiles, split = lin / p.stiles;
     const int r = t * SRT + (SKEYS ? 0 : 32 * wave) + (lane & 31);
     const int b = r / p.group;
     const Row row = row_of(b, kv * p.group + r % p.group, b < p.seqs);
@@ -967,7 +1079,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(Params p) {
     const int n = ceil_div(p.shared, SBN);
     const int tbeg = static_cast<int>(static_cast<int64_t>(n) * split / p.ssplits);
     const int tend = static_cast<int>(static_cast<int64_t>(n) * (split + 1) / p.ssplits);
-    Slot slot = {p.part + static_cast<size_t>(blockIdx.x) * slot_floats(SRT, DP), SRT};
+    Slot slot = {p.part + (static_cast<size_t>(t * p.ssplits + split) * p.hkv + kv) * slot_floats(SRT, DP), SRT};
     if constexpr (SKEYS) {
       keys_workgroup<T, DP, false>(p, lds, joint, row, runs, Pages{}, n, tbeg, tend, 0x7fffffff, slot);
     } else {
@@ -980,12 +1092,12 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(Params p) {
   const int own = lin;
   const int kv = lin % p.hkv;
   lin /= p.hkv;
-  const int split = lin % p.osplits;
-  lin /= p.osplits;
-  const int rt = lin % p.otiles, b = lin / p.otiles;
+  const int rt = lin % p.otiles;
+  Part part;
+  if (!find_part(p, lin / p.otiles, true, part)) return;
+  const int b = part.seq, len = part.len;
   const int orows = own_rows(p.group), r = rt * kKeyTile + (lane & 31);
   const Row row = row_of(b, kv * p.group + r, r < p.group);
-  const int len = uniform(min(max(p.lengths[b], 0), p.k_len));
   KeyRuns runs = {{}, {p.k + kv * p.k_head, p.v + kv * p.v_head, p.k_tok, p.v_tok, len, p.shared}};
   const Pages pages = {p.pages == nullptr ? nullptr : p.pages + static_cast<size_t>(b) * p.max_pages, p.page, p.num_pages, p.k_seq, p.v_seq};
   if (p.pages == nullptr) {
@@ -993,10 +1105,10 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(Params p) {
     runs.own.v += b * p.v_seq;
   }
   const int n = ceil_div(len, 32);
-  const int tbeg = static_cast<int>(static_cast<int64_t>(n) * split / p.osplits);
-  const int tend = static_cast<int>(static_cast<int64_t>(n) * (split + 1) / p.osplits);
+  const int tbeg = static_cast<int>(static_cast<int64_t>(n) * part.split / part.splits);
+  const int tend = static_cast<int>(static_cast<int64_t>(n) * (part.split + 1) / part.splits);
   Slot slot = {nullptr, orows};
-  if (parts > 1) slot.at = p.part + static_cast<size_t>(nshared) * slot_floats(SRT, DP) + static_cast<size_t>(own) * slot_floats(orows, DP);
+  if (p.stiles > 0 || part.splits > 1) slot.at = p.part + static_cast<size_t>(nshared) * slot_floats(SRT, DP) + static_cast<size_t>(own) * slot_floats(orows, DP);
   keys_workgroup<T, DP, true>(p, lds, joint, row, runs, pages, 0, tbeg, tend, 0x7fffffff, slot);
 }
 
@@ -1008,7 +1120,9 @@ __global__ __launch_bounds__(kThreads) void decode_join_kernel(Params p, int srt
   const int ns = p.stiles > 0 ? p.ssplits : 0, orows = own_rows(p.group);
   const size_t nshared = static_cast<size_t>(p.stiles) * p.ssplits * p.hkv;
   const int sr = b * p.group + g;
-  join_row<T, DP>(p.out + static_cast<int64_t>(row) * p.d * static_cast<int>(sizeof(T)), p.d, ns + p.osplits,
+  Part part;
+  if (!find_part(p, b, false, part) || ns + part.splits == 1) return;
+  join_row<T, DP>(p.out + static_cast<int64_t>(row) * p.d * static_cast<int>(sizeof(T)), p.d, ns + part.splits,
                   [&](int i, const float*& o, const float*& m, int& rows) {
                     const float* slot;
                     int r;
@@ -1017,7 +1131,7 @@ __global__ __launch_bounds__(kThreads) void decode_join_kernel(Params p, int srt
                       r = sr % srt;
                       rows = srt;
                     } else {
-                      const size_t at = ((static_cast<size_t>(b) * p.otiles + g / kKeyTile) * p.osplits + (i - ns)) * p.hkv + kv;
+                      const size_t at = (static_cast<size_t>(part.first + i - ns) * p.otiles + g / kKeyTile) * p.hkv + kv;
                       slot = p.part + nshared * slot_floats(srt, DP) + at * slot_floats(orows, DP);
                       r = g % kKeyTile;
                       rows = orows;
@@ -1125,6 +1239,9 @@ Params params(const g16_attention_args& a) {
   return p;
 }
 
+// Tiles of 32 keys that a workgroup of four wavefronts on their own keys gets at least.
+constexpr int kLeastKeys = 16;
+
 // Splits of `tiles` key tiles so that `items` workgroups become about two a CU, with at least `least` tiles
 // a split.
 int splits_for(int64_t items, int64_t tiles, int cus, int least) {
@@ -1152,30 +1269,37 @@ PromptPlan plan_prompt(const g16_attention_args& a) {
   // keys of an average sequence (packed lengths are known on the device only)
   const int64_t keys = a.shared + (a.q_offsets == nullptr ? a.k_len : a.k_len / a.seqs);
   const int64_t busy = a.q_offsets == nullptr ? tiles : (rows + r.rt - 1) / r.rt * a.seqs;
-  r.splits = splits_for(busy * a.hkv, (keys + bn - 1) / bn, cus_of(a), r.keys ? 16 : 4);
+  r.splits = splits_for(busy * a.hkv, (keys + bn - 1) / bn, cus_of(a), r.keys ? kLeastKeys : 4);
   if (r.splits > 1) r.bytes = static_cast<size_t>(r.tiles) * r.splits * a.hkv * slot_floats(r.rt, dp) * sizeof(float);
   return r;
 }
 
 struct DecodePlan {
-  bool skeys;
-  int stiles, ssplits, otiles, osplits;
+  bool skeys, join;
+  int stiles, ssplits, otiles, oitems, least;
+  int64_t own;  // workgroups a key head for the own keys
   size_t bytes;
 };
 DecodePlan plan_decode(const g16_attention_args& a) {
   DecodePlan r = {};
   const int group = a.hq / a.hkv, dp = a.d <= 64 ? 64 : 128, cus = cus_of(a);
   const int64_t rows = static_cast<int64_t>(a.seqs) * group;
-  r.skeys = rows <= kKeyTile;
+  r.skeys = rows <= 2 * kKeyTile;
   const int srt = r.skeys ? kKeyTile : kRowTile, sbn = r.skeys || a.is_f32 ? 32 : 64;
   r.stiles = a.shared > 0 ? static_cast<int>((rows + srt - 1) / srt) : 0;
-  r.ssplits = splits_for(static_cast<int64_t>(r.stiles) * a.hkv, (a.shared + sbn - 1) / sbn, cus, r.skeys ? 16 : 4);
+  r.ssplits = splits_for(static_cast<int64_t>(r.stiles) * a.hkv, (a.shared + sbn - 1) / sbn, cus, r.skeys ? kLeastKeys : 4);
   r.otiles = (group + kKeyTile - 1) / kKeyTile;
-  r.osplits = splits_for(static_cast<int64_t>(a.seqs) * r.otiles * a.hkv, (a.k_len + 31) / 32, cus, 16);
-  if (r.stiles > 0 || r.osplits > 1) {
+  const int64_t items = (2 * cus + static_cast<int64_t>(r.otiles) * a.hkv - 1) / (static_cast<int64_t>(r.otiles) * a.hkv);
+  // (at most as many parts as there are requests: one each, and no need to look for it)
+  const bool split = (a.k_len + 31) / 32 > kLeastKeys && items > 1;
+  r.oitems = static_cast<int>(items);
+  // (8 x 8 heads' parts of 16 requests up to 1500 keys: 24.8 us with 16 tiles at least, 22.4 with 8)
+  r.least = split ? kLeastKeys / 2 : 0;
+  r.own = (split ? items + a.seqs : a.seqs) * r.otiles;
+  r.join = r.stiles > 0 || split;
+  if (r.join)
     r.bytes = (static_cast<size_t>(r.stiles) * r.ssplits * a.hkv * slot_floats(srt, dp) +
-               static_cast<size_t>(a.seqs) * r.otiles * r.osplits * a.hkv * slot_floats(own_rows(group), dp)) * sizeof(float);
-  }
+               static_cast<size_t>(r.own) * a.hkv * slot_floats(own_rows(group), dp)) * sizeof(float);
   return r;
 }
 
@@ -1191,10 +1315,10 @@ int run_prompt(const Params& p, const PromptPlan& plan, hipStream_t stream) {
 }
 template <typename T, int DP>
 int run_decode(const Params& p, const DecodePlan& plan, hipStream_t stream) {
-  const dim3 grid((static_cast<unsigned>(p.stiles) * p.ssplits + static_cast<unsigned>(p.seqs) * p.otiles * p.osplits) * p.hkv);
+  const dim3 grid((static_cast<unsigned>(p.stiles) * p.ssplits + static_cast<unsigned>(plan.own)) * p.hkv);
   int rc = plan.skeys ? launch(decode_kernel<T, DP, true>, grid, dim3(kThreads), stream, p)
                       : launch(decode_kernel<T, DP, false>, grid, dim3(kThreads), stream, p);
-  if (rc == 0 && plan.bytes > 0)
+  if (rc == 0 && plan.join)
     rc = launch(decode_join_kernel<T, DP>, dim3(static_cast<unsigned>((static_cast<int64_t>(p.seqs) * p.hq + 3) / 4)), dim3(kThreads), stream, p,
                 plan.skeys ? kKeyTile : kRowTile);
   return rc;
@@ -1244,7 +1368,7 @@ extern "C" int g16_attention_decode(const g16_attention_args* args, void* stream
   const DecodePlan plan = plan_decode(a);
   if (plan.bytes > 0 && (a.workspace == nullptr || static_cast<size_t>(a.workspace_bytes) < plan.bytes)) return G16_E_WORKSPACE;
   if (!aligned16(a.workspace)) return G16_E_ALIGN;
-  if (!fits_grid((static_cast<int64_t>(plan.stiles) * plan.ssplits + static_cast<int64_t>(a.seqs) * plan.otiles * plan.osplits) * a.hkv) ||
+  if (!fits_grid((static_cast<int64_t>(plan.stiles) * plan.ssplits + plan.own) * a.hkv) ||
       !fits_grid((static_cast<int64_t>(a.seqs) * a.hq + 3) / 4))
     return G16_E_SHAPE;
   Params p = params(a);
@@ -1252,7 +1376,8 @@ extern "C" int g16_attention_decode(const g16_attention_args* args, void* stream
   p.stiles = plan.stiles;
   p.ssplits = plan.ssplits;
   p.otiles = plan.otiles;
-  p.osplits = plan.osplits;
+  p.oitems = plan.oitems;
+  p.least = plan.least;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (a.is_f32) return a.d <= 64 ? run_decode<float, 64>(p, plan, s) : run_decode<float, 128>(p, plan, s);
   return a.d <= 64 ? run_decode<_Float16, 64>(p, plan, s) : run_decode<_Float16, 128>(p, plan, s);
