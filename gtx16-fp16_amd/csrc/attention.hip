@@ -508,6 +508,7 @@ __device__ void rows_workgroup(const Params& p, char* lds, const Row& row, const
   for (int t = tbeg; t < tend; ++t) {
     const uint32_t buf = static_cast<uint32_t>((t - tbeg) & 1);
     wait_dma_le<0>();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     phase_barrier();  // tile t has arrived for every wavefront, and every one is done with tile t - 1
     pos0 = next_pos0;
     left = next_left;

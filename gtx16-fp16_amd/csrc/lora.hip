@@ -4,11 +4,22 @@
 //
 // Both products work on tiles of 16 rows on the 16x16 MFMA blocks, one adapter at a time, for whichever
 // rows of the tile have it; the rows of a tile are looked at once (a ballot per adapter among them), so
-// they may come in any order and need no sorting. fp32 activations, and the second product, whose left
-// side is fp32 sums, run on v_mfma_f32_16x16x4_f32, so nothing is rounded on the way to the output.
-// A tile's adapters may be dealt to several workgroups (`slots`): their rows are disjoint, so nothing has
-// to be added across them. Decode batches, where every row has its own adapter, are bound by reading the
-// adapters (rank * (K + N) * 2 bytes each) and need the parallel loads.
+// they may come in any order and need no sorting. The work of a workgroup is dealt to its 8 wavefronts by
+// what the tile turns out to hold: one adapter, and they share its K or its columns; 16, and each takes two.
+// (Workgroups for adapters that a tile may have cost more than they gave: 2048 of them with nothing to do
+// took 10 us.)
+//   * shrink, few rows: operands straight from memory, as the adapters (rank * (K + N) * 2 bytes for nearly every
+//     row of a decode batch) are what there is to read. K is split over workgroups as well; expand adds the
+//     parts up.
+//   * shrink, many rows: x and `down` come by DMA into LDS. A fragment straight from memory is 16 rows of 64
+//     bytes, whose lanes come in fours of different rows: 64 pieces, and the address unit takes them one by
+//     one (4096 x 4096 fp16, rank 32: 22 us).
+//   * expand: low is fp32, far from fp16's range in rows of massive activations. A row is scaled by a power of
+//     two to 2^14 .. 2^15 and taken as two fp16 parts (its largest value to 2^-22, smaller ones to 2^-22 of
+//     that), so two 16x16x32 MFMAs replace eight fp32 ones of twice the cycles each. The result passes
+//     through LDS, so that y is read and the output written in whole rows of 64 columns.
+//   * few rows whose adapters are small: expand computes low itself, in every workgroup (one launch less).
+// fp32 activations run on v_mfma_f32_16x16x4_f32: nothing is rounded.
 #include "g16_common.hpp"
 
 namespace g16 {
@@ -17,7 +28,10 @@ namespace {
 typedef float float8v __attribute__((ext_vector_type(8)));
 
 constexpr int kRows = 16;  // rows of a tile
-constexpr int kThreads = 256, kWaves = 4;
+// weights of `down` (rows * rank * K) up to which every workgroup of expand computes low itself
+constexpr int64_t kFusedWeights = 1 << 16;
+constexpr int kStagedTiles = 16;  // tiles from which shrink takes its operands through LDS
+constexpr int kThreads = 512, kWaves = 8;
 
 __device__ inline float4v mma16(half8 a, half8 b, float4v c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 __device__ inline float4v mma16(float8v a, float8v b, float4v c) {
@@ -45,126 +59,347 @@ struct Params {
   const float *scale, *y;
   void* out;
   float* low;  // [splits][M][rank]
-  int M, K, N, rank, adapters, slots, splits;
+  int M, K, N, rank, adapters, tiles, slots, splits, chunks;
 };
 
-// Calls f(adapter, rows) for every `slots`-th adapter (from `slot` on) among the tile's rows; rows: bit i
-// for row i. `mine` is the adapter of row lane % 16, negative for none.
-template <typename F>
-__device__ inline void each_adapter(int mine, int slot, int slots, const F& f) {
-  uint32_t left = static_cast<uint32_t>(__ballot(mine >= 0)) & 0xffffu;
-  for (int i = 0; left != 0; ++i) {
-    const int a = __builtin_amdgcn_readlane(mine, __builtin_ctz(left));
-    const uint32_t rows = static_cast<uint32_t>(__ballot(mine == a)) & 0xffffu;
-    left &= ~rows;
-    if (i % slots == slot) f(a, rows);
+// The adapters among a tile's 16 rows. mine: that of row lane % 16 (negative: none); ids: lane i, the i-th.
+struct Adapters {
+  int mine, count, ids;
+};
+__device__ inline Adapters adapters_of(const Params& p, int m0) {
+  const int lane = threadIdx.x & 63, row = m0 + (lane & 15);
+  Adapters t;
+  t.mine = row < p.M ? p.index[row] : -1;
+  if (t.mine >= p.adapters) t.mine = -1;
+  t.ids = -1;
+  t.count = 0;
+  for (uint32_t left = static_cast<uint32_t>(__ballot(t.mine >= 0)) & 0xffffu; left != 0; ++t.count) {
+    const int a = __builtin_amdgcn_readlane(t.mine, __builtin_ctz(left));
+    left &= ~static_cast<uint32_t>(__ballot(t.mine == a));
+    if (lane == t.count) t.ids = a;
+  }
+  return t;
+}
+
+// Steps s0 .. s1 - 1 of 32 values of K of low for the tile's rows and every `groups`-th adapter from `group` on:
+// block b of 16 rank columns, lane l: column 16 b + l % 16 of rows 4 (l / 16) .. + 3; other adapters' rows
+// stay as they are.
+template <typename T, int RB>
+__device__ inline void shrink_steps(const Params& p, int m0, const Adapters& t, int group, int groups, int s0, int s1, float4v (&low)[RB]) {
+  using V8 = typename Vec8<T>::V;
+  const int lane = threadIdx.x & 63, kl = (lane >> 4) * 8;
+  const T* xrow = static_cast<const T*>(p.x) + static_cast<size_t>(min(m0 + (lane & 15), p.M - 1)) * p.K;
+  for (int i = group; i < t.count; i += groups) {
+    const int a = __builtin_amdgcn_readlane(t.ids, i);
+    const uint32_t rows = static_cast<uint32_t>(__ballot(t.mine == a));
+    const _Float16* drow[RB];
+#pragma unroll
+    for (int b = 0; b < RB; ++b) drow[b] = p.down + (static_cast<size_t>(a) * p.rank + min(16 * b + (lane & 15), p.rank - 1)) * p.K;
+    float4v acc[RB] = {};
+    // kG steps' loads at a time. They are unconditional, from clamped places: past the share or past K, x counts
+    // as zeros (and `down` as values of the same row, which reach no other sum); columns past the rank are
+    // not stored.
+    constexpr int kG = RB == 1 ? 8 : (RB == 2 ? 4 : 2);
+    for (int s = s0; s < s1; s += kG) {
+      V8 xv[kG];
+      half8 dv[kG][RB];
+#pragma unroll
+      for (int g = 0; g < kG; ++g) {
+        const int k = min(s + g, s1 - 1) * 32 + kl, at = min(k, p.K - 8);
+        xv[g] = *reinterpret_cast<const V8*>(xrow + at);
+#pragma unroll
+        for (int b = 0; b < RB; ++b) dv[g][b] = *reinterpret_cast<const half8*>(drow[b] + at);
+        if (s + g >= s1 || k >= p.K) xv[g] = V8{};
+      }
+#pragma unroll
+      for (int g = 0; g < kG; ++g)
+#pragma unroll
+        for (int b = 0; b < RB; ++b) acc[b] = mma16(xv[g], as_operand(dv[g][b], T{}), acc[b]);
+    }
+#pragma unroll
+    for (int b = 0; b < RB; ++b)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if ((rows >> (4 * (lane >> 4) + j)) & 1u) low[b][j] = acc[b][j];
   }
 }
 
-__device__ inline int adapter_of(const Params& p, int row) {
-  const int a = row < p.M ? p.index[row] : -1;
-  return a < p.adapters ? a : -1;
+// The wavefronts' sums (part, in LDS) added up and stored for split `split`, for the rows of every `slots`-th adapter.
+template <int RB>
+__device__ inline void store_low(const Params& p, int m0, const Adapters& t, int slot, int slots, int split, const float4v (&part)[kWaves][RB][kWave]) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const float scale = t.mine >= 0 && p.scale != nullptr ? p.scale[t.mine] : 1.f;
+  uint32_t rows = 0;
+  for (int i = slot; i < t.count; i += slots) rows |= static_cast<uint32_t>(__ballot(t.mine == __builtin_amdgcn_readlane(t.ids, i)));
+  for (int b = wave; b < RB; b += kWaves) {
+    float4v v = part[0][b][lane];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) v += part[w][b][lane];
+    const int col = 16 * b + (lane & 15);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 4 * (lane >> 4) + i;
+      const float sc = __shfl(scale, r);
+      if (((rows >> r) & 1u) && col < p.rank) p.low[(static_cast<size_t>(split) * p.M + m0 + r) * p.rank + col] = v[i] * sc;
+    }
+  }
 }
 
-// low: split blockIdx.y of K, a quarter of it to each wavefront; RB blocks of 16 rank columns.
+// How 8 wavefronts share `count` adapters and a range of K: groups of wavefronts on different adapters, those
+// of a group on different parts of K.
+__device__ inline int groups_for(int count) { return count >= 5 ? 8 : (count >= 3 ? 4 : (count == 2 ? 2 : 1)); }
+
+// low from memory: a tile's every `slots`-th adapter (workgroups of one tile are `tiles` apart: neighbours go to
+// different XCDs), split blockIdx.y of K.
 template <typename T, int RB>
 __global__ __launch_bounds__(kThreads) void shrink_kernel(Params p) {
   __shared__ float4v part[kWaves][RB][kWave];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int slot = blockIdx.x % p.slots, m0 = static_cast<int>(blockIdx.x / p.slots) * kRows, split = blockIdx.y;
-  const int mine = adapter_of(p, m0 + (lane & 15));
-  const int steps = ceil_div(p.K, 32), parts = p.splits * kWaves, at = split * kWaves + wave;
-  const int s0 = static_cast<int>(static_cast<int64_t>(steps) * at / parts), s1 = static_cast<int>(static_cast<int64_t>(steps) * (at + 1) / parts);
-  const int kl = (lane >> 4) * 8;
-  const T* xrow = static_cast<const T*>(p.x) + static_cast<size_t>(min(m0 + (lane & 15), p.M - 1)) * p.K;
-  each_adapter(mine, slot, p.slots, [&](int a, uint32_t rows) {
-    const _Float16* drow = p.down + (static_cast<size_t>(a) * p.rank + (lane & 15)) * p.K;
-    float4v acc[RB] = {};
-#pragma unroll 4
-    for (int s = s0; s < s1; ++s) {
-      const int k = s * 32 + kl;
-      typename Vec8<T>::V xv = {};
-      half8 dv[RB] = {};
-      if (k < p.K) {
-        xv = *reinterpret_cast<const typename Vec8<T>::V*>(xrow + k);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int m0 = static_cast<int>(blockIdx.x % p.tiles) * kRows, slot = blockIdx.x / p.tiles, split = blockIdx.y;
+  const Adapters t = adapters_of(p, m0);
+  if (slot >= t.count) return;
+  const int steps = ceil_div(p.K, 32), of = p.splits * kWaves, at = split * kWaves + wave;
+  float4v low[RB] = {};
+  shrink_steps<T, RB>(p, m0, t, slot, p.slots, static_cast<int>(static_cast<int64_t>(steps) * at / of),
+                      static_cast<int>(static_cast<int64_t>(steps) * (at + 1) / of), low);
 #pragma unroll
-        for (int b = 0; b < RB; ++b)
-          if (16 * b + (lane & 15) < p.rank) dv[b] = *reinterpret_cast<const half8*>(drow + static_cast<size_t>(16 * b) * p.K + k);
-      }
-#pragma unroll
-      for (int b = 0; b < RB; ++b) acc[b] = mma16(xv, as_operand(dv[b], T{}), acc[b]);
-    }
-#pragma unroll
-    for (int b = 0; b < RB; ++b) part[wave][b][lane] = acc[b];
-    __syncthreads();
-    const float sc = p.scale != nullptr ? p.scale[a] : 1.f;
-    // lane l of block b holds column 16 b + l % 16 of rows 4 (l / 16) .. + 3
-    for (int b = wave; b < RB; b += kWaves) {
-      float4v v = part[0][b][lane];
-#pragma unroll
-      for (int w = 1; w < kWaves; ++w) v += part[w][b][lane];
-      const int col = 16 * b + (lane & 15);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = 4 * (lane >> 4) + i;
-        if (((rows >> r) & 1u) && col < p.rank) p.low[(static_cast<size_t>(split) * p.M + m0 + r) * p.rank + col] = v[i] * sc;
-      }
-    }
-    __syncthreads();
-  });
+  for (int b = 0; b < RB; ++b) part[wave][b][lane] = low[b];
+  __syncthreads();
+  store_low<RB>(p, m0, t, slot, p.slots, split, part);
 }
 
-// out = y + low @ up^T: a wavefront computes 64 columns of the tile's rows, transposed, so that a lane
-// ends up with 16 consecutive columns of one row (rows of block t of the left side: n0 + 16 (i / 4) + 4 t
-// + i % 4).
-template <bool OUT_F16>
-__global__ __launch_bounds__(kThreads) void expand_kernel(Params p) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int slot = blockIdx.x % p.slots, m0 = static_cast<int>(blockIdx.x / p.slots) * kRows;
-  const int n0 = (static_cast<int>(blockIdx.y) * kWaves + wave) * 64;
-  if (n0 >= p.N) return;
-  const int row = m0 + (lane & 15), mine = adapter_of(p, row), q = lane >> 4;
-  auto finish = [&](const float4v (&acc)[4]) {
-    const size_t at = static_cast<size_t>(row) * p.N + n0 + 16 * q;
+// low by way of LDS: kChunk values of K at a time, of x's 16 rows and an adapter's 16 RB rows of `down`, a
+// wavefront on 32 of them; the next chunks on their way meanwhile. 16-byte piece c of row r at c ^ r % 16.
+constexpr int kChunk = 32 * kWaves;
+template <typename T, int RB>
+struct Stage {
+  static constexpr int XROW = kChunk * sizeof(T), DROW = kChunk * 2;  // bytes
+  static constexpr int BYTES = 16 * XROW + 16 * RB * DROW;
+  static constexpr int XI = 16 * XROW / 1024 / kWaves, DI = 16 * RB * DROW / 1024 / kWaves;  // DMA instructions of a wavefront
+  static constexpr int COUNT = 3 * BYTES <= 80 * 1024 ? 3 : 2;
+};
+template <typename T, int RB>
+__global__ __launch_bounds__(kThreads) void shrink_tiles_kernel(Params p) {
+  using S = Stage<T, RB>;
+  constexpr int kLds = S::COUNT * S::BYTES > kWaves * RB * kWave * 16 ? S::COUNT * S::BYTES : kWaves * RB * kWave * 16;
+  __shared__ __attribute__((aligned(1024))) char lds[kLds];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int m0 = blockIdx.x * kRows, split = blockIdx.y;
+  const Adapters t = adapters_of(p, m0);
+  if (t.count == 0) return;
+  const int all = ceil_div(p.K, kChunk), c0 = static_cast<int>(static_cast<int64_t>(all) * split / p.splits),
+            c1 = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / p.splits), each = c1 - c0;
+  const uint32_t base = lds_base(lds);
+  constexpr int XC = S::XROW / 16, DC = S::DROW / 16;  // pieces of a row
+  auto issue = [&](int it) {
+    const int a = __builtin_amdgcn_readlane(t.ids, it / each), k0 = (c0 + it % each) * kChunk;
+    const uint32_t to = base + (it % S::COUNT) * S::BYTES;
+    const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<T*>(static_cast<const T*>(p.x) + static_cast<size_t>(m0) * p.K + k0), 0, 0x7fffffff, kRawBufferDword3);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (n0 + 16 * q + 8 * h >= p.N) break;
-      const float4v a = acc[2 * h] + *reinterpret_cast<const float4v*>(p.y + at + 8 * h);
-      const float4v b = acc[2 * h + 1] + *reinterpret_cast<const float4v*>(p.y + at + 8 * h + 4);
-      if constexpr (OUT_F16) {
-        const float8v v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-        *reinterpret_cast<half8*>(static_cast<_Float16*>(p.out) + at + 8 * h) = __builtin_convertvector(v, half8);
-      } else {
-        *reinterpret_cast<float4v*>(static_cast<float*>(p.out) + at + 8 * h) = a;
-        *reinterpret_cast<float4v*>(static_cast<float*>(p.out) + at + 8 * h + 4) = b;
+    for (int n = 0; n < S::XI; ++n) {
+      const int row = (wave * S::XI + n) * (64 / XC) + lane / XC, c = (lane % XC) ^ (row & 15);
+      const bool ok = m0 + row < p.M && k0 + c * static_cast<int>(16 / sizeof(T)) < p.K;
+      dma16(rx, to + (wave * S::XI + n) * 1024, ok ? static_cast<uint32_t>(row) * p.K * static_cast<uint32_t>(sizeof(T)) + c * 16 : kOob);
+    }
+    const __amdgpu_buffer_rsrc_t rd = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<_Float16*>(p.down + static_cast<size_t>(a) * p.rank * p.K + k0), 0, 0x7fffffff, kRawBufferDword3);
+#pragma unroll
+    for (int n = 0; n < S::DI; ++n) {
+      const int row = (wave * S::DI + n) * (64 / DC) + lane / DC, c = (lane % DC) ^ (row & 15);
+      const bool ok = row < p.rank && k0 + c * 8 < p.K;
+      dma16(rd, to + 16 * S::XROW + (wave * S::DI + n) * 1024, ok ? static_cast<uint32_t>(row) * p.K * 2u + c * 16 : kOob);
+    }
+  };
+  const int total = t.count * each, r16 = lane & 15, q = lane >> 4;
+  for (int i = 0; i < S::COUNT - 1; ++i)
+    if (i < total) issue(i);
+  float4v low[RB] = {}, acc[RB] = {};
+  for (int it = 0; it < total; ++it) {
+    // chunk `it` has arrived: only the younger ones may be in flight
+    if (S::COUNT == 3 && it + 1 < total) wait_dma_le<S::XI + S::DI>();
+    else wait_dma_le<0>();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    phase_barrier();  // ... for every wavefront, and every one has read the chunk whose place the next one takes
+    if (it + S::COUNT - 1 < total) issue(it + S::COUNT - 1);
+    const char* at = lds + (it % S::COUNT) * S::BYTES;
+    typename Vec8<T>::V xv;
+    if constexpr (sizeof(T) == 2) {
+      xv = *reinterpret_cast<const half8*>(at + r16 * S::XROW + (((wave * 4 + q) ^ r16) << 4));
+    } else {
+      const float4v a = *reinterpret_cast<const float4v*>(at + r16 * S::XROW + (((wave * 8 + 2 * q) ^ r16) << 4));
+      const float4v b = *reinterpret_cast<const float4v*>(at + r16 * S::XROW + (((wave * 8 + 2 * q + 1) ^ r16) << 4));
+      xv = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+      const half8 dv = *reinterpret_cast<const half8*>(at + 16 * S::XROW + (16 * b + r16) * S::DROW + (((wave * 4 + q) ^ r16) << 4));
+      acc[b] = mma16(xv, as_operand(dv, T{}), acc[b]);
+    }
+    if ((it + 1) % each == 0) {  // an adapter is done: its rows
+      const int a = __builtin_amdgcn_readlane(t.ids, it / each);
+      const uint32_t rows = static_cast<uint32_t>(__ballot(t.mine == a));
+#pragma unroll
+      for (int b = 0; b < RB; ++b) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if ((rows >> (4 * q + j)) & 1u) low[b][j] = acc[b][j];
+        acc[b] = float4v{};
+      }
+    }
+  }
+  __syncthreads();
+  auto& part = *reinterpret_cast<float4v(*)[kWaves][RB][kWave]>(lds);
+#pragma unroll
+  for (int b = 0; b < RB; ++b) part[wave][b][lane] = low[b];
+  __syncthreads();
+  store_low<RB>(p, m0, t, 0, 1, split, part);
+}
+
+// out = y + low @ up^T for tile blockIdx.x and p.chunks runs of 64 columns from blockIdx.y on; a wavefront takes
+// a share of all (adapter, run) pairs. RC: pieces of 32 rank columns. T: of x, FUSED: low is computed here.
+constexpr int kScrRow = 68;  // floats of a row of the wavefronts' LDS: rows start 4 banks apart
+template <typename T, bool OUT_F16, int RC, bool FUSED>
+__global__ __launch_bounds__(kThreads) void expand_kernel(Params p) {
+  constexpr int RB = FUSED ? 2 * RC : 1;
+  __shared__ float4v part[FUSED ? kWaves : 1][RB][FUSED ? kWave : 1];
+  __shared__ __attribute__((aligned(16))) float scratch[kWaves][kRows][kScrRow];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int m0 = blockIdx.x * kRows, q = lane >> 4, row = m0 + (lane & 15);
+  const Adapters t = adapters_of(p, m0);
+  if constexpr (FUSED) {
+    const int steps = ceil_div(p.K, 32), groups = groups_for(t.count), parts = kWaves / groups, at = wave % parts;
+    float4v low[RB] = {};
+    shrink_steps<T, RB>(p, m0, t, wave / parts, groups, steps * at / parts, steps * (at + 1) / parts, low);
+#pragma unroll
+    for (int b = 0; b < RB; ++b) part[wave][b][lane] = low[b];
+    __syncthreads();
+    for (int i = tid; i < RB * kWave; i += kThreads) {
+      float4v v = part[0][i / kWave][i % kWave];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) v += part[w][i / kWave][i % kWave];
+      part[0][i / kWave][i % kWave] = v;
+    }
+    __syncthreads();
+  }
+  // The pairs: rows without an adapter count as one more (number t.count) where y has to be copied.
+  const int n_first = static_cast<int>(blockIdx.y) * p.chunks * 64, runs = min(p.chunks, ceil_div(p.N - n_first, 64));
+  const bool copy = p.y != p.out && __ballot(t.mine < 0 && row < p.M) != 0;
+  const int pairs = (t.count + (copy ? 1 : 0)) * runs;
+  const int waves = kWaves * gridDim.z, w = wave + kWaves * blockIdx.z, p0 = pairs * w / waves, p1 = pairs * (w + 1) / waves;
+  if (p0 >= p1) return;
+  float(*scr)[kScrRow] = scratch[wave];
+  half8 hi[RC], lo[RC];
+  float back = 1.f;
+  int at = -1, a = -1;
+  half8 up[RC][4];
+  float4v y[4];
+  // y and the output: lane l holds columns 4 (l % 16) .. + 3 of rows l / 16 + 4 j
+  const int col = (lane & 15) * 4;
+  bool ours[4];
+  auto load = [&](int pair) {
+    const int which = pair / runs, n = n_first + (pair % runs) * 64;
+    const int id = which < t.count ? __builtin_amdgcn_readlane(t.ids, which) : -1;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int r = q + 4 * j, of = __shfl(t.mine, r);  // (by every lane)
+      ours[j] = of == id && m0 + r < p.M && n + col < p.N;
+      if (ours[j]) y[j] = *reinterpret_cast<const float4v*>(p.y + static_cast<size_t>(m0 + r) * p.N + n + col);
+    }
+    if (id >= 0) {
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        // (clamped: low is zero past the rank, and columns past the end are not stored)
+        const _Float16* from = p.up + (static_cast<size_t>(id) * p.N + min(n + 16 * b + (lane & 15), p.N - 1)) * p.rank;
+#pragma unroll
+        for (int c = 0; c < RC; ++c) up[c][b] = *reinterpret_cast<const half8*>(from + min(32 * c + 8 * q, p.rank - 8));
       }
     }
   };
-  // rows without an adapter: y as it is (where it is the output already, they are done)
-  if (slot == 0 && row < p.M && mine < 0 && p.y != p.out) {
-    const float4v none[4] = {};
-    finish(none);
-  }
-  each_adapter(mine, slot, p.slots, [&](int a, uint32_t) {
-    const bool ours = mine == a;
-    float4v acc[4] = {};
-    for (int r0 = 0; r0 < p.rank; r0 += 32) {
-      const int r = r0 + 8 * q;
-      float8v low = {};
-      if (ours && r < p.rank) {
-        for (int s = 0; s < p.splits; ++s)
-          low += *reinterpret_cast<const float8v*>(p.low + (static_cast<size_t>(s) * p.M + row) * p.rank + r);
+  // this lane's row (lane % 16) of low: 8 values of every piece, of other adapters' rows zeros
+  auto load_low = [&]() {
+    float8v low[RC];
+    float top = 0.f;
+#pragma unroll
+    for (int c = 0; c < RC; ++c) {
+      const int r = 32 * c + 8 * q;
+      low[c] = float8v{};
+      if (t.mine == a && r < p.rank) {
+        if constexpr (FUSED) {
+          const float sc = p.scale != nullptr ? p.scale[a] : 1.f;
+          const int rr = lane & 15;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) low[c][i] = part[0][(r + i) >> 4][((r + i) & 15) + 16 * (rr >> 2)][rr & 3] * sc;
+        } else {
+          const float* from = p.low + static_cast<size_t>(row) * p.rank + r;
+          for (int s = 0; s < p.splits; s += 4) {  // (four splits' loads at a time)
+            float8v v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              v[i] = *reinterpret_cast<const float8v*>(from + static_cast<size_t>(min(s + i, p.splits - 1)) * p.M * p.rank);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (s + i < p.splits) low[c] += v[i];
+          }
+        }
       }
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const int n = n0 + 16 * ((lane & 15) >> 2) + 4 * t + (lane & 3);
-        half8 u = {};
-        if (n < p.N && r < p.rank) u = *reinterpret_cast<const half8*>(p.up + (static_cast<size_t>(a) * p.N + n) * p.rank + r);
-        acc[t] = mma16(widen(u), low, acc[t]);
+      for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(low[c][i]));
+    }
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    // 2^e with top * 2^e in [2^14, 2^15), e held to what fp32 has both ways; infinities stay as they are
+    const int e = top > 0.f && top < __builtin_huge_valf() ? min(max(14 - ilogbf(top), -120), 120) : 0;
+    const float by = ldexpf(1.f, e);
+    back = ldexpf(1.f, -e);
+#pragma unroll
+    for (int c = 0; c < RC; ++c) {
+      const float8v v = low[c] * by;
+      hi[c] = __builtin_convertvector(v, half8);
+      lo[c] = __builtin_convertvector(v - widen(hi[c]), half8);
+    }
+  };
+  load(p0);
+  for (int pair = p0; pair < p1; ++pair) {
+    const int which = pair / runs, n = n_first + (pair % runs) * 64;
+    if (which != at) {
+      at = which;
+      a = which < t.count ? __builtin_amdgcn_readlane(t.ids, which) : -1;
+      if (a >= 0) load_low();
+    }
+    if (a >= 0) {
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        float4v acc = {};
+#pragma unroll
+        for (int c = 0; c < RC; ++c) {
+          acc = mma16(up[c][b], hi[c], acc);
+          acc = mma16(up[c][b], lo[c], acc);
+        }
+        // lane l: columns 16 b + 4 (l / 16) .. + 3 of row l % 16
+        *reinterpret_cast<float4v*>(&scr[lane & 15][16 * b + 4 * q]) = acc * back;
       }
     }
-    if (ours) finish(acc);
-  });
+    float4v v[4];
+    bool mine[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[j] = y[j];
+      mine[j] = ours[j];
+    }
+    if (pair + 1 < p1) load(pair + 1);
+    if (a >= 0) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] += *reinterpret_cast<const float4v*>(&scr[q + 4 * j][col]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (!mine[j]) continue;
+      const size_t to = static_cast<size_t>(m0 + q + 4 * j) * p.N + n + col;
+      if constexpr (OUT_F16) *reinterpret_cast<half4*>(static_cast<_Float16*>(p.out) + to) = __builtin_convertvector(v[j], half4);
+      else *reinterpret_cast<float4v*>(static_cast<float*>(p.out) + to) = v[j];
+    }
+  }
 }
 
 // ---- host ------------------------------------------------------------------------------------------------
@@ -181,35 +416,55 @@ int check(const g16_lora_args& a) {
 }
 
 struct Plan {
-  int tiles, slots, splits;
+  bool fused, staged;
+  int tiles, slots, splits, chunks, wide;  // wide: workgroups that share a tile's columns in expand
 };
 Plan plan_of(const g16_lora_args& a) {
   const int cus = a.num_cus > 0 ? a.num_cus : 256;
   Plan p;
   p.tiles = ceil_div(a.M, kRows);
-  // few tiles: an adapter a workgroup (a tile has at most 16), and K split so that about two land on a CU
-  p.slots = p.tiles >= cus ? 1 : (p.tiles * 4 >= cus ? 4 : 16);
-  if (p.slots > a.M) p.slots = a.M;
-  const int steps = ceil_div(a.K, 32);
-  const int want = (2 * cus + p.tiles * p.slots - 1) / (p.tiles * p.slots);
-  p.splits = want < 1 ? 1 : (want > 8 ? 8 : want);
-  if (p.splits > (steps + 7) / 8) p.splits = (steps + 7) / 8;
+  p.fused = a.M <= kRows && static_cast<int64_t>(a.M) * a.rank * a.K <= kFusedWeights;
+  p.staged = p.tiles >= kStagedTiles && a.K >= 2 * kChunk;
+  // staged: K in as many parts as make about two workgroups a CU, of at least two chunks; else an adapter a
+  // workgroup (a tile has at most 16, and there are few tiles), and up to 8 steps of K a wavefront
+  p.slots = p.staged ? 1 : (a.M < 16 ? a.M : 16);
+  p.splits = p.staged ? (2 * cus + p.tiles - 1) / p.tiles : ceil_div(ceil_div(a.K, 32), 8 * kWaves);
+  const int most = p.staged ? (a.K / (2 * kChunk) < 4 ? a.K / (2 * kChunk) : 4) : 8;
+  if (p.splits > most) p.splits = most;
   if (p.splits < 1) p.splits = 1;
+  // expand: about four workgroups a CU, of 1 to 32 runs of 64 columns, two for one run where that leaves
+  // CUs without any
+  const int runs = ceil_div(a.N, 64);
+  const int64_t each = (static_cast<int64_t>(p.tiles) * runs + 4 * cus - 1) / (4 * cus);
+  p.chunks = each < 1 ? 1 : (each > 32 ? 32 : static_cast<int>(each));
+  p.wide = a.M > kWaves && static_cast<int64_t>(p.tiles) * runs <= cus ? 2 : 1;
   return p;
 }
 
 Params params(const g16_lora_args& a, const Plan& plan) {
   return Params{a.x, reinterpret_cast<const _Float16*>(a.down), reinterpret_cast<const _Float16*>(a.up), a.index, a.scale, a.y, a.out,
-                static_cast<float*>(a.workspace), a.M, a.K, a.N, a.rank, a.adapters, plan.slots, plan.splits};
+                static_cast<float*>(a.workspace), a.M, a.K, a.N, a.rank, a.adapters, plan.tiles, plan.slots, plan.splits, plan.chunks};
 }
 
+template <typename T, int RB>
+int run_shrink_as(const Params& p, const Plan& plan, hipStream_t s) {
+  const dim3 grid(plan.tiles * plan.slots, plan.splits), block(kThreads);
+  return plan.staged ? launch(shrink_tiles_kernel<T, RB>, grid, block, s, p) : launch(shrink_kernel<T, RB>, grid, block, s, p);
+}
 template <typename T>
 int run_shrink(const Params& p, const Plan& plan, hipStream_t s) {
-  const dim3 grid(static_cast<unsigned>(plan.tiles) * plan.slots, plan.splits), block(kThreads);
-  if (p.rank <= 16) return launch(shrink_kernel<T, 1>, grid, block, s, p);
-  if (p.rank <= 32) return launch(shrink_kernel<T, 2>, grid, block, s, p);
-  if (p.rank <= 64) return launch(shrink_kernel<T, 4>, grid, block, s, p);
-  return launch(shrink_kernel<T, 8>, grid, block, s, p);
+  if (p.rank <= 16) return run_shrink_as<T, 1>(p, plan, s);
+  if (p.rank <= 32) return run_shrink_as<T, 2>(p, plan, s);
+  if (p.rank <= 64) return run_shrink_as<T, 4>(p, plan, s);
+  return run_shrink_as<T, 8>(p, plan, s);
+}
+
+template <typename T, bool OUT_F16, bool FUSED>
+int run_expand(const Params& p, const Plan& plan, hipStream_t s) {
+  const dim3 grid(plan.tiles, ceil_div(ceil_div(p.N, 64), plan.chunks), plan.wide), block(kThreads);
+  if (p.rank <= 32) return launch(expand_kernel<T, OUT_F16, 1, FUSED>, grid, block, s, p);
+  if (p.rank <= 64) return launch(expand_kernel<T, OUT_F16, 2, FUSED>, grid, block, s, p);
+  return launch(expand_kernel<T, OUT_F16, 4, FUSED>, grid, block, s, p);
 }
 
 }  // namespace
@@ -219,13 +474,15 @@ using namespace g16;
 
 extern "C" size_t g16_lora_workspace_bytes(const g16_lora_args* args) {
   if (args == nullptr || check(*args) != G16_OK || args->M == 0 || args->N == 0) return 0;
-  return static_cast<size_t>(plan_of(*args).splits) * args->M * args->rank * sizeof(float);
+  const Plan plan = plan_of(*args);
+  return plan.fused ? 0 : static_cast<size_t>(plan.splits) * args->M * args->rank * sizeof(float);
 }
 
 extern "C" int g16_lora_shrink(const g16_lora_args* args, void* stream) {
   if (args == nullptr) return G16_E_NULL;
   const int st = check(*args);
   if (st != G16_OK || args->M == 0 || args->N == 0 || args->rank == 0 || args->adapters == 0) return st;
+  if (plan_of(*args).fused) return G16_OK;
   if (args->workspace == nullptr || static_cast<size_t>(args->workspace_bytes) < g16_lora_workspace_bytes(args)) return G16_E_WORKSPACE;
   if (!aligned16(args->workspace)) return G16_E_ALIGN;
   const Plan plan = plan_of(*args);
@@ -238,13 +495,14 @@ extern "C" int g16_lora_expand(const g16_lora_args* args, void* stream) {
   if (args == nullptr) return G16_E_NULL;
   const int st = check(*args);
   if (st != G16_OK || args->M == 0 || args->N == 0) return st;
-  if (args->rank > 0 && args->adapters > 0 &&
+  const Plan plan = plan_of(*args);
+  if (args->rank > 0 && args->adapters > 0 && !plan.fused &&
       (args->workspace == nullptr || static_cast<size_t>(args->workspace_bytes) < g16_lora_workspace_bytes(args)))
     return G16_E_WORKSPACE;
   if (!aligned16(args->workspace)) return G16_E_ALIGN;
-  const Plan plan = plan_of(*args);
   const Params p = params(*args, plan);
-  const dim3 grid(static_cast<unsigned>(plan.tiles) * plan.slots, (args->N + 64 * kWaves - 1) / (64 * kWaves)), block(kThreads);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  return args->out_is_f16 ? launch(expand_kernel<true>, grid, block, s, p) : launch(expand_kernel<false>, grid, block, s, p);
+  if (!plan.fused) return args->out_is_f16 ? run_expand<_Float16, true, false>(p, plan, s) : run_expand<_Float16, false, false>(p, plan, s);
+  if (args->x_is_f32) return args->out_is_f16 ? run_expand<float, true, true>(p, plan, s) : run_expand<float, false, true>(p, plan, s);
+  return args->out_is_f16 ? run_expand<_Float16, true, true>(p, plan, s) : run_expand<_Float16, false, true>(p, plan, s);
 }

@@ -45,7 +45,11 @@ def test_nothing_to_do_is_no_error():
     assert _clib.load().g16_lora_expand(None, None) == NULL
 
 
-@pytest.mark.parametrize("M,K,rank", [(1, 8, 8), (20, 4096, 16), (5000, 512, 128)])
+def test_few_rows_need_no_workspace():
+    assert size(M=1, K=8, rank=8) == 0
+
+
+@pytest.mark.parametrize("M,K,rank", [(20, 4096, 16), (300, 4096, 40), (5000, 512, 128)])
 def test_workspace_holds_whole_splits(M, K, rank):
     n = size(M=M, K=K, rank=rank)
     assert n > 0 and n % (4 * M * rank) == 0
