@@ -87,7 +87,7 @@ def build_fastcall(verbose: bool = False) -> Path:
     if cc is None:
         raise RuntimeError("no C compiler (gcc) for the _g16fast extension")
     _run([cc, "-O2", "-fPIC", "-shared", "-Wall", "-Wextra", "-Wno-cast-function-type",
-          f"-I{sysconfig.get_paths()['include']}", str(CSRC / "fastcall.c"), "-o", str(tmp)], verbose)
+          f"-I{sysconfig.get_paths()['include']}", f"-I{INCLUDE}", str(CSRC / "fastcall.c"), "-o", str(tmp), "-lm"], verbose)
     os.replace(tmp, out)
     return out
 

@@ -11,9 +11,12 @@
  */
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
+#include <math.h>
 #include <stddef.h>
 #include <stdint.h>
 #include <string.h>
+
+#include "g16.h"
 
 typedef int (*skinny_fn)(const void*, const void*, void*, const void*, int, int, int, int, void*, size_t, void*,
                          size_t, void*);
@@ -230,6 +233,422 @@ static PyObject* fast_args_call(PyObject* self, PyObject* const* args, Py_ssize_
   return PyLong_FromLong(st);
 }
 
+/* ---- the usual calls of attention, attention_decode and lora_mm_t, checked and packed here -------------
+ * Each takes what its Python function takes and returns the output, or None for anything but a call that
+ * could go straight to the kernels: operands of another type, shape, layout or device, a gradient wanted,
+ * a scratch buffer that has to grow. The Python function then looks at the arguments one by one, copies
+ * what has to be copied or says what is wrong with them. A tensor is read through its public attributes
+ * (about 0.3 us of calls each, where the same checks in Python take 1). */
+typedef struct {
+  void* ptr;
+  int64_t shape[4], stride[4]; /* in elements */
+  int nd, device;
+  PyObject* dtype; /* torch's own dtype objects live as long as torch */
+} tensor_t;
+
+static PyObject *s_dtype, *s_shape, *s_stride, *s_data_ptr, *s_get_device, *s_requires_grad, *s_new_empty;
+static PyObject *g_f16 = NULL, *g_f32 = NULL, *g_i32 = NULL, *g_raw_stream = NULL, *g_grad_enabled = NULL, *g_ready = NULL,
+                *g_scratch = NULL;
+typedef size_t (*attention_size_fn)(const g16_attention_args*);
+typedef int (*attention_fn)(const g16_attention_args*, void*);
+static attention_size_fn g_attention_size[2];
+static attention_fn g_attention[2];
+
+#define MAX_DEVICES 64
+static int g_device_cus[MAX_DEVICES]; /* 0: not asked yet, -1: not a device of these kernels */
+
+static int int_tuple(PyObject* o, int64_t* out, int* n) {
+  if (o == NULL || !PyTuple_Check(o) || PyTuple_GET_SIZE(o) > 4) {
+    Py_XDECREF(o);
+    return -1;
+  }
+  *n = (int)PyTuple_GET_SIZE(o);
+  for (int i = 0; i < *n; ++i) out[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(o, i));
+  Py_DECREF(o);
+  return PyErr_Occurred() ? -1 : 0;
+}
+
+/* 0: t is filled in; -1: not a tensor that can be looked at (no error is left set) */
+static int read_tensor(PyObject* o, tensor_t* t) {
+  int n = 0;
+  PyObject* x;
+  if (int_tuple(PyObject_GetAttr(o, s_shape), t->shape, &t->nd) || int_tuple(PyObject_CallMethodNoArgs(o, s_stride), t->stride, &n) ||
+      n != t->nd)
+    goto no;
+  x = PyObject_CallMethodNoArgs(o, s_data_ptr);
+  if (x == NULL) goto no;
+  t->ptr = PyLong_AsVoidPtr(x);
+  Py_DECREF(x);
+  x = PyObject_CallMethodNoArgs(o, s_get_device);
+  if (x == NULL) goto no;
+  t->device = (int)PyLong_AsLong(x);
+  Py_DECREF(x);
+  t->dtype = PyObject_GetAttr(o, s_dtype);
+  if (t->dtype == NULL || PyErr_Occurred()) goto no;
+  Py_DECREF(t->dtype);
+  return 0;
+no:
+  PyErr_Clear();
+  return -1;
+}
+
+/* Compute units of a device these kernels run on; -1 else */
+static int device_cus(int device) {
+  if (device < 0 || device >= MAX_DEVICES) return -1;
+  if (g_device_cus[device] == 0) {
+    PyObject* r = PyObject_CallFunction(g_ready, "i", device);
+    long n = r == NULL ? -1 : PyLong_AsLong(r);
+    Py_XDECREF(r);
+    PyErr_Clear();
+    g_device_cus[device] = n > 0 ? (int)n : -1;
+  }
+  return g_device_cus[device];
+}
+
+static int wants_grad(PyObject* const* tensors, int n) {
+  PyObject* r = PyObject_CallNoArgs(g_grad_enabled);
+  int on = r != Py_False;
+  Py_XDECREF(r);
+  if (!on) return 0;
+  for (int i = 0; i < n; ++i) {
+    r = PyObject_GetAttr(tensors[i], s_requires_grad);
+    on = r != Py_False;
+    Py_XDECREF(r);
+    if (on) return 1;
+  }
+  return 0;
+}
+
+static int raw_stream(int device, void** out) {
+  PyObject *i = PyLong_FromLong(device), *r = i == NULL ? NULL : PyObject_CallOneArg(g_raw_stream, i);
+  Py_XDECREF(i);
+  if (r == NULL) return -1;
+  *out = PyLong_AsVoidPtr(r);
+  Py_DECREF(r);
+  return PyErr_Occurred() ? -1 : 0;
+}
+
+/* Pointer of the scratch buffer of (device, stream), at least `bytes` long */
+static int scratch(int device, void* stream, size_t bytes, void** out) {
+  PyObject* r = PyObject_CallFunction(g_scratch, "iKn", device, (unsigned long long)(uintptr_t)stream, (Py_ssize_t)bytes);
+  if (r == NULL) return -1;
+  *out = PyLong_AsVoidPtr(r);
+  Py_DECREF(r);
+  return PyErr_Occurred() ? -1 : 0;
+}
+
+static PyObject* empty_like(PyObject* o) {
+  PyObject* shape = PyObject_GetAttr(o, s_shape);
+  if (shape == NULL) return NULL;
+  PyObject* argv[2] = {o, shape};
+  PyObject* r = PyObject_VectorcallMethod(s_new_empty, argv, 2, NULL);
+  Py_DECREF(shape);
+  return r;
+}
+
+static int aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+/* Rows [.., token, head, d] that the kernels read in place (attn.py: _rows) */
+static int rows_ok(const tensor_t* t, int size, int64_t d, int keys) {
+  if (t->stride[t->nd - 1] != 1 || !aligned(t->ptr)) return 0;
+  for (int i = 0; i < t->nd - 1; ++i)
+    if (t->stride[i] * size % 16 != 0) return 0;
+  const int64_t token = t->stride[t->nd - 3];
+  return !keys || (token >= d && token * size < G16_ATTENTION_MAX_STRIDE);
+}
+
+/* A contiguous int32 or fp32 vector (NULL for None) */
+static int vector(PyObject* o, PyObject* dtype, int64_t n, int device, const void** out) {
+  tensor_t t;
+  *out = NULL;
+  if (o == Py_None) return 0;
+  if (read_tensor(o, &t) || t.dtype != dtype || t.nd != 1 || t.shape[0] != n || t.device != device || (n > 1 && t.stride[0] != 1)) return -1;
+  *out = t.ptr;
+  return 0;
+}
+
+static int fits(int64_t v) { return v >= 0 && v <= INT32_MAX; }
+
+static int heads_ok(const tensor_t* q, const tensor_t* k, const tensor_t* v, g16_attention_args* a) {
+  const int64_t hq = q->shape[q->nd - 2], d = q->shape[q->nd - 1], hkv = k->shape[k->nd - 2];
+  if ((q->dtype != g_f16 && q->dtype != g_f32) || k->dtype != q->dtype || v->dtype != q->dtype || k->device != q->device ||
+      v->device != q->device || memcmp(k->shape, v->shape, sizeof(int64_t) * (size_t)k->nd) != 0 || k->shape[k->nd - 1] != d || d <= 0 ||
+      d % 8 != 0 || d > G16_ATTENTION_MAX_D || !fits(hq) || !fits(hkv) || hkv == 0 || hq == 0 || hq % hkv != 0)
+    return 0;
+  a->hq = (int)hq;
+  a->hkv = (int)hkv;
+  a->d = (int)d;
+  a->is_f32 = q->dtype == g_f32;
+  a->num_cus = device_cus(q->device);
+  const int size = a->is_f32 ? 4 : 2;
+  return a->num_cus > 0 && rows_ok(q, size, d, 0) && rows_ok(k, size, d, 1) && rows_ok(v, size, d, 1);
+}
+
+/* scale, softcap, shared keys, slopes */
+static int rest_ok(PyObject* scale, PyObject* cap, PyObject* sk, PyObject* sv, PyObject* slopes, int device, PyObject* dtype, g16_attention_args* a) {
+  double c = PyFloat_AsDouble(cap), s = scale == Py_None ? 0.0 : PyFloat_AsDouble(scale);
+  if (PyErr_Occurred()) return 0;
+  if (scale == Py_None) {
+    s = 1.0 / sqrt((double)a->d);
+  }
+  if (s != s || !(c >= 0.0 && c < 1e300)) return 0;
+  a->scale = (float)s;
+  a->softcap = (float)c;
+  if (vector(slopes, g_f32, a->hq, device, (const void**)&a->slopes)) return 0;
+  if ((sk == Py_None) != (sv == Py_None)) return 0;
+  if (sk != Py_None) {
+    tensor_t tk, tv;
+    const int size = a->is_f32 ? 4 : 2;
+    if (read_tensor(sk, &tk) || read_tensor(sv, &tv) || tk.nd != 3 || tv.nd != 3 || tk.dtype != dtype || tv.dtype != dtype ||
+        tk.device != device || tv.device != device || memcmp(tk.shape, tv.shape, sizeof(int64_t) * 3) != 0 || tk.shape[1] != a->hkv ||
+        tk.shape[2] != a->d || tk.shape[0] == 0 || !fits(tk.shape[0]) || !rows_ok(&tk, size, a->d, 1) || !rows_ok(&tv, size, a->d, 1))
+      return 0;
+    a->shared_k = tk.ptr;
+    a->shared_v = tv.ptr;
+    a->shared = (int)tk.shape[0];
+    a->shared_k_token = tk.stride[0];
+    a->shared_k_head = tk.stride[1];
+    a->shared_v_token = tv.stride[0];
+    a->shared_v_head = tv.stride[1];
+  }
+  return 1;
+}
+
+static PyObject* none_clear(void) {
+  PyErr_Clear();
+  Py_RETURN_NONE;
+}
+
+/* The output, or None with no error set where the library rejects the arguments (the Python function then
+ * makes the same call and raises) */
+static PyObject* run_attention(PyObject* q, int device, g16_attention_args* a, int decode) {
+  void* stream;
+  PyObject* out;
+  int st;
+  const size_t bytes = g_attention_size[decode](a);
+  if (raw_stream(device, &stream) || (bytes > 0 && scratch(device, stream, bytes, &a->workspace))) return none_clear();
+  if (bytes > 0 && a->workspace == NULL) Py_RETURN_NONE;
+  a->workspace_bytes = (int64_t)bytes;
+  out = empty_like(q);
+  tensor_t t;
+  if (out == NULL || read_tensor(out, &t)) {
+    Py_XDECREF(out);
+    return none_clear();
+  }
+  a->out = t.ptr;
+  Py_BEGIN_ALLOW_THREADS
+  st = g_attention[decode](a, stream);
+  Py_END_ALLOW_THREADS
+  if (st != 0) {
+    Py_DECREF(out);
+    Py_RETURN_NONE;
+  }
+  return out;
+}
+
+/* attention(q, k, v, q_offsets, k_offsets, causal, visible, shared_k, shared_v, scale, softcap, slopes) */
+static PyObject* fast_attention(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  tensor_t q, k, v;
+  g16_attention_args a;
+  if (check_nargs("attention", nargs, 12)) return NULL;
+  if (g_ready == NULL) Py_RETURN_NONE;
+  memset(&a, 0, sizeof(a));
+  const int packed = args[3] != Py_None;
+  if (read_tensor(args[0], &q) || read_tensor(args[1], &k) || read_tensor(args[2], &v) || q.nd != (packed ? 3 : 4) || k.nd != q.nd ||
+      v.nd != q.nd || !heads_ok(&q, &k, &v, &a) || wants_grad(args, 3))
+    return none_clear();
+  if (packed) {
+    tensor_t o;
+    const PyObject* ko = args[4] == Py_None ? args[3] : args[4];
+    if (read_tensor(args[3], &o) || o.nd != 1 || o.shape[0] < 2 || !fits(o.shape[0] - 1) ||
+        vector(args[3], g_i32, o.shape[0], q.device, (const void**)&a.q_offsets) ||
+        vector((PyObject*)ko, g_i32, o.shape[0], q.device, (const void**)&a.k_offsets))
+      return none_clear();
+    a.seqs = (int)(o.shape[0] - 1);
+    a.q_token = q.stride[0], a.q_head = q.stride[1];
+    a.k_token = k.stride[0], a.k_head = k.stride[1];
+    a.v_token = v.stride[0], a.v_head = v.stride[1];
+  } else {
+    if (args[4] != Py_None || k.shape[0] != q.shape[0] || !fits(q.shape[0])) return none_clear();
+    a.seqs = (int)q.shape[0];
+    a.q_seq = q.stride[0], a.q_token = q.stride[1], a.q_head = q.stride[2];
+    a.k_seq = k.stride[0], a.k_token = k.stride[1], a.k_head = k.stride[2];
+    a.v_seq = v.stride[0], a.v_token = v.stride[1], a.v_head = v.stride[2];
+  }
+  const int64_t q_len = q.shape[q.nd - 3], k_len = k.shape[k.nd - 3];
+  const int causal = PyObject_IsTrue(args[5]);
+  if (!fits(q_len) || !fits(k_len) || q_len == 0 || a.seqs == 0 || causal < 0 || (!causal && args[6] != Py_None)) return none_clear();
+  a.q_len = (int)q_len;
+  a.k_len = (int)k_len;
+  a.causal = causal;
+  if (vector(args[6], g_i32, a.seqs, q.device, (const void**)&a.visible) ||
+      !rest_ok(args[9], args[10], args[7], args[8], args[11], q.device, q.dtype, &a))
+    return none_clear();
+  a.q = q.ptr, a.k = k.ptr, a.v = v.ptr;
+  return run_attention(args[0], q.device, &a, 0);
+}
+
+/* attention_decode(q, k_cache, v_cache, lengths, pages, shared_k, shared_v, scale, softcap, slopes) */
+static PyObject* fast_attention_decode(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  tensor_t q, k, v;
+  g16_attention_args a;
+  if (check_nargs("attention_decode", nargs, 10)) return NULL;
+  if (g_ready == NULL) Py_RETURN_NONE;
+  memset(&a, 0, sizeof(a));
+  if (read_tensor(args[0], &q) || read_tensor(args[1], &k) || read_tensor(args[2], &v) || q.nd != 3 || k.nd != 4 || v.nd != 4 ||
+      q.shape[0] == 0 || !fits(q.shape[0]) || !fits(k.shape[0]) || !fits(k.shape[1]) || k.shape[1] == 0 || !heads_ok(&q, &k, &v, &a) ||
+      wants_grad(args, 3) || vector(args[3], g_i32, q.shape[0], q.device, (const void**)&a.lengths) || a.lengths == NULL)
+    return none_clear();
+  a.seqs = (int)q.shape[0];
+  a.q_len = 1;
+  a.page = (int)k.shape[1];
+  a.num_pages = (int)k.shape[0];
+  a.k_len = a.page;
+  if (args[4] != Py_None) {
+    tensor_t t;
+    if (read_tensor(args[4], &t) || t.dtype != g_i32 || t.nd != 2 || t.shape[0] != a.seqs || t.device != q.device || t.stride[1] != 1 ||
+        t.stride[0] != t.shape[1] || t.shape[1] == 0 || !fits(t.shape[1] * a.page))
+      return none_clear();
+    a.pages = t.ptr;
+    a.max_pages = (int)t.shape[1];
+    a.k_len = a.max_pages * a.page;
+  } else if (k.shape[0] != a.seqs) {
+    Py_RETURN_NONE;
+  }
+  if (!rest_ok(args[7], args[8], args[5], args[6], args[9], q.device, q.dtype, &a)) return none_clear();
+  a.q = q.ptr, a.k = k.ptr, a.v = v.ptr;
+  a.q_seq = q.stride[0], a.q_head = q.stride[1];
+  a.k_seq = k.stride[0], a.k_token = k.stride[1], a.k_head = k.stride[2];
+  a.v_seq = v.stride[0], a.v_token = v.stride[1], a.v_head = v.stride[2];
+  return run_attention(args[0], q.device, &a, 1);
+}
+
+typedef int (*plan_fn)(int, int, int, int);
+typedef size_t (*plan_size_fn)(int, int, int, int);
+typedef size_t (*lora_size_fn)(const g16_lora_args*);
+typedef int (*lora_fn)(const g16_lora_args*, void*);
+static plan_fn g_skinny_plan;
+static plan_size_fn g_skinny_partials, g_skinny_counters;
+static lora_size_fn g_lora_size;
+static lora_fn g_lora_shrink, g_lora_expand;
+static PyObject *g_split = NULL, *s_dtype_names = NULL;
+
+static int packed_rows(const tensor_t* t, PyObject* dtype, int nd, int device) {
+  int64_t step = 1;
+  if (t->nd != nd || t->dtype != dtype || t->device != device || !aligned(t->ptr)) return 0;
+  for (int i = nd - 1; i >= 0; --i) {
+    if (t->shape[i] <= 0 || !fits(t->shape[i]) || (t->shape[i] > 1 && t->stride[i] != step)) return 0;
+    step *= t->shape[i];
+  }
+  return 1;
+}
+
+static PyObject* new_matrix(PyObject* like, int64_t M, int64_t N, PyObject* dtype) {
+  PyObject* shape = Py_BuildValue("(LL)", (long long)M, (long long)N);
+  if (shape == NULL) return NULL;
+  PyObject* argv[3] = {like, shape, dtype};
+  PyObject* r = PyObject_VectorcallMethod(s_new_empty, argv, 2, s_dtype_names);
+  Py_DECREF(shape);
+  return r;
+}
+
+/* lora_mm_t(x2d, w_t, down, up, index, scale, bias, out_dtype) of up to 8 rows */
+static PyObject* fast_lora_mm_t(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  tensor_t x, w, down, up, t;
+  g16_lora_args a;
+  const void* bias;
+  void *stream, *ws[2] = {NULL, NULL};
+  size_t ws_bytes[2] = {0, 0};
+  PyObject *y = NULL, *out = NULL;
+  int st;
+  if (check_nargs("lora_mm_t", nargs, 8)) return NULL;
+  if (g_ready == NULL) Py_RETURN_NONE;
+  memset(&a, 0, sizeof(a));
+  if (read_tensor(args[0], &x) || x.nd != 2 || x.shape[0] > G16_SKINNY_MAX_M || (x.dtype != g_f16 && x.dtype != g_f32) ||
+      !packed_rows(&x, x.dtype, 2, x.device) || (a.num_cus = device_cus(x.device)) <= 0 || read_tensor(args[1], &w) ||
+      !packed_rows(&w, g_f16, 2, x.device) || w.shape[0] != x.shape[1] || w.shape[0] % 8 != 0 || w.shape[1] % 8 != 0 ||
+      read_tensor(args[2], &down) || !packed_rows(&down, g_f16, 3, x.device) || read_tensor(args[3], &up) ||
+      !packed_rows(&up, g_f16, 3, x.device) || down.shape[2] != w.shape[0] || up.shape[1] != w.shape[1] || up.shape[0] != down.shape[0] ||
+      up.shape[2] != down.shape[1] || down.shape[1] % 8 != 0 || down.shape[1] > G16_LORA_MAX_RANK ||
+      vector(args[4], g_i32, x.shape[0], x.device, (const void**)&a.index) || a.index == NULL ||
+      vector(args[5], g_f32, down.shape[0], x.device, (const void**)&a.scale) || vector(args[6], g_f32, w.shape[1], x.device, &bias) ||
+      !aligned(bias) || (args[7] != g_f16 && args[7] != g_f32) || wants_grad(args, 4) || raw_stream(x.device, &stream))
+    return none_clear();
+  a.M = (int)x.shape[0], a.K = (int)w.shape[0], a.N = (int)w.shape[1];
+  a.adapters = (int)down.shape[0], a.rank = (int)down.shape[1];
+  a.x_is_f32 = x.dtype == g_f32, a.out_is_f16 = args[7] == g_f16;
+  a.x = x.ptr, a.down = down.ptr, a.up = up.ptr;
+  const int ksplit = g_skinny_plan(a.M, a.N, a.K, a.num_cus);
+  const size_t pb = g_skinny_partials(a.M, a.N, a.K, ksplit), cb = g_skinny_counters(a.M, a.N, a.K, ksplit);
+  if (pb > 0 || cb > 0) {
+    PyObject* r = PyObject_CallFunction(g_split, "iKnn", x.device, (unsigned long long)(uintptr_t)stream, (Py_ssize_t)pb, (Py_ssize_t)cb);
+    const int bad = r == NULL || !PyTuple_Check(r) || PyTuple_GET_SIZE(r) != 4 || as_ptr(PyTuple_GET_ITEM(r, 0), &ws[0]) ||
+                    as_size(PyTuple_GET_ITEM(r, 1), &ws_bytes[0]) || as_ptr(PyTuple_GET_ITEM(r, 2), &ws[1]) ||
+                    as_size(PyTuple_GET_ITEM(r, 3), &ws_bytes[1]);
+    Py_XDECREF(r);
+    if (bad) return none_clear();
+  }
+  y = new_matrix(args[0], a.M, a.N, g_f32);
+  out = y == NULL ? NULL : (a.out_is_f16 ? new_matrix(args[0], a.M, a.N, g_f16) : Py_NewRef(y));
+  if (out == NULL || read_tensor(y, &t)) goto no;
+  a.y = t.ptr;
+  if (read_tensor(out, &t)) goto no;
+  a.out = t.ptr;
+  const size_t bytes = g_lora_size(&a);
+  if (bytes > 0 && (scratch(x.device, stream, bytes, &a.workspace) || a.workspace == NULL)) goto no;
+  a.workspace_bytes = (int64_t)bytes;
+  Py_BEGIN_ALLOW_THREADS
+  st = g_skinny(x.ptr, a.x_is_f32, w.ptr, t.ptr == a.y ? t.ptr : (void*)a.y, 0, bias, a.M, a.N, a.K, ksplit, ws[0], ws_bytes[0], ws[1],
+                ws_bytes[1], stream);
+  if (st == 0 && bytes > 0) st = g_lora_shrink(&a, stream);
+  if (st == 0) st = g_lora_expand(&a, stream);
+  Py_END_ALLOW_THREADS
+  if (st != 0) goto no;
+  Py_DECREF(y);
+  return out;
+no:
+  Py_XDECREF(y);
+  Py_XDECREF(out);
+  return none_clear();
+}
+
+/* bind_torch(float16, float32, int32, raw_stream(device), is_grad_enabled(), ready(device) -> compute units or
+ * -1, scratch(device, stream, bytes) -> pointer, split_buffers(device, stream, partial bytes, counter bytes),
+ * [addresses of g16_attention_workspace_bytes, g16_attention, g16_attention_decode_workspace_bytes,
+ * g16_attention_decode, g16_skinny_plan, g16_skinny_workspace_bytes, g16_skinny_counter_bytes,
+ * g16_lora_workspace_bytes, g16_lora_shrink, g16_lora_expand]) */
+static PyObject* fast_bind_torch(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  void* fn[10];
+  if (check_nargs("bind_torch", nargs, 9)) return NULL;
+  for (int i = 0; i < 10; ++i) {
+    PyObject* o = PySequence_GetItem(args[8], i);
+    const int bad = o == NULL || as_ptr(o, &fn[i]) || check_bound(fn[i]);
+    Py_XDECREF(o);
+    if (bad) return NULL;
+  }
+  for (int i = 0; i < 2; ++i) {
+    g_attention_size[i] = (attention_size_fn)fn[2 * i];
+    g_attention[i] = (attention_fn)fn[2 * i + 1];
+  }
+  g_skinny_plan = (plan_fn)fn[4];
+  g_skinny_partials = (plan_size_fn)fn[5];
+  g_skinny_counters = (plan_size_fn)fn[6];
+  g_lora_size = (lora_size_fn)fn[7];
+  g_lora_shrink = (lora_fn)fn[8];
+  g_lora_expand = (lora_fn)fn[9];
+  PyObject** to[8] = {&g_f16, &g_f32, &g_i32, &g_raw_stream, &g_grad_enabled, &g_ready, &g_scratch, &g_split};
+  for (int i = 0; i < 8; ++i) {
+    Py_INCREF(args[i]);
+    Py_XSETREF(*to[i], args[i]);
+  }
+  memset(g_device_cus, 0, sizeof(g_device_cus));
+  Py_RETURN_NONE;
+}
+
 static PyMethodDef fast_methods[] = {
     {"bind", (PyCFunction)(void (*)(void))fast_bind, METH_FASTCALL,
      "bind(skinny_f32in_addr, mm_t_gemm_addr, skinny_strips_f32in_addr, skinny_addr, skinny_strips_addr)"},
@@ -243,6 +662,13 @@ static PyMethodDef fast_methods[] = {
      "g16_skinny_f32in with fast argument parsing; returns its status"},
     {"mm_t_gemm", (PyCFunction)(void (*)(void))fast_mm_t_gemm, METH_FASTCALL,
      "g16_mm_t_gemm with fast argument parsing; returns its status"},
+    {"bind_torch", (PyCFunction)(void (*)(void))fast_bind_torch, METH_FASTCALL, "torch's types and the callbacks of the calls below"},
+    {"attention", (PyCFunction)(void (*)(void))fast_attention, METH_FASTCALL,
+     "attention for arguments that need no copy; None for any others"},
+    {"attention_decode", (PyCFunction)(void (*)(void))fast_attention_decode, METH_FASTCALL,
+     "attention_decode for arguments that need no copy; None for any others"},
+    {"lora_mm_t", (PyCFunction)(void (*)(void))fast_lora_mm_t, METH_FASTCALL,
+     "lora_mm_t of up to 8 rows for arguments that need no copy; None for any others"},
     {"args_size", (PyCFunction)(void (*)(void))fast_args_size, METH_FASTCALL,
      "a *_workspace_bytes entry point, by address, on a struct of arguments; returns its size"},
     {"args_call", (PyCFunction)(void (*)(void))fast_args_call, METH_FASTCALL,
@@ -253,4 +679,14 @@ static PyMethodDef fast_methods[] = {
 static struct PyModuleDef fast_module = {PyModuleDef_HEAD_INIT, "_g16fast", NULL, -1, fast_methods,
                                          NULL, NULL, NULL, NULL};
 
-PyMODINIT_FUNC PyInit__g16fast(void) { return PyModule_Create(&fast_module); }
+PyMODINIT_FUNC PyInit__g16fast(void) {
+  s_dtype = PyUnicode_InternFromString("dtype");
+  s_shape = PyUnicode_InternFromString("shape");
+  s_stride = PyUnicode_InternFromString("stride");
+  s_data_ptr = PyUnicode_InternFromString("data_ptr");
+  s_get_device = PyUnicode_InternFromString("get_device");
+  s_requires_grad = PyUnicode_InternFromString("requires_grad");
+  s_new_empty = PyUnicode_InternFromString("new_empty");
+  s_dtype_names = PyTuple_Pack(1, s_dtype);
+  return PyModule_Create(&fast_module);
+}

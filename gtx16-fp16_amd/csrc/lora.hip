@@ -267,27 +267,12 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(Params p) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int m0 = blockIdx.x * kRows, q = lane >> 4, row = m0 + (lane & 15);
   const Adapters t = adapters_of(p, m0);
-  if constexpr (FUSED) {
-    const int steps = ceil_div(p.K, 32), groups = groups_for(t.count), parts = kWaves / groups, at = wave % parts;
-    float4v low[RB] = {};
-    shrink_steps<T, RB>(p, m0, t, wave / parts, groups, steps * at / parts, steps * (at + 1) / parts, low);
-#pragma unroll
-    for (int b = 0; b < RB; ++b) part[wave][b][lane] = low[b];
-    __syncthreads();
-    for (int i = tid; i < RB * kWave; i += kThreads) {
-      float4v v = part[0][i / kWave][i % kWave];
-#pragma unroll
-      for (int w = 1; w < kWaves; ++w) v += part[w][i / kWave][i % kWave];
-      part[0][i / kWave][i % kWave] = v;
-    }
-    __syncthreads();
-  }
   // The pairs: rows without an adapter count as one more (number t.count) where y has to be copied.
   const int n_first = static_cast<int>(blockIdx.y) * p.chunks * 64, runs = min(p.chunks, ceil_div(p.N - n_first, 64));
   const bool copy = p.y != p.out && __ballot(t.mine < 0 && row < p.M) != 0;
   const int pairs = (t.count + (copy ? 1 : 0)) * runs;
   const int waves = kWaves * gridDim.z, w = wave + kWaves * blockIdx.z, p0 = pairs * w / waves, p1 = pairs * (w + 1) / waves;
-  if (p0 >= p1) return;
+  if (!FUSED && p0 >= p1) return;
   float(*scr)[kScrRow] = scratch[wave];
   half8 hi[RC], lo[RC];
   float back = 1.f;
@@ -359,7 +344,22 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(Params p) {
       lo[c] = __builtin_convertvector(v - widen(hi[c]), half8);
     }
   };
-  load(p0);
+  if (p0 < p1) load(p0);
+  if constexpr (FUSED) {
+    const int steps = ceil_div(p.K, 32), groups = groups_for(t.count), parts = kWaves / groups, at = wave % parts;
+    float4v low[RB] = {};
+    shrink_steps<T, RB>(p, m0, t, wave / parts, groups, steps * at / parts, steps * (at + 1) / parts, low);
+#pragma unroll
+    for (int b = 0; b < RB; ++b) part[wave][b][lane] = low[b];
+    __syncthreads();
+    for (int i = tid; i < RB * kWave; i += kThreads) {
+      float4v v = part[0][i / kWave][i % kWave];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) v += part[w][i / kWave][i % kWave];
+      part[0][i / kWave][i % kWave] = v;
+    }
+    __syncthreads();
+  }
   for (int pair = p0; pair < p1; ++pair) {
     const int which = pair / runs, n = n_first + (pair % runs) * 64;
     if (which != at) {

@@ -11,6 +11,7 @@ import struct
 import torch
 
 from . import _clib
+from .direct import direct
 from .kernels import scratch_buffer, stream_handle
 from .ops import _is_target, _sm_count
 
@@ -133,6 +134,9 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_offsets: t
     Scores are ``scale * q.k`` (scale: 1 / sqrt(d)), then ``softcap * tanh(score / softcap)`` if softcap is not 0,
     then less ``slopes[head]`` (fp32) times the distance of the two positions. Returns q's shape and type,
     contiguous. Scores, softmax and sums are fp32; with fp16 inputs the weights are rounded to fp16."""
+    out = direct().attention(q, k, v, q_offsets, k_offsets, causal, visible, shared_k, shared_v, scale, softcap, slopes)
+    if out is not None:
+        return out
     packed = q_offsets is not None
     if q.dim() != (3 if packed else 4) or k.dim() != q.dim() or v.dim() != q.dim():
         raise ValueError("attention: q, k and v must be [rows, heads, d] with q_offsets, [sequences, tokens, heads, d] without")
@@ -188,6 +192,9 @@ def attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     it holds, and a page number outside the cache reads as zeros. ``shared_k`` and ``shared_v`` [prefix, key heads, d]
     come before every request's own keys. The token stands at its last key's position. Types, heads, scores
     and the result are ``attention``'s; a request without any key gives zeros."""
+    out = direct().attention_decode(q, k_cache, v_cache, lengths, pages, shared_k, shared_v, scale, softcap, slopes)
+    if out is not None:
+        return out
     if q.dim() != 3 or k_cache.dim() != 4 or v_cache.dim() != 4 or lengths.dim() != 1:
         raise ValueError("attention_decode: q must be [requests, heads, d], the caches have four dimensions, lengths one")
     seqs, hq, d = q.shape

@@ -10,6 +10,7 @@ import struct
 import torch
 
 from . import _clib
+from .direct import direct
 from .kernels import scratch_buffer, stream_handle
 from .ops import _aligned, _sm_count, mm_t
 
@@ -52,6 +53,9 @@ def lora_mm_t(x2d: torch.Tensor, w_t: torch.Tensor, down: torch.Tensor, up: torc
     negative (or past the last adapter) for none; scale fp32 [adapters] or None. x2d, w_t, bias and out_dtype
     are mm_t's, and so is the shared product, rounding of fp32 activations included; the adapters' part is
     computed from the activations as they are, in fp32, and added before the one rounding to out_dtype."""
+    out = direct().lora_mm_t(x2d, w_t, down, up, index, scale, bias, out_dtype)
+    if out is not None:
+        return out
     if out_dtype not in (torch.float32, torch.float16):
         raise ValueError(f"out_dtype must be float32 or float16, got {out_dtype}")
     _check(x2d, w_t, down, up, index, scale)
