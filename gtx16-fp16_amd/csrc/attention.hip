@@ -15,8 +15,13 @@
 //     than 2^kLag above it (the weights grow to at most 2^(kShift + kLag), far inside fp16), which after
 //     the first tiles spares almost every rescale of O. Weights are computed 2^kShift above their value,
 //     which keeps those far below the maximum out of fp16's subnormals.
-//   * fp32 inputs run the same code on v_mfma_f32_32x32x2_f32, eight of them where fp16 has one 32x32x16:
-//     the lanes' eight values per step are the same, only their order along the sum differs.
+//   * fp32 values are multiplied as two fp16 parts each, to 2^-22 of the value: three products (that of the two
+//     small parts is below it) of 32 cycles where eight v_mfma_f32_32x32x2_f32 take 512 for the same step. The
+//     small part of a key or value is kept 2^11 above its size, that of its large part, so that it stays
+//     out of fp16's subnormals, and meets the other side 2^11 below it. Query rows are scaled by a power of two
+//     to 2^13 .. 2^14 first. Keys and values have to lie in fp16's range, and a tile's largest be at least
+//     2^-10 (a value is exact to 2^-36); a tile where that does not hold, which every wavefront sees from the
+//     part it loaded, takes the fp32 instructions. Weights, 0 .. 2^15, always fit.
 //   * Keys arrive by DMA into LDS with the row swizzles of Tile. A tile that ends past its sequence is cut
 //     off by the buffer descriptor's range, which writes zeros: no value from behind a sequence's end
 //     reaches a product.
@@ -57,6 +62,45 @@ __device__ inline float16v mma(float8v a, float8v b, float16v c) {
   for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
   return c;
 }
+
+// fp32 as two fp16 parts: hi + lo for what is multiplied from the right, hi + 2^-11 lo from the left (Left8).
+struct Split8 {
+  half8 hi, lo;
+};
+struct Left8 : Split8 {};
+__device__ inline float8v widen(half8 h) { return __builtin_convertvector(h, float8v); }
+__device__ inline Split8 split(float8v v) {
+  const half8 hi = __builtin_convertvector(v, half8);
+  float8v rest;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) rest[j] = fmaf(static_cast<float>(hi[j]), -1.f, v[j]);  // one mixed-precision instruction
+  return Split8{hi, __builtin_convertvector(rest, half8)};
+}
+__device__ inline float16v mma(const Left8& a, const Split8& b, float16v c) {
+  c = mma(a.hi, b.hi, c);
+  c = mma(a.hi, b.lo, c);
+  return mma(a.lo, b.hi * static_cast<_Float16>(0x1p-11f), c);
+}
+// What becomes of 8 values that are multiplied: fp16 as it is, fp32 in parts.
+__device__ inline half8 left(half8 v) { return v; }
+__device__ inline half8 right(half8 v) { return v; }
+__device__ inline Left8 left(float8v v) {
+  const half8 hi = __builtin_convertvector(v, half8);
+  float8v rest;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) rest[j] = fmaf(static_cast<float>(hi[j]), -0x1p11f, v[j] * 0x1p11f);  // exact
+  return Left8{{hi, __builtin_convertvector(rest, half8)}};
+}
+__device__ inline Split8 right(float8v v) { return split(v); }
+
+// Which of a tile's values a lane has seen: whether one is past fp16's range, whether one is not small.
+struct Range {
+  float top = 0.f;
+  __device__ void see(float4v v) { top = fmaxf(fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w))); }
+  // bit 0: past, bit 1: not small, over the wavefront
+  __device__ int bits() const { return (__any(top > 65504.f) ? 1 : 0) | (__any(top >= 0x1p-10f) ? 2 : 0); }
+};
+__device__ inline bool exact_needed(int bits) { return (bits & 3) != 2; }
 
 // The value of the lane 32 away.
 __device__ inline float other_half(float v) {
@@ -255,19 +299,35 @@ __device__ inline float score_of(const Scoring& s, float x, float slope, float d
 template <typename T, int DP>
 struct Wave {
   using V8 = typename Vec8<T>::V;
-  V8 q[DP / 16];
+  decltype(right(V8{})) q[DP / 16];
   float16v o[DP / 32];
   float m, l;  // the reference maximum (log2 units) and this lane's part of the sum of weights
+  float back;  // fp32: what the scores are multiplied by for the scaling of the row (1 for fp16)
 
   __device__ void start(const Row& row, float sign, int d, int lane) {
     const int h = lane >> 5;
+V8 v[DP / 16];
 #pragma unroll
     for (int ks = 0; ks < DP / 16; ++ks) {
       const int at = 16 * ks + 8 * h;
-      V8 v = {};
-      if (row.q != nullptr && at < d) v = *reinterpret_cast<const V8*>(row.q + at * sizeof(T));
-      q[ks] = sign == 1.f ? v : v * static_cast<T>(sign);
+      v[ks] = V8{};
+      if (row.q != nullptr && at < d) v[ks] = *reinterpret_cast<const V8*>(row.q + at * sizeof(T));
     }
+    float by = sign;
+    back = 1.f;
+    if constexpr (sizeof(T) == 4) {  // the row's largest value to 2^13 .. 2^14
+      float top = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < DP / 16; ++ks)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[ks][j]));
+      top = fmaxf(top, other_half(top));
+      const int e = top > 0.f && top < __builtin_huge_valf() ? min(max(13 - ilogbf(top), -120), 120) : 0;
+      by *= ldexpf(1.f, e);
+      back = ldexpf(1.f, -e);
+    }
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks) q[ks] = right(by == 1.f ? v[ks] : v[ks] * static_cast<T>(by));
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i) o[i] = float16v{};
     m = -__builtin_huge_valf();
@@ -281,15 +341,31 @@ struct Wave {
     for (int i = 0; i < DP / 32; ++i) asm volatile("" : "+v"(o[i]));
   }
 
-  // S^T of the tile's NB blocks of 32 keys
-  template <int NB, typename TL>
+  // S^T of the tile's NB blocks of 32 keys. EXACT: fp32 keys that do not fit fp16 (see Range).
+  template <int NB, typename TL, bool EXACT>
   __device__ void products(uint32_t kt, float16v (&s)[NB]) const {
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb) {
       s[kb] = float16v{};
 #pragma unroll
-      for (int ks = 0; ks < DP / 16; ++ks) s[kb] = mma(TL::k_frag(kt, kb, ks), q[ks], s[kb]);
+      for (int ks = 0; ks < DP / 16; ++ks) {
+        if constexpr (EXACT) {
+          half8 hi = q[ks].hi;
+          asm volatile("" : "+v"(hi));  // (or the sums would be kept in registers for the whole loop)
+          s[kb] = mma(TL::k_frag(kt, kb, ks), widen(hi) + widen(q[ks].lo), s[kb]);
+        } else s[kb] = mma(left(TL::k_frag(kt, kb, ks)), q[ks], s[kb]);
+      }
     }
+  }
+  template <int NB, typename TL>
+  __device__ void products(uint32_t kt, float16v (&s)[NB], bool exact) const {
+    if constexpr (sizeof(T) == 4) {
+      if (__builtin_expect(exact, 0)) {
+        products<NB, TL, true>(kt, s);
+        return;
+      }
+    }
+    products<NB, TL, false>(kt, s);
   }
 
   // The weights of the tile's keys: positions pos0 .., `left` of them in the sequence.
@@ -297,7 +373,7 @@ struct Wave {
   __device__ void weights(float16v (&s)[NB], const Scoring& sc, const Row& row, int pos0, int left, int last_seen, int lane) {
     const int h4 = (lane >> 5) * 4;
     // t = s * c + off
-    float c = sc.c, off = 0.f;
+    float c = sizeof(T) == 4 ? sc.c * back : sc.c, off = 0.f;
     if (sc.capped) {
       if (sizeof(T) == 2 && !sc.fine) {
         // tanh(y) = 1 - 2 / (e^2y + 1): s becomes -1 / (e^2y + 1), and the rest of it joins c and off
@@ -308,10 +384,11 @@ struct Wave {
         c = 2.f * sc.cap;
         off = sc.cap;
       } else {
+        const float inv = sizeof(T) == 4 ? sc.inv * back : sc.inv;
 #pragma unroll
         for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[kb][r] = tanh_of(s[kb][r] * sc.inv);
+          for (int r = 0; r < 16; ++r) s[kb][r] = tanh_of(s[kb][r] * inv);
         c = sc.cap;
       }
     }
@@ -368,16 +445,32 @@ struct Wave {
   }
 
   // O^T += V^T P^T
-  template <int NB, typename TL>
+  template <int NB, typename TL, bool EXACT>
   __device__ void add(uint32_t vt, const float16v (&s)[NB]) {
 #pragma unroll
     for (int ks = 0; ks < 2 * NB; ++ks) {
       V8 w;
 #pragma unroll
       for (int j = 0; j < 8; ++j) w[j] = static_cast<T>(s[ks >> 1][8 * (ks & 1) + j]);
+      if constexpr (EXACT) {
 #pragma unroll
-      for (int db = 0; db < DP / 32; ++db) o[db] = mma(TL::v_frag(vt, ks, db), w, o[db]);
+        for (int db = 0; db < DP / 32; ++db) o[db] = mma(TL::v_frag(vt, ks, db), w, o[db]);
+      } else {
+        const auto wp = right(w);
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db) o[db] = mma(left(TL::v_frag(vt, ks, db)), wp, o[db]);
+      }
     }
+  }
+  template <int NB, typename TL>
+  __device__ void add(uint32_t vt, const float16v (&s)[NB], bool exact) {
+    if constexpr (sizeof(T) == 4) {
+      if (__builtin_expect(exact, 0)) {
+        add<NB, TL, true>(vt, s);
+        return;
+      }
+    }
+    add<NB, TL, false>(vt, s);
   }
 };
 
@@ -468,7 +561,7 @@ __device__ inline float inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
 // Wavefront w holds rows 32 w .. 32 w + 31. last_seen: a position up to which every valid row of this
 // wavefront sees; wave_limit: the last position that any of them sees.
 template <typename T, int DP>
-__device__ void rows_workgroup(const Params& p, char* lds, const Row& row, const KeyRuns& runs, int n0, int tbeg, int tend,
+__device__ void rows_workgroup(const Params& p, char* lds, int* ranges, const Row& row, const KeyRuns& runs, int n0, int tbeg, int tend,
                                int last_seen, int wave_limit, const Slot& slot) {
   constexpr int BN = sizeof(T) == 2 ? 64 : 32, NB = BN / 32;
   using TL = Tile<T, DP, BN>;
@@ -508,16 +601,29 @@ __device__ void rows_workgroup(const Params& p, char* lds, const Row& row, const
   for (int t = tbeg; t < tend; ++t) {
     const uint32_t buf = static_cast<uint32_t>((t - tbeg) & 1);
     wait_dma_le<0>();
+    if constexpr (sizeof(T) == 4) {  // the range of what this wavefront loaded, for all four
+      Range k, v;
+#pragma unroll
+      for (int n = 0; n < NIW; ++n) {
+        const uint32_t from = base + buf * 2 * TL::BYTES + (wave * NIW + n) * 1024 + lane * 16;
+        k.see(*lds_at<float4v>(from));
+        v.see(*lds_at<float4v>(from + TL::BYTES));
+      }
+      const int bits = k.bits() | (v.bits() << 2);
+      if (lane == 0) ranges[buf * 4 + wave] = bits;
+    }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     phase_barrier();  // tile t has arrived for every wavefront, and every one is done with tile t - 1
+    int bits = 0;
+    if constexpr (sizeof(T) == 4) bits = uniform(ranges[buf * 4] | ranges[buf * 4 + 1] | ranges[buf * 4 + 2] | ranges[buf * 4 + 3]);
     pos0 = next_pos0;
     left = next_left;
     if (t + 1 < tend) issue(t + 1, buf ^ 1);
     if (pos0 <= wave_limit) {
       float16v s[NB];
-      w.template products<NB, TL>(klane + buf * 2 * TL::BYTES, s);
+      w.template products<NB, TL>(klane + buf * 2 * TL::BYTES, s, exact_needed(bits));
       w.template weights<NB>(s, sc, row, pos0, left, last_seen, lane);
-      w.template add<NB, TL>(vlane + buf * 2 * TL::BYTES, s);
+      w.template add<NB, TL>(vlane + buf * 2 * TL::BYTES, s, exact_needed(bits >> 2));
     }
   }
   w.settle();
@@ -679,6 +785,13 @@ __device__ void keys_workgroup(const Params& p, char* lds, float* joint, const R
     }
   };
   const uint32_t klane = kl + TL::k_lane(lane), vlane = kl + TL::BYTES + TL::v_lane(lane);
+  auto exact = [&](uint32_t tile) {
+    if constexpr (sizeof(T) == 2) return false;
+    Range r;
+#pragma unroll
+    for (int n = 0; n < NI; ++n) r.see(*lds_at<float4v>(tile + n * 1024 + lane * 16));
+    return exact_needed(r.bits());
+  };
   Wave<T, DP> w;
   int t = tbeg + wave;
   if (t < tend) {
@@ -699,13 +812,13 @@ __device__ void keys_workgroup(const Params& p, char* lds, float* joint, const R
     // Waits for K, then for V: only the instructions issued after it may be in flight (others among them only
     // make it wait longer).
     wait_dma_le<NI>();
-    w.template products<1, TL>(klane, s);
+    w.template products<1, TL>(klane, s, exact(kl));
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K has been read before the next K overwrites it
     if (more) issue(t + 4, next, false);
     w.template weights<1>(s, sc, row, pos0, left, last_seen, lane);
     if (more) wait_dma_le<NI>();
     else wait_dma_le<0>();
-    w.template add<1, TL>(vlane, s);
+    w.template add<1, TL>(vlane, s, exact(kl + TL::BYTES));
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if (more) issue(t + 4, next, true);
     next = page_of(t + 8);
@@ -866,11 +979,13 @@ __device__ inline Row prompt_row(const Params& p, const Where& w, int kv, int r,
   return row;
 }
 
+// (three workgroups of 128 rows fit a CU at 64 values a row, two at 128)
 template <typename T, int DP, bool KEYS>
-__global__ __launch_bounds__(kThreads, 2) void prompt_kernel(Params p) {
+__global__ __launch_bounds__(kThreads, !KEYS && DP == 64 ? 3 : 2) void prompt_kernel(Params p) {
   constexpr int RT = KEYS ? kKeyTile : kRowTile, BN = KEYS ? 32 : (sizeof(T) == 2 ? 64 : 32);
   __shared__ __attribute__((aligned(1024))) char lds[KEYS ? keys_lds<T, DP>() : rows_lds<T, DP>()];
   __shared__ float joint[KEYS ? 257 : 1];
+  __shared__ int ranges[8];  // fp32: of the two tiles in LDS, from each wavefront
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   int lin = blockIdx.x;
   const int kv = lin % p.hkv;
@@ -905,7 +1020,7 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_kernel(Params p) {
   if constexpr (KEYS) {
     keys_workgroup<T, DP, false>(p, lds, joint, row, runs, Pages{}, n0, tbeg, tend, last_seen, slot);
   } else {
-    rows_workgroup<T, DP>(p, lds, row, runs, n0, tbeg, tend, last_seen, wave_limit, slot);
+    rows_workgroup<T, DP>(p, lds, ranges, row, runs, n0, tbeg, tend, last_seen, wave_limit, slot);
   }
 }
 
@@ -1055,6 +1170,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(Params p) {
   constexpr int SRT = SKEYS ? kKeyTile : kRowTile, SBN = SKEYS ? 32 : (sizeof(T) == 2 ? 64 : 32);
   __shared__ __attribute__((aligned(1024))) char lds[SKEYS ? keys_lds<T, DP>() : cmax(keys_lds<T, DP>(), rows_lds<T, DP>())];
   __shared__ float joint[257];
+  __shared__ int ranges[8];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int nshared = p.stiles * p.ssplits * p.hkv;
   auto row_of = [&](int b, int head, bool ok) {
@@ -1085,7 +1201,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(Params p) {
       keys_workgroup<T, DP, false>(p, lds, joint, row, runs, Pages{}, n, tbeg, tend, 0x7fffffff, slot);
     } else {
       const bool some = t * SRT + 32 * wave < p.seqs * p.group;  // a wavefront without rows computes nothing
-      rows_workgroup<T, DP>(p, lds, row, runs, n, tbeg, tend, 0x7fffffff, some ? 0x7fffffff : -1, slot);
+      rows_workgroup<T, DP>(p, lds, ranges, row, runs, n, tbeg, tend, 0x7fffffff, some ? 0x7fffffff : -1, slot);
     }
     return;
   }

@@ -478,7 +478,7 @@ static PyObject* fast_attention(PyObject* self, PyObject* const* args, Py_ssize_
   }
   const int64_t q_len = q.shape[q.nd - 3], k_len = k.shape[k.nd - 3];
   const int causal = PyObject_IsTrue(args[5]);
-  if (!fits(q_len) || !fits(k_len) || q_len == 0 || a.seqs == 0 || causal < 0 || (!causal && args[6] != Py_None)) return none_clear();
+  if (!fits(q_len) || !fits(k_len) || q_len == 0 || a.seqs == 0 || causal < 0) return none_clear();
   a.q_len = (int)q_len;
   a.k_len = (int)k_len;
   a.causal = causal;

@@ -129,7 +129,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_offsets: t
     ``shared_k`` and ``shared_v`` [prefix, key heads, d] every sequence's keys follow that common prefix, and
     positions count from the prefix's first. ``causal``: a row sees the keys up to its own position, and the
     first ``visible[b]`` (int32, one a sequence) in any case (a prefix mask); otherwise all keys of its
-    sequence. Rows that see no key give zeros; values a row does not see do not reach it, whatever they are.
+    sequence, whatever ``visible`` says. Rows that see no key give zeros; values a row does not see do not reach it, whatever they are.
 
     Scores are ``scale * q.k`` (scale: 1 / sqrt(d)), then ``softcap * tanh(score / softcap)`` if softcap is not 0,
     then less ``slopes[head]`` (fp32) times the distance of the two positions. Returns q's shape and type,
@@ -155,8 +155,6 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_offsets: t
             raise ValueError("attention: k and v must have q's sequences, and offsets come with packed tensors")
         seqs = q.shape[0]
     if visible is not None:
-        if not causal:
-            raise ValueError("attention: visible widens a causal mask")
         visible = _ints("attention", visible, (seqs,), dev, "visible")
     scale, softcap = _numbers("attention", scale, softcap, d)
     slopes = _slopes("attention", slopes, hq, dev)

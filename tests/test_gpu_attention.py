@@ -93,6 +93,10 @@ def test_prefix_mask(cuda, dtype, visible, shared):
     run_prompts(cuda, [100, 130], [100, 135], 2, 1, 64, dtype, shared=shared, causal=True, visible=visible)
 
 
+def test_prefix_mask_without_a_causal_one_hides_nothing(cuda):
+    run_prompts(cuda, [40, 50], [40, 55], 2, 1, 64, F16, visible=[3, 7])
+
+
 @pytest.mark.parametrize("dtype", [F16, F32])
 @pytest.mark.parametrize("softcap", [0.0, 1.0, 30.0])
 @pytest.mark.parametrize("slopes", [False, True])
@@ -194,6 +198,19 @@ def test_wide_ranges_of_scores(cuda):
             a, b, c = (t.to(dtype) for t in (q, k, v))
             y = g.attention(a.to(cuda), b.to(cuda), c.to(cuda), q_offsets=offsets([40]).to(cuda), k_offsets=offsets([333]).to(cuda))
             check(y, prompts(a, b, c, [40], [333]), f"{dtype} {order}")
+
+
+@pytest.mark.parametrize("k_scale,v_scale", [(1e-6, 1.0), (1.0, 1e-6), (1e6, 1.0), (1.0, 1e6), (1e-30, 1e30), (1e6, 1e-12), (300.0, 1e-3)])
+@pytest.mark.parametrize("rows", [20, 140])
+def test_fp32_values_of_all_sizes(cuda, k_scale, v_scale, rows):
+    # past fp16's range and far below it: the tiles that need them take the fp32 instructions
+    gen = torch.Generator().manual_seed(17)
+    q = normal(gen, rows, 2, 64, dtype=F32, scale=1 / max(k_scale, 1e-6))
+    k, v = normal(gen, 150, 1, 64, dtype=F32, scale=k_scale), normal(gen, 150, 1, 64, dtype=F32, scale=v_scale)
+    k[70:80] *= 7.0
+    y = g.attention(q.to(cuda), k.to(cuda), v.to(cuda), q_offsets=offsets([rows]).to(cuda), k_offsets=offsets([150]).to(cuda))
+    out, tol = prompts(q, k, v, [rows], [150])
+    check(y, (out, tol + 2.0 ** -36 * min(v_scale, 1.0) * (v_scale >= 2.0 ** -12)))
 
 
 def test_offsets_outside_the_tensors_are_held_to_them(cuda):
@@ -383,7 +400,7 @@ def test_refusals(cuda):
         lambda: g.attention(p, pk, pk, q_offsets=off.cpu()),
         lambda: g.attention(p, pk, pk, q_offsets=off, k_offsets=off[:2]),
         lambda: g.attention(q, k, k, k_offsets=off),
-        lambda: g.attention(q, k, k, visible=n),
+        lambda: g.attention(q, k, k, visible=n.long()),
         lambda: g.attention(q, k, k, causal=True, visible=n[:1]),
         lambda: g.attention(q, k, k, shared_k=pk),
         lambda: g.attention(q, k, k, shared_k=pk, shared_v=pk[:3]),
