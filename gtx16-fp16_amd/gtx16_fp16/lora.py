@@ -1,7 +1,7 @@
 """Low-rank adapters of many requests beside one linear layer's product (``lora_mm_t``).
 
 No counterpart in the reference; arguments and checks follow ``mm_t``. The kernels are those of
-``csrc/lora.hip``.
+``csrc/lora.hip``; ``AdapterLinear`` is a ``FastLinear`` with adapters of its own.
 """
 from __future__ import annotations
 
@@ -12,6 +12,7 @@ import torch
 from . import _clib
 from .direct import direct
 from .kernels import scratch_buffer, stream_handle
+from .linear import FastLinear
 from .ops import _aligned, _sm_count, mm_t
 
 MAX_RANK = 128  # G16_LORA_MAX_RANK
@@ -85,6 +86,47 @@ def lora_mm_t(x2d: torch.Tensor, w_t: torch.Tensor, down: torch.Tensor, up: torc
         if status != 0:
             _clib.check(status, "adapters")
     return out
+
+
+class AdapterLinear(FastLinear):
+    """A ``FastLinear`` with ``adapters`` low-rank adapters beside its weight, one of them, or none, for each
+    row: ``layer(x, index)`` with index as in ``lora_mm_t``, one value for each row of x (all leading
+    dimensions flattened, in their order); ``layer(x)`` is the FastLinear.
+
+    State: FastLinear's ``weight_t`` and ``bias``, and ``down`` [adapters, rank, in_features], ``up`` [adapters,
+    out_features, rank] in fp16, ``scale`` [adapters] in fp32. A new layer's adapters change nothing (``up`` is
+    zero)."""
+
+    def __init__(self, in_features: int, out_features: int, adapters: int, rank: int, bias: bool = True, device=None):
+        super().__init__(in_features, out_features, bias, device)
+        if rank % 8 or not 0 < rank <= MAX_RANK:
+            raise ValueError(f"AdapterLinear: the rank must be a multiple of 8 up to {MAX_RANK}, got {rank}")
+        self.register_buffer("down", torch.zeros(adapters, rank, in_features, dtype=torch.float16, device=device))
+        self.register_buffer("up", torch.zeros(adapters, out_features, rank, dtype=torch.float16, device=device))
+        self.register_buffer("scale", torch.ones(adapters, dtype=torch.float32, device=device))
+
+    @classmethod
+    def from_fast(cls, layer: FastLinear, adapters: int, rank: int) -> "AdapterLinear":
+        """``layer``'s own weight and bias (not copies) with ``adapters`` new adapters beside them."""
+        m = cls(layer.in_features, layer.out_features, adapters, rank, layer.bias is not None, device="meta")
+        dev = layer.weight_t.device
+        m.weight_t, m.bias = layer.weight_t, layer.bias
+        m.down = torch.zeros(m.down.shape, dtype=torch.float16, device=dev)
+        m.up = torch.zeros(m.up.shape, dtype=torch.float16, device=dev)
+        m.scale = torch.ones(adapters, dtype=torch.float32, device=dev)
+        return m
+
+    def forward(self, x: torch.Tensor, index: torch.Tensor | None = None) -> torch.Tensor:
+        if index is None:
+            return super().forward(x)
+        dtype = x.dtype if x.dtype in (torch.float16, torch.float32) else torch.float32
+        x2 = x.reshape(-1, self.in_features)
+        y = lora_mm_t(x2 if x2.dtype == dtype else x2.float(), self.weight_t, self.down, self.up, index.reshape(-1), scale=self.scale,
+                      bias=self.bias, out_dtype=dtype)
+        return y.view(*x.shape[:-1], self.out_features)
+
+    def extra_repr(self) -> str:
+        return f"{super().extra_repr()}, adapters={self.down.shape[0]}, rank={self.down.shape[1]}"
 
 
 _entry: tuple[int, ...] = ()
