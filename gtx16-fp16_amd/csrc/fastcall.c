@@ -525,15 +525,11 @@ static PyObject* fast_attention_decode(PyObject* self, PyObject* const* args, Py
   return run_attention(args[0], q.device, &a, 1);
 }
 
-typedef int (*plan_fn)(int, int, int, int);
-typedef size_t (*plan_size_fn)(int, int, int, int);
 typedef size_t (*lora_size_fn)(const g16_lora_args*);
 typedef int (*lora_fn)(const g16_lora_args*, void*);
-static plan_fn g_skinny_plan;
-static plan_size_fn g_skinny_partials, g_skinny_counters;
 static lora_size_fn g_lora_size;
 static lora_fn g_lora_shrink, g_lora_expand;
-static PyObject *g_split = NULL, *s_dtype_names = NULL;
+static PyObject* s_dtype_names = NULL;
 
 static int packed_rows(const tensor_t* t, PyObject* dtype, int nd, int device) {
   int64_t step = 1;
@@ -554,20 +550,60 @@ static PyObject* new_matrix(PyObject* like, int64_t M, int64_t N, PyObject* dtyp
   return r;
 }
 
-/* lora_mm_t(x2d, w_t, down, up, index, scale, bias, out_dtype) of up to 8 rows */
+typedef int (*raw_fn)(const void*, const void*, int, void*, int, const void*, int, int, int, int, void*);
+typedef int (*direct_fn)(const void*, const void*, int, void*, int, const void*, float, int, int, int, int, void*);
+static raw_fn g_mm_t_raw;
+static direct_fn g_mm_t_direct;
+static PyObject* g_route = NULL;
+
+/* The shared product as mm_t makes it, fp32 out */
+typedef struct {
+  int kind, ksplit; /* 0: skinny, 1: mm_t_gemm, 2: one launch that reads x itself */
+  double thresh;
+  void* ptr[3]; /* scratch, partials, counters */
+  size_t bytes[3];
+} product_t;
+
+/* g_route(device, stream, M, N, K, x is fp32) -> (kind, ksplit, threshold, scratch, bytes, partials, bytes, counters,
+ * bytes), or None where a buffer is not kept between calls */
+static int product_route(int device, void* stream, const g16_lora_args* a, product_t* p) {
+  PyObject* r = PyObject_CallFunction(g_route, "iKiiii", device, (unsigned long long)(uintptr_t)stream, a->M, a->N, a->K, a->x_is_f32);
+  int bad = r == NULL || !PyTuple_Check(r) || PyTuple_GET_SIZE(r) != 9 || as_int(PyTuple_GET_ITEM(r, 0), &p->kind) ||
+            as_int(PyTuple_GET_ITEM(r, 1), &p->ksplit);
+  if (!bad) {
+    p->thresh = PyFloat_AsDouble(PyTuple_GET_ITEM(r, 2));
+    for (int i = 0; i < 3; ++i)
+      bad = bad || as_ptr(PyTuple_GET_ITEM(r, 3 + 2 * i), &p->ptr[i]) || as_size(PyTuple_GET_ITEM(r, 4 + 2 * i), &p->bytes[i]);
+  }
+  Py_XDECREF(r);
+  return bad || PyErr_Occurred() ? -1 : 0;
+}
+
+static int run_product(const product_t* p, const g16_lora_args* a, const void* w, const void* bias, void* stream) {
+  void* y = (void*)a->y;
+  if (p->kind == 0)
+    return g_skinny(a->x, a->x_is_f32, w, y, 0, bias, a->M, a->N, a->K, p->ksplit, p->ptr[1], p->bytes[1], p->ptr[2], p->bytes[2], stream);
+  if (p->kind == 1)
+    return g_mm_t_gemm(a->x, a->x_is_f32, w, y, 0, bias, (float)p->thresh, a->M, a->N, a->K, a->num_cus, p->ptr[0], p->bytes[0], p->ptr[1],
+                       p->bytes[1], p->ptr[2], p->bytes[2], stream);
+  return a->x_is_f32 ? g_mm_t_direct(a->x, w, 0, y, 0, bias, (float)p->thresh, a->M, a->N, a->K, a->num_cus, stream)
+                     : g_mm_t_raw(a->x, w, 0, y, 0, bias, a->M, a->N, a->K, a->num_cus, stream);
+}
+
+/* lora_mm_t(x2d, w_t, down, up, index, scale, bias, out_dtype) */
 static PyObject* fast_lora_mm_t(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
   (void)self;
   tensor_t x, w, down, up, t;
   g16_lora_args a;
   const void* bias;
-  void *stream, *ws[2] = {NULL, NULL};
-  size_t ws_bytes[2] = {0, 0};
+  void* stream;
+  product_t product;
   PyObject *y = NULL, *out = NULL;
   int st;
   if (check_nargs("lora_mm_t", nargs, 8)) return NULL;
   if (g_ready == NULL) Py_RETURN_NONE;
   memset(&a, 0, sizeof(a));
-  if (read_tensor(args[0], &x) || x.nd != 2 || x.shape[0] > G16_SKINNY_MAX_M || (x.dtype != g_f16 && x.dtype != g_f32) ||
+  if (read_tensor(args[0], &x) || x.nd != 2 || (x.dtype != g_f16 && x.dtype != g_f32) ||
       !packed_rows(&x, x.dtype, 2, x.device) || (a.num_cus = device_cus(x.device)) <= 0 || read_tensor(args[1], &w) ||
       !packed_rows(&w, g_f16, 2, x.device) || w.shape[0] != x.shape[1] || w.shape[0] % 8 != 0 || w.shape[1] % 8 != 0 ||
       read_tensor(args[2], &down) || !packed_rows(&down, g_f16, 3, x.device) || read_tensor(args[3], &up) ||
@@ -581,16 +617,7 @@ static PyObject* fast_lora_mm_t(PyObject* self, PyObject* const* args, Py_ssize_
   a.adapters = (int)down.shape[0], a.rank = (int)down.shape[1];
   a.x_is_f32 = x.dtype == g_f32, a.out_is_f16 = args[7] == g_f16;
   a.x = x.ptr, a.down = down.ptr, a.up = up.ptr;
-  const int ksplit = g_skinny_plan(a.M, a.N, a.K, a.num_cus);
-  const size_t pb = g_skinny_partials(a.M, a.N, a.K, ksplit), cb = g_skinny_counters(a.M, a.N, a.K, ksplit);
-  if (pb > 0 || cb > 0) {
-    PyObject* r = PyObject_CallFunction(g_split, "iKnn", x.device, (unsigned long long)(uintptr_t)stream, (Py_ssize_t)pb, (Py_ssize_t)cb);
-    const int bad = r == NULL || !PyTuple_Check(r) || PyTuple_GET_SIZE(r) != 4 || as_ptr(PyTuple_GET_ITEM(r, 0), &ws[0]) ||
-                    as_size(PyTuple_GET_ITEM(r, 1), &ws_bytes[0]) || as_ptr(PyTuple_GET_ITEM(r, 2), &ws[1]) ||
-                    as_size(PyTuple_GET_ITEM(r, 3), &ws_bytes[1]);
-    Py_XDECREF(r);
-    if (bad) return none_clear();
-  }
+  if (product_route(x.device, stream, &a, &product)) return none_clear();
   y = new_matrix(args[0], a.M, a.N, g_f32);
   out = y == NULL ? NULL : (a.out_is_f16 ? new_matrix(args[0], a.M, a.N, g_f16) : Py_NewRef(y));
   if (out == NULL || read_tensor(y, &t)) goto no;
@@ -601,8 +628,7 @@ static PyObject* fast_lora_mm_t(PyObject* self, PyObject* const* args, Py_ssize_
   if (bytes > 0 && (scratch(x.device, stream, bytes, &a.workspace) || a.workspace == NULL)) goto no;
   a.workspace_bytes = (int64_t)bytes;
   Py_BEGIN_ALLOW_THREADS
-  st = g_skinny(x.ptr, a.x_is_f32, w.ptr, t.ptr == a.y ? t.ptr : (void*)a.y, 0, bias, a.M, a.N, a.K, ksplit, ws[0], ws_bytes[0], ws[1],
-                ws_bytes[1], stream);
+  st = run_product(&product, &a, w.ptr, bias, stream);
   if (st == 0 && bytes > 0) st = g_lora_shrink(&a, stream);
   if (st == 0) st = g_lora_expand(&a, stream);
   Py_END_ALLOW_THREADS
@@ -616,15 +642,14 @@ no:
 }
 
 /* bind_torch(float16, float32, int32, raw_stream(device), is_grad_enabled(), ready(device) -> compute units or
- * -1, scratch(device, stream, bytes) -> pointer, split_buffers(device, stream, partial bytes, counter bytes),
- * [addresses of g16_attention_workspace_bytes, g16_attention, g16_attention_decode_workspace_bytes,
- * g16_attention_decode, g16_skinny_plan, g16_skinny_workspace_bytes, g16_skinny_counter_bytes,
- * g16_lora_workspace_bytes, g16_lora_shrink, g16_lora_expand]) */
+ * -1, scratch(device, stream, bytes) -> pointer, route (see product_route), [addresses of
+ * g16_attention_workspace_bytes, g16_attention, g16_attention_decode_workspace_bytes, g16_attention_decode,
+ * g16_mm_t_raw, g16_mm_t_direct, g16_lora_workspace_bytes, g16_lora_shrink, g16_lora_expand]) */
 static PyObject* fast_bind_torch(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
   (void)self;
-  void* fn[10];
+  void* fn[9];
   if (check_nargs("bind_torch", nargs, 9)) return NULL;
-  for (int i = 0; i < 10; ++i) {
+  for (int i = 0; i < 9; ++i) {
     PyObject* o = PySequence_GetItem(args[8], i);
     const int bad = o == NULL || as_ptr(o, &fn[i]) || check_bound(fn[i]);
     Py_XDECREF(o);
@@ -634,13 +659,12 @@ static PyObject* fast_bind_torch(PyObject* self, PyObject* const* args, Py_ssize
     g_attention_size[i] = (attention_size_fn)fn[2 * i];
     g_attention[i] = (attention_fn)fn[2 * i + 1];
   }
-  g_skinny_plan = (plan_fn)fn[4];
-  g_skinny_partials = (plan_size_fn)fn[5];
-  g_skinny_counters = (plan_size_fn)fn[6];
-  g_lora_size = (lora_size_fn)fn[7];
-  g_lora_shrink = (lora_fn)fn[8];
-  g_lora_expand = (lora_fn)fn[9];
-  PyObject** to[8] = {&g_f16, &g_f32, &g_i32, &g_raw_stream, &g_grad_enabled, &g_ready, &g_scratch, &g_split};
+  g_mm_t_raw = (raw_fn)fn[4];
+  g_mm_t_direct = (direct_fn)fn[5];
+  g_lora_size = (lora_size_fn)fn[6];
+  g_lora_shrink = (lora_fn)fn[7];
+  g_lora_expand = (lora_fn)fn[8];
+  PyObject** to[8] = {&g_f16, &g_f32, &g_i32, &g_raw_stream, &g_grad_enabled, &g_ready, &g_scratch, &g_route};
   for (int i = 0; i < 8; ++i) {
     Py_INCREF(args[i]);
     Py_XSETREF(*to[i], args[i]);
@@ -668,7 +692,7 @@ static PyMethodDef fast_methods[] = {
     {"attention_decode", (PyCFunction)(void (*)(void))fast_attention_decode, METH_FASTCALL,
      "attention_decode for arguments that need no copy; None for any others"},
     {"lora_mm_t", (PyCFunction)(void (*)(void))fast_lora_mm_t, METH_FASTCALL,
-     "lora_mm_t of up to 8 rows for arguments that need no copy; None for any others"},
+     "lora_mm_t for arguments that need no copy; None for any others"},
     {"args_size", (PyCFunction)(void (*)(void))fast_args_size, METH_FASTCALL,
      "a *_workspace_bytes entry point, by address, on a struct of arguments; returns its size"},
     {"args_call", (PyCFunction)(void (*)(void))fast_args_call, METH_FASTCALL,

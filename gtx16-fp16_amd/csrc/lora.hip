@@ -65,12 +65,14 @@ struct Params {
 // The adapters among a tile's 16 rows. mine: that of row lane % 16 (negative: none); ids: lane i, the i-th.
 struct Adapters {
   int mine, count, ids;
+  float scale;  // of `mine`
 };
 __device__ inline Adapters adapters_of(const Params& p, int m0) {
   const int lane = threadIdx.x & 63, row = m0 + (lane & 15);
   Adapters t;
   t.mine = row < p.M ? p.index[row] : -1;
   if (t.mine >= p.adapters) t.mine = -1;
+  t.scale = t.mine >= 0 && p.scale != nullptr ? p.scale[t.mine] : 1.f;
   t.ids = -1;
   t.count = 0;
   for (uint32_t left = static_cast<uint32_t>(__ballot(t.mine >= 0)) & 0xffffu; left != 0; ++t.count) {
@@ -128,7 +130,6 @@ __device__ inline void shrink_steps(const Params& p, int m0, const Adapters& t, 
 template <int RB>
 __device__ inline void store_low(const Params& p, int m0, const Adapters& t, int slot, int slots, int split, const float4v (&part)[kWaves][RB][kWave]) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const float scale = t.mine >= 0 && p.scale != nullptr ? p.scale[t.mine] : 1.f;
   uint32_t rows = 0;
   for (int i = slot; i < t.count; i += slots) rows |= static_cast<uint32_t>(__ballot(t.mine == __builtin_amdgcn_readlane(t.ids, i)));
   for (int b = wave; b < RB; b += kWaves) {
@@ -139,7 +140,7 @@ __device__ inline void store_low(const Params& p, int m0, const Adapters& t, int
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int r = 4 * (lane >> 4) + i;
-      const float sc = __shfl(scale, r);
+      const float sc = __shfl(t.scale, r);
       if (((rows >> r) & 1u) && col < p.rank) p.low[(static_cast<size_t>(split) * p.M + m0 + r) * p.rank + col] = v[i] * sc;
     }
   }
@@ -184,15 +185,16 @@ __global__ __launch_bounds__(kThreads) void shrink_tiles_kernel(Params p) {
   constexpr int kLds = S::COUNT * S::BYTES > kWaves * RB * kWave * 16 ? S::COUNT * S::BYTES : kWaves * RB * kWave * 16;
   __shared__ __attribute__((aligned(1024))) char lds[kLds];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int m0 = blockIdx.x * kRows, split = blockIdx.y;
+  const int m0 = static_cast<int>(blockIdx.x % p.tiles) * kRows, slot = blockIdx.x / p.tiles, split = blockIdx.y;
   const Adapters t = adapters_of(p, m0);
-  if (t.count == 0) return;
+  if (slot >= t.count) return;
+  const int count = (t.count - slot + p.slots - 1) / p.slots;  // this slot's adapters: slot, slot + slots, ..
   const int all = ceil_div(p.K, kChunk), c0 = static_cast<int>(static_cast<int64_t>(all) * split / p.splits),
             c1 = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / p.splits), each = c1 - c0;
   const uint32_t base = lds_base(lds);
   constexpr int XC = S::XROW / 16, DC = S::DROW / 16;  // pieces of a row
   auto issue = [&](int it) {
-    const int a = __builtin_amdgcn_readlane(t.ids, it / each), k0 = (c0 + it % each) * kChunk;
+    const int a = __builtin_amdgcn_readlane(t.ids, slot + it / each * p.slots), k0 = (c0 + it % each) * kChunk;
     const uint32_t to = base + (it % S::COUNT) * S::BYTES;
     const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc(
         const_cast<T*>(static_cast<const T*>(p.x) + static_cast<size_t>(m0) * p.K + k0), 0, 0x7fffffff, kRawBufferDword3);
@@ -211,7 +213,7 @@ __global__ __launch_bounds__(kThreads) void shrink_tiles_kernel(Params p) {
       dma16(rd, to + 16 * S::XROW + (wave * S::DI + n) * 1024, ok ? static_cast<uint32_t>(row) * p.K * 2u + c * 16 : kOob);
     }
   };
-  const int total = t.count * each, r16 = lane & 15, q = lane >> 4;
+  const int total = count * each, r16 = lane & 15, q = lane >> 4;
   for (int i = 0; i < S::COUNT - 1; ++i)
     if (i < total) issue(i);
   float4v low[RB] = {}, acc[RB] = {};
@@ -237,7 +239,7 @@ __global__ __launch_bounds__(kThreads) void shrink_tiles_kernel(Params p) {
       acc[b] = mma16(xv, as_operand(dv, T{}), acc[b]);
     }
     if ((it + 1) % each == 0) {  // an adapter is done: its rows
-      const int a = __builtin_amdgcn_readlane(t.ids, it / each);
+      const int a = __builtin_amdgcn_readlane(t.ids, slot + it / each * p.slots);
       const uint32_t rows = static_cast<uint32_t>(__ballot(t.mine == a));
 #pragma unroll
       for (int b = 0; b < RB; ++b) {
@@ -253,7 +255,7 @@ __global__ __launch_bounds__(kThreads) void shrink_tiles_kernel(Params p) {
 #pragma unroll
   for (int b = 0; b < RB; ++b) part[wave][b][lane] = low[b];
   __syncthreads();
-  store_low<RB>(p, m0, t, 0, 1, split, part);
+  store_low<RB>(p, m0, t, slot, p.slots, split, part);
 }
 
 // out = y + low @ up^T for tile blockIdx.x and p.chunks runs of 64 columns from blockIdx.y on; a wavefront takes
@@ -311,10 +313,9 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(Params p) {
       low[c] = float8v{};
       if (t.mine == a && r < p.rank) {
         if constexpr (FUSED) {
-          const float sc = p.scale != nullptr ? p.scale[a] : 1.f;
           const int rr = lane & 15;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) low[c][i] = part[0][(r + i) >> 4][((r + i) & 15) + 16 * (rr >> 2)][rr & 3] * sc;
+          for (int i = 0; i < 8; ++i) low[c][i] = part[0][(r + i) >> 4][((r + i) & 15) + 16 * (rr >> 2)][rr & 3] * t.scale;
         } else {
           const float* from = p.low + static_cast<size_t>(row) * p.rank + r;
           for (int s = 0; s < p.splits; s += 4) {  // (four splits' loads at a time)
@@ -425,13 +426,17 @@ Plan plan_of(const g16_lora_args& a) {
   p.tiles = ceil_div(a.M, kRows);
   p.fused = a.M <= kRows && static_cast<int64_t>(a.M) * a.rank * a.K <= kFusedWeights;
   p.staged = p.tiles >= kStagedTiles && a.K >= 2 * kChunk;
-  // staged: K in as many parts as make about two workgroups a CU, of at least two chunks; else an adapter a
-  // workgroup (a tile has at most 16, and there are few tiles), and up to 8 steps of K a wavefront
-  p.slots = p.staged ? 1 : (a.M < 16 ? a.M : 16);
+  // Staged: K in as many parts as make about two workgroups a CU, of at least two chunks, then the adapters a
+  // tile may have on as many as still do; else an adapter a workgroup (a tile has at most 16, and there are
+  // few tiles), and up to 8 steps of K a wavefront.
   p.splits = p.staged ? (2 * cus + p.tiles - 1) / p.tiles : ceil_div(ceil_div(a.K, 32), 8 * kWaves);
   const int most = p.staged ? (a.K / (2 * kChunk) < 4 ? a.K / (2 * kChunk) : 4) : 8;
   if (p.splits > most) p.splits = most;
   if (p.splits < 1) p.splits = 1;
+  p.slots = p.staged ? 2 * cus / (p.tiles * p.splits) : kRows;
+  if (p.slots > kRows) p.slots = kRows;
+  if (p.slots > a.M) p.slots = a.M;
+  if (p.slots < 1) p.slots = 1;
   // expand: about four workgroups a CU, of 1 to 32 runs of 64 columns, two for one run where that leaves
   // CUs without any
   const int runs = ceil_div(a.N, 64);

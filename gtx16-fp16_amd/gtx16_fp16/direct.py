@@ -9,13 +9,12 @@ from __future__ import annotations
 
 import torch
 
-from . import _clib
-from .kernels import _MAX_CACHED_SCRATCH, scratch_buffer, split_buffers
+from . import _clib, ops
+from .kernels import _MAX_CACHED_SCRATCH, SKINNY_MAX_M, scratch_buffer, split_buffers
 from .ops import _is_target, _sm_count
 
 _ENTRY_POINTS = ("g16_attention_workspace_bytes", "g16_attention", "g16_attention_decode_workspace_bytes", "g16_attention_decode",
-                 "g16_skinny_plan", "g16_skinny_workspace_bytes", "g16_skinny_counter_bytes", "g16_lora_workspace_bytes",
-                 "g16_lora_shrink", "g16_lora_expand")
+                 "g16_mm_t_raw", "g16_mm_t_direct", "g16_lora_workspace_bytes", "g16_lora_shrink", "g16_lora_expand")
 
 
 def _ready(device: int) -> int:
@@ -29,8 +28,24 @@ def _scratch_ptr(device: int, stream: int, nbytes: int) -> int:
     return scratch_buffer(torch.device("cuda", device), stream, nbytes).data_ptr()
 
 
-def _split_ptrs(device: int, stream: int, partial_bytes: int, counter_bytes: int) -> tuple:
-    return split_buffers(torch.device("cuda", device), stream, partial_bytes, counter_bytes)
+def _route(device: int, stream: int, M: int, N: int, K: int, x_is_f32: int):
+    """How mm_t makes this product, with its buffers (see ``product_route`` in csrc/fastcall.c); None where
+    it takes a buffer that is not kept between calls."""
+    dev = torch.device("cuda", device)
+    lib = _clib.load()
+    if M <= SKINNY_MAX_M:
+        ksplit, partials, counters = ops._skinny_plan(lib, M, N, K, dev)
+        return (0, ksplit, 0.0, 0, 0, *split_buffers(dev, stream, partials, counters))
+    if not x_is_f32:
+        ops._enable_history(lib, device, stream)
+    kind, scratch, ksplit, partials, counters, alone, raw, _ = ops._gemm_route(lib, M, N, K, dev)
+    if (alone and ops._direct_thresh()) if x_is_f32 else raw:
+        return 2, 1, ops.ROW_SCALE_THRESHOLD, 0, 0, 0, 0, 0, 0
+    if scratch > _MAX_CACHED_SCRATCH:
+        return None
+    ptr = scratch_buffer(dev, stream, scratch).data_ptr() if scratch else 0
+    bufs = split_buffers(dev, stream, partials, counters) if kind == "splitk" else (0, 0, 0, 0)
+    return (1, ksplit, ops.ROW_SCALE_THRESHOLD, ptr, scratch, *bufs)
 
 
 _bound = None
@@ -42,6 +57,6 @@ def direct():
     if _bound is None:
         fast = _clib.fast()
         fast.bind_torch(torch.float16, torch.float32, torch.int32, torch._C._cuda_getCurrentRawStream, torch.is_grad_enabled, _ready,
-                        _scratch_ptr, _split_ptrs, [_clib.address(n) for n in _ENTRY_POINTS])
+                        _scratch_ptr, _route, [_clib.address(n) for n in _ENTRY_POINTS])
         _bound = fast
     return _bound

@@ -128,6 +128,25 @@ def _remember(key: tuple, value: tuple) -> None:
     _routes[key] = value
 
 
+def _skinny_plan(lib, M: int, N: int, K: int, dev: torch.device) -> tuple:
+    """(ksplit, partial bytes, counter bytes) of the skinny path for this shape."""
+    key = (-M, N, K, dev.index or 0)
+    plan = _routes.get(key)
+    if plan is None:
+        ksplit = lib.g16_skinny_plan(M, N, K, _sm_count(dev))
+        plan = (ksplit, lib.g16_skinny_workspace_bytes(M, N, K, ksplit), lib.g16_skinny_counter_bytes(M, N, K, ksplit))
+        _remember(key, plan)
+    return plan
+
+
+def _enable_history(lib, index: int, stream: int) -> None:
+    # The speculation history lets a weight whose fp16 call needed a tile computed again take the
+    # two-launch route for a while; it is enabled once per device (a small pinned allocation,
+    # retried on a later call if this one is being captured into a graph).
+    if index not in _spec_history and lib.g16_mm_t_spec_history(stream) == 0:
+        _spec_history.add(index)
+
+
 def _check_operands(x2d: torch.Tensor, w_t: torch.Tensor, bias: torch.Tensor | None) -> None:
     # The reference leaves validation to supported() (ops.py:29-35, "Check supported() first"); a
     # call that skips it must still not hand the kernels a pointer they cannot read (a bias or
@@ -193,13 +212,7 @@ def mm_t(x2d: torch.Tensor, w_t: torch.Tensor, bias: torch.Tensor | None = None,
     f32 = x2d.dtype == torch.float32
     if M <= SKINNY_MAX_M:  # memory-bound path, fp32 math
         out = torch.empty(M, N, device=dev, dtype=out_dtype)
-        key = (-M, N, K, dev.index or 0)
-        plan = _routes.get(key)
-        if plan is None:
-            ksplit = lib.g16_skinny_plan(M, N, K, _sm_count(dev))
-            plan = (ksplit, lib.g16_skinny_workspace_bytes(M, N, K, ksplit),
-                    lib.g16_skinny_counter_bytes(M, N, K, ksplit))
-            _remember(key, plan)
+        plan = _skinny_plan(lib, M, N, K, dev)
         ksplit = plan[0]
         bufs = split_buffers(dev, stream, plan[1], plan[2])
         _clib.check(_clib.fast().skinny(x2d.data_ptr(), f32, w_t.data_ptr(),
@@ -214,12 +227,8 @@ def mm_t(x2d: torch.Tensor, w_t: torch.Tensor, bias: torch.Tensor | None = None,
     # fp32 rows itself (into LDS at once on the unsplit 32x128 tile with K <= 1280, step by step on the
     # other small tiles) or streams fp16 x as it is (32-, 64- and 128-row tiles: a row within the
     # threshold is its own cast).
-    # The speculation history lets a weight whose fp16 call needed a tile computed again take the
-    # two-launch route for a while; it is enabled once per device (a small pinned allocation,
-    # retried on a later call if this one is being captured into a graph).
-    if not f32 and dev.index not in _spec_history:
-        if lib.g16_mm_t_spec_history(stream) == 0:
-            _spec_history.add(dev.index)
+    if not f32:
+        _enable_history(lib, dev.index, stream)
     kind, scratch_bytes, _ks, ws_bytes, cnt_bytes, direct, raw, _pb = _gemm_route(lib, M, N, K, dev)
     out = torch.empty(M, N, device=dev, dtype=out_dtype)
     if (direct and _direct_thresh()) if f32 else raw:
