@@ -606,7 +606,7 @@ static PyObject* fast_lora_mm_t(PyObject* self, PyObject* const* args, Py_ssize_
   if (read_tensor(args[0], &x) || x.nd != 2 || (x.dtype != g_f16 && x.dtype != g_f32) ||
       !packed_rows(&x, x.dtype, 2, x.device) || (a.num_cus = device_cus(x.device)) <= 0 || read_tensor(args[1], &w) ||
       !packed_rows(&w, g_f16, 2, x.device) || w.shape[0] != x.shape[1] || w.shape[0] % 8 != 0 || w.shape[1] % 8 != 0 ||
-      read_tensor(args[2], &down) || !packed_rows(&down, g_f16, 3, x.device) || read_tensor(args[3], &up) ||
+      w.shape[0] > G16_LORA_MAX_SIDE || w.shape[1] > G16_LORA_MAX_SIDE || read_tensor(args[2], &down) || !packed_rows(&down, g_f16, 3, x.device) || read_tensor(args[3], &up) ||
       !packed_rows(&up, g_f16, 3, x.device) || down.shape[2] != w.shape[0] || up.shape[1] != w.shape[1] || up.shape[0] != down.shape[0] ||
       up.shape[2] != down.shape[1] || down.shape[1] % 8 != 0 || down.shape[1] > G16_LORA_MAX_RANK ||
       vector(args[4], g_i32, x.shape[0], x.device, (const void**)&a.index) || a.index == NULL ||

@@ -258,13 +258,173 @@ __global__ __launch_bounds__(kThreads) void shrink_tiles_kernel(Params p) {
   store_low<RB>(p, m0, t, slot, p.slots, split, part);
 }
 
-// out = y + low @ up^T for tile blockIdx.x and p.chunks runs of 64 columns from blockIdx.y on; a wavefront takes
-// a share of all (adapter, run) pairs. RC: pieces of 32 rank columns. T: of x, FUSED: low is computed here.
-constexpr int kScrRow = 68;  // floats of a row of the wavefronts' LDS: rows start 4 banks apart
-template <typename T, bool OUT_F16, int RC, bool FUSED>
-__global__ __launch_bounds__(kThreads) void expand_kernel(Params p) {
-  constexpr int RB = FUSED ? 2 * RC : 1;
-  __shared__ float4v part[FUSED ? kWaves : 1][RB][FUSED ? kWave : 1];
+// out = y + low @ up^T for 64 rows and p.chunks runs of 64 columns from blockIdx.y on. The wavefronts, and the
+// gridDim.z workgroups of the same rows and columns, share all (adapter, run) pairs; a pair's part of `up` is
+// loaded once for its rows (its fragments are 64 pieces a load, like shrink's: with 16 rows a workgroup they
+// took more time than y and the output, 4096 x 4096, rank 64: 47 us). The rows' low is summed up, scaled and
+// split once, into LDS. Bound by y and the output: 4111 x 4096, rank 32, fp16, is 101 MB in 25 us, 4 TB/s.
+// RC: pieces of 32 rank columns.
+constexpr int kScrRow = 68;   // floats of a row of the wavefronts' LDS: rows start 4 banks apart
+constexpr int kManyRows = 64;
+template <bool OUT_F16>
+__device__ inline void store4(const Params& p, size_t at, float4v v) {
+  if constexpr (OUT_F16) *reinterpret_cast<half4*>(static_cast<_Float16*>(p.out) + at) = __builtin_convertvector(v, half4);
+  else *reinterpret_cast<float4v*>(static_cast<float*>(p.out) + at) = v;
+}
+// 2^e that takes `top`, a row's largest value, to 2^14 .. 2^15 (e held to what fp32 has both ways; infinities
+// stay as they are)
+__device__ inline int exponent_for(float top) {
+  return top > 0.f && top < __builtin_huge_valf() ? min(max(14 - ilogbf(top), -120), 120) : 0;
+}
+template <bool OUT_F16, int RC>
+__global__ __launch_bounds__(kThreads, RC == 1 ? 4 : 2) void expand_kernel(Params p) {
+  constexpr int kLow = 32 * RC + 8;  // halves of a row: rows start 4 banks times an odd number apart
+  __shared__ __attribute__((aligned(16))) _Float16 s_hi[kManyRows][kLow], s_lo[kManyRows][kLow];
+  __shared__ float s_back[kManyRows];
+  __shared__ __attribute__((aligned(16))) float scratch[kWaves][kRows][kScrRow];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int m0 = blockIdx.x * kManyRows, q = lane >> 4;
+  // the adapter of row m0 + lane, and the list of all
+  int mine = m0 + lane < p.M ? p.index[m0 + lane] : -1, ids = -1, count = 0;
+  if (mine >= p.adapters) mine = -1;
+  for (uint64_t left = __ballot(mine >= 0); left != 0; ++count) {
+    const int a = __builtin_amdgcn_readlane(mine, __builtin_ctzll(left));
+    left &= ~__ballot(mine == a);
+    if (lane == count) ids = a;
+  }
+  {
+    const int r = tid >> 3, part = tid & 7;  // 8 threads a row
+    const bool some = __shfl(mine, r) >= 0;
+    float4v v[RC];
+    float top = 0.f;
+#pragma unroll
+    for (int c = 0; c < RC; ++c) {
+      const int e = 32 * c + 4 * part;
+      v[c] = float4v{0.f, 0.f, 0.f, 0.f};
+      if (some && e < p.rank) {
+        const float* from = p.low + static_cast<size_t>(m0 + r) * p.rank + e;
+        for (int s = 0; s < p.splits; s += 4) {  // (four splits' loads at a time)
+          float4v u[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            u[i] = *reinterpret_cast<const float4v*>(from + static_cast<size_t>(min(s + i, p.splits - 1)) * p.M * p.rank);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (s + i < p.splits) v[c] += u[i];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(v[c][i]));
+    }
+#pragma unroll
+    for (int i = 1; i < 8; i *= 2) top = fmaxf(top, __shfl_xor(top, i));
+    const int e = exponent_for(top);
+    const float by = ldexpf(1.f, e);
+#pragma unroll
+    for (int c = 0; c < RC; ++c) {
+      const float4v x = v[c] * by;
+      const half4 hi = __builtin_convertvector(x, half4);
+      *reinterpret_cast<half4*>(&s_hi[r][32 * c + 4 * part]) = hi;
+      *reinterpret_cast<half4*>(&s_lo[r][32 * c + 4 * part]) = __builtin_convertvector(x - __builtin_convertvector(hi, float4v), half4);
+    }
+    if (part == 0) s_back[r] = ldexpf(1.f, -e);
+  }
+  __syncthreads();
+  // The pairs: rows without an adapter count as one more (number `count`) where y has to be copied.
+  const int n_first = static_cast<int>(blockIdx.y) * p.chunks * 64, runs = min(p.chunks, ceil_div(p.N - n_first, 64));
+  const bool copy = p.y != p.out && __ballot(mine < 0 && m0 + lane < p.M) != 0;
+  const int pairs = (count + (copy ? 1 : 0)) * runs;
+  const int waves = kWaves * gridDim.z, w = wave + kWaves * blockIdx.z;
+  const int p0 = static_cast<int>(static_cast<int64_t>(pairs) * w / waves), p1 = static_cast<int>(static_cast<int64_t>(pairs) * (w + 1) / waves);
+  float(*scr)[kScrRow] = scratch[wave];
+  const int col = (lane & 15) * 4;  // y and the output: lane l holds columns col .. + 3 of rows l / 16 + 4 j
+  for (int pair = p0; pair < p1; ++pair) {
+    const int which = pair / runs, n = n_first + (pair % runs) * 64;
+    const int a = which < count ? __builtin_amdgcn_readlane(ids, which) : -1;
+    const uint64_t rows = __ballot(mine == a && m0 + lane < p.M);
+    half8 up[RC][4];
+    if (a >= 0) {
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        // (clamped: low is zero past the rank, and columns past the end are not stored)
+        const _Float16* from = p.up + (static_cast<size_t>(a) * p.N + min(n + 16 * b + (lane & 15), p.N - 1)) * p.rank;
+#pragma unroll
+        for (int c = 0; c < RC; ++c) up[c][b] = *reinterpret_cast<const half8*>(from + min(32 * c + 8 * q, p.rank - 8));
+      }
+    }
+    // The pair's rows, in order: lane k holds the k-th one's number (the others' follow), so that rows in no order
+    // at all cost a pair one tile of 16 rather than four (2000 x 2048 x 2048, rank 16, 32 adapters at random:
+    // 22 us against 38).
+    const int here = __popcll(rows);
+    const int before = static_cast<int>(__builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(rows >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(rows), 0)));
+    const int order = __builtin_amdgcn_ds_permute(4 * (((rows >> lane) & 1u) != 0 ? before : here + lane - before), lane);
+    // y and the output by buffer accesses, out of range (no load, no store) for lanes without a row or column:
+    // under a branch, the compiler could not tell how many stores are in flight and would wait for all of
+    // them wherever it waits for a load.
+    const bool inside = n + col < p.N;
+    auto base = [&](const void* m, uint32_t size) {
+      return __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<char*>(static_cast<const char*>(m)) + (static_cast<size_t>(m0) * p.N + n) * size, 0, 0x7fffffff, kRawBufferDword3);
+    };
+    const __amdgpu_buffer_rsrc_t r_y = base(p.y, 4), r_out = base(p.out, OUT_F16 ? 2 : 4);
+    uint32_t at[2][4];  // elements from there on
+    float4v y[2][4];
+    auto load_y = [&](int s) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int k = 16 * s + 4 * j + q, r = __shfl(order, k);
+        const bool ok = inside && k < here;
+        at[s & 1][j] = ok ? static_cast<uint32_t>(r) * static_cast<uint32_t>(p.N) + col : kOob;
+        y[s & 1][j] = __builtin_bit_cast(float4v, __builtin_amdgcn_raw_buffer_load_b128(r_y, static_cast<int>(ok ? at[s & 1][j] * 4 : kOob), 0, 0));
+      }
+    };
+    load_y(0);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      float4v(&v)[4] = y[s & 1];
+      if (s < 3) load_y(s + 1);
+      if (a >= 0) {
+        const int r = __shfl(order, 16 * s + (lane & 15));
+        const float back = s_back[r];
+        half8 hi[RC], lo[RC];
+#pragma unroll
+        for (int c = 0; c < RC; ++c) {
+          hi[c] = *reinterpret_cast<const half8*>(&s_hi[r][32 * c + 8 * q]);
+          lo[c] = *reinterpret_cast<const half8*>(&s_lo[r][32 * c + 8 * q]);
+        }
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          float4v acc = {};
+#pragma unroll
+          for (int c = 0; c < RC; ++c) {
+            acc = mma16(up[c][b], hi[c], acc);
+            acc = mma16(up[c][b], lo[c], acc);
+          }
+          // lane l: columns 16 b + 4 (l / 16) .. + 3 of row l % 16
+          *reinterpret_cast<float4v*>(&scr[lane & 15][16 * b + 4 * q]) = acc * back;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] += *reinterpret_cast<const float4v*>(&scr[q + 4 * j][col]);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t e = at[s & 1][j];
+        if constexpr (OUT_F16)
+          __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, __builtin_convertvector(v[j], half4)), r_out, static_cast<int>(e == kOob ? kOob : e * 2), 0, 0);
+        else
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v[j]), r_out, static_cast<int>(e == kOob ? kOob : e * 4), 0, 0);
+      }
+      if (16 * s + 16 >= here) break;
+    }
+  }
+}
+
+// Few rows whose adapters are small (one tile): low is computed here, by every workgroup for its 64 columns.
+// T: of x.
+template <typename T, bool OUT_F16, int RC>
+__global__ __launch_bounds__(kThreads) void fused_kernel(Params p) {
+  constexpr int RB = 2 * RC;
+  __shared__ float4v part[kWaves][RB][kWave];
   __shared__ __attribute__((aligned(16))) float scratch[kWaves][kRows][kScrRow];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int m0 = blockIdx.x * kRows, q = lane >> 4, row = m0 + (lane & 15);
@@ -274,7 +434,6 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(Params p) {
   const bool copy = p.y != p.out && __ballot(t.mine < 0 && row < p.M) != 0;
   const int pairs = (t.count + (copy ? 1 : 0)) * runs;
   const int waves = kWaves * gridDim.z, w = wave + kWaves * blockIdx.z, p0 = pairs * w / waves, p1 = pairs * (w + 1) / waves;
-  if (!FUSED && p0 >= p1) return;
   float(*scr)[kScrRow] = scratch[wave];
   half8 hi[RC], lo[RC];
   float back = 1.f;
@@ -312,30 +471,16 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(Params p) {
       const int r = 32 * c + 8 * q;
       low[c] = float8v{};
       if (t.mine == a && r < p.rank) {
-        if constexpr (FUSED) {
-          const int rr = lane & 15;
+        const int rr = lane & 15;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) low[c][i] = part[0][(r + i) >> 4][((r + i) & 15) + 16 * (rr >> 2)][rr & 3] * t.scale;
-        } else {
-          const float* from = p.low + static_cast<size_t>(row) * p.rank + r;
-          for (int s = 0; s < p.splits; s += 4) {  // (four splits' loads at a time)
-            float8v v[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              v[i] = *reinterpret_cast<const float8v*>(from + static_cast<size_t>(min(s + i, p.splits - 1)) * p.M * p.rank);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (s + i < p.splits) low[c] += v[i];
-          }
-        }
+        for (int i = 0; i < 8; ++i) low[c][i] = part[0][(r + i) >> 4][((r + i) & 15) + 16 * (rr >> 2)][rr & 3] * t.scale;
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(low[c][i]));
     }
     top = fmaxf(top, __shfl_xor(top, 16));
     top = fmaxf(top, __shfl_xor(top, 32));
-    // 2^e with top * 2^e in [2^14, 2^15), e held to what fp32 has both ways; infinities stay as they are
-    const int e = top > 0.f && top < __builtin_huge_valf() ? min(max(14 - ilogbf(top), -120), 120) : 0;
+    const int e = exponent_for(top);
     const float by = ldexpf(1.f, e);
     back = ldexpf(1.f, -e);
 #pragma unroll
@@ -346,7 +491,7 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(Params p) {
     }
   };
   if (p0 < p1) load(p0);
-  if constexpr (FUSED) {
+  {
     const int steps = ceil_div(p.K, 32), groups = groups_for(t.count), parts = kWaves / groups, at = wave % parts;
     float4v low[RB] = {};
     shrink_steps<T, RB>(p, m0, t, wave / parts, groups, steps * at / parts, steps * (at + 1) / parts, low);
@@ -396,9 +541,7 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(Params p) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if (!mine[j]) continue;
-      const size_t to = static_cast<size_t>(m0 + q + 4 * j) * p.N + n + col;
-      if constexpr (OUT_F16) *reinterpret_cast<half4*>(static_cast<_Float16*>(p.out) + to) = __builtin_convertvector(v[j], half4);
-      else *reinterpret_cast<float4v*>(static_cast<float*>(p.out) + to) = v[j];
+      store4<OUT_F16>(p, static_cast<size_t>(m0 + q + 4 * j) * p.N + n + col, v[j]);
     }
   }
 }
@@ -408,7 +551,7 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(Params p) {
 int check(const g16_lora_args& a) {
   if ((a.x_is_f32 | a.out_is_f16) & ~1) return G16_E_DTYPE;
   if (a.M < 0 || a.K < 0 || a.N < 0 || a.adapters < 0 || a.rank < 0 || a.K % 8 != 0 || a.N % 8 != 0 || a.rank % 8 != 0 ||
-      a.rank > G16_LORA_MAX_RANK)
+      a.rank > G16_LORA_MAX_RANK || a.K > G16_LORA_MAX_SIDE || a.N > G16_LORA_MAX_SIDE)
     return G16_E_SHAPE;
   if (a.M == 0 || a.N == 0) return G16_OK;
   if (a.x == nullptr || a.down == nullptr || a.up == nullptr || a.index == nullptr || a.y == nullptr || a.out == nullptr) return G16_E_NULL;
@@ -437,12 +580,14 @@ Plan plan_of(const g16_lora_args& a) {
   if (p.slots > kRows) p.slots = kRows;
   if (p.slots > a.M) p.slots = a.M;
   if (p.slots < 1) p.slots = 1;
-  // expand: about four workgroups a CU, of 1 to 32 runs of 64 columns, two for one run where that leaves
-  // CUs without any
-  const int runs = ceil_div(a.N, 64);
-  const int64_t each = (static_cast<int64_t>(p.tiles) * runs + 4 * cus - 1) / (4 * cus);
-  p.chunks = each < 1 ? 1 : (each > 32 ? 32 : static_cast<int>(each));
-  p.wide = a.M > kWaves && static_cast<int64_t>(p.tiles) * runs <= cus ? 2 : 1;
+  // expand: about two workgroups a CU, of 1 to 32 runs of 64 columns, several for the same rows and columns
+  // where that leaves CUs without any; fused: a run each
+  const int runs = ceil_div(a.N, 64), many = ceil_div(a.M, kManyRows);
+  const int64_t each = (static_cast<int64_t>(many) * runs + 2 * cus - 1) / (2 * cus);
+  p.chunks = p.fused || each < 1 ? 1 : (each > 32 ? 32 : static_cast<int>(each));
+  const int64_t groups = static_cast<int64_t>(many) * ceil_div(runs, p.chunks);
+  p.wide = p.fused || a.M <= kWaves || groups >= cus ? 1 : static_cast<int>(2 * cus / groups);
+  if (p.wide > 8) p.wide = 8;
   return p;
 }
 
@@ -464,12 +609,19 @@ int run_shrink(const Params& p, const Plan& plan, hipStream_t s) {
   return run_shrink_as<T, 8>(p, plan, s);
 }
 
-template <typename T, bool OUT_F16, bool FUSED>
+template <bool OUT_F16>
 int run_expand(const Params& p, const Plan& plan, hipStream_t s) {
-  const dim3 grid(plan.tiles, ceil_div(ceil_div(p.N, 64), plan.chunks), plan.wide), block(kThreads);
-  if (p.rank <= 32) return launch(expand_kernel<T, OUT_F16, 1, FUSED>, grid, block, s, p);
-  if (p.rank <= 64) return launch(expand_kernel<T, OUT_F16, 2, FUSED>, grid, block, s, p);
-  return launch(expand_kernel<T, OUT_F16, 4, FUSED>, grid, block, s, p);
+  const dim3 grid(ceil_div(p.M, kManyRows), ceil_div(ceil_div(p.N, 64), plan.chunks), plan.wide), block(kThreads);
+  if (p.rank <= 32) return launch(expand_kernel<OUT_F16, 1>, grid, block, s, p);
+  if (p.rank <= 64) return launch(expand_kernel<OUT_F16, 2>, grid, block, s, p);
+  return launch(expand_kernel<OUT_F16, 4>, grid, block, s, p);
+}
+template <typename T, bool OUT_F16>
+int run_fused(const Params& p, hipStream_t s) {
+  const dim3 grid(1, ceil_div(p.N, 64)), block(kThreads);
+  if (p.rank <= 32) return launch(fused_kernel<T, OUT_F16, 1>, grid, block, s, p);
+  if (p.rank <= 64) return launch(fused_kernel<T, OUT_F16, 2>, grid, block, s, p);
+  return launch(fused_kernel<T, OUT_F16, 4>, grid, block, s, p);
 }
 
 }  // namespace
@@ -507,7 +659,7 @@ extern "C" int g16_lora_expand(const g16_lora_args* args, void* stream) {
   if (!aligned16(args->workspace)) return G16_E_ALIGN;
   const Params p = params(*args, plan);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (!plan.fused) return args->out_is_f16 ? run_expand<_Float16, true, false>(p, plan, s) : run_expand<_Float16, false, false>(p, plan, s);
-  if (args->x_is_f32) return args->out_is_f16 ? run_expand<float, true, true>(p, plan, s) : run_expand<float, false, true>(p, plan, s);
-  return args->out_is_f16 ? run_expand<_Float16, true, true>(p, plan, s) : run_expand<_Float16, false, true>(p, plan, s);
+  if (!plan.fused) return args->out_is_f16 ? run_expand<true>(p, plan, s) : run_expand<false>(p, plan, s);
+  if (args->x_is_f32) return args->out_is_f16 ? run_fused<float, true>(p, s) : run_fused<float, false>(p, s);
+  return args->out_is_f16 ? run_fused<_Float16, true>(p, s) : run_fused<_Float16, false>(p, s);
 }

@@ -16,6 +16,7 @@ from .linear import FastLinear
 from .ops import _aligned, _sm_count, mm_t
 
 MAX_RANK = 128  # G16_LORA_MAX_RANK
+MAX_SIDE = 1 << 21  # G16_LORA_MAX_SIDE
 
 # g16_lora_args without its workspace
 _ARGS = struct.Struct("@7P8i")
@@ -35,6 +36,8 @@ def _check(x2d: torch.Tensor, w_t: torch.Tensor, down: torch.Tensor, up: torch.T
                          f"[adapters, {N}, rank]")
     if r % 8 or r > MAX_RANK:
         raise ValueError(f"lora_mm_t: the rank must be a multiple of 8 up to {MAX_RANK}, got {r}")
+    if K > MAX_SIDE or N > MAX_SIDE:
+        raise ValueError(f"lora_mm_t: K and N may be up to {MAX_SIDE}, got {K} and {N}")
     if not (index.dtype == torch.int32 and index.shape == (x2d.shape[0],) and index.device == dev):
         raise ValueError(f"lora_mm_t: index must be an int32 tensor of shape ({x2d.shape[0]},) on {dev}")
     if scale is not None and not (scale.dtype == torch.float32 and scale.shape == (n,) and scale.device == dev):

@@ -10,7 +10,7 @@ import pytest
 import torch
 
 import gtx16_fp16 as g
-from gtx16_fp16 import ops
+from gtx16_fp16 import lora, ops
 
 pytestmark = pytest.mark.gpu
 
@@ -192,3 +192,23 @@ def test_refusals(cuda):
             pytest.fail(f"{list(changes)} was taken")
     with pytest.raises(RuntimeError, match="no_grad"):
         call(x=c["x"].clone().requires_grad_())
+
+
+def test_sides_past_32_bit_offsets_are_refused(cuda):
+    n = lora.MAX_SIDE + 8
+    index = torch.zeros(1, dtype=torch.int32, device=cuda)
+
+    def zeros(*shape):
+        return torch.zeros(*shape, device=cuda, dtype=F16)
+
+    with pytest.raises(ValueError, match="up to"):
+        g.lora_mm_t(zeros(1, 8), zeros(8, n), zeros(1, 8, 8), zeros(1, n, 8), index)
+    with pytest.raises(ValueError, match="up to"):
+        g.lora_mm_t(zeros(1, n), zeros(n, 8), zeros(1, 8, n), zeros(1, 8, 8), index)
+
+
+@pytest.mark.parametrize("M,n", [(64, 2), (64, 5), (200, 3), (333, 40)])
+def test_adapters_interleaved_row_by_row(cuda, M, n):
+    c = make(M, 256, 136, 24, n)
+    c["index"] = torch.arange(M, dtype=torch.int32) % (n + 1)
+    check(cuda, c)

@@ -53,3 +53,10 @@ def test_few_rows_need_no_workspace():
 def test_workspace_holds_whole_splits(M, K, rank):
     n = size(M=M, K=K, rank=rank)
     assert n > 0 and n % (4 * M * rank) == 0
+
+
+@pytest.mark.parametrize("name", ["g16_lora_shrink", "g16_lora_expand"])
+@pytest.mark.parametrize("side", ["K", "N"])
+def test_sides_past_32_bit_offsets_are_rejected(name, side):
+    assert call(name, **{side: lora.MAX_SIDE + 8}) == SHAPE
+    assert size(**{side: lora.MAX_SIDE}) > 0
