@@ -170,7 +170,10 @@ __global__ __launch_bounds__(kThreads) void shrink_kernel(Params p) {
 }
 
 // low by way of LDS: kChunk values of K at a time, of x's 16 rows and an adapter's 16 RB rows of `down`, a
-// wavefront on 32 of them; the next chunks on their way meanwhile. 16-byte piece c of row r at c ^ r % 16.
+// wavefront on 32 of them; the next chunks on their way meanwhile. 16-byte piece c of row r at c ^ r % 16. All
+// adapters of a chunk in turn, so that x is read once (1024 x 4096, rank 16, 32 adapters at random: 24.8 us an
+// adapter at a time, 23.1 so: 142 MB, mostly of `down`, out of L2 and the Infinity Cache, which twice as many
+// steps in flight slowed down to 27).
 constexpr int kChunk = 32 * kWaves;
 template <typename T, int RB>
 struct Stage {
@@ -185,70 +188,92 @@ __global__ __launch_bounds__(kThreads) void shrink_tiles_kernel(Params p) {
   constexpr int kLds = S::COUNT * S::BYTES > kWaves * RB * kWave * 16 ? S::COUNT * S::BYTES : kWaves * RB * kWave * 16;
   __shared__ __attribute__((aligned(1024))) char lds[kLds];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int m0 = static_cast<int>(blockIdx.x % p.tiles) * kRows, slot = blockIdx.x / p.tiles, split = blockIdx.y;
+  const int lin = static_cast<int>(blockIdx.x), m0 = lin % p.tiles * kRows, slot = lin / p.tiles, split = blockIdx.y;
   const Adapters t = adapters_of(p, m0);
   if (slot >= t.count) return;
   const int count = (t.count - slot + p.slots - 1) / p.slots;  // this slot's adapters: slot, slot + slots, ..
   const int all = ceil_div(p.K, kChunk), c0 = static_cast<int>(static_cast<int64_t>(all) * split / p.splits),
-            c1 = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / p.splits), each = c1 - c0;
+            c1 = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / p.splits);
   const uint32_t base = lds_base(lds);
   constexpr int XC = S::XROW / 16, DC = S::DROW / 16;  // pieces of a row
-  auto issue = [&](int it) {
-    const int a = __builtin_amdgcn_readlane(t.ids, slot + it / each * p.slots), k0 = (c0 + it % each) * kChunk;
-    const uint32_t to = base + (it % S::COUNT) * S::BYTES;
-    const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<T*>(static_cast<const T*>(p.x) + static_cast<size_t>(m0) * p.K + k0), 0, 0x7fffffff, kRawBufferDword3);
+  // Where this lane's pieces of a chunk are, in its rows (`in`: at which value of K).
+  uint32_t x_off[S::XI], d_off[S::DI];
+  int x_in[S::XI], d_in[S::DI];
 #pragma unroll
-    for (int n = 0; n < S::XI; ++n) {
-      const int row = (wave * S::XI + n) * (64 / XC) + lane / XC, c = (lane % XC) ^ (row & 15);
-      const bool ok = m0 + row < p.M && k0 + c * static_cast<int>(16 / sizeof(T)) < p.K;
-      dma16(rx, to + (wave * S::XI + n) * 1024, ok ? static_cast<uint32_t>(row) * p.K * static_cast<uint32_t>(sizeof(T)) + c * 16 : kOob);
+  for (int n = 0; n < S::XI; ++n) {
+    const int row = (wave * S::XI + n) * (64 / XC) + lane / XC, c = (lane % XC) ^ (row & 15);
+    x_in[n] = c * static_cast<int>(16 / sizeof(T));
+    x_off[n] = m0 + row < p.M ? static_cast<uint32_t>(row) * p.K * static_cast<uint32_t>(sizeof(T)) + c * 16 : kOob;
+  }
+#pragma unroll
+  for (int n = 0; n < S::DI; ++n) {
+    const int row = (wave * S::DI + n) * (64 / DC) + lane / DC, c = (lane % DC) ^ (row & 15);
+    d_in[n] = c * 8;
+    d_off[n] = row < p.rank ? static_cast<uint32_t>(row) * p.K * 2u + c * 16 : kOob;
+  }
+  // step `it`: chunk it / count for the slot's adapter it % count, x with the chunk's first
+  int chunk = c0, which = 0, to = 0;  // of the next step to load, and its place
+  const size_t adapter = static_cast<size_t>(p.rank) * p.K;
+  auto issue = [&]() {
+    const int k0 = chunk * kChunk, left = p.K - k0;
+    const uint32_t at = base + to * S::BYTES + wave * (S::XI * 1024);
+    if (which == 0) {
+      const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<T*>(static_cast<const T*>(p.x) + static_cast<size_t>(m0) * p.K + k0), 0, 0x7fffffff, kRawBufferDword3);
+#pragma unroll
+      for (int n = 0; n < S::XI; ++n) dma16(rx, at + n * 1024, x_in[n] < left ? x_off[n] : kOob);
     }
-    const __amdgpu_buffer_rsrc_t rd = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<_Float16*>(p.down + static_cast<size_t>(a) * p.rank * p.K + k0), 0, 0x7fffffff, kRawBufferDword3);
+    const int a = __builtin_amdgcn_readlane(t.ids, slot + which * p.slots);
+    const __amdgpu_buffer_rsrc_t rd =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<_Float16*>(p.down + a * adapter + k0), 0, 0x7fffffff, kRawBufferDword3);
 #pragma unroll
-    for (int n = 0; n < S::DI; ++n) {
-      const int row = (wave * S::DI + n) * (64 / DC) + lane / DC, c = (lane % DC) ^ (row & 15);
-      const bool ok = row < p.rank && k0 + c * 8 < p.K;
-      dma16(rd, to + 16 * S::XROW + (wave * S::DI + n) * 1024, ok ? static_cast<uint32_t>(row) * p.K * 2u + c * 16 : kOob);
+    for (int n = 0; n < S::DI; ++n)
+      dma16(rd, base + to * S::BYTES + 16 * S::XROW + (wave * S::DI + n) * 1024, d_in[n] < left ? d_off[n] : kOob);
+    to = to + 1 == S::COUNT ? 0 : to + 1;
+    if (++which == count) {
+      which = 0;
+      ++chunk;
     }
   };
-  const int total = count * each, r16 = lane & 15, q = lane >> 4;
+  const int total = count * (c1 - c0), r16 = lane & 15, q = lane >> 4;
   for (int i = 0; i < S::COUNT - 1; ++i)
-    if (i < total) issue(i);
-  float4v low[RB] = {}, acc[RB] = {};
-  for (int it = 0; it < total; ++it) {
-    // chunk `it` has arrived: only the younger ones may be in flight
-    if (S::COUNT == 3 && it + 1 < total) wait_dma_le<S::XI + S::DI>();
-    else wait_dma_le<0>();
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    phase_barrier();  // ... for every wavefront, and every one has read the chunk whose place the next one takes
-    if (it + S::COUNT - 1 < total) issue(it + S::COUNT - 1);
-    const char* at = lds + (it % S::COUNT) * S::BYTES;
-    typename Vec8<T>::V xv;
-    if constexpr (sizeof(T) == 2) {
-      xv = *reinterpret_cast<const half8*>(at + r16 * S::XROW + (((wave * 4 + q) ^ r16) << 4));
+    if (i < total) issue();
+  int row_of[4];  // the adapters of rows 4 q .. 4 q + 3
+#pragma unroll
+  for (int j = 0; j < 4; ++j) row_of[j] = __shfl(t.mine, 4 * q + j);
+  float4v low[RB] = {};
+  typename Vec8<T>::V xv = {};
+  const char* at = lds;
+  for (int it = 0, now = 0; it < total; ++it, now = now + 1 == count ? 0 : now + 1) {
+    // step `it` has arrived: only the younger ones may be in flight (one with x in it is XI instructions longer)
+    if (S::COUNT == 3 && it + 1 < total) {
+      if (now + 1 == count) wait_dma_le<S::XI + S::DI>();
+      else wait_dma_le<S::DI>();
     } else {
-      const float4v a = *reinterpret_cast<const float4v*>(at + r16 * S::XROW + (((wave * 8 + 2 * q) ^ r16) << 4));
-      const float4v b = *reinterpret_cast<const float4v*>(at + r16 * S::XROW + (((wave * 8 + 2 * q + 1) ^ r16) << 4));
-      xv = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+      wait_dma_le<0>();
     }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    phase_barrier();  // ... for every wavefront, and every one has read the step whose place the next one takes
+    if (it + S::COUNT - 1 < total) issue();
+    if (now == 0) {
+      if constexpr (sizeof(T) == 2) {
+        xv = *reinterpret_cast<const half8*>(at + r16 * S::XROW + (((wave * 4 + q) ^ r16) << 4));
+      } else {
+        const float4v a = *reinterpret_cast<const float4v*>(at + r16 * S::XROW + (((wave * 8 + 2 * q) ^ r16) << 4));
+        const float4v b = *reinterpret_cast<const float4v*>(at + r16 * S::XROW + (((wave * 8 + 2 * q + 1) ^ r16) << 4));
+        xv = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+      }
+    }
+    // the adapter's rows take the new sums, the others keep theirs
+    const int a = __builtin_amdgcn_readlane(t.ids, slot + now * p.slots);
 #pragma unroll
     for (int b = 0; b < RB; ++b) {
       const half8 dv = *reinterpret_cast<const half8*>(at + 16 * S::XROW + (16 * b + r16) * S::DROW + (((wave * 4 + q) ^ r16) << 4));
-      acc[b] = mma16(xv, as_operand(dv, T{}), acc[b]);
-    }
-    if ((it + 1) % each == 0) {  // an adapter is done: its rows
-      const int a = __builtin_amdgcn_readlane(t.ids, slot + it / each * p.slots);
-      const uint32_t rows = static_cast<uint32_t>(__ballot(t.mine == a));
+      const float4v sum = mma16(xv, as_operand(dv, T{}), low[b]);
 #pragma unroll
-      for (int b = 0; b < RB; ++b) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if ((rows >> (4 * q + j)) & 1u) low[b][j] = acc[b][j];
-        acc[b] = float4v{};
-      }
+      for (int j = 0; j < 4; ++j) low[b][j] = row_of[j] == a ? sum[j] : low[b][j];
     }
+    at = at == lds + (S::COUNT - 1) * S::BYTES ? lds : at + S::BYTES;
   }
   __syncthreads();
   auto& part = *reinterpret_cast<float4v(*)[kWaves][RB][kWave]>(lds);
@@ -598,7 +623,8 @@ Params params(const g16_lora_args& a, const Plan& plan) {
 
 template <typename T, int RB>
 int run_shrink_as(const Params& p, const Plan& plan, hipStream_t s) {
-  const dim3 grid(plan.tiles * plan.slots, plan.splits), block(kThreads);
+  const dim3 block(kThreads);
+  const dim3 grid(plan.tiles * plan.slots, plan.splits);
   return plan.staged ? launch(shrink_tiles_kernel<T, RB>, grid, block, s, p) : launch(shrink_kernel<T, RB>, grid, block, s, p);
 }
 template <typename T>
