@@ -27,10 +27,10 @@
 //     reaches a product.
 // Two shapes of workgroup, both of 4 wavefronts:
 //   * rows: 128 query rows, 32 per wavefront, all on the same keys, two tiles in LDS, one barrier a tile.
-//   * keys: 32 query rows, every wavefront on its own tiles of 32 keys, joined at the end; for few rows,
-//     where the time is that of reading the keys.
+//   * keys: 32 query rows, every wavefront on its own tiles of 32 keys, joined at the end; for few rows, whose
+//     time is that of one workgroup or of reading the keys.
 // With too few tiles to fill the card, the keys are split over workgroups as well, which leave (O, maximum,
-// sum) in the workspace; a second launch joins them in split order (no atomics: repeated calls agree).
+// sum) in the workspace (prompt_time weighs shapes and splits); a second launch joins them in split order (no atomics: repeated calls agree).
 #include "g16_common.hpp"
 
 namespace g16 {
@@ -1363,13 +1363,43 @@ Params params(const g16_attention_args& a) {
 // Tiles of 32 keys that a workgroup of four wavefronts on their own keys gets at least.
 constexpr int kLeastKeys = 16;
 
-// Splits of `tiles` key tiles so that `items` workgroups become about two a CU, with at least `least` tiles
-// a split.
-int splits_for(int64_t items, int64_t tiles, int cus, int least) {
+// Splits of `tiles` key tiles so that `items` workgroups become about `many`, with at least `least` tiles a
+// split.
+int splits_for(int64_t items, int64_t tiles, int many, int least) {
   if (items <= 0 || tiles <= 0) return 1;
-  int64_t s = (2 * cus + items - 1) / items;
+  int64_t s = (many + items - 1) / items;
   if (s > tiles / least) s = tiles / least;
   return s < 1 ? 1 : static_cast<int>(s > 256 ? 256 : s);
+}
+
+// What a prompt takes in one shape and number of splits, in us. A CU gets through so many steps (tiles of 64 fp16
+// or 32 fp32 keys; 128 keys for the four wavefronts of 32 rows) in a time that two workgroups on it mostly share;
+// a split's sums go through the workspace and a second launch. Measured for this, us (causal unless said otherwise,
+// query heads on key heads): 3 x 597 tokens, 32 on 8 of 128, no mask: 35 whole, 76 in two splits; 4 x 1611, 6 on 2,
+// no mask: 60 and 82; 512, 32 on 8: 12.8 in 32 rows, 18 in 128, 31 in two splits; 2048, 8 on 2: 26 in 32 rows, 48 in
+// 128, 37 in four splits; 128 rows on 16128 keys, 32 on 8: 60 in 16 splits, 69 in 8, 70 in 32 rows and 4; 2 x 298 after
+// 2531, 2 on 2: 18 in 32 rows and 4 splits, 20 in 128 and 16; 46 x 35 in fp32, 20 on 5 of 80: 32 in 32 rows, 16 in 128.
+struct Step {
+  float alone, shared;
+};
+Step step_of(bool keys, bool f32, int dp) {
+  if (keys) return f32 ? (dp == 64 ? Step{2.4f, 1.9f} : Step{4.6f, 4.6f}) : (dp == 64 ? Step{0.7f, 0.6f} : Step{0.9f, 0.8f});
+  if (f32) return dp == 64 ? Step{1.5f, 1.06f} : Step{3.f, 2.9f};
+  return dp == 64 ? Step{0.9f, 0.55f} : Step{1.45f, 1.2f};
+}
+float prompt_time(bool keys, bool f32, int dp, int64_t items, int64_t steps, float average, int splits, int cus) {
+  const Step t = step_of(keys, f32, dp);
+  const int64_t workgroups = items * splits, each = (steps + splits - 1) / splits, share = (workgroups + cus - 1) / cus;
+  const float mean = average / static_cast<float>(splits) > 1.f ? average / static_cast<float>(splits) : 1.f;
+  // (a CU's share of workgroups: the largest and the mean one, as CUs with fewer leave memory and power to the rest)
+  const float part = share > 1 ? 0.5f * (static_cast<float>(share) + static_cast<float>(workgroups) / static_cast<float>(cus)) : 1.f;
+  const float longest = static_cast<float>(each) * t.alone, all = part * mean * t.shared;
+  const int at_once = keys && f32 && dp == 128 ? 1 : 2;  // on a CU; further ones start after them
+  float us = (keys ? 6.5f : 8.f) + (longest > all ? longest : all);
+  if (share > at_once) us += (at_once == 1 ? 5.f : 2.f) * static_cast<float>(share - at_once);
+  // (what is written and read again, at 5 TB/s)
+  if (splits > 1) us += 4.f + static_cast<float>(workgroups) * static_cast<float>(slot_floats(keys ? kKeyTile : kRowTile, dp)) * 1.6e-6f;
+  return us;
 }
 
 struct PromptPlan {
@@ -1379,18 +1409,30 @@ struct PromptPlan {
 };
 PromptPlan plan_prompt(const g16_attention_args& a) {
   PromptPlan r = {};
-  const int group = a.hq / a.hkv, dp = a.d <= 64 ? 64 : 128;
+  const int group = a.hq / a.hkv, dp = a.d <= 64 ? 64 : 128, cus = cus_of(a);
   const int64_t rows = a.q_offsets == nullptr ? static_cast<int64_t>(a.q_len) * group : static_cast<int64_t>(a.q_len) * group / a.seqs;
-  r.keys = rows <= 64;
+  // keys of an average sequence (packed lengths are known on the device only), and what its rows see on average
+  const int64_t own = a.q_offsets == nullptr ? a.k_len : a.k_len / a.seqs, keys = a.shared + own;
+  const int64_t tokens = a.q_offsets == nullptr ? a.q_len : a.q_len / a.seqs;
+  const float seen = static_cast<float>(keys) - (a.causal ? 0.5f * static_cast<float>(tokens < own ? tokens : own) : 0.f);
+  float best = 0.f;
+  for (int m = 0; m < 2; ++m) {
+    const bool by_keys = m == 1;
+    const int rt = by_keys ? kKeyTile : kRowTile, step = by_keys ? 128 : (a.is_f32 ? 32 : 64);
+    const int64_t items = (rows + rt - 1) / rt * a.seqs * a.hkv, steps = (keys + step - 1) / step;
+    for (int s = 1; s <= 256; s = s < 4 ? s + 1 : (s & (s - 1) ? s / 3 * 4 : s / 2 * 3)) {  // 1 2 3 4 6 8 12 16 ..
+      if (s > 1 && steps / s < (by_keys ? 1 : 2)) break;
+      const float us = prompt_time(by_keys, a.is_f32 != 0, dp, items, steps, seen / static_cast<float>(step), s, cus);
+      if (r.splits > 0 && us >= best) continue;
+      best = us;
+      r.keys = by_keys;
+      r.splits = s;
+    }
+  }
   r.rt = r.keys ? kKeyTile : kRowTile;
   const int64_t tiles = a.q_offsets == nullptr ? (rows + r.rt - 1) / r.rt * a.seqs
                                                : static_cast<int64_t>(a.q_len) * group / r.rt + a.seqs;
   r.tiles = static_cast<int>(tiles);
-  const int bn = r.keys || a.is_f32 ? 32 : 64;
-  // keys of an average sequence (packed lengths are known on the device only)
-  const int64_t keys = a.shared + (a.q_offsets == nullptr ? a.k_len : a.k_len / a.seqs);
-  const int64_t busy = a.q_offsets == nullptr ? tiles : (rows + r.rt - 1) / r.rt * a.seqs;
-  r.splits = splits_for(busy * a.hkv, (keys + bn - 1) / bn, cus_of(a), r.keys ? kLeastKeys : 4);
   if (r.splits > 1) r.bytes = static_cast<size_t>(r.tiles) * r.splits * a.hkv * slot_floats(r.rt, dp) * sizeof(float);
   return r;
 }
@@ -1408,7 +1450,10 @@ DecodePlan plan_decode(const g16_attention_args& a) {
   r.skeys = rows <= 2 * kKeyTile;
   const int srt = r.skeys ? kKeyTile : kRowTile, sbn = r.skeys || a.is_f32 ? 32 : 64;
   r.stiles = a.shared > 0 ? static_cast<int>((rows + srt - 1) / srt) : 0;
-  r.ssplits = splits_for(static_cast<int64_t>(r.stiles) * a.hkv, (a.shared + sbn - 1) / sbn, cus, r.skeys ? kLeastKeys : 4);
+  // (two workgroups a CU; 128 rows of more than 64 values: one, as a second one adds no speed and the requests' own
+  // keys take its place: 64 requests, 32768 shared keys, 8 heads of 128: 86 us, with two 88; of 64: 42 and 39.)
+  r.ssplits = splits_for(static_cast<int64_t>(r.stiles) * a.hkv, (a.shared + sbn - 1) / sbn, r.skeys || dp == 64 ? 2 * cus : cus,
+                         r.skeys ? kLeastKeys : 4);
   r.otiles = (group + kKeyTile - 1) / kKeyTile;
   const int64_t items = (2 * cus + static_cast<int64_t>(r.otiles) * a.hkv - 1) / (static_cast<int64_t>(r.otiles) * a.hkv);
   // (at most as many parts as there are requests: one each, and no need to look for it)
