@@ -566,8 +566,10 @@ __device__ inline float inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
 
 // ---- workgroup of 128 rows ---------------------------------------------------------------------------
 // Wavefront w holds rows 32 w .. 32 w + 31. last_seen: a position up to which every valid row of this
-// wavefront sees; wave_limit: the last position that any of them sees.
-template <typename T, int DP>
+// wavefront sees; wave_limit: the last position that any of them sees. DU: of a row's DP places in LDS, those that
+// the products go over, half of them for heads of up to 32 values, three quarters for up to 96 (8192 causal tokens, 32
+// heads on 8 of 96: 489 us, all 128 places 542; 16 x 512 in fp32, 12 of 32: 35 and 44).
+template <typename T, int DP, int DU>
 __device__ void rows_workgroup(const Params& p, char* lds, int* ranges, const Row& row, const KeyRuns& runs, int n0, int tbeg, int tend,
                                int last_seen, int wave_limit, const Slot& slot) {
   constexpr int BN = sizeof(T) == 2 ? 64 : 32, NB = BN / 32;
@@ -601,7 +603,7 @@ __device__ void rows_workgroup(const Params& p, char* lds, int* ranges, const Ro
     at.pos0 += BN;
     at.len -= BN;
   };
-  Wave<T, DP> w;
+  Wave<T, DU> w;
   if (tbeg < tend) issue(tbeg, 0);
   w.start(row, p.sign, p.d, lane);
   const uint32_t klane = base + TL::k_lane(lane), vlane = base + TL::BYTES + TL::v_lane(lane);
@@ -640,7 +642,7 @@ __device__ void rows_workgroup(const Params& p, char* lds, int* ranges, const Ro
   if (slot.at != nullptr) {
     float* o = slot.at + static_cast<size_t>(r) * DP;
 #pragma unroll
-    for (int db = 0; db < DP / 32; ++db)
+    for (int db = 0; db < DU / 32; ++db)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const float16v& a = w.o[db];
@@ -653,7 +655,7 @@ __device__ void rows_workgroup(const Params& p, char* lds, int* ranges, const Ro
   } else if (row.out != nullptr) {
     const float inv = inverse(l);
 #pragma unroll
-    for (int db = 0; db < DP / 32; ++db)
+    for (int db = 0; db < DU / 32; ++db)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int d0 = 32 * db + 8 * q + 4 * h;
@@ -663,7 +665,7 @@ __device__ void rows_workgroup(const Params& p, char* lds, int* ranges, const Ro
   }
   if (!p.causal) return;
 #pragma unroll
-  for (int db = 0; db < DP / 32; ++db)
+  for (int db = 0; db < DU / 32; ++db)
 #pragma unroll
     for (int i = 0; i < 16; ++i) bad = fmaf(w.o[db][i], 0.f, bad);
   const uint64_t which = __ballot(bad != 0.f && row.q != nullptr);
@@ -987,7 +989,7 @@ __device__ inline Row prompt_row(const Params& p, const Where& w, int kv, int r,
 }
 
 // (three workgroups of 128 rows fit a CU at 64 values a row, two at 128)
-template <typename T, int DP, bool KEYS>
+template <typename T, int DP, int DU, bool KEYS>
 __global__ __launch_bounds__(kThreads, !KEYS && DP == 64 ? 3 : 2) void prompt_kernel(Params p) {
   constexpr int RT = KEYS ? kKeyTile : kRowTile, BN = KEYS ? 32 : (sizeof(T) == 2 ? 64 : 32);
   __shared__ __attribute__((aligned(1024))) char lds[KEYS ? keys_lds<T, DP>() : rows_lds<T, DP>()];
@@ -1026,7 +1028,7 @@ __global__ __launch_bounds__(kThreads, !KEYS && DP == 64 ? 3 : 2) void prompt_ke
   if constexpr (KEYS) {
     keys_workgroup<T, DP, false>(p, lds, joint, row, runs, Pages{}, n0, tbeg, tend, last_seen, slot);
   } else {
-    rows_workgroup<T, DP>(p, lds, ranges, row, runs, n0, tbeg, tend, last_seen, wave_limit, slot);
+    rows_workgroup<T, DP, DU>(p, lds, ranges, row, runs, n0, tbeg, tend, last_seen, wave_limit, slot);
   }
 }
 
@@ -1206,7 +1208,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(Params p) {
       keys_workgroup<T, DP, false>(p, lds, joint, row, runs, Pages{}, n, tbeg, tend, 0x7fffffff, slot);
     } else {
       const bool some = t * SRT + 32 * wave < p.seqs * p.group;  // a wavefront without rows computes nothing
-      rows_workgroup<T, DP>(p, lds, ranges, row, runs, n, tbeg, tend, 0x7fffffff, some ? 0x7fffffff : -1, slot);
+      rows_workgroup<T, DP, DP>(p, lds, ranges, row, runs, n, tbeg, tend, 0x7fffffff, some ? 0x7fffffff : -1, slot);
     }
     return;
   }
@@ -1472,8 +1474,10 @@ DecodePlan plan_decode(const g16_attention_args& a) {
 template <typename T, int DP>
 int run_prompt(const Params& p, const PromptPlan& plan, hipStream_t stream) {
   const dim3 grid(static_cast<unsigned>(plan.tiles) * plan.splits * p.hkv);
-  int rc = plan.keys ? launch(prompt_kernel<T, DP, true>, grid, dim3(kThreads), stream, p)
-                     : launch(prompt_kernel<T, DP, false>, grid, dim3(kThreads), stream, p);
+  constexpr int kLess = DP == 64 ? 32 : 96;
+  int rc = plan.keys      ? launch(prompt_kernel<T, DP, DP, true>, grid, dim3(kThreads), stream, p)
+           : p.d <= kLess ? launch(prompt_kernel<T, DP, kLess, false>, grid, dim3(kThreads), stream, p)
+                          : launch(prompt_kernel<T, DP, DP, false>, grid, dim3(kThreads), stream, p);
   if (rc == 0 && plan.splits > 1)
     rc = launch(prompt_join_kernel<T, DP>, dim3(static_cast<unsigned>(plan.tiles) * p.hkv * (plan.rt / kJoinRows)), dim3(kThreads), stream, p,
                 plan.rt);
