@@ -1454,9 +1454,14 @@ DecodePlan plan_decode(const g16_attention_args& a) {
   r.stiles = a.shared > 0 ? static_cast<int>((rows + srt - 1) / srt) : 0;
   // (two workgroups a CU; 128 rows of more than 64 values: one, as a second one adds no speed and the requests' own
   // keys take its place: 64 requests, 32768 shared keys, 8 heads of 128: 86 us, with two 88; of 64: 42 and 39.)
-  r.ssplits = splits_for(static_cast<int64_t>(r.stiles) * a.hkv, (a.shared + sbn - 1) / sbn, r.skeys || dp == 64 ? 2 * cus : cus,
-                         r.skeys ? kLeastKeys : 4);
+  // 32 rows of more than 64 fp32 values: the LDS holds one workgroup a CU, all of which should start at once, and a
+  // tile takes five times as long as in fp16, so shorter splits pay (4 requests of up to 1000, 2000 shared, 8 heads of
+  // 128: 26.5 us in 10 splits, 39.5 in 3; 11 of up to 22, 11081, 2 of 72: 27 in 48, 35 in 21).
   r.otiles = (group + kKeyTile - 1) / kKeyTile;
+  const bool single = r.skeys && a.is_f32 && dp == 128;
+  const int64_t others = a.seqs * static_cast<int64_t>(r.otiles) * a.hkv;
+  const int many = single ? static_cast<int>(others < cus / 2 ? cus - others : cus / 2) : (r.skeys || dp == 64 ? 2 * cus : cus);
+  r.ssplits = splits_for(static_cast<int64_t>(r.stiles) * a.hkv, (a.shared + sbn - 1) / sbn, many, single ? 6 : (r.skeys ? kLeastKeys : 4));
   const int64_t items = (2 * cus + static_cast<int64_t>(r.otiles) * a.hkv - 1) / (static_cast<int64_t>(r.otiles) * a.hkv);
   // (at most as many parts as there are requests: one each, and no need to look for it)
   const bool split = (a.k_len + 31) / 32 > kLeastKeys && items > 1;
