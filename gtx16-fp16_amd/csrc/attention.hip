@@ -30,7 +30,8 @@
 //   * keys: 32 query rows, every wavefront on its own tiles of 32 keys, joined at the end; for few rows, whose
 //     time is that of one workgroup or of reading the keys.
 // With too few tiles to fill the card, the keys are split over workgroups as well, which leave (O, maximum,
-// sum) in the workspace (prompt_time weighs shapes and splits); a second launch joins them in split order (no atomics: repeated calls agree).
+// sum) in the workspace (prompt_time weighs shapes and splits); a second launch joins them in split order (no
+// atomics: repeated calls agree).
 #include "g16_common.hpp"
 
 namespace g16 {
@@ -1453,7 +1454,7 @@ DecodePlan plan_decode(const g16_attention_args& a) {
   const int srt = r.skeys ? kKeyTile : kRowTile, sbn = r.skeys || a.is_f32 ? 32 : 64;
   r.stiles = a.shared > 0 ? static_cast<int>((rows + srt - 1) / srt) : 0;
   // (two workgroups a CU; 128 rows of more than 64 values: one, as a second one adds no speed and the requests' own
-  // keys take its place: 64 requests, 32768 shared keys, 8 heads of 128: 86 us, with two 88; of 64: 42 and 39.)
+  // keys take its place: 64 requests, 32768 shared keys, 8 heads of 128: 75 us, with two 83; of 64: 42 and 39.)
   // 32 rows of more than 64 fp32 values: the LDS holds one workgroup a CU, all of which should start at once, and a
   // tile takes five times as long as in fp16, so shorter splits pay (4 requests of up to 1000, 2000 shared, 8 heads of
   // 128: 26.5 us in 10 splits, 39.5 in 3; 11 of up to 22, 11081, 2 of 72: 27 in 48, 35 in 21).
