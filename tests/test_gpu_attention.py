@@ -425,3 +425,16 @@ def test_refusals(cuda):
         g.attention(q.requires_grad_(), k, k)
     with torch.no_grad():
         g.attention(q, k, k)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("d", [8, 24, 32, 40, 72, 88, 96, 104])
+def test_many_short_sequences_of_every_width(cuda, dtype, d):
+    lengths = [(37 * i) % 70 for i in range(100)]
+    run_prompts(cuda, lengths, lengths, 6, 6, d, dtype, causal=d % 16 == 0, seed=d)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("lens_q,lens_k", [([130, 0, 7], [1500, 3, 40]), ([1], [3000]), ([300], [300])])
+def test_few_tiles_split_over_the_keys(cuda, dtype, lens_q, lens_k):
+    run_prompts(cuda, lens_q, lens_k, 2, 1, 72, dtype, causal=True, shared=100, slopes=True)
