@@ -62,7 +62,13 @@ struct Params {
   int M, K, N, rank, adapters, tiles, slots, splits, chunks;
 };
 
-// The adapters among a tile's 16 rows. mine: that of row lane % 16 (negative: none); ids: lane i, the i-th.
+// A row's adapter: -1 for every index that names none.
+__device__ inline int adapter_of(const Params& p, int row) {
+  const int a = row < p.M ? p.index[row] : -1;
+  return a >= 0 && a < p.adapters ? a : -1;
+}
+
+// The adapters among a tile's 16 rows. mine: that of row lane % 16 (-1: none); ids: lane i, the i-th.
 struct Adapters {
   int mine, count, ids;
   float scale;  // of `mine`
@@ -70,8 +76,7 @@ struct Adapters {
 __device__ inline Adapters adapters_of(const Params& p, int m0) {
   const int lane = threadIdx.x & 63, row = m0 + (lane & 15);
   Adapters t;
-  t.mine = row < p.M ? p.index[row] : -1;
-  if (t.mine >= p.adapters) t.mine = -1;
+  t.mine = adapter_of(p, row);
   t.scale = t.mine >= 0 && p.scale != nullptr ? p.scale[t.mine] : 1.f;
   t.ids = -1;
   t.count = 0;
@@ -310,8 +315,8 @@ __global__ __launch_bounds__(kThreads, RC == 1 ? 4 : 2) void expand_kernel(Param
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int m0 = blockIdx.x * kManyRows, q = lane >> 4;
   // the adapter of row m0 + lane, and the list of all
-  int mine = m0 + lane < p.M ? p.index[m0 + lane] : -1, ids = -1, count = 0;
-  if (mine >= p.adapters) mine = -1;
+  const int mine = adapter_of(p, m0 + lane);
+  int ids = -1, count = 0;
   for (uint64_t left = __ballot(mine >= 0); left != 0; ++count) {
     const int a = __builtin_amdgcn_readlane(mine, __builtin_ctzll(left));
     left &= ~__ballot(mine == a);

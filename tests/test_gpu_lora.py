@@ -212,3 +212,16 @@ def test_adapters_interleaved_row_by_row(cuda, M, n):
     c = make(M, 256, 136, 24, n)
     c["index"] = torch.arange(M, dtype=torch.int32) % (n + 1)
     check(cuda, c)
+
+
+@pytest.mark.parametrize("M,K", [(5, 64), (16, 256), (40, 256), (300, 512)])
+@pytest.mark.parametrize("x,out", [(F16, F16), (F32, F16), (F16, F32)])
+def test_every_negative_index_means_no_adapter(cuda, M, K, x, out):
+    c = make(M, K, 136, 16, 3, x, seed=M)
+    c["index"][::2] = torch.tensor([-2, -1, -7, -(1 << 31)], dtype=torch.int32).repeat(M)[:c["index"][::2].numel()]
+    rows = c["index"] < 0
+    want = ops.mm_t(c["x"].to(cuda), c["w"].to(cuda), c["bias"].to(cuda), F32).to(out)
+    for _ in range(2):
+        torch.full((M, 136), float("nan"), dtype=out, device=cuda)  # (freed at once: likely the next output's memory)
+        y = check(cuda, c, out)
+        assert torch.equal(y[rows.to(cuda)], want[rows.to(cuda)])
