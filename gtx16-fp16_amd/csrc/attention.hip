@@ -1295,8 +1295,7 @@ int check(const g16_attention_args& a, bool decode) {
     return t % 16 == 0 && h % 16 == 0 && (!longest || (token >= a.d && t < G16_ATTENTION_MAX_STRIDE));
   };
   if (!aligned16(a.q) || !aligned16(a.out) || !row(decode ? 0 : a.q_token, a.q_head, false) || a.q_seq * size % 16 != 0) return G16_E_ALIGN;
-  const bool own = decode ? a.k_len > 0 : a.k_len > 0;
-  if (own) {
+  if (a.k_len > 0) {
     if (a.k == nullptr || a.v == nullptr) return G16_E_NULL;
     if (!aligned16(a.k) || !aligned16(a.v) || a.k_seq * size % 16 != 0 || a.v_seq * size % 16 != 0) return G16_E_ALIGN;
     if (!row(a.k_token, a.k_head, true) || !row(a.v_token, a.v_head, true)) return G16_E_SHAPE;
@@ -1405,9 +1404,11 @@ float prompt_time(bool keys, bool f32, int dp, int64_t items, int64_t steps, flo
   return us;
 }
 
+bool fits_grid(int64_t workgroups) { return workgroups <= (1LL << 24) - 1; }  // 2^32 threads a launch
+
 struct PromptPlan {
   bool keys;
-  int rt, tiles, splits;
+  int rt, tiles, splits;  // splits 0: no shape whose launches are small enough
   size_t bytes;
 };
 PromptPlan plan_prompt(const g16_attention_args& a) {
@@ -1423,19 +1424,20 @@ PromptPlan plan_prompt(const g16_attention_args& a) {
     const bool by_keys = m == 1;
     const int rt = by_keys ? kKeyTile : kRowTile, step = by_keys ? 128 : (a.is_f32 ? 32 : 64);
     const int64_t items = (rows + rt - 1) / rt * a.seqs * a.hkv, steps = (keys + step - 1) / step;
+    // row tiles; packed: at most
+    const int64_t tiles = a.q_offsets == nullptr ? (rows + rt - 1) / rt * a.seqs : static_cast<int64_t>(a.q_len) * group / rt + a.seqs;
     for (int s = 1; s <= 256; s = s < 4 ? s + 1 : (s & (s - 1) ? s / 3 * 4 : s / 2 * 3)) {  // 1 2 3 4 6 8 12 16 ..
       if (s > 1 && steps / s < (by_keys ? 1 : 2)) break;
+      if (!fits_grid(tiles * s * a.hkv) || (s > 1 && !fits_grid(tiles * a.hkv * (rt / kJoinRows)))) break;
       const float us = prompt_time(by_keys, a.is_f32 != 0, dp, items, steps, seen / static_cast<float>(step), s, cus);
       if (r.splits > 0 && us >= best) continue;
       best = us;
       r.keys = by_keys;
+      r.rt = rt;
+      r.tiles = static_cast<int>(tiles);
       r.splits = s;
     }
   }
-  r.rt = r.keys ? kKeyTile : kRowTile;
-  const int64_t tiles = a.q_offsets == nullptr ? (rows + r.rt - 1) / r.rt * a.seqs
-                                               : static_cast<int64_t>(a.q_len) * group / r.rt + a.seqs;
-  r.tiles = static_cast<int>(tiles);
   if (r.splits > 1) r.bytes = static_cast<size_t>(r.tiles) * r.splits * a.hkv * slot_floats(r.rt, dp) * sizeof(float);
   return r;
 }
@@ -1500,8 +1502,6 @@ int run_decode(const Params& p, const DecodePlan& plan, hipStream_t stream) {
   return rc;
 }
 
-bool fits_grid(int64_t workgroups) { return workgroups <= (1LL << 24) - 1; }  // 2^32 threads a launch
-
 }  // namespace
 }  // namespace g16
 
@@ -1512,17 +1512,27 @@ extern "C" size_t g16_attention_workspace_bytes(const g16_attention_args* args) 
   return plan_prompt(*args).bytes;
 }
 
+extern "C" int g16_attention_plan(const g16_attention_args* args, int* row_tile, int* splits) {
+  if (args == nullptr || row_tile == nullptr || splits == nullptr) return G16_E_NULL;
+  *row_tile = *splits = 0;
+  const int st = check(*args, false);
+  if (st != G16_OK || args->seqs == 0 || args->hq == 0 || args->q_len == 0) return st;
+  const PromptPlan plan = plan_prompt(*args);
+  if (plan.splits == 0) return G16_E_SHAPE;
+  *row_tile = plan.rt;
+  *splits = plan.splits;
+  return G16_OK;
+}
+
 extern "C" int g16_attention(const g16_attention_args* args, void* stream) {
   if (args == nullptr) return G16_E_NULL;
   const g16_attention_args& a = *args;
   const int st = check(a, false);
   if (st != G16_OK || a.seqs == 0 || a.hq == 0 || a.q_len == 0) return st;
   const PromptPlan plan = plan_prompt(a);
+  if (plan.splits == 0) return G16_E_SHAPE;
   if (plan.bytes > 0 && (a.workspace == nullptr || static_cast<size_t>(a.workspace_bytes) < plan.bytes)) return G16_E_WORKSPACE;
   if (!aligned16(a.workspace)) return G16_E_ALIGN;
-  if (!fits_grid(static_cast<int64_t>(plan.tiles) * plan.splits * a.hkv) ||
-      !fits_grid(static_cast<int64_t>(plan.tiles) * a.hkv * (plan.rt / kJoinRows)))
-    return G16_E_SHAPE;
   Params p = params(a);
   p.tiles = plan.tiles;
   p.splits = plan.splits;

@@ -16,7 +16,7 @@ from pathlib import Path
 import torch  # noqa: F401  (loads torch's HIP runtime before libg16.so)
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libg16.so"
-ABI_VERSION = 17
+ABI_VERSION = 18
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
@@ -69,6 +69,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "g16_skinny_strips": (_I, [_P, _I, _P, _P, _I, _P, _I, _I, _I, _P]),
     "g16_skinny_strips_route": (_I, [_I, _I, _I, _I]),
     "g16_attention_workspace_bytes": (_SZ, [_P]),
+    "g16_attention_plan": (_I, [_P, _P, _P]),
     "g16_attention": (_I, [_P, _P]),
     "g16_attention_decode_workspace_bytes": (_SZ, [_P]),
     "g16_attention_decode": (_I, [_P, _P]),

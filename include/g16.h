@@ -47,7 +47,7 @@
 extern "C" {
 #endif
 
-#define G16_ABI_VERSION 17
+#define G16_ABI_VERSION 18
 
 /* Status codes (negative: rejected by the library before any launch). */
 #define G16_OK 0
@@ -398,6 +398,11 @@ typedef struct {
 } g16_attention_args;
 size_t g16_attention_workspace_bytes(const g16_attention_args* args);
 int g16_attention(const g16_attention_args* args, void* stream);
+/* How g16_attention runs these arguments: the query rows of a workgroup (128, or 32 whose wavefronts take keys of
+ * their own) and over how many workgroups a row's keys are split (0 and 0 where there is nothing to do). Returns what
+ * the call would be rejected with, the workspace apart; G16_E_SHAPE too where no shape fits a launch (2^24 - 1
+ * workgroups: one for every row tile, key head and split). */
+int g16_attention_plan(const g16_attention_args* args, int* row_tile, int* splits);
 size_t g16_attention_decode_workspace_bytes(const g16_attention_args* args);
 int g16_attention_decode(const g16_attention_args* args, void* stream);
 

@@ -84,3 +84,45 @@ def test_struct_size_is_checked_by_the_binding():
     with pytest.raises(TypeError):
         fast.args_size(_clib.address("g16_attention"))
     assert ctypes.sizeof(ctypes.c_void_p) == 8
+
+
+def plan(**changes):
+    """(status, rows of a workgroup, splits) of g16_attention for these arguments."""
+    args = ctypes.create_string_buffer(head(**changes) + bytes(16))
+    rows, splits = ctypes.c_int(-1), ctypes.c_int(-1)
+    st = _clib.load().g16_attention_plan(args, ctypes.byref(rows), ctypes.byref(splits))
+    return st, rows.value, splits.value
+
+
+def documents(n, tokens, heads, **changes):
+    rows = n * tokens
+    return dict(dict(q_offsets=4096, k_offsets=4096, seqs=n, q_len=rows, k_len=rows, hq=heads, hkv=heads, q_token=heads * 64, k_token=heads * 64,
+                     v_token=heads * 64), **changes)
+
+
+def test_plan_follows_the_checks():
+    assert plan(d=60) == (SHAPE, 0, 0)
+    assert plan(q=0) == (NULL, 0, 0)
+    assert plan(q_len=0) == (0, 0, 0)
+    st, rows, splits = plan()
+    assert st == 0 and rows in (32, 128) and splits == 1
+    assert plan(k_len=8000, q_len=4, k_seq=8000 * 64, v_seq=8000 * 64)[2] > 1
+    rows = ctypes.c_int()
+    assert _clib.load().g16_attention_plan(None, ctypes.byref(rows), ctypes.byref(rows)) == NULL
+    assert _clib.load().g16_attention_plan(ctypes.create_string_buffer(head() + bytes(16)), None, ctypes.byref(rows)) == NULL
+
+
+@pytest.mark.parametrize("n,tokens,heads", [(50000, 10, 12), (100000, 10, 12), (100000, 100, 12), (1000000, 3, 12)])
+def test_many_documents_fit_a_launch_where_nothing_is_joined(n, tokens, heads):
+    # one workgroup for every 128 (or 32) rows of a document and head, of which a launch takes 2^24 - 1
+    st, rows, splits = plan(**documents(n, tokens, heads))
+    assert st == 0 and splits == 1 and (n * tokens // rows + n) * heads < 1 << 24
+
+
+def test_what_no_launch_takes_is_rejected():
+    assert plan(**documents(1 << 24, 1, 2)) == (SHAPE, 0, 0)
+    assert size("g16_attention", **documents(1 << 24, 1, 2)) == 0
+    assert call("g16_attention", **documents(1 << 24, 1, 2)) == SHAPE
+    # rows of all sequences past 32 bits
+    equal = dict(seqs=1 << 22, q_len=1 << 22, k_len=8, hq=2, hkv=2)
+    assert plan(**equal) == (SHAPE, 0, 0) and call("g16_attention", **equal) == SHAPE
