@@ -13,15 +13,16 @@
 //     row-major V in LDS in that order through the transposing reads (fp16) or plain dword reads (fp32).
 //   * One pass over the keys with a running maximum. A maximum only moves when a row's new one is more
 //     than 2^kLag above it (the weights grow to at most 2^(kShift + kLag), far inside fp16), which after
-//     the first tiles spares almost every rescale of O. Weights are computed 2^kShift above their value,
+//     the first tiles spares almost every rescale of O. fp16 weights are 2^kShift above their value,
 //     which keeps those far below the maximum out of fp16's subnormals.
-//   * fp32 values are multiplied as two fp16 parts each, to 2^-22 of the value: three products (that of the two
-//     small parts is below it) of 32 cycles where eight v_mfma_f32_32x32x2_f32 take 512 for the same step. The
-//     small part of a key or value is kept 2^11 above its size, that of its large part, so that it stays
-//     out of fp16's subnormals, and meets the other side 2^11 below it. Query rows are scaled by a power of two
-//     to 2^13 .. 2^14 first. Keys and values have to lie in fp16's range, and a tile's largest be at least
-//     2^-10 (a value is exact to 2^-36); a tile where that does not hold, which every wavefront sees from the
-//     part it loaded, takes the fp32 instructions. Weights, 0 .. 2^15, always fit.
+//   * fp32 values are multiplied as three bf16 parts each, v = hi + mid + lo: 8 bits a part, all 24 of the value, in
+//     fp32's own range, so neither the size of a value nor that of its neighbours matters. Of the nine products of
+//     parts the three below 2^-24 of the whole are left out; the other six take 192 cycles where eight
+//     v_mfma_f32_32x32x2_f32 take 512 for the same step. Infinities have no parts (inf - inf), and the last parts of
+//     values below 2^-110 are lost, which matters only beside huge ones: a tile of keys or values that holds one of
+//     2^64 or more, or NaN, which every wavefront sees from the part it loaded, takes the fp32 instructions, and so do
+//     all tiles of rows whose queries do. (32 x 256 tokens, 12 heads of 64, distance bias: 56 us; everything on the
+//     fp32 instructions 71; two fp16 parts of 22 bits, right only for values of like size, 41.)
 //   * Keys arrive by DMA into LDS with the row swizzles of Tile. A tile that ends past its sequence is cut
 //     off by the buffer descriptor's range, which writes zeros: no value from behind a sequence's end
 //     reaches a product.
@@ -32,6 +33,8 @@
 // With too few tiles to fill the card, the keys are split over workgroups as well, which leave (O, maximum,
 // sum) in the workspace (prompt_time weighs shapes and splits); a second launch joins them in split order (no
 // atomics: repeated calls agree).
+#include <cfloat>
+
 #include "g16_common.hpp"
 
 namespace g16 {
@@ -40,7 +43,14 @@ namespace {
 typedef float float8v __attribute__((ext_vector_type(8)));
 typedef float float2v __attribute__((ext_vector_type(2)));
 
-constexpr float kShift = 8.f, kLag = 7.f;
+constexpr float kLag = 7.f;
+// fp16 weights are 2^kShift above their value, by way of the exponent. fp32 ones would lose bits of the exponent by that
+// (2^-20 of a weight at 23), and are made 2^kScale of theirs by a product: at most 2^-16, so that the sums over 65536
+// keys of the largest weight stay within the values' range.
+template <typename T>
+constexpr float kShift = sizeof(T) == 2 ? 8.f : 0.f;
+template <typename T>
+constexpr float kScale = sizeof(T) == 2 ? 1.f : 0x1p-23f;
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kPlainCap = 256.f;  // largest tanh cap that fp16 inputs take the plain form for (tanh_of)
 constexpr int kRowTile = 128, kKeyTile = 32;  // query rows of the two workgroup shapes
@@ -64,44 +74,77 @@ __device__ inline float16v mma(float8v a, float8v b, float16v c) {
   return c;
 }
 
-// fp32 as two fp16 parts: hi + lo for what is multiplied from the right, hi + 2^-11 lo from the left (Left8).
+// fp32 as three bf16 parts, hi + mid + lo.
+typedef __bf16 bhalf8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bhalf2 __attribute__((ext_vector_type(2)));
 struct Split8 {
-  half8 hi, lo;
+  bhalf8 hi, mid, lo;
 };
-struct Left8 : Split8 {};
-__device__ inline float8v widen(half8 h) { return __builtin_convertvector(h, float8v); }
-__device__ inline Split8 split(float8v v) {
-  const half8 hi = __builtin_convertvector(v, half8);
-  float8v rest;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) rest[j] = fmaf(static_cast<float>(hi[j]), -1.f, v[j]);  // one mixed-precision instruction
-  return Split8{hi, __builtin_convertvector(rest, half8)};
-}
-__device__ inline float16v mma(const Left8& a, const Split8& b, float16v c) {
-  c = mma(a.hi, b.hi, c);
+__device__ inline float16v mma(bhalf8 a, bhalf8 b, float16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ inline float8v widen(bhalf8 v) { return __builtin_convertvector(v, float8v); }
+__device__ inline float8v whole(const Split8& s) { return widen(s.hi) + widen(s.mid) + widen(s.lo); }  // (no part rounds)
+// ... all products of parts but the largest
+__device__ inline float16v mma_small(const Split8& a, const Split8& b, float16v c) {
+  c = mma(a.lo, b.hi, c);
+  c = mma(a.mid, b.mid, c);
   c = mma(a.hi, b.lo, c);
-  return mma(a.lo, b.hi * static_cast<_Float16>(0x1p-11f), c);
+  c = mma(a.mid, b.hi, c);
+  return mma(a.hi, b.mid, c);
 }
+__device__ inline float16v mma(const Split8& a, const Split8& b, float16v c) { return mma(a.hi, b.hi, mma_small(a, b, c)); }
 // What becomes of 8 values that are multiplied: fp16 as it is, fp32 in parts.
-__device__ inline half8 left(half8 v) { return v; }
-__device__ inline half8 right(half8 v) { return v; }
-__device__ inline Left8 left(float8v v) {
-  const half8 hi = __builtin_convertvector(v, half8);
+__device__ inline half8 operand(half8 v) { return v; }
+// Values rounded to bf16, taken off them: 20 instructions for 8. (A dot product with (-1, 0) would save the unpacking,
+// but v_dot2_f32_bf16 does not give the difference exactly, and takes as long.)
+__device__ inline bhalf8 take_part(float8v& v) {
+  bhalf8 part;
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) {
+    const bhalf2 two = __builtin_convertvector((float2v{v[j], v[j + 1]}), bhalf2);
+    const uint32_t bits = __builtin_bit_cast(uint32_t, two);
+    part[j] = two[0];
+    part[j + 1] = two[1];
+    v[j] -= __uint_as_float(bits << 16);
+    v[j + 1] -= __uint_as_float(bits & 0xffff0000u);
+  }
+  return part;
+}
+__device__ inline Split8 operand(float8v v) {
+  Split8 s;
+  s.hi = take_part(v);
+  s.mid = take_part(v);
+  s.lo = __builtin_convertvector(v, bhalf8);
+  return s;
+}
+// The same for any fp32 value: whole() gives it back, NaN, infinities and those that round to one included.
+__device__ inline Split8 operand_of_any(float8v v) {
+  bhalf8 hi = __builtin_convertvector(v, bhalf8);
   float8v rest;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) rest[j] = fmaf(static_cast<float>(hi[j]), -0x1p11f, v[j] * 0x1p11f);  // exact
-  return Left8{{hi, __builtin_convertvector(rest, half8)}};
+  for (int j = 0; j < 8; ++j) {
+    if (fabsf(static_cast<float>(hi[j])) <= FLT_MAX || v[j] != v[j]) {
+      rest[j] = v[j] - static_cast<float>(hi[j]);
+    } else {  // its first 8 bits, cut off
+      const float cut = __uint_as_float(__float_as_uint(v[j]) & 0xffff0000u);
+      hi[j] = static_cast<__bf16>(cut);
+      rest[j] = fabsf(cut) <= FLT_MAX ? v[j] - cut : 0.f;
+    }
+  }
+  Split8 s = operand(rest);
+  // (at most 16 bits are left: two parts)
+  return Split8{hi, s.hi, s.mid};
 }
-__device__ inline Split8 right(float8v v) { return split(v); }
 
-// Which of a tile's values a lane has seen: whether one is past fp16's range, whether one is not small.
+// Whether what a lane has seen is to be split: not where a value is 2^64 or more or not a number (or, which does no
+// harm, where a sum of large ones is).
 struct Range {
-  float top = 0.f;
-  __device__ void see(float4v v) { top = fmaxf(fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w))); }
-  // bit 0: past, bit 1: not small, over the wavefront
-  __device__ int bits() const { return (__any(top > 65504.f) ? 1 : 0) | (__any(top >= 0x1p-10f) ? 2 : 0); }
+  float sum = 0.f;
+  __device__ void see(float4v v) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum = fmaf(fabsf(v[j]), 0x1p64f, sum);
+  }
+  __device__ bool past() const { return __any(!(sum <= FLT_MAX)); }  // over the wavefront
 };
-__device__ inline bool exact_needed(int bits) { return (bits & 3) != 2; }
 
 // The value of the lane 32 away.
 __device__ inline float other_half(float v) {
@@ -307,10 +350,10 @@ __device__ inline float score_of(const Scoring& s, float x, float slope, float d
 template <typename T, int DP>
 struct Wave {
   using V8 = typename Vec8<T>::V;
-  decltype(right(V8{})) q[DP / 16];
+  decltype(operand(V8{})) q[DP / 16];
   float16v o[DP / 32];
   float m, l;  // the reference maximum (log2 units) and this lane's part of the sum of weights
-  float back;  // fp32: what the scores are multiplied by for the scaling of the row (1 for fp16)
+  bool exact;  // fp32: whether a row of the wavefront is not to be split
 
   __device__ void start(const Row& row, float sign, int d, int lane) {
     const int h = lane >> 5;
@@ -320,22 +363,26 @@ struct Wave {
       const int at = 16 * ks + 8 * h;
       v[ks] = V8{};
       if (row.q != nullptr && at < d) v[ks] = *reinterpret_cast<const V8*>(row.q + at * sizeof(T));
+      if (sign != 1.f) v[ks] *= static_cast<T>(sign);
     }
-    float by = sign;
-    back = 1.f;
-    if constexpr (sizeof(T) == 4) {  // the row's largest value to 2^13 .. 2^14
-      float top = 0.f;
+    exact = false;
+    if constexpr (sizeof(T) == 4) {
+      Range r;
 #pragma unroll
-      for (int ks = 0; ks < DP / 16; ++ks)
+      for (int ks = 0; ks < DP / 16; ++ks) {
+        r.see(__builtin_shufflevector(v[ks], v[ks], 0, 1, 2, 3));
+        r.see(__builtin_shufflevector(v[ks], v[ks], 4, 5, 6, 7));
+      }
+      exact = r.past();
+      if (__builtin_expect(exact, 0)) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[ks][j]));
-      top = fmaxf(top, other_half(top));
-      const int e = top > 0.f && top < __builtin_huge_valf() ? min(max(13 - ilogbf(top), -120), 120) : 0;
-      by *= ldexpf(1.f, e);
-      back = ldexpf(1.f, -e);
+        for (int ks = 0; ks < DP / 16; ++ks) q[ks] = operand_of_any(v[ks]);
+      }
     }
+    if (!exact) {
 #pragma unroll
-    for (int ks = 0; ks < DP / 16; ++ks) q[ks] = right(by == 1.f ? v[ks] : v[ks] * static_cast<T>(by));
+      for (int ks = 0; ks < DP / 16; ++ks) q[ks] = operand(v[ks]);
+    }
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i) o[i] = float16v{};
     m = -__builtin_huge_valf();
@@ -349,26 +396,40 @@ struct Wave {
     for (int i = 0; i < DP / 32; ++i) asm volatile("" : "+v"(o[i]));
   }
 
-  // S^T of the tile's NB blocks of 32 keys. EXACT: fp32 keys that do not fit fp16 (see Range).
+  // S^T of the tile's NB blocks of 32 keys. EXACT: fp32 keys or queries that are not to be split (see Range).
   template <int NB, typename TL, bool EXACT>
   __device__ void products(uint32_t kt, float16v (&s)[NB]) const {
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb) {
       s[kb] = float16v{};
+      if constexpr (sizeof(T) == 4 && !EXACT) {
+        // The small products first: each one added to the large ones' sum would round it (single tokens on 300 keys of
+        // 64: 1.4e-7 from the exact result, 2.5e-7 a step at a time, in the same time).
+        bhalf8 hi[DP / 16];
 #pragma unroll
-      for (int ks = 0; ks < DP / 16; ++ks) {
-        if constexpr (EXACT) {
-          half8 hi = q[ks].hi;
-          asm volatile("" : "+v"(hi));  // (or the sums would be kept in registers for the whole loop)
-          s[kb] = mma(TL::k_frag(kt, kb, ks), widen(hi) + widen(q[ks].lo), s[kb]);
-        } else s[kb] = mma(left(TL::k_frag(kt, kb, ks)), q[ks], s[kb]);
+        for (int ks = 0; ks < DP / 16; ++ks) {
+          const Split8 key = operand(TL::k_frag(kt, kb, ks));
+          s[kb] = mma_small(key, q[ks], s[kb]);
+          hi[ks] = key.hi;
+        }
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) s[kb] = mma(hi[ks], q[ks].hi, s[kb]);
+      } else {
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) {
+          if constexpr (EXACT) {
+            Split8 part = q[ks];
+            asm volatile("" : "+v"(part.hi));  // (or the sums would be kept in registers for the whole loop)
+            s[kb] = mma(TL::k_frag(kt, kb, ks), whole(part), s[kb]);
+          } else s[kb] = mma(TL::k_frag(kt, kb, ks), q[ks], s[kb]);
+        }
       }
     }
   }
   template <int NB, typename TL>
-  __device__ void products(uint32_t kt, float16v (&s)[NB], bool exact) const {
+  __device__ void products(uint32_t kt, float16v (&s)[NB], bool past) const {
     if constexpr (sizeof(T) == 4) {
-      if (__builtin_expect(exact, 0)) {
+      if (__builtin_expect(past || exact, 0)) {
         products<NB, TL, true>(kt, s);
         return;
       }
@@ -381,7 +442,7 @@ struct Wave {
   __device__ void weights(float16v (&s)[NB], const Scoring& sc, const Row& row, int pos0, int left, int last_seen, int lane) {
     const int h4 = (lane >> 5) * 4;
     // t = s * c + off
-    float c = sizeof(T) == 4 ? sc.c * back : sc.c, off = 0.f;
+    float c = sc.c, off = 0.f;
     if (sc.capped) {
       if (sizeof(T) == 2 && !sc.fine) {
         // tanh(y) = 1 - 2 / (e^2y + 1): s becomes -1 / (e^2y + 1), and the rest of it joins c and off
@@ -392,11 +453,10 @@ struct Wave {
         c = 2.f * sc.cap;
         off = sc.cap;
       } else {
-        const float inv = sizeof(T) == 4 ? sc.inv * back : sc.inv;
 #pragma unroll
         for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[kb][r] = tanh_of(s[kb][r] * inv);
+          for (int r = 0; r < 16; ++r) s[kb][r] = tanh_of(s[kb][r] * sc.inv);
         c = sc.cap;
       }
     }
@@ -439,13 +499,13 @@ struct Wave {
         for (int r = 0; r < 16; ++r) o[i][r] *= f;
     }
     // a row that has seen no key yet (m = -inf): every score is -inf, every weight 0
-    const float ref = (m == -__builtin_huge_valf() ? 0.f : m) - kShift - off;
+    const float ref = (m == -__builtin_huge_valf() ? 0.f : m) - kShift<T> - off;
     float sum = 0.f;
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const float w = __builtin_amdgcn_exp2f(fmaf(s[kb][r], c, -ref));
+        const float w = __builtin_amdgcn_exp2f(fmaf(s[kb][r], c, -ref)) * kScale<T>;
         s[kb][r] = w;
         sum += w;
       }
@@ -464,16 +524,16 @@ struct Wave {
 #pragma unroll
         for (int db = 0; db < DP / 32; ++db) o[db] = mma(TL::v_frag(vt, ks, db), w, o[db]);
       } else {
-        const auto wp = right(w);
+        const auto wp = operand(w);
 #pragma unroll
-        for (int db = 0; db < DP / 32; ++db) o[db] = mma(left(TL::v_frag(vt, ks, db)), wp, o[db]);
+        for (int db = 0; db < DP / 32; ++db) o[db] = mma(operand(TL::v_frag(vt, ks, db)), wp, o[db]);
       }
     }
   }
   template <int NB, typename TL>
-  __device__ void add(uint32_t vt, const float16v (&s)[NB], bool exact) {
+  __device__ void add(uint32_t vt, const float16v (&s)[NB], bool past) {
     if constexpr (sizeof(T) == 4) {
-      if (__builtin_expect(exact, 0)) {
+      if (__builtin_expect(past, 0)) {
         add<NB, TL, true>(vt, s);
         return;
       }
@@ -532,13 +592,13 @@ __device__ __attribute__((noinline)) void careful_row(const char* q, float sign,
     for (int j = (g ? from1 : from0) + lane; j < end && s.pos0 + j <= limit; j += kWave) top = fmaxf(top, score(s, j));
   }
   for (int i = 1; i < kWave; i *= 2) top = fmaxf(top, __shfl_xor(top, i));
-  const float ref = (top == -__builtin_huge_valf() ? 0.f : top) - kShift;
+  const float ref = (top == -__builtin_huge_valf() ? 0.f : top) - kShift<T>;
   float l = 0.f, o[DP / 64] = {};
   for (int g = 0; g < 2; ++g) {
     const Keys& s = g ? runs.own : runs.shared;
     const int end = min(min(g ? to1 : to0, s.len), limit < s.pos0 ? 0 : limit - s.pos0 + 1);
     for (int j0 = g ? from1 : from0; j0 < end; j0 += kWave) {
-      const float w = j0 + lane < end ? __builtin_amdgcn_exp2f(score(s, j0 + lane) - ref) : 0.f;
+      const float w = j0 + lane < end ? __builtin_amdgcn_exp2f(score(s, j0 + lane) - ref) * kScale<T> : 0.f;
       l += w;
       for (int i = 0; i < min(kWave, end - j0); ++i) {
         const float wi = __shfl(w, i);
@@ -619,7 +679,7 @@ __device__ void rows_workgroup(const Params& p, char* lds, int* ranges, const Ro
         k.see(*lds_at<float4v>(from));
         v.see(*lds_at<float4v>(from + TL::BYTES));
       }
-      const int bits = k.bits() | (v.bits() << 2);
+      const int bits = (k.past() ? 1 : 0) | (v.past() ? 2 : 0);
       if (lane == 0) ranges[buf * 4 + wave] = bits;
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -631,9 +691,9 @@ __device__ void rows_workgroup(const Params& p, char* lds, int* ranges, const Ro
     if (t + 1 < tend) issue(t + 1, buf ^ 1);
     if (pos0 <= wave_limit) {
       float16v s[NB];
-      w.template products<NB, TL>(klane + buf * 2 * TL::BYTES, s, exact_needed(bits));
+      w.template products<NB, TL>(klane + buf * 2 * TL::BYTES, s, (bits & 1) != 0);
       w.template weights<NB>(s, sc, row, pos0, left, last_seen, lane);
-      w.template add<NB, TL>(vlane + buf * 2 * TL::BYTES, s, exact_needed(bits >> 2));
+      w.template add<NB, TL>(vlane + buf * 2 * TL::BYTES, s, (bits & 2) != 0);
     }
   }
   w.settle();
@@ -795,12 +855,12 @@ __device__ void keys_workgroup(const Params& p, char* lds, float* joint, const R
     }
   };
   const uint32_t klane = kl + TL::k_lane(lane), vlane = kl + TL::BYTES + TL::v_lane(lane);
-  auto exact = [&](uint32_t tile) {
+  auto past = [&](uint32_t tile) {
     if constexpr (sizeof(T) == 2) return false;
     Range r;
 #pragma unroll
     for (int n = 0; n < NI; ++n) r.see(*lds_at<float4v>(tile + n * 1024 + lane * 16));
-    return exact_needed(r.bits());
+    return r.past();
   };
   Wave<T, DP> w;
   int t = tbeg + wave;
@@ -822,13 +882,13 @@ __device__ void keys_workgroup(const Params& p, char* lds, float* joint, const R
     // Waits for K, then for V: only the instructions issued after it may be in flight (others among them only
     // make it wait longer).
     wait_dma_le<NI>();
-    w.template products<1, TL>(klane, s, exact(kl));
+    w.template products<1, TL>(klane, s, past(kl));
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K has been read before the next K overwrites it
     if (more) issue(t + 4, next, false);
     w.template weights<1>(s, sc, row, pos0, left, last_seen, lane);
     if (more) wait_dma_le<NI>();
     else wait_dma_le<0>();
-    w.template add<1, TL>(vlane, s, exact(kl + TL::BYTES));
+    w.template add<1, TL>(vlane, s, past(kl + TL::BYTES));
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if (more) issue(t + 4, next, true);
     next = page_of(t + 8);

@@ -133,7 +133,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_offsets: t
 
     Scores are ``scale * q.k`` (scale: 1 / sqrt(d)), then ``softcap * tanh(score / softcap)`` if softcap is not 0,
     then less ``slopes[head]`` (fp32) times the distance of the two positions. Returns q's shape and type,
-    contiguous. Scores, softmax and sums are fp32; with fp16 inputs the weights are rounded to fp16."""
+    contiguous. Scores, softmax and sums are fp32. With fp16 inputs the weights are rounded to fp16 (2^-12 of each at
+    most) for their product with the values; fp32 inputs are multiplied with all their bits, whatever their size."""
     out = direct().attention(q, k, v, q_offsets, k_offsets, causal, visible, shared_k, shared_v, scale, softcap, slopes)
     if out is not None:
         return out

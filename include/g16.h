@@ -362,8 +362,9 @@ int g16_peak_mfma_data(int blocks, int iters, const uint16_t* operands, int ngro
  *     s_ij -= slopes[head] * |p_i - p_j|                               (slopes NULL: nothing),
  *     out_i = sum_j softmax_j(s_ij) v_j,
  * zeros where a row sees no key. Query head h reads key head h / (hq / hkv). Types: fp16 or fp32 (is_f32),
- * head dimension d a multiple of 8 up to G16_ATTENTION_MAX_D; scores, softmax and sums in fp32 (fp16
- * weights are rounded to fp16 for their product with v).
+ * head dimension d a multiple of 8 up to G16_ATTENTION_MAX_D; scores, softmax and sums in fp32. With
+ * fp16 inputs the weights are rounded to fp16 for their product with v; fp32 inputs and their weights are multiplied
+ * with all their 24 bits, over fp32's range, each product to 2^-24.
  *   The keys of a sequence are `shared` common ones (positions 0 ..), then its own (positions shared ..).
  * g16_attention: its query rows stand at the end of its own keys, row t of lq at position
  * shared + lk - lq + t. q_offsets and k_offsets (int32, seqs + 1 values) give the sequences' runs in
