@@ -15,9 +15,10 @@
 //     bytes, whose lanes come in fours of different rows: 64 pieces, and the address unit takes them one by
 //     one (4096 x 4096 fp16, rank 32: 22 us).
 //   * expand: low is fp32, far from fp16's range in rows of massive activations. A row is scaled by a power of
-//     two to 2^14 .. 2^15 and taken as two fp16 parts (its largest value to 2^-22, smaller ones to 2^-22 of
-//     that), so two 16x16x32 MFMAs replace eight fp32 ones of twice the cycles each. The result passes
-//     through LDS, so that y is read and the output written in whole rows of 64 columns.
+//     two to 2^14 .. 2^15 and taken as three fp16 parts, each kept 2^11 above its size: all 24 bits of every value
+//     down to 2^-38 of the row's largest, past which it adds nothing that fp32 sums keep (`up` is fp16, so columns
+//     differ by 2^40 at most). Three 16x16x32 MFMAs, with a sum for each part, replace eight fp32 ones of twice the
+//     cycles each. The result passes through LDS, so that y is read and the output written in whole rows of 64 columns.
 //   * few rows whose adapters are small: expand computes low itself, in every workgroup (one launch less).
 // fp32 activations run on v_mfma_f32_16x16x4_f32: nothing is rounded.
 #include "g16_common.hpp"
@@ -291,8 +292,8 @@ __global__ __launch_bounds__(kThreads) void shrink_tiles_kernel(Params p) {
 // out = y + low @ up^T for 64 rows and p.chunks runs of 64 columns from blockIdx.y on. The wavefronts, and the
 // gridDim.z workgroups of the same rows and columns, share all (adapter, run) pairs; a pair's part of `up` is
 // loaded once for its rows (its fragments are 64 pieces a load, like shrink's: with 16 rows a workgroup they
-// took more time than y and the output, 4096 x 4096, rank 64: 47 us). The rows' low is summed up, scaled and
-// split once, into LDS. Bound by y and the output: 4111 x 4096, rank 32, fp16, is 101 MB in 25 us, 4 TB/s.
+// took more time than y and the output, 4096 x 4096, rank 64: 47 us). The rows' low is summed up and
+// scaled once, into LDS. Bound by y and the output: 4111 x 4096, rank 32, fp16, is 101 MB in 25 us, 4 TB/s.
 // RC: pieces of 32 rank columns.
 constexpr int kScrRow = 68;   // floats of a row of the wavefronts' LDS: rows start 4 banks apart
 constexpr int kManyRows = 64;
@@ -301,16 +302,44 @@ __device__ inline void store4(const Params& p, size_t at, float4v v) {
   if constexpr (OUT_F16) *reinterpret_cast<half4*>(static_cast<_Float16*>(p.out) + at) = __builtin_convertvector(v, half4);
   else *reinterpret_cast<float4v*>(static_cast<float*>(p.out) + at) = v;
 }
-// 2^e that takes `top`, a row's largest value, to 2^14 .. 2^15 (e held to what fp32 has both ways; infinities
-// stay as they are)
+// 2^e that takes `top`, a row's largest value, to 2^14 .. 2^15 (e held to what fp32 has both ways; 0 for infinities)
 __device__ inline int exponent_for(float top) {
   return top > 0.f && top < __builtin_huge_valf() ? min(max(14 - ilogbf(top), -120), 120) : 0;
 }
+// A value of a row with infinities: what is finite in it changes nothing, and might not fit fp16.
+__device__ inline float beside_infinity(float v) { return fabsf(v) < __builtin_huge_valf() ? 0.f : v; }
+
+// v = hi + 2^-11 (mid + 2^-11 lo). odd: rows with infinities, which have one part.
+struct Parts {
+  half8 hi, mid, lo;
+};
+__device__ inline Parts parts_of(float8v v, bool odd) {
+  Parts p;
+  p.hi = __builtin_convertvector(v, half8);
+  v = (v - widen(p.hi)) * 0x1p11f;
+  p.mid = __builtin_convertvector(v, half8);
+  v = (v - widen(p.mid)) * 0x1p11f;
+  p.lo = __builtin_convertvector(v, half8);
+  if (odd) p.mid = p.lo = half8{};
+  return p;
+}
+// 4 columns of `up` times a row's parts
+template <int RC>
+__device__ inline float4v mma_parts(const half8 (&up)[RC][4], int b, const Parts (&low)[RC]) {
+  float4v hi = {}, mid = {}, lo = {};
+#pragma unroll
+  for (int c = 0; c < RC; ++c) {
+    hi = mma16(up[c][b], low[c].hi, hi);
+    mid = mma16(up[c][b], low[c].mid, mid);
+    lo = mma16(up[c][b], low[c].lo, lo);
+  }
+  return hi + 0x1p-11f * (mid + 0x1p-11f * lo);
+}
 template <bool OUT_F16, int RC>
 __global__ __launch_bounds__(kThreads, RC == 1 ? 4 : 2) void expand_kernel(Params p) {
-  constexpr int kLow = 32 * RC + 8;  // halves of a row: rows start 4 banks times an odd number apart
-  __shared__ __attribute__((aligned(16))) _Float16 s_hi[kManyRows][kLow], s_lo[kManyRows][kLow];
-  __shared__ float s_back[kManyRows];
+  constexpr int kLow = 32 * RC + 4;  // floats of a row: rows start 4 banks times an odd number apart
+  __shared__ __attribute__((aligned(16))) float s_low[kManyRows][kLow];
+  __shared__ float s_back[kManyRows];  // negative: a row with infinities
   __shared__ __attribute__((aligned(16))) float scratch[kWaves][kRows][kScrRow];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int m0 = blockIdx.x * kManyRows, q = lane >> 4;
@@ -350,14 +379,14 @@ __global__ __launch_bounds__(kThreads, RC == 1 ? 4 : 2) void expand_kernel(Param
     for (int i = 1; i < 8; i *= 2) top = fmaxf(top, __shfl_xor(top, i));
     const int e = exponent_for(top);
     const float by = ldexpf(1.f, e);
+    const bool odd = top == __builtin_huge_valf();
 #pragma unroll
     for (int c = 0; c < RC; ++c) {
-      const float4v x = v[c] * by;
-      const half4 hi = __builtin_convertvector(x, half4);
-      *reinterpret_cast<half4*>(&s_hi[r][32 * c + 4 * part]) = hi;
-      *reinterpret_cast<half4*>(&s_lo[r][32 * c + 4 * part]) = __builtin_convertvector(x - __builtin_convertvector(hi, float4v), half4);
+      float4v x = v[c] * by;
+      if (odd) x = float4v{beside_infinity(x[0]), beside_infinity(x[1]), beside_infinity(x[2]), beside_infinity(x[3])};
+      *reinterpret_cast<float4v*>(&s_low[r][32 * c + 4 * part]) = x;
     }
-    if (part == 0) s_back[r] = ldexpf(1.f, -e);
+    if (part == 0) s_back[r] = odd ? -1.f : ldexpf(1.f, -e);
   }
   __syncthreads();
   // The pairs: rows without an adapter count as one more (number `count`) where y has to be copied.
@@ -416,22 +445,17 @@ __global__ __launch_bounds__(kThreads, RC == 1 ? 4 : 2) void expand_kernel(Param
       if (a >= 0) {
         const int r = __shfl(order, 16 * s + (lane & 15));
         const float back = s_back[r];
-        half8 hi[RC], lo[RC];
+        Parts low[RC];
 #pragma unroll
         for (int c = 0; c < RC; ++c) {
-          hi[c] = *reinterpret_cast<const half8*>(&s_hi[r][32 * c + 8 * q]);
-          lo[c] = *reinterpret_cast<const half8*>(&s_lo[r][32 * c + 8 * q]);
+          const float4v x = *reinterpret_cast<const float4v*>(&s_low[r][32 * c + 8 * q]);
+          const float4v y = *reinterpret_cast<const float4v*>(&s_low[r][32 * c + 8 * q + 4]);
+          low[c] = parts_of(__builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7), back < 0.f);
         }
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-          float4v acc = {};
-#pragma unroll
-          for (int c = 0; c < RC; ++c) {
-            acc = mma16(up[c][b], hi[c], acc);
-            acc = mma16(up[c][b], lo[c], acc);
-          }
           // lane l: columns 16 b + 4 (l / 16) .. + 3 of row l % 16
-          *reinterpret_cast<float4v*>(&scr[lane & 15][16 * b + 4 * q]) = acc * back;
+          *reinterpret_cast<float4v*>(&scr[lane & 15][16 * b + 4 * q]) = mma_parts<RC>(up, b, low) * fabsf(back);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] += *reinterpret_cast<const float4v*>(&scr[q + 4 * j][col]);
@@ -465,7 +489,7 @@ __global__ __launch_bounds__(kThreads) void fused_kernel(Params p) {
   const int pairs = (t.count + (copy ? 1 : 0)) * runs;
   const int waves = kWaves * gridDim.z, w = wave + kWaves * blockIdx.z, p0 = pairs * w / waves, p1 = pairs * (w + 1) / waves;
   float(*scr)[kScrRow] = scratch[wave];
-  half8 hi[RC], lo[RC];
+  Parts parts[RC];
   float back = 1.f;
   int at = -1, a = -1;
   half8 up[RC][4];
@@ -512,12 +536,16 @@ __global__ __launch_bounds__(kThreads) void fused_kernel(Params p) {
     top = fmaxf(top, __shfl_xor(top, 32));
     const int e = exponent_for(top);
     const float by = ldexpf(1.f, e);
+    const bool odd = top == __builtin_huge_valf();
     back = ldexpf(1.f, -e);
 #pragma unroll
     for (int c = 0; c < RC; ++c) {
-      const float8v v = low[c] * by;
-      hi[c] = __builtin_convertvector(v, half8);
-      lo[c] = __builtin_convertvector(v - widen(hi[c]), half8);
+      float8v v = low[c] * by;
+      if (odd) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = beside_infinity(v[i]);
+      }
+      parts[c] = parts_of(v, odd);
     }
   };
   if (p0 < p1) load(p0);
@@ -546,14 +574,8 @@ __global__ __launch_bounds__(kThreads) void fused_kernel(Params p) {
     if (a >= 0) {
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
-        float4v acc = {};
-#pragma unroll
-        for (int c = 0; c < RC; ++c) {
-          acc = mma16(up[c][b], hi[c], acc);
-          acc = mma16(up[c][b], lo[c], acc);
-        }
         // lane l: columns 16 b + 4 (l / 16) .. + 3 of row l % 16
-        *reinterpret_cast<float4v*>(&scr[lane & 15][16 * b + 4 * q]) = acc * back;
+        *reinterpret_cast<float4v*>(&scr[lane & 15][16 * b + 4 * q]) = mma_parts<RC>(up, b, parts) * back;
       }
     }
     float4v v[4];

@@ -416,7 +416,8 @@ int g16_attention_decode(const g16_attention_args* args, void* stream);
  * G16_LORA_MAX_SIDE (offsets within a tile of rows are 32 bits); all contiguous, 16-byte aligned.
  * g16_lora_shrink leaves scale * x @ down^T in the workspace (fp32), g16_lora_expand does the rest: two launches,
  * between which the projection may run. Both take the same arguments and a workspace of
- * g16_lora_workspace_bytes(). Sums are fp32, and nothing is rounded before the output.
+ * g16_lora_workspace_bytes(). Sums are fp32, and no operand is rounded
+ * before the output.
  */
 #define G16_LORA_MAX_RANK 128
 #define G16_LORA_MAX_SIDE (1 << 21)

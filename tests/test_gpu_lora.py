@@ -225,3 +225,31 @@ def test_every_negative_index_means_no_adapter(cuda, M, K, x, out):
         torch.full((M, 136), float("nan"), dtype=out, device=cuda)  # (freed at once: likely the next output's memory)
         y = check(cuda, c, out)
         assert torch.equal(y[rows.to(cuda)], want[rows.to(cuda)])
+
+
+@pytest.mark.parametrize("M,K,r", [(1, 512, 16), (7, 256, 24), (40, 256, 16), (300, 512, 48), (300, 264, 128)])
+@pytest.mark.parametrize("x", [F16, F32])
+def test_channels_of_the_rank_of_unlike_size(cuda, M, K, r, x):
+    # large sums that meet small columns of `up` beside small ones that meet large columns, and make the result
+    c = make(M, K, 136, r, 3, x, seed=M + r)
+    c["w"] *= 2.0 ** -14
+    c["bias"] *= 0
+    c["down"] = (c["down"].float() * torch.where(torch.arange(r) % 3 == 0, 2.0 ** 15, 2.0 ** -13)[:, None]).half()
+    c["up"] = (c["up"].float() * torch.where(torch.arange(r) % 3 == 0, 2.0 ** -22, 2.0 ** 13)).half()
+    check(cuda, c, F32)
+
+
+@pytest.mark.parametrize("M", [3, 40, 300])
+def test_infinite_sums_of_an_adapter_stay_infinite(cuda, M):
+    # one sum past fp32 beside a huge finite one of the other sign, from finite activations
+    c = make(M, 64, 136, 16, 2, F32, seed=M, bias=False)
+    c["index"][:] = 1
+    c["down"].zero_()
+    c["down"][1, 0, 3], c["down"][1, 1, 4] = 1000.0, -1.0
+    c["up"] = c["up"].abs() + 0.1
+    plain = c["x"].clone()
+    c["x"][0, 3], c["x"][0, 4] = 1e38, 1e30
+    y = run(cuda, c, F32).cpu()
+    assert (y[0] == float("inf")).all()
+    ref, tol = reference(dict(c, x=plain), F32)
+    assert ((y.double() - ref).abs() / tol)[1:].max() <= 1.0
