@@ -3,7 +3,7 @@
 A small call is bound by the host: checked and packed in Python, one costs 8 us besides its launches, about
 as long as its kernels run. ``_g16fast`` does the same for arguments that need no copy, and returns None for
 any others; the Python functions then check them one by one, copy or raise. What it needs of this package
-(the device, the buffers kept per stream) it asks the functions here for.
+(the device, the buffers kept per stream and thread) it asks the functions here for.
 """
 from __future__ import annotations
 

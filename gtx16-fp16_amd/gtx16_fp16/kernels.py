@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import contextlib
 import threading
+from threading import get_ident
 
 import torch
 
@@ -211,21 +212,24 @@ _ARITY = {"rowscale_f32": 5, "rowscale_f16": 5, "hgemm_f32out": 8, "hgemm_f16out
 # ---- split-reduction buffers ----------------------------------------------------------------
 # The split-K GEMM and the skinny GEMV sum their K slices through two buffers: fp32 partials (no
 # initialisation needed) and per-tile arrival counters, which must be zero before first use and
-# which every call leaves zero again. One pair is kept per (device, stream) and grown on demand:
-# calls on one stream are ordered, so they can share it; calls on different streams get
-# different buffers.
+# which every call leaves zero again. One pair is kept per (device, stream, thread) and grown on
+# demand: calls of one thread on one stream are ordered, launch for launch, so they can share it.
+# Calls on different streams get different buffers, and so do threads that share a stream: a call
+# of several launches that meet in a buffer (a cast and its GEMM, the parts of an attention and their
+# join, the two products of an adapter) may have another thread's launches between its own. A
+# thread that reuses an ended one's identifier takes over its buffers, in stream order.
 #   A buffer that is replaced by a larger one is kept alive, never freed: a HIP graph captured
 # while it was current still writes to it on every replay, and if its memory went back to the
 # caching allocator, a later tensor could be placed there and overwritten by such a replay.
 # Growth doubles the size, so the retired buffers of a key add up to less than its current one.
 _ws_lock = threading.Lock()
-_partials: dict[tuple[int, int], torch.Tensor] = {}
-_counters: dict[tuple[int, int], torch.Tensor] = {}
-_scratch: dict[tuple[int, int], torch.Tensor] = {}
+_partials: dict[tuple[int, int, int], torch.Tensor] = {}
+_counters: dict[tuple[int, int, int], torch.Tensor] = {}
+_scratch: dict[tuple[int, int, int], torch.Tensor] = {}
 _retired: list[torch.Tensor] = []
-# (device index, stream) -> (partial bytes, counter bytes, the pointer tuple split_buffers returns):
-# the per-call lookup of a stream whose buffers are already large enough
-_current: dict[tuple[int, int], tuple] = {}
+# (device index, stream, thread) -> (partial bytes, counter bytes, the pointer tuple split_buffers
+# returns): the per-call lookup of a stream whose buffers are already large enough
+_current: dict[tuple[int, int, int], tuple] = {}
 _MIN_PARTIAL_BYTES = 1 << 20
 _MIN_COUNTER_BYTES = 64 << 10
 # mm_t's cast scratch is kept per stream up to this size (small GEMMs are bound by host time, and
@@ -254,7 +258,7 @@ def split_buffers(device: torch.device, stream: int, partial_bytes: int, counter
     ``stream``; (0, 0, 0, 0) when the call needs none."""
     if partial_bytes <= 0 and counter_bytes <= 0:
         return 0, 0, 0, 0
-    key = (device.index or 0, stream)
+    key = (device.index or 0, stream, get_ident())
     hit = _current.get(key)
     if hit is not None and hit[0] >= partial_bytes and hit[1] >= counter_bytes:
         return hit[2]
@@ -266,13 +270,14 @@ def split_buffers(device: torch.device, stream: int, partial_bytes: int, counter
 
 
 def scratch_buffer(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
-    """A uint8 device buffer of at least ``nbytes`` for the cast of one mm_t call on ``stream``:
-    kept per (device, stream) and reused by the next call there (calls on one stream are ordered)
-    up to 16 MiB; above that a fresh allocation per call. A buffer that is outgrown stays alive,
-    like the split buffers, since a captured graph may still use it."""
+    """A uint8 device buffer of at least ``nbytes`` for the cast of one mm_t call on ``stream``, or what else the
+    launches of one call pass on: kept per (device, stream, calling thread) and reused by the thread's next
+    call there (those are ordered) up to 16 MiB; above that a fresh allocation per call, which the caller holds until
+    its last launch is enqueued. A buffer that is outgrown stays alive, like the split buffers, since a captured graph
+    may still use it."""
     if nbytes > _MAX_CACHED_SCRATCH:
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
-    key = (device.index or 0, stream)
+    key = (device.index or 0, stream, get_ident())
     buf = _scratch.get(key)
     if buf is None or buf.numel() < nbytes:
         buf = _grown(_scratch, key, nbytes, 1 << 20, device, zero=False)

@@ -33,7 +33,10 @@
  *                    before the first use, and every call leaves them all zero again, so one
  *                    zero-filled counter buffer serves any sequence of calls on one stream.
  *     With ksplit == 1 neither is used (NULL/0 is fine). Calls that use the same buffers
- *     concurrently (different streams) race.
+ *     concurrently (different streams) race. So do calls of different threads on one stream that use
+ *     the same buffers, scratch and workspaces of every kind among them: a call may be several
+ *     launches, and another thread's may come between them. Every thread passes buffers of its own, or
+ *     the threads take turns, whole calls at a time (g16_lora_shrink to g16_lora_expand is one).
  *   - Results are deterministic: no floating-point atomics; split reductions sum partials in a
  *     fixed order, so repeated calls return identical bits.
  */
