@@ -82,10 +82,10 @@ def lora_mm_t(x2d: torch.Tensor, w_t: torch.Tensor, down: torch.Tensor, up: torc
     size, shrink, expand = _entry_points()
     stream = stream_handle(dev.index or 0)
     nbytes = fast.args_size(size, head)
-    # (without a workspace, expand computes both products)
-    ws = scratch_buffer(dev, stream, nbytes).data_ptr() if nbytes else None
+    # (without a workspace, expand computes both products; the tensor is held until both are enqueued)
+    ws = scratch_buffer(dev, stream, nbytes) if nbytes else None
     for fn in (shrink, expand) if nbytes else (expand,):
-        status = fast.args_call(fn, head, ws, nbytes, stream)
+        status = fast.args_call(fn, head, None if ws is None else ws.data_ptr(), nbytes, stream)
         if status != 0:
             _clib.check(status, "adapters")
     return out

@@ -253,3 +253,7 @@ def test_infinite_sums_of_an_adapter_stay_infinite(cuda, M):
     assert (y[0] == float("inf")).all()
     ref, tol = reference(dict(c, x=plain), F32)
     assert ((y.double() - ref).abs() / tol)[1:].max() <= 1.0
+
+
+def test_a_workspace_that_is_not_kept(cuda):
+    check(cuda, make(40000, 64, 64, 128, 3))

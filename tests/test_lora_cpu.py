@@ -1,7 +1,10 @@
 """CPU tests of the adapters' entry points: what the library rejects before a launch, and the workspace it asks for."""
 from __future__ import annotations
 
+import weakref
+
 import pytest
+import torch
 
 from gtx16_fp16 import _clib, lora
 
@@ -60,3 +63,33 @@ def test_workspace_holds_whole_splits(M, K, rank):
 def test_sides_past_32_bit_offsets_are_rejected(name, side):
     assert call(name, **{side: lora.MAX_SIDE + 8}) == SHAPE
     assert size(**{side: lora.MAX_SIDE}) > 0
+
+
+def test_the_workspace_lives_until_both_products_are_enqueued(monkeypatch):
+    # past the size that is kept between calls, nothing but the call holds it
+    made, seen = [], []
+
+    def scratch(dev, stream, nbytes):
+        t = torch.empty(nbytes, dtype=torch.uint8)
+        made.append(weakref.ref(t))
+        return t
+
+    class Fast:
+        lora_mm_t = staticmethod(lambda *args: None)
+        args_size = staticmethod(lambda fn, head: 20 << 20)
+
+        @staticmethod
+        def args_call(fn, head, ws, nbytes, stream):
+            seen.append(made[0]() is not None and made[0]().data_ptr() == ws and nbytes == 20 << 20)
+            return 0
+
+    monkeypatch.setattr(lora, "direct", Fast)
+    monkeypatch.setattr(lora._clib, "fast", Fast)
+    monkeypatch.setattr(lora, "scratch_buffer", scratch)
+    monkeypatch.setattr(lora, "stream_handle", lambda index: 0)
+    monkeypatch.setattr(lora, "_sm_count", lambda dev: 256)
+    monkeypatch.setattr(lora, "mm_t", lambda x, w, bias, dtype: torch.zeros(x.shape[0], w.shape[1], dtype=dtype))
+    x, w = torch.zeros(4, 8, dtype=torch.float16), torch.zeros(8, 8, dtype=torch.float16)
+    index = torch.zeros(4, dtype=torch.int32)
+    lora.lora_mm_t(x, w, torch.zeros(1, 8, 8, dtype=torch.float16), torch.zeros(1, 8, 8, dtype=torch.float16), index)
+    assert seen == [True, True] and made[0]() is None
