@@ -705,8 +705,9 @@ extern "C" int g16_lora_expand(const g16_lora_args* args, void* stream) {
   if (args == nullptr) return G16_E_NULL;
   const int st = check(*args);
   if (st != G16_OK || args->M == 0 || args->N == 0) return st;
+  if (args->rank == 0 && args->adapters > 0) return G16_E_SHAPE;  // (the kernels clamp to a row's last 8 values)
   const Plan plan = plan_of(*args);
-  if (args->rank > 0 && args->adapters > 0 && !plan.fused &&
+  if (args->adapters > 0 && !plan.fused &&
       (args->workspace == nullptr || static_cast<size_t>(args->workspace_bytes) < g16_lora_workspace_bytes(args)))
     return G16_E_WORKSPACE;
   if (!aligned16(args->workspace)) return G16_E_ALIGN;

@@ -93,3 +93,11 @@ def test_the_workspace_lives_until_both_products_are_enqueued(monkeypatch):
     index = torch.zeros(4, dtype=torch.int32)
     lora.lora_mm_t(x, w, torch.zeros(1, 8, 8, dtype=torch.float16), torch.zeros(1, 8, 8, dtype=torch.float16), index)
     assert seen == [True, True] and made[0]() is None
+
+
+def test_expand_rejects_adapters_of_rank_0():
+    # (few rows, where expand would compute both products, and many)
+    for M in (1, 20, 5000):
+        for out_is_f16 in (0, 1):
+            assert call("g16_lora_expand", rank=0, M=M, out_is_f16=out_is_f16) == SHAPE
+    assert call("g16_lora_expand", rank=0, M=0) == 0
