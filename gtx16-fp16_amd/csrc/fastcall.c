@@ -305,13 +305,15 @@ static int device_cus(int device) {
   return g_device_cus[device];
 }
 
-static int wants_grad(PyObject* const* tensors, int n) {
+/* Whether a gradient is wanted of one of args[which[0]] .. (tensors or None) */
+static int wants_grad(PyObject* const* args, const int* which, int n) {
   PyObject* r = PyObject_CallNoArgs(g_grad_enabled);
   int on = r != Py_False;
   Py_XDECREF(r);
   if (!on) return 0;
   for (int i = 0; i < n; ++i) {
-    r = PyObject_GetAttr(tensors[i], s_requires_grad);
+    if (args[which[i]] == Py_None) continue;
+    r = PyObject_GetAttr(args[which[i]], s_requires_grad);
     on = r != Py_False;
     Py_XDECREF(r);
     if (on) return 1;
@@ -447,6 +449,7 @@ static PyObject* run_attention(PyObject* q, int device, g16_attention_args* a, i
 }
 
 /* attention(q, k, v, q_offsets, k_offsets, causal, visible, shared_k, shared_v, scale, softcap, slopes) */
+static const int kGradAttention[6] = {0, 1, 2, 7, 8, 11};
 static PyObject* fast_attention(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
   (void)self;
   tensor_t q, k, v;
@@ -456,7 +459,7 @@ static PyObject* fast_attention(PyObject* self, PyObject* const* args, Py_ssize_
   memset(&a, 0, sizeof(a));
   const int packed = args[3] != Py_None;
   if (read_tensor(args[0], &q) || read_tensor(args[1], &k) || read_tensor(args[2], &v) || q.nd != (packed ? 3 : 4) || k.nd != q.nd ||
-      v.nd != q.nd || !heads_ok(&q, &k, &v, &a) || wants_grad(args, 3))
+      v.nd != q.nd || !heads_ok(&q, &k, &v, &a) || wants_grad(args, kGradAttention, 6))
     return none_clear();
   if (packed) {
     tensor_t o;
@@ -490,6 +493,7 @@ static PyObject* fast_attention(PyObject* self, PyObject* const* args, Py_ssize_
 }
 
 /* attention_decode(q, k_cache, v_cache, lengths, pages, shared_k, shared_v, scale, softcap, slopes) */
+static const int kGradDecode[6] = {0, 1, 2, 5, 6, 9};
 static PyObject* fast_attention_decode(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
   (void)self;
   tensor_t q, k, v;
@@ -499,7 +503,7 @@ static PyObject* fast_attention_decode(PyObject* self, PyObject* const* args, Py
   memset(&a, 0, sizeof(a));
   if (read_tensor(args[0], &q) || read_tensor(args[1], &k) || read_tensor(args[2], &v) || q.nd != 3 || k.nd != 4 || v.nd != 4 ||
       q.shape[0] == 0 || !fits(q.shape[0]) || !fits(k.shape[0]) || !fits(k.shape[1]) || k.shape[1] == 0 || !heads_ok(&q, &k, &v, &a) ||
-      wants_grad(args, 3) || vector(args[3], g_i32, q.shape[0], q.device, (const void**)&a.lengths) || a.lengths == NULL)
+      wants_grad(args, kGradDecode, 6) || vector(args[3], g_i32, q.shape[0], q.device, (const void**)&a.lengths) || a.lengths == NULL)
     return none_clear();
   a.seqs = (int)q.shape[0];
   a.q_len = 1;
@@ -591,6 +595,7 @@ static int run_product(const product_t* p, const g16_lora_args* a, const void* w
 }
 
 /* lora_mm_t(x2d, w_t, down, up, index, scale, bias, out_dtype) */
+static const int kGradLora[6] = {0, 1, 2, 3, 5, 6};
 static PyObject* fast_lora_mm_t(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
   (void)self;
   tensor_t x, w, down, up, t;
@@ -611,7 +616,7 @@ static PyObject* fast_lora_mm_t(PyObject* self, PyObject* const* args, Py_ssize_
       up.shape[2] != down.shape[1] || down.shape[1] % 8 != 0 || down.shape[1] > G16_LORA_MAX_RANK ||
       vector(args[4], g_i32, x.shape[0], x.device, (const void**)&a.index) || a.index == NULL ||
       vector(args[5], g_f32, down.shape[0], x.device, (const void**)&a.scale) || vector(args[6], g_f32, w.shape[1], x.device, &bias) ||
-      !aligned(bias) || (args[7] != g_f16 && args[7] != g_f32) || wants_grad(args, 4) || raw_stream(x.device, &stream))
+      !aligned(bias) || (args[7] != g_f16 && args[7] != g_f32) || wants_grad(args, kGradLora, 6) || raw_stream(x.device, &stream))
     return none_clear();
   a.M = (int)x.shape[0], a.K = (int)w.shape[0], a.N = (int)w.shape[1];
   a.adapters = (int)down.shape[0], a.rank = (int)down.shape[1];

@@ -11,7 +11,7 @@ import struct
 import torch
 
 from . import _clib
-from .direct import direct
+from .direct import direct, refuse_gradients
 from .kernels import scratch_buffer, stream_handle
 from .ops import _is_target, _sm_count
 
@@ -75,8 +75,6 @@ def _check(name: str, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, hq: int
         raise ValueError(f"{name}: the head dimension must be a multiple of 8 up to {MAX_HEAD_DIM}, got {d}")
     if hq and (not hkv or hq % hkv):
         raise ValueError(f"{name}: {hq} query heads do not share {hkv} key heads evenly")
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad()")
 
 
 def _shared(name: str, shared_k, shared_v, q: torch.Tensor, hkv: int, d: int, size: int):
@@ -144,6 +142,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_offsets: t
     hq, d = q.shape[-2:]
     hkv = k.shape[-2]
     _check("attention", q, k, v, hq, hkv, d)
+    refuse_gradients("attention", q, k, v, shared_k, shared_v, slopes)
     dev, size = q.device, q.element_size()
     if packed:
         if q_offsets.dim() != 1 or q_offsets.shape[0] < 1:
@@ -199,6 +198,7 @@ def attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     seqs, hq, d = q.shape
     hkv = k_cache.shape[2]
     _check("attention_decode", q, k_cache, v_cache, hq, hkv, d)
+    refuse_gradients("attention_decode", q, k_cache, v_cache, shared_k, shared_v, slopes)
     dev, size = q.device, q.element_size()
     lengths = _ints("attention_decode", lengths, (seqs,), dev, "lengths")
     page, max_pages = k_cache.shape[1], 0

@@ -48,6 +48,12 @@ def _route(device: int, stream: int, M: int, N: int, K: int, x_is_f32: int):
     return (1, ksplit, ops.ROW_SCALE_THRESHOLD, ptr, scratch, *bufs)
 
 
+def refuse_gradients(name: str, *tensors) -> None:
+    """Raise for the first of ``tensors`` (None among them) that a gradient is wanted of: the kernels have none."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad()")
+
+
 _bound = None
 
 

@@ -10,7 +10,7 @@ import struct
 import torch
 
 from . import _clib
-from .direct import direct
+from .direct import direct, refuse_gradients
 from .kernels import scratch_buffer, stream_handle
 from .linear import FastLinear
 from .ops import _aligned, _sm_count, mm_t
@@ -42,8 +42,6 @@ def _check(x2d: torch.Tensor, w_t: torch.Tensor, down: torch.Tensor, up: torch.T
         raise ValueError(f"lora_mm_t: index must be an int32 tensor of shape ({x2d.shape[0]},) on {dev}")
     if scale is not None and not (scale.dtype == torch.float32 and scale.shape == (n,) and scale.device == dev):
         raise ValueError(f"lora_mm_t: scale must be an fp32 tensor of shape ({n},) on {dev}")
-    if torch.is_grad_enabled() and (x2d.requires_grad or down.requires_grad or up.requires_grad):
-        raise RuntimeError("lora_mm_t has no gradient: call it under torch.no_grad()")
 
 
 def lora_mm_t(x2d: torch.Tensor, w_t: torch.Tensor, down: torch.Tensor, up: torch.Tensor, index: torch.Tensor, *,
@@ -63,6 +61,7 @@ def lora_mm_t(x2d: torch.Tensor, w_t: torch.Tensor, down: torch.Tensor, up: torc
     if out_dtype not in (torch.float32, torch.float16):
         raise ValueError(f"out_dtype must be float32 or float16, got {out_dtype}")
     _check(x2d, w_t, down, up, index, scale)
+    refuse_gradients("lora_mm_t", x2d, w_t, down, up, scale, bias)
     x2d = _aligned(x2d)
     y = mm_t(x2d, w_t, bias, torch.float32)
     M, K = x2d.shape

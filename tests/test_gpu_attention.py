@@ -438,3 +438,22 @@ def test_many_short_sequences_of_every_width(cuda, dtype, d):
 @pytest.mark.parametrize("lens_q,lens_k", [([130, 0, 7], [1500, 3, 40]), ([1], [3000]), ([300], [300])])
 def test_few_tiles_split_over_the_keys(cuda, dtype, lens_q, lens_k):
     run_prompts(cuda, lens_q, lens_k, 2, 1, 72, dtype, causal=True, shared=100, slopes=True)
+
+
+def test_a_gradient_of_any_operand_is_refused(cuda):
+    q, k = torch.zeros(2, 8, 4, 64, dtype=F16, device=cuda), torch.zeros(2, 8, 2, 64, dtype=F16, device=cuda)
+    given = dict(shared_k=k[0].clone(), shared_v=k[1].clone(), slopes=torch.zeros(4, device=cuda))
+    n = torch.tensor([1, 2], dtype=torch.int32, device=cuda)
+    odd = torch.zeros(2, 8, 2, 72, dtype=F16, device=cuda)[..., 4:68]  # (a view that is copied: checked in Python)
+    for kk in (k, odd):
+        for name in ("q", "k", "v", *given):
+            ops = dict(q=q, k=kk, v=kk, **given)
+            ops[name] = ops[name].detach().clone().requires_grad_()
+            rest = {a: ops[a] for a in given}
+            for call in (lambda: g.attention(ops["q"], ops["k"], ops["v"], **rest),  # noqa: B023
+                         lambda: g.attention_decode(ops["q"][:, 0], ops["k"], ops["v"], n, **rest)):  # noqa: B023
+                with pytest.raises(RuntimeError, match="no_grad"):
+                    call()
+                    pytest.fail(f"{name} was taken")
+                with torch.no_grad():
+                    call()

@@ -257,3 +257,18 @@ def test_infinite_sums_of_an_adapter_stay_infinite(cuda, M):
 
 def test_a_workspace_that_is_not_kept(cuda):
     check(cuda, make(40000, 64, 64, 128, 3))
+
+
+@pytest.mark.parametrize("M", [4, 40])
+def test_a_gradient_of_any_operand_is_refused(cuda, M):
+    c = {k: v.to(cuda) for k, v in make(M, 64, 64, 8, 2).items()}
+    for view in (False, True):
+        for name in ("x", "w", "down", "up", "scale", "bias"):
+            d = dict(c, x=c["x"].t().contiguous().t()) if view else dict(c)
+            d[name] = d[name].detach().clone(memory_format=torch.preserve_format).requires_grad_()
+            call = lambda: g.lora_mm_t(d["x"], d["w"], d["down"], d["up"], d["index"], scale=d["scale"], bias=d["bias"])  # noqa: E731,B023
+            with pytest.raises(RuntimeError, match="no_grad"):
+                call()
+                pytest.fail(f"{name} was taken")
+            with torch.no_grad():
+                call()
