@@ -9,9 +9,10 @@ from __future__ import annotations
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _clib
-from .direct import direct, refuse_gradients
+from .direct import direct, refuse_gradients, refuse_tangents
 from .kernels import scratch_buffer, stream_handle
 from .ops import _is_target, _sm_count
 
@@ -133,6 +134,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_offsets: t
     then less ``slopes[head]`` (fp32) times the distance of the two positions. Returns q's shape and type,
     contiguous. Scores, softmax and sums are fp32. With fp16 inputs the weights are rounded to fp16 (2^-12 of each at
     most) for their product with the values; fp32 inputs are multiplied with all their bits, whatever their size."""
+    if forward_ad._current_level >= 0:
+        refuse_tangents("attention", q, k, v, shared_k, shared_v, slopes)
     out = direct().attention(q, k, v, q_offsets, k_offsets, causal, visible, shared_k, shared_v, scale, softcap, slopes)
     if out is not None:
         return out
@@ -190,6 +193,8 @@ def attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     it holds, and a page number outside the cache reads as zeros. ``shared_k`` and ``shared_v`` [prefix, key heads, d]
     come before every request's own keys. The token stands at its last key's position. Types, heads, scores
     and the result are ``attention``'s; a request without any key gives zeros."""
+    if forward_ad._current_level >= 0:
+        refuse_tangents("attention_decode", q, k_cache, v_cache, shared_k, shared_v, slopes)
     out = direct().attention_decode(q, k_cache, v_cache, lengths, pages, shared_k, shared_v, scale, softcap, slopes)
     if out is not None:
         return out

@@ -8,6 +8,7 @@ any others; the Python functions then check them one by one, copy or raise. What
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _clib, ops
 from .kernels import _MAX_CACHED_SCRATCH, SKINNY_MAX_M, scratch_buffer, split_buffers
@@ -46,6 +47,13 @@ def _route(device: int, stream: int, M: int, N: int, K: int, x_is_f32: int):
     ptr = scratch_buffer(dev, stream, scratch).data_ptr() if scratch else 0
     bufs = split_buffers(dev, stream, partials, counters) if kind == "splitk" else (0, 0, 0, 0)
     return (1, ksplit, ops.ROW_SCALE_THRESHOLD, ptr, scratch, *bufs)
+
+
+def refuse_tangents(name: str, *tensors) -> None:
+    """Raise for the first of ``tensors`` (None among them) with a forward-mode tangent. Called only inside a
+    ``forward_ad.dual_level()``; outside there are none."""
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{name} has no forward-mode derivative: pass it the tensors without their tangents")
 
 
 def refuse_gradients(name: str, *tensors) -> None:

@@ -8,9 +8,10 @@ from __future__ import annotations
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _clib
-from .direct import direct, refuse_gradients
+from .direct import direct, refuse_gradients, refuse_tangents
 from .kernels import scratch_buffer, stream_handle
 from .linear import FastLinear
 from .ops import _aligned, _sm_count, mm_t
@@ -55,6 +56,8 @@ def lora_mm_t(x2d: torch.Tensor, w_t: torch.Tensor, down: torch.Tensor, up: torc
     negative (or past the last adapter) for none; scale fp32 [adapters] or None. x2d, w_t, bias and out_dtype
     are mm_t's, and so is the shared product, rounding of fp32 activations included; the adapters' part is
     computed from the activations as they are, in fp32, and added before the one rounding to out_dtype."""
+    if forward_ad._current_level >= 0:
+        refuse_tangents("lora_mm_t", x2d, w_t, down, up, scale, bias)
     out = direct().lora_mm_t(x2d, w_t, down, up, index, scale, bias, out_dtype)
     if out is not None:
         return out
