@@ -53,6 +53,7 @@ template <typename T>
 constexpr float kScale = sizeof(T) == 2 ? 1.f : 0x1p-23f;
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kPlainCap = 256.f;  // largest tanh cap that fp16 inputs take the plain form for (tanh_of)
+constexpr float kNoCap = 0x1p100f;  // a cap from here on changes no fp32 score below 2^88, and would not fit in log2 units
 constexpr int kRowTile = 128, kKeyTile = 32;  // query rows of the two workgroup shapes
 constexpr int kThreads = 256;
 
@@ -316,11 +317,12 @@ struct Scoring {
 __device__ inline Scoring scoring(const Params& p) {
   Scoring s;
   s.c = p.scale * kLog2e;
-  s.capped = p.softcap != 0.f;
+  s.capped = p.softcap != 0.f && p.softcap < kNoCap;
   s.fine = p.softcap > kPlainCap;
   s.biased = p.slopes != nullptr;
   s.cap = p.softcap * kLog2e;
-  s.inv = s.capped ? p.scale / p.softcap : 0.f;
+  // (held to where no score's product with it is 0 times infinity; past that every score is at a cap of nearly 0)
+  s.inv = s.capped ? fminf(p.scale / p.softcap, 1e37f) : 0.f;
   s.inv2 = s.inv * (2.f * kLog2e);
   return s;
 }
@@ -1345,7 +1347,7 @@ int check(const g16_attention_args& a, bool decode) {
       a.d > G16_ATTENTION_MAX_D)
     return G16_E_SHAPE;
   if (a.seqs == 0 || a.hq == 0 || (!decode && a.q_len == 0)) return G16_OK;
-  if (a.hkv == 0 || a.hq % a.hkv != 0 || !(a.softcap >= 0.f) || !(a.scale == a.scale)) return G16_E_SHAPE;
+  if (a.hkv == 0 || a.hq % a.hkv != 0 || !(a.softcap >= 0.f && a.softcap <= FLT_MAX) || !(a.scale == a.scale)) return G16_E_SHAPE;
   if (static_cast<int64_t>(a.shared) + a.k_len > (1 << 30) || static_cast<int64_t>(a.q_len) * a.hq > (1LL << 31) - 1 ||
       static_cast<int64_t>(a.seqs) * a.hq > (1LL << 31) - 1)
     return G16_E_SHAPE;

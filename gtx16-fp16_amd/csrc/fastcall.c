@@ -11,6 +11,7 @@
  */
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
+#include <float.h>
 #include <math.h>
 #include <stddef.h>
 #include <stdint.h>
@@ -393,7 +394,8 @@ static int rest_ok(PyObject* scale, PyObject* cap, PyObject* sk, PyObject* sv, P
   if (scale == Py_None) {
     s = 1.0 / sqrt((double)a->d);
   }
-  if (s != s || !(c >= 0.0 && c < 1e300)) return 0;
+  /* (what fp32 cannot hold is left to the Python function, which says so) */
+  if (s != s || (fabs(s) > FLT_MAX && !isinf(s)) || !(c >= 0.0 && c <= FLT_MAX) || (c > 0.0 && (float)c == 0.0f)) return 0;
   a->scale = (float)s;
   a->softcap = (float)c;
   if (vector(slopes, g_f32, a->hq, device, (const void**)&a->slopes)) return 0;

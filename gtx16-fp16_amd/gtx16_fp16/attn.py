@@ -19,6 +19,7 @@ from .ops import _is_target, _sm_count
 MAX_HEAD_DIM = 128          # G16_ATTENTION_MAX_D
 _MAX_STRIDE = 1 << 24       # G16_ATTENTION_MAX_STRIDE: bytes between a key row and the next
 _F16, _F32 = torch.float16, torch.float32
+_FLT_MAX = torch.finfo(torch.float32).max
 
 # g16_attention_args without its workspace
 _ARGS = struct.Struct("@12P13q13i2fi")
@@ -102,8 +103,10 @@ def _slopes(name: str, slopes, hq: int, dev: torch.device):
 def _numbers(name: str, scale, softcap: float, d: int) -> tuple[float, float]:
     scale = d ** -0.5 if scale is None else float(scale)
     softcap = float(softcap or 0.0)
-    if scale != scale or not 0.0 <= softcap < float("inf"):
-        raise ValueError(f"{name}: scale must be a number and softcap at least 0, got {scale} and {softcap}")
+    if scale != scale or _FLT_MAX < abs(scale) < float("inf"):
+        raise ValueError(f"{name}: scale must be a number that fp32 holds, got {scale}")
+    if not 0.0 <= softcap <= _FLT_MAX or (softcap and not struct.unpack("f", struct.pack("f", softcap))[0]):
+        raise ValueError(f"{name}: softcap must be 0 (none) or a positive number that fp32 holds, got {softcap}")
     return scale, softcap
 
 

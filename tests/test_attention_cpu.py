@@ -126,3 +126,17 @@ def test_what_no_launch_takes_is_rejected():
     # rows of all sequences past 32 bits
     equal = dict(seqs=1 << 22, q_len=1 << 22, k_len=8, hq=2, hkv=2)
     assert plan(**equal) == (SHAPE, 0, 0) and call("g16_attention", **equal) == SHAPE
+
+
+@pytest.mark.parametrize("name", ["g16_attention", "g16_attention_decode"])
+def test_an_infinite_cap_is_rejected(name):
+    assert call(name, softcap=float("inf")) == SHAPE
+
+
+def test_numbers_that_fp32_does_not_hold_are_refused():
+    assert attn._numbers("attention", None, 0.0, 64) == (0.125, 0.0)
+    assert attn._numbers("attention", -3.0, 1e-40, 64) == (-3.0, 1e-40)
+    for scale, cap in ((1e39, 0.0), (-1e300, 0.0), (float("nan"), 0.0), (1.0, 1e39), (1.0, float("inf")), (1.0, float("nan")), (1.0, -1.0),
+                       (1.0, 1e-60)):
+        with pytest.raises(ValueError, match="attention: s"):
+            attn._numbers("attention", scale, cap, 64)

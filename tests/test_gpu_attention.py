@@ -457,3 +457,19 @@ def test_a_gradient_of_any_operand_is_refused(cuda):
                     pytest.fail(f"{name} was taken")
                 with torch.no_grad():
                     call()
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_caps_of_all_sizes(cuda, dtype):
+    q, k = torch.zeros(1, 8, 4, 64, dtype=dtype, device=cuda), torch.zeros(1, 8, 2, 64, dtype=dtype, device=cuda)
+    n = torch.ones(1, dtype=torch.int32, device=cuda)
+    for bad in (1e39, 1e100, 1e299, 1e-60, float("inf")):
+        for call in (lambda: g.attention(q, k, k, softcap=bad), lambda: g.attention_decode(q[:, 0], k, k, n, softcap=bad),  # noqa: B023
+                     lambda: g.attention(q, k, k, scale=bad if 1 < bad < 1e300 else float("nan"))):  # noqa: B023
+            with pytest.raises(ValueError):
+                call()
+                pytest.fail(f"{bad} was taken")
+    for cap in (1e-44, 1e-38, 1e-6, 257.0, 1e6, 1e30, 3e38):
+        run_prompts(cuda, [40, 1], [50, 3], 4, 2, 64, dtype, softcap=cap, causal=True, seed=3, what=str(cap))
+        # (scores of exactly 0 have a weight, whatever the cap)
+        assert (g.attention(q, k, k + 1, softcap=cap) == 1).all()
