@@ -179,6 +179,18 @@ class FastLinear(nn.Module):
             self._wp_key = key
         return self._wp
 
+    def _packed_for(self, x2: torch.Tensor) -> torch.Tensor | None:
+        # the prepacked copy of weight_t where a call with these rows gains by it
+        # On 256x128 tiles a prepacked weight gains where the batch has more rows than the layer columns, up
+        # to 6 % (8241 x 896 x 744 fp16 33.1 -> 31.9 us, 2339 x 5760 x 2056 105.0 -> 100.6, 3291 x 4256 x 1304
+        # 88.7 -> 83.4), and loses below, up to 4 % (777 x 3072 x 8192 57.0 -> 59.5, 2086 x 3728 x 3072 76.7 ->
+        # 79.4): there it serves them only where it lets layers share one cast.
+        M = x2.shape[0]
+        cols = _gemm_route(_clib.load(), M, self.out_features, self.in_features, x2.device)[7]
+        if cols == 256 or (cols and (M >= self.out_features or self.share_cast)):
+            return self._packed_weight()
+        return None
+
     def _decode_weight(self) -> int:
         # pointer of the decode-layout copy of weight_t, (re)built like the prepacked copy; 0 when it
         # is not current and the stream is being captured
@@ -275,15 +287,7 @@ class FastLinear(nn.Module):
             odt = torch.float32 if out_dtype == torch.float32 else torch.float16
             M = x2.shape[0]
             b = self.bias
-            wp = None
-            # On 256x128 tiles a prepacked weight gains where the batch has more rows than the layer columns, up
-            # to 6 % (8241 x 896 x 744 fp16 33.1 -> 31.9 us, 2339 x 5760 x 2056 105.0 -> 100.6, 3291 x 4256 x 1304
-            # 88.7 -> 83.4), and loses below, up to 4 % (777 x 3072 x 8192 57.0 -> 59.5, 2086 x 3728 x 3072 76.7 ->
-            # 79.4): there it serves them only where it lets layers share one cast.
-            if self.prepack_weight and M > SKINNY_MAX_M:
-                cols = _gemm_route(_clib.load(), M, self.out_features, self.in_features, x2.device)[7]
-                if cols == 256 or (cols and (M >= self.out_features or self.share_cast)):
-                    wp = self._packed_weight()
+            wp = self._packed_for(x2) if self.prepack_weight and M > SKINNY_MAX_M else None
             if wp is not None:
                 y = mm_t_prepacked(x2, self.weight_t, wp, b, odt, _cast_source=x if self.share_cast else None)
             elif (self.prepack_decode and M <= STRIPS_MAX_M and x2.device == self.weight_t.device

@@ -12,9 +12,9 @@ from torch.autograd import forward_ad
 
 from . import _clib
 from .direct import direct, refuse_gradients, refuse_tangents
-from .kernels import scratch_buffer, stream_handle
+from .kernels import SKINNY_MAX_M, scratch_buffer, stream_handle
 from .linear import FastLinear
-from .ops import _aligned, _sm_count, mm_t
+from .ops import _aligned, _gemm_route, _sm_count, mm_t, mm_t_prepacked
 
 MAX_RANK = 128  # G16_LORA_MAX_RANK
 MAX_SIDE = 1 << 21  # G16_LORA_MAX_SIDE
@@ -66,9 +66,14 @@ def lora_mm_t(x2d: torch.Tensor, w_t: torch.Tensor, down: torch.Tensor, up: torc
     _check(x2d, w_t, down, up, index, scale)
     refuse_gradients("lora_mm_t", x2d, w_t, down, up, scale, bias)
     x2d = _aligned(x2d)
-    y = mm_t(x2d, w_t, bias, torch.float32)
-    M, K = x2d.shape
-    N, (n, r) = w_t.shape[1], down.shape[:2]
+    return _add_adapters(x2d, mm_t(x2d, w_t, bias, torch.float32), down, up, index, scale, out_dtype)
+
+
+def _add_adapters(x2d: torch.Tensor, y: torch.Tensor, down: torch.Tensor, up: torch.Tensor, index: torch.Tensor, scale,
+                  out_dtype: torch.dtype) -> torch.Tensor:
+    """The adapters' part beside the shared product ``y`` (fp32, written to where out_dtype is fp32); checked operands."""
+    (M, K), N = x2d.shape, y.shape[1]
+    n, r = down.shape[:2]
     dev = x2d.device
     out = y if out_dtype == torch.float32 else torch.empty(M, N, device=dev, dtype=out_dtype)
     if out.numel() == 0:
@@ -98,6 +103,13 @@ class AdapterLinear(FastLinear):
     row: ``layer(x, index)`` with index as in ``lora_mm_t``, one value for each row of x (all leading
     dimensions flattened, in their order); ``layer(x)`` is the FastLinear.
 
+    Types, shapes and fallbacks are FastLinear's: with an index, too, large batches read the prepacked copy of the
+    weight, and what the kernels cannot take (CPU tensors, other devices, sizes that are no multiples of 8, converted
+    buffers) or have no gradient for is computed by torch operations, the adapters' part in fp32; gradients then reach
+    x and, where they require them, ``down``, ``up`` and ``scale``. ``prepack_decode`` has no effect on calls with an
+    index: token by token the host makes the shared product and the adapters' part in one go, which costs less than
+    the decode layout saves.
+
     State: FastLinear's ``weight_t`` and ``bias``, and ``down`` [adapters, rank, in_features], ``up`` [adapters,
     out_features, rank] in fp16, ``scale`` [adapters] in fp32. A new layer's adapters change nothing (``up`` is
     zero)."""
@@ -121,13 +133,59 @@ class AdapterLinear(FastLinear):
         m.scale = torch.ones(adapters, dtype=torch.float32, device=dev)
         return m
 
+    def _plain(self, x: torch.Tensor, index: torch.Tensor) -> torch.Tensor:
+        # FastLinear's result and the adapters, by torch operations
+        y = super().forward(x)
+        acc = torch.promote_types(y.dtype, torch.float32)
+        x2, add = x.reshape(-1, self.in_features).to(acc), []
+        for a in index.unique().tolist():
+            if 0 <= a < self.down.shape[0]:
+                at = (index == a).nonzero().flatten()
+                add.append((at, self.scale[a].to(acc) * (x2[at] @ self.down[a].to(acc).t() @ self.up[a].to(acc).t())))
+        if not add:
+            return y
+        part = torch.zeros(x2.shape[0], self.out_features, device=x2.device, dtype=acc).index_copy(
+            0, torch.cat([at for at, _ in add]), torch.cat([z for _, z in add]))
+        return (y.reshape(part.shape).to(acc) + part).to(y.dtype).view(y.shape)
+
+    def _takes(self, x: torch.Tensor) -> bool:
+        # what lora_mm_t computes with these buffers
+        d, u = self.down, self.up
+        return (x.is_cuda and self._operands_ok(self.weight_t, None, x.device) and d.dtype == u.dtype == torch.float16
+                and d.device == u.device == self.scale.device == x.device
+                and not (torch.is_grad_enabled() and any(t.requires_grad for t in (x, d, u, self.scale))))
+
+    def _may_pack(self, M: int, dev: torch.device) -> bool:
+        # whether a prepacked weight can serve M rows
+        K, N = self.in_features, self.out_features
+        return self.prepack_weight and M > SKINNY_MAX_M and not (K | N) % 8 and _gemm_route(_clib.load(), M, N, K, dev)[7] != 0
+
     def forward(self, x: torch.Tensor, index: torch.Tensor | None = None) -> torch.Tensor:
         if index is None:
             return super().forward(x)
+        w, scale, bias = self.weight_t, self.scale, self.bias
         dtype = x.dtype if x.dtype in (torch.float16, torch.float32) else torch.float32
-        x2 = x.reshape(-1, self.in_features)
-        y = lora_mm_t(x2 if x2.dtype == dtype else x2.float(), self.weight_t, self.down, self.up, index.reshape(-1), scale=self.scale,
-                      bias=self.bias, out_dtype=dtype)
+        x2, rows = x.reshape(-1, self.in_features), index.reshape(-1)
+        M, y = x2.shape[0], None
+        # (first what needs no look at the operands here: small calls are bound by the host)
+        if M and x.is_cuda and forward_ad._current_level < 0 and not self._may_pack(M, x.device):
+            y = direct().lora_mm_t(x2, w, self.down, self.up, rows, scale, bias, dtype)
+        if y is None:
+            if not (rows.dtype == torch.int32 and rows.shape[0] == M and rows.device == x.device):
+                raise ValueError(f"AdapterLinear: index must hold {M} int32 values on {x.device}, one for each row of x")
+            if M == 0 or not self._takes(x):
+                return self._plain(x, rows)
+            x2 = x2 if x2.dtype == dtype else x2.float()
+            scale = scale if scale.dtype == torch.float32 else scale.float()
+            wp = self._packed_for(x2) if self._may_pack(M, x.device) else None
+            if wp is None:
+                y = lora_mm_t(x2, w, self.down, self.up, rows, scale=scale, bias=bias, out_dtype=dtype)
+            else:  # (lora_mm_t with the shared product from the prepacked weight, whose bits are mm_t's)
+                _check(x2, w, self.down, self.up, rows, scale)
+                refuse_tangents("AdapterLinear", x, self.down, self.up, scale)
+                x2 = _aligned(x2)
+                y = mm_t_prepacked(x2, w, wp, bias, torch.float32, _cast_source=x if self.share_cast else None)
+                y = _add_adapters(x2, y, self.down, self.up, rows, scale, dtype)
         return y.view(*x.shape[:-1], self.out_features)
 
     def extra_repr(self) -> str:
