@@ -61,6 +61,7 @@ struct Params {
   void* out;
   float* low;  // [splits][M][rank]
   int M, K, N, rank, adapters, tiles, slots, splits, chunks;
+  int first;  // row of the launch's first tile
 };
 
 // A row's adapter: -1 for every index that names none.
@@ -162,7 +163,7 @@ template <typename T, int RB>
 __global__ __launch_bounds__(kThreads) void shrink_kernel(Params p) {
   __shared__ float4v part[kWaves][RB][kWave];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int m0 = static_cast<int>(blockIdx.x % p.tiles) * kRows, slot = blockIdx.x / p.tiles, split = blockIdx.y;
+  const int m0 = p.first + static_cast<int>(blockIdx.x % p.tiles) * kRows, slot = blockIdx.x / p.tiles, split = blockIdx.y;
   const Adapters t = adapters_of(p, m0);
   if (slot >= t.count) return;
   const int steps = ceil_div(p.K, 32), of = p.splits * kWaves, at = split * kWaves + wave;
@@ -194,7 +195,7 @@ __global__ __launch_bounds__(kThreads) void shrink_tiles_kernel(Params p) {
   constexpr int kLds = S::COUNT * S::BYTES > kWaves * RB * kWave * 16 ? S::COUNT * S::BYTES : kWaves * RB * kWave * 16;
   __shared__ __attribute__((aligned(1024))) char lds[kLds];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int lin = static_cast<int>(blockIdx.x), m0 = lin % p.tiles * kRows, slot = lin / p.tiles, split = blockIdx.y;
+  const int lin = static_cast<int>(blockIdx.x), m0 = p.first + lin % p.tiles * kRows, slot = lin / p.tiles, split = blockIdx.y;
   const Adapters t = adapters_of(p, m0);
   if (slot >= t.count) return;
   const int count = (t.count - slot + p.slots - 1) / p.slots;  // this slot's adapters: slot, slot + slots, ..
@@ -342,7 +343,7 @@ __global__ __launch_bounds__(kThreads, RC == 1 ? 4 : 2) void expand_kernel(Param
   __shared__ float s_back[kManyRows];  // negative: a row with infinities
   __shared__ __attribute__((aligned(16))) float scratch[kWaves][kRows][kScrRow];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int m0 = blockIdx.x * kManyRows, q = lane >> 4;
+  const int m0 = p.first + static_cast<int>(blockIdx.x) * kManyRows, q = lane >> 4;
   // the adapter of row m0 + lane, and the list of all
   const int mine = adapter_of(p, m0 + lane);
   int ids = -1, count = 0;
@@ -602,7 +603,7 @@ __global__ __launch_bounds__(kThreads) void fused_kernel(Params p) {
 
 int check(const g16_lora_args& a) {
   if ((a.x_is_f32 | a.out_is_f16) & ~1) return G16_E_DTYPE;
-  if (a.M < 0 || a.K < 0 || a.N < 0 || a.adapters < 0 || a.rank < 0 || a.K % 8 != 0 || a.N % 8 != 0 || a.rank % 8 != 0 ||
+  if (a.M < 0 || a.M > INT32_MAX - kManyRows || a.K < 0 || a.N < 0 || a.adapters < 0 || a.rank < 0 || a.K % 8 != 0 || a.N % 8 != 0 || a.rank % 8 != 0 ||
       a.rank > G16_LORA_MAX_RANK || a.K > G16_LORA_MAX_SIDE || a.N > G16_LORA_MAX_SIDE)
     return G16_E_SHAPE;
   if (a.M == 0 || a.N == 0) return G16_OK;
@@ -621,14 +622,15 @@ Plan plan_of(const g16_lora_args& a) {
   p.tiles = ceil_div(a.M, kRows);
   p.fused = a.M <= kRows && static_cast<int64_t>(a.M) * a.rank * a.K <= kFusedWeights;
   p.staged = p.tiles >= kStagedTiles && a.K >= 2 * kChunk;
-  // Staged: K in as many parts as make about two workgroups a CU, of at least two chunks, then the adapters a
-  // tile may have on as many as still do; else an adapter a workgroup (a tile has at most 16, and there are
-  // few tiles), and up to 8 steps of K a wavefront.
+  // Staged: K in as many parts as make about two workgroups a CU, of at least two chunks; else up to 8 steps of K a
+  // wavefront. Few tiles: an adapter a workgroup (a tile has at most 16). More: the adapters a tile may have on as many
+  // workgroups as still make two a CU, eight where they read little each (with 16 for every tile, 100000 rows of
+  // 256, rank 16, 8 adapters: 499 us in runs 228, so 431 and 165; 4000 rows, 32 at random: 70, with two a CU 75).
   p.splits = p.staged ? (2 * cus + p.tiles - 1) / p.tiles : ceil_div(ceil_div(a.K, 32), 8 * kWaves);
   const int most = p.staged ? (a.K / (2 * kChunk) < 4 ? a.K / (2 * kChunk) : 4) : 8;
   if (p.splits > most) p.splits = most;
   if (p.splits < 1) p.splits = 1;
-  p.slots = p.staged ? 2 * cus / (p.tiles * p.splits) : kRows;
+  p.slots = p.tiles < kStagedTiles ? kRows : static_cast<int>((p.staged ? 2 : 8) * cus / (static_cast<int64_t>(p.tiles) * p.splits));
   if (p.slots > kRows) p.slots = kRows;
   if (p.slots > a.M) p.slots = a.M;
   if (p.slots < 1) p.slots = 1;
@@ -645,14 +647,24 @@ Plan plan_of(const g16_lora_args& a) {
 
 Params params(const g16_lora_args& a, const Plan& plan) {
   return Params{a.x, reinterpret_cast<const _Float16*>(a.down), reinterpret_cast<const _Float16*>(a.up), a.index, a.scale, a.y, a.out,
-                static_cast<float*>(a.workspace), a.M, a.K, a.N, a.rank, a.adapters, plan.tiles, plan.slots, plan.splits, plan.chunks};
+                static_cast<float*>(a.workspace), a.M, a.K, a.N, a.rank, a.adapters, plan.tiles, plan.slots, plan.splits, plan.chunks, 0};
 }
 
+// A launch's workgroups in x: 2^32 threads, which the rows of the largest batches pass; they are dealt to several.
+constexpr int kMostGroups = (1 << 23) - 1;
+
 template <typename T, int RB>
-int run_shrink_as(const Params& p, const Plan& plan, hipStream_t s) {
+int run_shrink_as(Params p, const Plan& plan, hipStream_t s) {
   const dim3 block(kThreads);
-  const dim3 grid(plan.tiles * plan.slots, plan.splits);
-  return plan.staged ? launch(shrink_tiles_kernel<T, RB>, grid, block, s, p) : launch(shrink_kernel<T, RB>, grid, block, s, p);
+  const int all = plan.tiles, most = kMostGroups / plan.slots;
+  int rc = 0;
+  for (int t = 0; t < all && rc == 0; t += most) {
+    p.tiles = all - t < most ? all - t : most;
+    p.first = t * kRows;
+    const dim3 grid(p.tiles * plan.slots, plan.splits);
+    rc = plan.staged ? launch(shrink_tiles_kernel<T, RB>, grid, block, s, p) : launch(shrink_kernel<T, RB>, grid, block, s, p);
+  }
+  return rc;
 }
 template <typename T>
 int run_shrink(const Params& p, const Plan& plan, hipStream_t s) {
@@ -663,11 +675,18 @@ int run_shrink(const Params& p, const Plan& plan, hipStream_t s) {
 }
 
 template <bool OUT_F16>
-int run_expand(const Params& p, const Plan& plan, hipStream_t s) {
-  const dim3 grid(ceil_div(p.M, kManyRows), ceil_div(ceil_div(p.N, 64), plan.chunks), plan.wide), block(kThreads);
-  if (p.rank <= 32) return launch(expand_kernel<OUT_F16, 1>, grid, block, s, p);
-  if (p.rank <= 64) return launch(expand_kernel<OUT_F16, 2>, grid, block, s, p);
-  return launch(expand_kernel<OUT_F16, 4>, grid, block, s, p);
+int run_expand(Params p, const Plan& plan, hipStream_t s) {
+  const dim3 block(kThreads);
+  const int all = ceil_div(p.M, kManyRows);
+  int rc = 0;
+  for (int t = 0; t < all && rc == 0; t += kMostGroups) {
+    p.first = t * kManyRows;
+    const dim3 grid(all - t < kMostGroups ? all - t : kMostGroups, ceil_div(ceil_div(p.N, 64), plan.chunks), plan.wide);
+    rc = p.rank <= 32   ? launch(expand_kernel<OUT_F16, 1>, grid, block, s, p)
+         : p.rank <= 64 ? launch(expand_kernel<OUT_F16, 2>, grid, block, s, p)
+                        : launch(expand_kernel<OUT_F16, 4>, grid, block, s, p);
+  }
+  return rc;
 }
 template <typename T, bool OUT_F16>
 int run_fused(const Params& p, hipStream_t s) {

@@ -417,7 +417,7 @@ int g16_attention_decode(const g16_attention_args* args, void* stream);
  * out [M,N] fp32 (y itself, too) or fp16. A row whose index is negative or not below `adapters` has no
  * adapter: out is y there. K, N and rank multiples of 8, rank 8 to G16_LORA_MAX_RANK (rank 0: shrink has nothing to do,
  * expand rejects it unless there are no adapters, either), K and N up to
- * G16_LORA_MAX_SIDE (offsets within a tile of rows are 32 bits); all contiguous, 16-byte aligned.
+ * G16_LORA_MAX_SIDE (offsets within a tile of rows are 32 bits), M up to 2^31 - 65; all contiguous, 16-byte aligned.
  * g16_lora_shrink leaves scale * x @ down^T in the workspace (fp32), g16_lora_expand does the rest: two launches,
  * between which the projection may run. Both take the same arguments and a workspace of
  * g16_lora_workspace_bytes(). Sums are fp32, and no operand is rounded

@@ -272,3 +272,20 @@ def test_a_gradient_of_any_operand_is_refused(cuda, M):
                 pytest.fail(f"{name} was taken")
             with torch.no_grad():
                 call()
+
+
+@pytest.mark.parametrize("M,K,rank", [((1 << 23) + 37, 64, 8), ((1 << 27) + 70, 8, 8)])
+def test_more_rows_than_a_launch_has_threads_for(cuda, M, K, rank):
+    # 2^32 threads a launch: workgroups of 512 for every 16 rows, several of them where a tile may hold several adapters
+    gen = torch.Generator(cuda).manual_seed(0)
+    x = torch.empty(M, K, dtype=F16, device=cuda).normal_(generator=gen)
+    w, down = torch.randn(K, 8, generator=gen, device=cuda).half(), torch.randn(3, rank, K, generator=gen, device=cuda).half()
+    up = torch.randn(3, 8, rank, generator=gen, device=cuda).half()
+    index = (torch.arange(M, device=cuda) % 5 - 1).int()
+    y = g.lora_mm_t(x, w, down, up, index, out_dtype=F16)
+    for a in (0, 1 << 20, 1 << 22, (1 << 23) - 50, M // 2, (1 << 27) - 50, M - 100):
+        if a + 100 <= M:
+            rows = slice(a, a + 100)
+            c = dict(x=x[rows].cpu(), w=w.cpu(), down=down.cpu(), up=up.cpu(), index=index[rows].cpu(), scale=None, bias=None)
+            ref, tol = reference(c, F16)
+            assert ((y[rows].double().cpu() - ref).abs() / tol).max() <= 1.0, a

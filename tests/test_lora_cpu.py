@@ -101,3 +101,9 @@ def test_expand_rejects_adapters_of_rank_0():
         for out_is_f16 in (0, 1):
             assert call("g16_lora_expand", rank=0, M=M, out_is_f16=out_is_f16) == SHAPE
     assert call("g16_lora_expand", rank=0, M=0) == 0
+
+
+def test_rows_past_32_bits_are_rejected():
+    for name in ("g16_lora_shrink", "g16_lora_expand"):
+        assert call(name, M=(1 << 31) - 2) == SHAPE
+        assert call(name, M=1 << 30, K=8, N=8, rank=8) == WORKSPACE
