@@ -34,6 +34,7 @@
 // sum) in the workspace (prompt_time weighs shapes and splits); a second launch joins them in split order (no
 // atomics: repeated calls agree).
 #include <cfloat>
+#include <type_traits>
 
 #include "g16_common.hpp"
 
@@ -297,6 +298,55 @@ __device__ inline void dma16_from(const char* at, uint32_t lds_addr) {
                : "memory", "m0");
 }
 
+// Where a wavefront takes a tile's operands from: LDS, or memory, where no other wavefront is needed (careful_rows).
+template <typename TL>
+struct InLds {
+  uint32_t k_at, v_at;
+  __device__ typename TL::V8 k(int kb, int ks) const { return TL::k_frag(k_at, kb, ks); }
+  __device__ typename TL::V8 v(int ks, int db) const { return TL::v_frag(v_at, ks, db); }
+};
+template <typename T, int DP, int NB>
+struct InMemory {
+  const Keys& run;
+  int j0, d, lane;
+  using V8 = typename Vec8<T>::V;
+  // (fp16 values are loaded as soon as the keys; fp32 ones would take too many registers)
+  static constexpr bool HELD = sizeof(T) == 2;
+  V8 held[HELD ? 2 * NB : 1][HELD ? DP / 32 : 1];
+  __device__ InMemory(const Keys& r, int first, int values, int l) : run(r), j0(first), d(values), lane(l) {
+    if constexpr (HELD) {
+#pragma unroll
+      for (int ks = 0; ks < 2 * NB; ++ks)
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db) held[ks][db] = load(ks, db);
+    }
+  }
+  __device__ V8 k(int kb, int ks) const {
+    const int j = j0 + 32 * kb + (lane & 31), at = 16 * ks + 8 * (lane >> 5);
+    // (Keys past the last one are the last one again: their weights are 0, and careful_rows takes the tile for one that
+    // hides keys. Without a branch for each, a tile's loads are under way together.)
+    const V8 x = *reinterpret_cast<const V8*>(run.k + static_cast<size_t>(min(j, run.len - 1)) * run.k_tok + min(at, d - 8) * sizeof(T));
+    return at < d ? x : V8{};
+  }
+  __device__ V8 v(int ks, int db) const {
+    if constexpr (HELD) return held[ks][db];
+    else {
+      asm volatile("" ::: "memory");
+      return load(ks, db);
+    }
+  }
+  __device__ V8 load(int ks, int db) const {
+    const int at = 32 * db + (lane & 31), first = j0 + 16 * ks + 4 * (lane >> 5);
+    V8 x = {};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int j = first + 8 * (i >> 2) + (i & 3);
+      x[i] = *reinterpret_cast<const T*>(run.v + static_cast<size_t>(min(j, run.len - 1)) * run.v_tok + min(at, d - 1) * sizeof(T));
+    }
+    return x;
+  }
+};
+
 // ---- one lane's query row ------------------------------------------------------------------------
 struct Row {
   const char* q;  // NULL: no such row
@@ -327,6 +377,14 @@ __device__ inline Scoring scoring(const Params& p) {
   return s;
 }
 
+// What a workgroup needs to know besides its rows and keys.
+struct What {
+  Scoring sc;
+  float sign;
+  int d, causal;
+};
+__device__ inline What what_of(const Params& p) { return What{scoring(p), p.sign, p.d, p.causal}; }
+
 // tanh to fp32's last bits near 0, where a cap leaves most scores (an odd polynomial fitted by least
 // squares to (tanh(y) / y - 1) / y^2 on [0, 0.625], largest relative error 4e-9), and 1 - 2 / (e^2y + 1)
 // past it. With fp16 inputs and a cap up to kPlainCap the second form's absolute error, 1e-7 of the cap, is
@@ -346,6 +404,23 @@ __device__ inline float tanh_of(float y) {
 __device__ inline float score_of(const Scoring& s, float x, float slope, float distance) {
   const float t = s.capped ? s.cap * tanh_of(x * s.inv) : x * s.c;
   return s.biased ? fmaf(-slope, fabsf(distance), t) : t;
+}
+
+// Of keys j0 .. j1 - 1 (at most 64), those with a value that is not finite.
+template <typename T>
+__device__ inline uint64_t infinite_keys(const Keys& run, int j0, int j1, int d, int lane) {
+  using V8 = typename Vec8<T>::V;
+  bool some = false;
+  if (j0 + lane < j1) {
+    const T* v = reinterpret_cast<const T*>(run.v + static_cast<size_t>(j0 + lane) * run.v_tok);
+#pragma unroll 4
+    for (int at = 0; at < d; at += 8) {
+      const V8 x = *reinterpret_cast<const V8*>(v + at);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) some |= !(fabsf(static_cast<float>(x[j])) <= FLT_MAX);
+    }
+  }
+  return __ballot(some);
 }
 
 // ---- the running softmax and product of 32 rows in one wavefront ---------------------------------
@@ -399,8 +474,8 @@ struct Wave {
   }
 
   // S^T of the tile's NB blocks of 32 keys. EXACT: fp32 keys or queries that are not to be split (see Range).
-  template <int NB, typename TL, bool EXACT>
-  __device__ void products(uint32_t kt, float16v (&s)[NB]) const {
+  template <int NB, bool EXACT, bool FRESH, typename S>
+  __device__ void products_as(const S& tile, float16v (&s)[NB]) const {
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb) {
       s[kb] = float16v{};
@@ -410,7 +485,7 @@ struct Wave {
         bhalf8 hi[DP / 16];
 #pragma unroll
         for (int ks = 0; ks < DP / 16; ++ks) {
-          const Split8 key = operand(TL::k_frag(kt, kb, ks));
+          const Split8 key = operand(tile.k(kb, ks));
           s[kb] = mma_small(key, q[ks], s[kb]);
           hi[ks] = key.hi;
         }
@@ -421,22 +496,27 @@ struct Wave {
         for (int ks = 0; ks < DP / 16; ++ks) {
           if constexpr (EXACT) {
             Split8 part = q[ks];
-            asm volatile("" : "+v"(part.hi));  // (or the sums would be kept in registers for the whole loop)
-            s[kb] = mma(TL::k_frag(kt, kb, ks), whole(part), s[kb]);
-          } else s[kb] = mma(TL::k_frag(kt, kb, ks), q[ks], s[kb]);
+            // (or their sums would be kept in registers for the whole loop)
+            if constexpr (FRESH) asm volatile("" : "+v"(part.hi), "+v"(part.mid), "+v"(part.lo));
+            else asm volatile("" : "+v"(part.hi));
+            s[kb] = mma(tile.k(kb, ks), whole(part), s[kb]);
+          } else s[kb] = mma(tile.k(kb, ks), q[ks], s[kb]);
         }
       }
     }
   }
-  template <int NB, typename TL>
-  __device__ void products(uint32_t kt, float16v (&s)[NB], bool past) const {
+  // FRESH: the queries' parts are put together in every tile that needs them whole. Prompts are faster where only a part
+  // of that is (32 x 256 tokens, 12 heads of 64: 59 us and 64), single tokens where all is (64 of 400 keys of 128 after
+  // 8192: 147 and 150).
+  template <int NB, bool FRESH, typename S>
+  __device__ void products(const S& tile, float16v (&s)[NB], bool past) const {
     if constexpr (sizeof(T) == 4) {
       if (__builtin_expect(past || exact, 0)) {
-        products<NB, TL, true>(kt, s);
+        products_as<NB, true, FRESH>(tile, s);
         return;
       }
     }
-    products<NB, TL, false>(kt, s);
+    products_as<NB, false, FRESH>(tile, s);
   }
 
   // The weights of the tile's keys: positions pos0 .., `left` of them in the sequence.
@@ -514,33 +594,84 @@ struct Wave {
     l += sum;
   }
 
-  // O^T += V^T P^T
-  template <int NB, typename TL, bool EXACT>
-  __device__ void add(uint32_t vt, const float16v (&s)[NB]) {
+  template <int NB>
+  __device__ static V8 weights_of(const float16v (&s)[NB], int ks) {
+    V8 w;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = static_cast<T>(s[ks >> 1][8 * (ks & 1) + j]);
+    return w;
+  }
+
+  // O^T += V^T P^T. FINITE: without the values that are not.
+  template <int NB, bool EXACT, bool FINITE, typename S>
+  __device__ void add_as(const S& tile, const float16v (&s)[NB]) {
+    auto values = [&](int ks, int db) {
+      V8 v = tile.v(ks, db);
+      if constexpr (FINITE) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (!(fabsf(static_cast<float>(v[j])) <= FLT_MAX)) v[j] = static_cast<T>(0.f);
+      }
+      return v;
+    };
 #pragma unroll
     for (int ks = 0; ks < 2 * NB; ++ks) {
-      V8 w;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = static_cast<T>(s[ks >> 1][8 * (ks & 1) + j]);
+      const V8 w = weights_of(s, ks);
       if constexpr (EXACT) {
 #pragma unroll
-        for (int db = 0; db < DP / 32; ++db) o[db] = mma(TL::v_frag(vt, ks, db), w, o[db]);
+        for (int db = 0; db < DP / 32; ++db) o[db] = mma(values(ks, db), w, o[db]);
       } else {
         const auto wp = operand(w);
 #pragma unroll
-        for (int db = 0; db < DP / 32; ++db) o[db] = mma(operand(TL::v_frag(vt, ks, db)), wp, o[db]);
+        for (int db = 0; db < DP / 32; ++db) o[db] = mma(operand(values(ks, db)), wp, o[db]);
       }
     }
   }
-  template <int NB, typename TL>
-  __device__ void add(uint32_t vt, const float16v (&s)[NB], bool past) {
-    if constexpr (sizeof(T) == 4) {
-      if (__builtin_expect(past, 0)) {
-        add<NB, TL, true>(vt, s);
+  // past: see Range. finite: without the tile's infinities and NaN.
+  template <int NB, bool CAREFUL, typename S>
+  __device__ void add(const S& tile, const float16v (&s)[NB], bool past, bool finite) {
+    constexpr bool kF32 = sizeof(T) == 4;
+    if constexpr (CAREFUL) {
+      if (finite && (!kF32 || past)) {
+        add_as<NB, kF32, true>(tile, s);
         return;
       }
     }
-    add<NB, TL, false>(vt, s);
+    if constexpr (kF32) {
+      if (__builtin_expect(past, 0)) {
+        add_as<NB, true, false>(tile, s);
+        return;
+      }
+    }
+    add_as<NB, false, false>(tile, s);
+  }
+
+  // Whether a sum of the wavefront's rows is not finite, other than of rows that are NaN by their weights already.
+  __device__ bool infinite(const Row& row) const {
+    float x = 0.f;
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x = fmaf(o[db][i], 0.f, x);
+    return __any(x != 0.f && l == l && row.out != nullptr);
+  }
+  // The values of keys j0 .. j1 - 1 (at most 64) that are not finite, added for the rows that see them: their weights are
+  // above 0, so that is what the product makes of them.
+  __device__ void add_infinite(const Keys& run, int j0, int j1, const Row& row, int d, int lane) {
+    for (uint64_t keys = infinite_keys<T>(run, j0, j1, d, lane); keys != 0; keys &= keys - 1) {
+      const int j = j0 + __builtin_ctzll(keys);
+      const T* v = reinterpret_cast<const T*>(run.v + static_cast<size_t>(j) * run.v_tok);
+      const bool sees = run.pos0 + j <= row.limit && l == l;  // (with NaN weights, the row is NaN already)
+      if (!__any(sees)) continue;
+#pragma unroll
+      for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int at = 32 * db + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3);
+          const float x = at < d ? static_cast<float>(v[at]) : 0.f;
+          if (sees && !(fabsf(x) <= FLT_MAX)) o[db][i] += x;
+        }
+    }
   }
 };
 
@@ -572,69 +703,98 @@ __device__ inline void store_out(char* out, int d0, const float (&v)[N]) {
   }
 }
 
-// One row again, key by key, for rows whose sums are not finite: an infinity or NaN behind a key that
-// the row does not see, times that key's weight 0, may be the reason. Only the keys that it sees are
-// read here. The whole wavefront works on the row.
-template <typename T, int DP>
-__device__ __attribute__((noinline)) void careful_row(const char* q, float sign, char* out, int pos, int limit, float slope, const Scoring sc,
-                                                      const KeyRuns runs, int from0, int to0, int from1, int to1, int d,
-                                                      float* part, float* part_m, float* part_l) {
-  const int lane = threadIdx.x & 63;
-  const T* qv = reinterpret_cast<const T*>(q);
-  auto score = [&](const Keys& s, int j) {
-    const T* kr = reinterpret_cast<const T*>(s.k + static_cast<size_t>(j) * s.k_tok);
-    float x = 0.f;
-    for (int i = 0; i < d; ++i) x = fmaf(to_f(qv[i]) * sign, to_f(kr[i]), x);
-    return score_of(sc, x, slope, static_cast<float>(pos - s.pos0 - j));
-  };
-  float top = -__builtin_huge_valf();
-  for (int g = 0; g < 2; ++g) {
-    const Keys& s = g ? runs.own : runs.shared;
-    const int end = min(g ? to1 : to0, s.len);
-    for (int j = (g ? from1 : from0) + lane; j < end && s.pos0 + j <= limit; j += kWave) top = fmaxf(top, score(s, j));
-  }
-  for (int i = 1; i < kWave; i *= 2) top = fmaxf(top, __shfl_xor(top, i));
-  const float ref = (top == -__builtin_huge_valf() ? 0.f : top) - kShift<T>;
-  float l = 0.f, o[DP / 64] = {};
-  for (int g = 0; g < 2; ++g) {
-    const Keys& s = g ? runs.own : runs.shared;
-    const int end = min(min(g ? to1 : to0, s.len), limit < s.pos0 ? 0 : limit - s.pos0 + 1);
-    for (int j0 = g ? from1 : from0; j0 < end; j0 += kWave) {
-      const float w = j0 + lane < end ? __builtin_amdgcn_exp2f(score(s, j0 + lane) - ref) * kScale<T> : 0.f;
-      l += w;
-      for (int i = 0; i < min(kWave, end - j0); ++i) {
-        const float wi = __shfl(w, i);
-        const T* vr = reinterpret_cast<const T*>(s.v + static_cast<size_t>(j0 + i) * s.v_tok);
-#pragma unroll
-        for (int e = 0; e < DP / 64; ++e)
-          if (lane + 64 * e < d) o[e] = fmaf(to_f(static_cast<T>(wi)), to_f(vr[lane + 64 * e]), o[e]);
-      }
-    }
-  }
-  for (int i = 1; i < kWave; i *= 2) l += __shfl_xor(l, i);
-#pragma unroll
-  for (int e = 0; e < DP / 64; ++e) {
-    const int at = lane + 64 * e;
-    if (part != nullptr) part[at] = at < d ? o[e] : 0.f;
-    else if (at < d) reinterpret_cast<T*>(out)[at] = static_cast<T>(l > 0.f || l != l ? o[e] / l : 0.f);
-  }
-  if (part != nullptr && lane == 0) {
-    *part_m = top;
-    *part_l = l;
-  }
-}
-
 // 1 / l, with 0 for a row that saw no key (a NaN stays one)
 __device__ inline float inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
 
+// The rows of wavefront `wave` of a workgroup of 128 to their places.
+template <typename T, int DP, int DU>
+__device__ inline void store_rows(const Wave<T, DU>& w, const Row& row, int d, const Slot& slot, int wave, int lane) {
+  const float l = w.l + other_half(w.l);
+  const int h = lane >> 5, r = wave * 32 + (lane & 31);
+  if (slot.at != nullptr) {
+    float* o = slot.at + static_cast<size_t>(r) * DP;
+#pragma unroll
+    for (int db = 0; db < DU / 32; ++db)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float16v& a = w.o[db];
+        *reinterpret_cast<float4v*>(o + 32 * db + 8 * q + 4 * h) = float4v{a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]};
+      }
+    if (h == 0) {
+      slot_m<DP>(slot)[r] = w.m;
+      slot_m<DP>(slot)[slot.rows + r] = l;
+    }
+  } else if (row.out != nullptr) {
+    const float inv = inverse(l);
+#pragma unroll
+    for (int db = 0; db < DU / 32; ++db)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int d0 = 32 * db + 8 * q + 4 * h;
+        const float v[4] = {w.o[db][4 * q] * inv, w.o[db][4 * q + 1] * inv, w.o[db][4 * q + 2] * inv, w.o[db][4 * q + 3] * inv};
+        if (d0 < d) store_out<T, 4>(row.out, d0, v);
+      }
+  }
+}
+
+// (What arrives here is the same for all lanes, but for the row, and has to be known to be.)
+__device__ inline What uniform(const What& c) {
+  auto f = [](float x) { return __uint_as_float(static_cast<uint32_t>(uniform(static_cast<int>(__float_as_uint(x))))); };
+  return What{{f(c.sc.c), f(c.sc.cap), f(c.sc.inv), f(c.sc.inv2), uniform(c.sc.capped) != 0, uniform(c.sc.fine) != 0, uniform(c.sc.biased) != 0},
+              f(c.sign), uniform(c.d), uniform(c.causal)};
+}
+
+// A row's weight for a key that it does not see is 0, which times an infinity or NaN would be NaN. Hardly any value is one,
+// so rows are computed as if none were. This computes those of a wavefront again whose sums are not finite, where such a
+// value stands in a tile that hides keys from one of them (the last tiles): without these tiles' infinities and NaN,
+// which are then added for the rows that see them. From memory: the workgroup's other wavefronts may have ended (waiting
+// for them at the end of every call costs 48 documents of 200 tokens 5 %). 4096 tokens, 8 heads of 64 on 4: 55 us; with a
+// NaN at key 40 66, at key 4086, for rows of which all keys are gone over again, 161; key by key and row by row it
+// was 17 ms.
+template <typename T, int DP, int DU>
+__device__ __attribute__((noinline)) void careful_rows(What what, Row row, KeyRuns runs, int from0, int to0, int from1, int to1, int last, int limit,
+                                                       Slot place) {
+  constexpr int NB = sizeof(T) == 2 ? 2 : 1, BN = 32 * NB;
+  const What c = uniform(what);
+  const int last_seen = uniform(last), wave_limit = uniform(limit), lane = threadIdx.x & 63, wave = uniform(static_cast<int>(threadIdx.x >> 6));
+  const Slot slot = {uniform(place.at), uniform(place.rows)};
+  auto hides = [&](int first, int keys) { return keys < BN || last_seen < first + BN - 1; };
+  auto tiles = [&](auto each) {  // of this wavefront, in order
+    for (int g = 0; g < 2; ++g) {
+      const Keys run = runs.run(g != 0);
+      const int end = min(uniform(g ? to1 : to0), run.len);
+      for (int j0 = uniform(g ? from1 : from0); j0 < end && run.pos0 + j0 <= wave_limit; j0 += BN) each(run, j0, run.pos0 + j0, run.len - j0);
+    }
+  };
+  bool again = false;
+  tiles([&](const Keys& run, int j0, int pos0, int left) {
+    if (hides(pos0, left)) again = again || infinite_keys<T>(run, j0, min(j0 + BN, run.len), c.d, lane) != 0;
+  });
+  if (!again) return;
+  Wave<T, DU> w;
+  w.start(row, c.sign, c.d, lane);
+  tiles([&](const Keys& run, int j0, int pos0, int left) {
+    const InMemory<T, DU, NB> tile(run, j0, c.d, lane);
+    float16v s[NB];
+    w.template products_as<NB, sizeof(T) == 4, true>(tile, s);
+    w.template weights<NB>(s, c.sc, row, pos0, left, last_seen, lane);
+    if (hides(pos0, left)) w.template add_as<NB, sizeof(T) == 4, true>(tile, s);
+    else w.template add_as<NB, sizeof(T) == 4, false>(tile, s);
+  });
+  tiles([&](const Keys& run, int j0, int pos0, int left) {
+    if (hides(pos0, left)) w.add_infinite(run, j0, min(j0 + BN, run.len), row, c.d, lane);
+  });
+  store_rows<T, DP, DU>(w, row, c.d, slot, wave, lane);
+}
+
 // ---- workgroup of 128 rows ---------------------------------------------------------------------------
 // Wavefront w holds rows 32 w .. 32 w + 31. last_seen: a position up to which every valid row of this
-// wavefront sees; wave_limit: the last position that any of them sees. DU: of a row's DP places in LDS, those that
+// wavefront sees; wave_limit: the last position that any of them sees. MASK: whether rows may not see keys. DU: of a row's DP places in LDS, those that
 // the products go over, half of them for heads of up to 32 values, three quarters for up to 96 (8192 causal tokens, 32
 // heads on 8 of 96: 489 us, all 128 places 542; 16 x 512 in fp32, 12 of 32: 35 and 44).
-template <typename T, int DP, int DU>
-__device__ void rows_workgroup(const Params& p, char* lds, int* ranges, const Row& row, const KeyRuns& runs, int n0, int tbeg, int tend,
-                               int last_seen, int wave_limit, const Slot& slot) {
+template <typename T, int DP, int DU, bool MASK, typename F>
+__device__ inline void rows_workgroup(const Params& p, char* lds, int* ranges, const Row& row, const KeyRuns& runs, int n0, int tbeg, int tend,
+                                      int last_seen, int wave_limit, const Slot& slot, const F& row_again) {
   constexpr int BN = sizeof(T) == 2 ? 64 : 32, NB = BN / 32;
   using TL = Tile<T, DP, BN>;
   constexpr int NIW = TL::NI / 4;  // DMA instructions of a wavefront per tile and operand
@@ -667,9 +827,9 @@ __device__ void rows_workgroup(const Params& p, char* lds, int* ranges, const Ro
     at.len -= BN;
   };
   Wave<T, DU> w;
+  const uint32_t klane = base + TL::k_lane(lane), vlane = base + TL::BYTES + TL::v_lane(lane);
   if (tbeg < tend) issue(tbeg, 0);
   w.start(row, p.sign, p.d, lane);
-  const uint32_t klane = base + TL::k_lane(lane), vlane = base + TL::BYTES + TL::v_lane(lane);
   for (int t = tbeg; t < tend; ++t) {
     const uint32_t buf = static_cast<uint32_t>((t - tbeg) & 1);
     wait_dma_le<0>();
@@ -693,60 +853,18 @@ __device__ void rows_workgroup(const Params& p, char* lds, int* ranges, const Ro
     if (t + 1 < tend) issue(t + 1, buf ^ 1);
     if (pos0 <= wave_limit) {
       float16v s[NB];
-      w.template products<NB, TL>(klane + buf * 2 * TL::BYTES, s, (bits & 1) != 0);
+      const InLds<TL> tile = {klane + buf * 2 * TL::BYTES, vlane + buf * 2 * TL::BYTES};
+      w.template products<NB, !MASK>(tile, s, (bits & 1) != 0);
       w.template weights<NB>(s, sc, row, pos0, left, last_seen, lane);
-      w.template add<NB, TL>(vlane + buf * 2 * TL::BYTES, s, (bits & 2) != 0);
+      w.template add<NB, false>(tile, s, (bits & 2) != 0, false);
     }
   }
   w.settle();
-  const float l = w.l + other_half(w.l);
-  const int h = lane >> 5, r = wave * 32 + (lane & 31);
-  float bad = 0.f;
-  if (slot.at != nullptr) {
-    float* o = slot.at + static_cast<size_t>(r) * DP;
-#pragma unroll
-    for (int db = 0; db < DU / 32; ++db)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float16v& a = w.o[db];
-        *reinterpret_cast<float4v*>(o + 32 * db + 8 * q + 4 * h) = float4v{a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]};
-      }
-    if (h == 0) {
-      slot_m<DP>(slot)[r] = w.m;
-      slot_m<DP>(slot)[slot.rows + r] = l;
-    }
-  } else if (row.out != nullptr) {
-    const float inv = inverse(l);
-#pragma unroll
-    for (int db = 0; db < DU / 32; ++db)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int d0 = 32 * db + 8 * q + 4 * h;
-        const float v[4] = {w.o[db][4 * q] * inv, w.o[db][4 * q + 1] * inv, w.o[db][4 * q + 2] * inv, w.o[db][4 * q + 3] * inv};
-        if (d0 < p.d) store_out<T, 4>(row.out, d0, v);
-      }
-  }
-  if (!p.causal) return;
-#pragma unroll
-  for (int db = 0; db < DU / 32; ++db)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) bad = fmaf(w.o[db][i], 0.f, bad);
-  const uint64_t which = __ballot(bad != 0.f && row.q != nullptr);
-  uint32_t rows = static_cast<uint32_t>(which) | static_cast<uint32_t>(which >> 32);
-  if (__builtin_expect(rows != 0u, 0)) {
-    __builtin_amdgcn_s_waitcnt(0);  // the rows' first results are stored before their second ones
-    while (rows) {
-      const int i = __builtin_ctz(rows);
-      rows &= rows - 1;
-      const int rr = wave * 32 + i;
-      float* pm = slot.at == nullptr ? nullptr : slot_m<DP>(slot) + rr;
-      careful_row<T, DP>(reinterpret_cast<const char*>(__shfl(reinterpret_cast<unsigned long long>(row.q), i)), p.sign,
-                         reinterpret_cast<char*>(__shfl(reinterpret_cast<unsigned long long>(row.out), i)), __shfl(row.pos, i),
-                         __shfl(row.limit, i), __shfl(row.slope, i), sc, runs, min(tbeg, n0) * BN, min(tend, n0) * BN,
-                         max(tbeg - n0, 0) * BN, max(tend - n0, 0) * BN, p.d,
-                         slot.at == nullptr ? nullptr : slot.at + static_cast<size_t>(rr) * DP, pm,
-                         pm == nullptr ? nullptr : pm + slot.rows);
-    }
+  store_rows<T, DP, DU>(w, row, p.d, slot, wave, lane);
+  if constexpr (MASK) {
+    if (p.causal && __builtin_expect(w.infinite(row), 0))
+      careful_rows<T, DP, DU>(what_of(p), row_again(), runs, min(tbeg, n0) * BN, min(tend, n0) * BN, max(tbeg - n0, 0) * BN, max(tend - n0, 0) * BN,
+                              last_seen, wave_limit, slot);
   }
 }
 
@@ -762,16 +880,19 @@ struct Pages {
   int page, num_pages;
   int64_t k_seq, v_seq;
 };
-template <typename T, int DP, bool PAGED>
-__device__ void keys_workgroup(const Params& p, char* lds, float* joint, const Row& row, const KeyRuns& runs, const Pages& pages,
-                               int n0, int tbeg, int tend, int last_seen, const Slot& slot) {
+template <typename T, int DP>
+__device__ void careful_keys(What c, char* lds, float* joint, Row row, KeyRuns runs, int n0, int tbeg, int tend, int last_seen, Slot slot);
+
+// CAREFUL: as careful_rows, by the whole workgroup, whose wavefronts meet at the end anyway.
+template <typename T, int DP, bool PAGED, bool MASK, bool CAREFUL = false>
+__device__ inline void keys_workgroup(const What& c, char* lds, float* joint, const Row& row, const KeyRuns& runs, const Pages& pages,
+                                      int n0, int tbeg, int tend, int last_seen, const Slot& slot) {
   constexpr int BN = 32;
   using TL = Tile<T, DP, BN>;
   constexpr int NI = TL::NI;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const uint32_t kl = lds_base(lds) + wave * (2 * TL::BYTES);  // K, then V
-  const Scoring sc = scoring(p);
-  const int row_bytes = p.d * static_cast<int>(sizeof(T));
+  const int row_bytes = c.d * static_cast<int>(sizeof(T));
   const bool paged = PAGED && pages.table != nullptr, whole = paged && pages.page % 16 == 0;
   uint32_t koff[NI], voff[NI];
   bool second = tbeg >= n0;  // the run that the offsets are for
@@ -856,7 +977,7 @@ __device__ void keys_workgroup(const Params& p, char* lds, float* joint, const R
       else dma_rows<NI>(cur.k + static_cast<size_t>(j0) * cur.k_tok, cur.k_tok, rows, koff, to);
     }
   };
-  const uint32_t klane = kl + TL::k_lane(lane), vlane = kl + TL::BYTES + TL::v_lane(lane);
+  const InLds<TL> tile = {kl + TL::k_lane(lane), kl + TL::BYTES + TL::v_lane(lane)};
   auto past = [&](uint32_t tile) {
     if constexpr (sizeof(T) == 2) return false;
     Range r;
@@ -865,6 +986,16 @@ __device__ void keys_workgroup(const Params& p, char* lds, float* joint, const R
     return r.past();
   };
   Wave<T, DP> w;
+  auto hides = [&](int first, int keys) { return last_seen < first + min(keys, BN) - 1; };
+  // this wavefront's tiles that hide keys, from the last one on
+  auto hidden = [&](auto each) {
+    for (int u = tend - 1; u >= tbeg; --u) {
+      const Keys run = runs.run(u >= n0);
+      const int j0 = (u - (u >= n0 ? n0 : 0)) * BN;
+      if (!hides(run.pos0 + j0, run.len - j0)) break;
+      if ((u - tbeg) % 4 == wave) each(run, j0, min(j0 + BN, run.len));
+    }
+  };
   int t = tbeg + wave;
   if (t < tend) {
     const Ids ids = page_of(t);
@@ -872,7 +1003,7 @@ __device__ void keys_workgroup(const Params& p, char* lds, float* joint, const R
     issue(t, ids, true);
   }
   Ids next = page_of(t + 4);
-  w.start(row, p.sign, p.d, lane);
+  w.start(row, c.sign, c.d, lane);
   // The rows' loads are done before the loop: its waits count DMA only, and the compiler, which does not
   // know of that, would wait for all of it before it first uses the rows.
   __builtin_amdgcn_s_waitcnt(0);
@@ -884,18 +1015,19 @@ __device__ void keys_workgroup(const Params& p, char* lds, float* joint, const R
     // Waits for K, then for V: only the instructions issued after it may be in flight (others among them only
     // make it wait longer).
     wait_dma_le<NI>();
-    w.template products<1, TL>(klane, s, past(kl));
+    w.template products<1, !MASK>(tile, s, past(kl));
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K has been read before the next K overwrites it
     if (more) issue(t + 4, next, false);
-    w.template weights<1>(s, sc, row, pos0, left, last_seen, lane);
+    w.template weights<1>(s, c.sc, row, pos0, left, last_seen, lane);
     if (more) wait_dma_le<NI>();
     else wait_dma_le<0>();
-    w.template add<1, TL>(vlane, s, past(kl + TL::BYTES));
+    w.template add<1, CAREFUL>(tile, s, past(kl + TL::BYTES), CAREFUL && hides(pos0, left));
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if (more) issue(t + 4, next, true);
     next = page_of(t + 8);
   }
   w.settle();
+  if constexpr (CAREFUL) hidden([&](const Keys& run, int j0, int j1) { w.add_infinite(run, j0, j1, row, c.d, lane); });
   // ---- join the four wavefronts: sums [wave][value][row] in LDS, then 8 threads a row ----
   const float l = w.l + other_half(w.l);
   const int h = lane >> 5, r = lane & 31;
@@ -909,7 +1041,7 @@ __device__ void keys_workgroup(const Params& p, char* lds, float* joint, const R
     joint[wave * 32 + r] = w.m;
     joint[128 + wave * 32 + r] = l;
   }
-  if (tid == 0) joint[256] = 0.f;
+  if (MASK && tid < 2) joint[256 + tid] = 0.f;
   __syncthreads();
   float top = -__builtin_huge_valf();
 #pragma unroll
@@ -927,52 +1059,48 @@ __device__ void keys_workgroup(const Params& p, char* lds, float* joint, const R
   float bad = 0.f;
   const bool stored = slot.at != nullptr ? r < slot.rows : row.out != nullptr;
 #pragma unroll
-  for (int c = 0; c < DT; c += 8) {
+  for (int e0 = 0; e0 < DT; e0 += 8) {
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       float x = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x = fmaf(f[i], so[(i * DP + d0 + c + e) * 32 + r], x);
+      for (int i = 0; i < 4; ++i) x = fmaf(f[i], so[(i * DP + d0 + e0 + e) * 32 + r], x);
       v[e] = x * inv;
       bad = fmaf(x, 0.f, bad);
     }
     if (stored && slot.at != nullptr) {
-      float* o = slot.at + static_cast<size_t>(r) * DP + d0 + c;
+      float* o = slot.at + static_cast<size_t>(r) * DP + d0 + e0;
       *reinterpret_cast<float4v*>(o) = float4v{v[0], v[1], v[2], v[3]};
       *reinterpret_cast<float4v*>(o + 4) = float4v{v[4], v[5], v[6], v[7]};
-    } else if (stored && d0 + c < p.d) {
-      store_out<T, 8>(row.out, d0 + c, v);
+    } else if (stored && d0 + e0 < c.d) {
+      store_out<T, 8>(row.out, d0 + e0, v);
     }
   }
   if (slot.at != nullptr && tid < 32 && r < slot.rows) {
     slot_m<DP>(slot)[r] = top;
     slot_m<DP>(slot)[slot.rows + r] = total;
   }
-  if constexpr (!PAGED) {
-    if (!p.causal) return;
+  if constexpr (MASK && !CAREFUL) {
+    if (!c.causal) return;
+    // whether sums are not finite, then whether hidden values are
     uint32_t* flags = reinterpret_cast<uint32_t*>(joint + 256);
-    const uint64_t which = __ballot(bad != 0.f && row.q != nullptr);
-    const uint32_t some = static_cast<uint32_t>(which) | static_cast<uint32_t>(which >> 32);
-    if (lane == 0 && some) atomicOr(flags, some);
-    __builtin_amdgcn_s_waitcnt(0);  // the rows' first results are stored before their second ones
+    if (__any(bad != 0.f && total == total && row.q != nullptr) && lane == 0) atomicOr(flags, 1u);
     __syncthreads();
-    uint32_t rows = *flags;
-    if (__builtin_expect(rows != 0u, 0)) {
-      for (int k = 0; rows; ++k) {
-        const int i = __builtin_ctz(rows);
-        rows &= rows - 1;
-        if ((k & 3) != wave) continue;
-        float* pm = slot.at == nullptr ? nullptr : slot_m<DP>(slot) + i;
-        careful_row<T, DP>(reinterpret_cast<const char*>(__shfl(reinterpret_cast<unsigned long long>(row.q), i)), p.sign,
-                           reinterpret_cast<char*>(__shfl(reinterpret_cast<unsigned long long>(row.out), i)), __shfl(row.pos, i),
-                           __shfl(row.limit, i), __shfl(row.slope, i), sc, runs, min(tbeg, n0) * BN, min(tend, n0) * BN,
-                         max(tbeg - n0, 0) * BN, max(tend - n0, 0) * BN, p.d,
-                           slot.at == nullptr ? nullptr : slot.at + static_cast<size_t>(i) * DP, pm,
-                           pm == nullptr ? nullptr : pm + slot.rows);
-      }
+    if (__builtin_expect(uniform(static_cast<int>(flags[0])), 0)) {
+      hidden([&](const Keys& run, int j0, int j1) {
+        if (infinite_keys<T>(run, j0, j1, c.d, lane) != 0 && lane == 0) atomicOr(flags + 1, 1u);
+      });
+      __syncthreads();
+      if (uniform(static_cast<int>(flags[1]))) careful_keys<T, DP>(c, lds, joint, row, runs, n0, tbeg, tend, last_seen, slot);
     }
   }
+}
+template <typename T, int DP>
+__device__ __attribute__((noinline)) void careful_keys(What c, char* lds, float* joint, Row row, KeyRuns runs, int n0, int tbeg, int tend, int last_seen,
+                                                       Slot slot) {
+  keys_workgroup<T, DP, false, true, true>(uniform(c), uniform(lds), uniform(joint), row, runs, Pages{}, uniform(n0), uniform(tbeg), uniform(tend),
+                                           uniform(last_seen), Slot{uniform(slot.at), uniform(slot.rows)});
 }
 
 template <typename T, int DP>
@@ -1053,10 +1181,10 @@ __device__ inline Row prompt_row(const Params& p, const Where& w, int kv, int r,
 
 // (three workgroups of 128 rows fit a CU at 64 values a row, two at 128)
 template <typename T, int DP, int DU, bool KEYS>
-__global__ __launch_bounds__(kThreads, !KEYS && DP == 64 ? 3 : 2) void prompt_kernel(Params p) {
+__global__ __launch_bounds__(kThreads, DP == 64 && (!KEYS || sizeof(T) == 2) ? 3 : 2) void prompt_kernel(Params p) {
   constexpr int RT = KEYS ? kKeyTile : kRowTile, BN = KEYS ? 32 : (sizeof(T) == 2 ? 64 : 32);
   __shared__ __attribute__((aligned(1024))) char lds[KEYS ? keys_lds<T, DP>() : rows_lds<T, DP>()];
-  __shared__ float joint[KEYS ? 257 : 1];
+  __shared__ float joint[KEYS ? 258 : 1];
   __shared__ int ranges[8];  // fp32: of the two tiles in LDS, from each wavefront
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   int lin = blockIdx.x;
@@ -1089,9 +1217,10 @@ __global__ __launch_bounds__(kThreads, !KEYS && DP == 64 ? 3 : 2) void prompt_ke
   Slot slot = {nullptr, RT};
   if (p.splits > 1) slot.at = p.part + static_cast<size_t>(blockIdx.x) * slot_floats(RT, DP);
   if constexpr (KEYS) {
-    keys_workgroup<T, DP, false>(p, lds, joint, row, runs, Pages{}, n0, tbeg, tend, last_seen, slot);
+    keys_workgroup<T, DP, false, true>(what_of(p), lds, joint, row, runs, Pages{}, n0, tbeg, tend, last_seen, slot);
   } else {
-    rows_workgroup<T, DP, DU>(p, lds, ranges, row, runs, n0, tbeg, tend, last_seen, wave_limit, slot);
+    rows_workgroup<T, DP, DU, true>(p, lds, ranges, row, runs, n0, tbeg, tend, last_seen, wave_limit, slot,
+                                    [&]() { return prompt_row(p, w, kv, first + (lane & 31), sizeof(T)); });
   }
 }
 
@@ -1240,7 +1369,7 @@ template <typename T, int DP, bool SKEYS>
 __global__ __launch_bounds__(kThreads, 2) void decode_kernel(Params p) {
   constexpr int SRT = SKEYS ? kKeyTile : kRowTile, SBN = SKEYS ? 32 : (sizeof(T) == 2 ? 64 : 32);
   __shared__ __attribute__((aligned(1024))) char lds[SKEYS ? keys_lds<T, DP>() : cmax(keys_lds<T, DP>(), rows_lds<T, DP>())];
-  __shared__ float joint[257];
+  __shared__ float joint[256];
   __shared__ int ranges[8];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int nshared = p.stiles * p.ssplits * p.hkv;
@@ -1268,10 +1397,10 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(Params p) {
     const int tbeg = share_begin(n, split, p.ssplits), tend = share_begin(n, split + 1, p.ssplits);
     Slot slot = {p.part + (static_cast<size_t>(t * p.ssplits + split) * p.hkv + kv) * slot_floats(SRT, DP), SRT};
     if constexpr (SKEYS) {
-      keys_workgroup<T, DP, false>(p, lds, joint, row, runs, Pages{}, n, tbeg, tend, 0x7fffffff, slot);
+      keys_workgroup<T, DP, false, false>(what_of(p), lds, joint, row, runs, Pages{}, n, tbeg, tend, 0x7fffffff, slot);
     } else {
       const bool some = t * SRT + 32 * wave < p.seqs * p.group;  // a wavefront without rows computes nothing
-      rows_workgroup<T, DP, DP>(p, lds, ranges, row, runs, n, tbeg, tend, 0x7fffffff, some ? 0x7fffffff : -1, slot);
+      rows_workgroup<T, DP, DP, false>(p, lds, ranges, row, runs, n, tbeg, tend, 0x7fffffff, some ? 0x7fffffff : -1, slot, [&]() { return row; });
     }
     return;
   }
@@ -1295,7 +1424,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(Params p) {
   const int tbeg = share_begin(n, part.split, part.splits), tend = share_begin(n, part.split + 1, part.splits);
   Slot slot = {nullptr, orows};
   if (p.stiles > 0 || part.splits > 1) slot.at = p.part + static_cast<size_t>(nshared) * slot_floats(SRT, DP) + static_cast<size_t>(own) * slot_floats(orows, DP);
-  keys_workgroup<T, DP, true>(p, lds, joint, row, runs, pages, 0, tbeg, tend, 0x7fffffff, slot);
+  keys_workgroup<T, DP, true, false>(what_of(p), lds, joint, row, runs, pages, 0, tbeg, tend, 0x7fffffff, slot);
 }
 
 template <typename T, int DP>
