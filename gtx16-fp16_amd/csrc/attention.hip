@@ -1565,28 +1565,40 @@ int splits_for(int64_t items, int64_t tiles, int many, int least) {
   return s < 1 ? 1 : static_cast<int>(s > 256 ? 256 : s);
 }
 
+// Places of a row that the products of 128 rows go over (see rows_workgroup).
+int places_of(int d) { return d <= 64 ? (d <= 32 ? 32 : 64) : (d <= 96 ? 96 : 128); }
+
 // What a prompt takes in one shape and number of splits, in us. A CU gets through so many steps (tiles of 64 fp16
 // or 32 fp32 keys; 128 keys for the four wavefronts of 32 rows) in a time that two workgroups on it mostly share;
 // a split's sums go through the workspace and a second launch. Measured for this, us (causal unless said otherwise,
 // query heads on key heads): 3 x 597 tokens, 32 on 8 of 128, no mask: 35 whole, 76 in two splits; 4 x 1611, 6 on 2,
 // no mask: 60 and 82; 512, 32 on 8: 12.8 in 32 rows, 18 in 128, 31 in two splits; 2048, 8 on 2: 26 in 32 rows, 48 in
 // 128, 37 in four splits; 128 rows on 16128 keys, 32 on 8: 60 in 16 splits, 69 in 8, 70 in 32 rows and 4; 2 x 298 after
-// 2531, 2 on 2: 18 in 32 rows and 4 splits, 20 in 128 and 16; 46 x 35 in fp32, 20 on 5 of 80: 32 in 32 rows, 16 in 128.
+// 2531, 2 on 2: 18 in 32 rows and 4 splits, 20 in 128 and 16. fp32: 46 x 35, 20 on 5 of 80: 54 in 32 rows, 14 in 128; 2048,
+// 32 on 8 of 128: 397 in 128 rows, 297 in two splits, 394 in 32 rows; 4 x 1611, 6 on 2 of 64, no mask: 131 in 32 rows,
+// 181 in 128, 141 in four splits; 128 after 3872, 16 heads of 128: 57 in 32 rows and 4 splits, 72 in 128 and 16;
+// 32 x 256, 12 heads of 64, no mask: 60 in 128 rows, 85 in 32; 1000, the same: 37 in 32 rows, 52 in 128 and 4 splits.
 struct Step {
-  float alone, shared;
+  float alone, shared, beside;  // one workgroup on a CU; each of several; the longest of several
 };
-Step step_of(bool keys, bool f32, int dp) {
-  if (keys) return f32 ? (dp == 64 ? Step{2.4f, 1.9f} : Step{4.6f, 4.6f}) : (dp == 64 ? Step{0.7f, 0.6f} : Step{0.9f, 0.8f});
-  if (f32) return dp == 64 ? Step{1.5f, 1.06f} : Step{3.f, 2.9f};
-  return dp == 64 ? Step{0.9f, 0.55f} : Step{1.45f, 1.2f};
+// places: of a row, that the products go over
+Step step_of(bool keys, bool f32, int dp, int places) {
+  if (f32) {
+    if (keys) return dp == 64 ? Step{2.4f, 2.1f, 2.7f} : Step{5.2f, 5.5f, 5.2f};
+    if (dp == 64) return places == 32 ? Step{1.6f, 1.f, 1.6f} : Step{2.4f, 2.08f, 3.2f};
+    return places == 96 ? Step{3.5f, 2.9f, 4.7f} : Step{4.8f, 3.8f, 6.2f};
+  }
+  if (keys) return dp == 64 ? Step{0.7f, 0.6f, 0.7f} : Step{0.9f, 0.8f, 0.9f};
+  return dp == 64 ? Step{0.9f, 0.55f, 0.9f} : Step{1.45f, 1.2f, 1.45f};
 }
-float prompt_time(bool keys, bool f32, int dp, int64_t items, int64_t steps, float average, int splits, int cus) {
-  const Step t = step_of(keys, f32, dp);
+float prompt_time(bool keys, bool f32, int d, int64_t items, int64_t steps, float average, int splits, int cus) {
+  const int dp = d <= 64 ? 64 : 128;
+  const Step t = step_of(keys, f32, dp, places_of(d));
   const int64_t workgroups = items * splits, each = (steps + splits - 1) / splits, share = (workgroups + cus - 1) / cus;
   const float mean = average / static_cast<float>(splits) > 1.f ? average / static_cast<float>(splits) : 1.f;
   // (a CU's share of workgroups: the largest and the mean one, as CUs with fewer leave memory and power to the rest)
   const float part = share > 1 ? 0.5f * (static_cast<float>(share) + static_cast<float>(workgroups) / static_cast<float>(cus)) : 1.f;
-  const float longest = static_cast<float>(each) * t.alone, all = part * mean * t.shared;
+  const float longest = static_cast<float>(each) * (share > 1 ? t.beside : t.alone), all = part * mean * t.shared;
   const int at_once = keys && f32 && dp == 128 ? 1 : 2;  // on a CU; further ones start after them
   float us = (keys ? 6.5f : 8.f) + (longest > all ? longest : all);
   if (share > at_once) us += (at_once == 1 ? 5.f : 2.f) * static_cast<float>(share - at_once);
@@ -1620,7 +1632,7 @@ PromptPlan plan_prompt(const g16_attention_args& a) {
     for (int s = 1; s <= 256; s = s < 4 ? s + 1 : (s & (s - 1) ? s / 3 * 4 : s / 2 * 3)) {  // 1 2 3 4 6 8 12 16 ..
       if (s > 1 && steps / s < (by_keys ? 1 : 2)) break;
       if (!fits_grid(tiles * s * a.hkv) || (s > 1 && !fits_grid(tiles * a.hkv * (rt / kJoinRows)))) break;
-      const float us = prompt_time(by_keys, a.is_f32 != 0, dp, items, steps, seen / static_cast<float>(step), s, cus);
+      const float us = prompt_time(by_keys, a.is_f32 != 0, a.d, items, steps, seen / static_cast<float>(step), s, cus);
       if (r.splits > 0 && us >= best) continue;
       best = us;
       r.keys = by_keys;
@@ -1675,7 +1687,7 @@ int run_prompt(const Params& p, const PromptPlan& plan, hipStream_t stream) {
   const dim3 grid(static_cast<unsigned>(plan.tiles) * plan.splits * p.hkv);
   constexpr int kLess = DP == 64 ? 32 : 96;
   int rc = plan.keys      ? launch(prompt_kernel<T, DP, DP, true>, grid, dim3(kThreads), stream, p)
-           : p.d <= kLess ? launch(prompt_kernel<T, DP, kLess, false>, grid, dim3(kThreads), stream, p)
+           : places_of(p.d) == kLess ? launch(prompt_kernel<T, DP, kLess, false>, grid, dim3(kThreads), stream, p)
                           : launch(prompt_kernel<T, DP, DP, false>, grid, dim3(kThreads), stream, p);
   if (rc == 0 && plan.splits > 1)
     rc = launch(prompt_join_kernel<T, DP>, dim3(static_cast<unsigned>(plan.tiles) * p.hkv * (plan.rt / kJoinRows)), dim3(kThreads), stream, p,

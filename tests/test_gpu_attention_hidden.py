@@ -17,10 +17,12 @@ INF, NAN = float("inf"), float("nan")
 # sequences, rows, keys, query heads, key heads, d, shared keys: (rows of a workgroup, whether the keys are split)
 CASES = [((2, 45, 50, 2, 1, 64, 0), (32, False)), ((1, 40, 2100, 2, 1, 128, 0), (32, True)), ((12, 140, 140, 24, 12, 64, 0), (128, False)),
          ((12, 140, 150, 24, 12, 128, 40), (128, False)), ((12, 140, 140, 24, 12, 32, 0), (128, False)),
-         ((1, 200, 3000, 64, 8, 64, 0), (128, True)), ((12, 140, 140, 24, 12, 96, 0), (128, False))]
+         {F16: ((1, 200, 3000, 64, 8, 64, 0), (128, True)), F32: ((1, 200, 1000, 16, 4, 96, 0), (128, True))},
+         ((12, 140, 140, 24, 12, 96, 0), (128, False))]
 
 
 def case(case, dtype, seed=0):
+    case = case[dtype] if isinstance(case, dict) else case
     (n, rows, keys, hq, hkv, d, shared), (tile, split) = case
     plan = prompt_plan(rows, keys, hq, hkv, d, dtype == F32, n, packed=False, causal=True, shared=shared)
     assert plan[0] == tile and (plan[1] > 1) == split, plan
