@@ -54,7 +54,7 @@ def test_groups_of_heads(cuda, dtype, hq, hkv):
 @pytest.mark.parametrize("causal", [False, True])
 def test_shared_prefix(cuda, dtype, shared, causal):
     lens_k = [n + (i % 3) * 20 for i, n in enumerate(DOCUMENTS)]
-    run(cuda, DOCUMENTS, lens_k, 64, 32, 64, dtype, shared=shared, causal=causal, seed=shared)
+    run(cuda, DOCUMENTS, lens_k, 48, 6, 64, dtype, shared=shared, causal=causal, seed=shared)
 
 
 @pytest.mark.parametrize("dtype", [F16, F32])
