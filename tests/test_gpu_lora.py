@@ -289,3 +289,28 @@ def test_more_rows_than_a_launch_has_threads_for(cuda, M, K, rank):
             c = dict(x=x[rows].cpu(), w=w.cpu(), down=down.cpu(), up=up.cpu(), index=index[rows].cpu(), scale=None, bias=None)
             ref, tol = reference(c, F16)
             assert ((y[rows].double().cpu() - ref).abs() / tol).max() <= 1.0, a
+
+
+@pytest.mark.parametrize("M,K,splits", [(300, 520, 1), (300, 1000, 1), (300, 2056, 4), (300, 4096, 4), (2000, 1032, 2), (2000, 4096, 4),
+                                        (4200, 1000, 1), (4200, 4096, 2)])
+@pytest.mark.parametrize("r", [8, 24, 32, 64, 128])
+@pytest.mark.parametrize("x", [F16, F32])
+def test_many_rows_by_way_of_lds(cuda, M, K, splits, r, x):
+    # both operands through LDS, for every number of rank blocks: K split over workgroups and not, a multiple of a chunk and
+    # not, rows of an adapter in runs, row by row and at random, one and several adapters to a workgroup
+    head = lora._ARGS.pack(*([4096] * 7), M, K, 136, r, 6, x == F32, 1, torch.cuda.get_device_properties(cuda).multi_processor_count)
+    nbytes = g._clib.fast().args_size(g._clib.address("g16_lora_workspace_bytes"), head)
+    assert nbytes == splits * M * r * 4
+    c = make(M, K, 136, r, 6, x, seed=M + K + r)
+    m = torch.arange(M, dtype=torch.int32)
+    for index in (m // 300, m % 7 - 1, torch.randint(-1, 6, (M,), generator=torch.Generator().manual_seed(r)).int()):
+        c["index"] = index
+        check(cuda, c, F32)
+
+
+@pytest.mark.parametrize("x", [F16, F32])
+def test_every_row_of_many_its_own_adapter(cuda, x):
+    # 16 adapters to a tile, on fewer workgroups
+    c = make(600, 1032, 136, 16, 600, x)
+    c["index"] = torch.randperm(600, generator=torch.Generator().manual_seed(0)).int()
+    check(cuda, c)
