@@ -11,6 +11,9 @@
 //     them: its 16-deep step s takes keys 16 s + 4 h + {0..3} and 16 s + 8 + 4 h + {0..3} from lane half h,
 //     which are registers 8 s .. 8 s + 7 of the block. No weight moves between lanes. V^T comes from
 //     row-major V in LDS in that order through the transposing reads (fp16) or plain dword reads (fp32).
+//     fp16 inputs: each weight is rounded to fp16 for that product (its sum is not), which puts results 2.8e-4 from the
+//     exact ones, where their own rounding to fp16 makes it 2.1e-4. Weights in two parts give 2.1e-4, and 8192 causal
+//     tokens, 32 heads on 8 of 128, take 858 us instead of 633 (4 x 2048, 16 heads of 64: 73 and 58).
 //   * One pass over the keys with a running maximum. A maximum only moves when a row's new one is more
 //     than 2^kLag above it (the weights grow to at most 2^(kShift + kLag), far inside fp16), which after
 //     the first tiles spares almost every rescale of O. fp16 weights are 2^kShift above their value,
@@ -46,7 +49,7 @@ typedef float float2v __attribute__((ext_vector_type(2)));
 
 constexpr float kLag = 7.f;
 // fp16 weights are 2^kShift above their value, by way of the exponent. fp32 ones would lose bits of the exponent by that
-// (2^-20 of a weight at 23), and are made 2^kScale of theirs by a product: at most 2^-16, so that the sums over 65536
+// (2^-20 of a weight at 23), and are multiplied by kScale: at most 2^-16, so that the sums over 65536
 // keys of the largest weight stay within the values' range.
 template <typename T>
 constexpr float kShift = sizeof(T) == 2 ? 8.f : 0.f;
@@ -791,7 +794,7 @@ __device__ __attribute__((noinline)) void careful_rows(What what, Row row, KeyRu
 // Wavefront w holds rows 32 w .. 32 w + 31. last_seen: a position up to which every valid row of this
 // wavefront sees; wave_limit: the last position that any of them sees. MASK: whether rows may not see keys. DU: of a row's DP places in LDS, those that
 // the products go over, half of them for heads of up to 32 values, three quarters for up to 96 (8192 causal tokens, 32
-// heads on 8 of 96: 489 us, all 128 places 542; 16 x 512 in fp32, 12 of 32: 35 and 44).
+// heads on 8 of 96: 483 us, all 128 places 569; 16 x 512 in fp32, 12 of 32: 64 and 95).
 template <typename T, int DP, int DU, bool MASK, typename F>
 __device__ inline void rows_workgroup(const Params& p, char* lds, int* ranges, const Row& row, const KeyRuns& runs, int n0, int tbeg, int tend,
                                       int last_seen, int wave_limit, const Slot& slot, const F& row_again) {
@@ -1662,7 +1665,7 @@ DecodePlan plan_decode(const g16_attention_args& a) {
   // keys take its place: 64 requests, 32768 shared keys, 8 heads of 128: 75 us, with two 83; of 64: 42 and 39.)
   // 32 rows of more than 64 fp32 values: the LDS holds one workgroup a CU, all of which should start at once, and a
   // tile takes five times as long as in fp16, so shorter splits pay (4 requests of up to 1000, 2000 shared, 8 heads of
-  // 128: 26.5 us in 10 splits, 39.5 in 3; 11 of up to 22, 11081, 2 of 72: 27 in 48, 35 in 21).
+  // 128: 27.6 us in 10 splits, 42.7 in 3; 11 of up to 22, 11081, 2 of 72: 24.8 in 48, 36 in 21).
   r.otiles = (group + kKeyTile - 1) / kKeyTile;
   const bool single = r.skeys && a.is_f32 && dp == 128;
   const int64_t others = a.seqs * static_cast<int64_t>(r.otiles) * a.hkv;

@@ -100,6 +100,19 @@ def test_gradients_reach_the_input_and_trained_adapters(device):
         assert all(ops[k].grad is None for k in ops if k not in wanted)
 
 
+def test_gradients_against_differences():
+    m, x, index = layer(K=24, N=16)
+    m, x = m.double(), x[:2].double()
+    index = index[:2]
+    given = [t.detach().clone().requires_grad_() for t in (x, m.down, m.up, m.scale)]
+
+    def call(x, down, up, scale):
+        m.down, m.up, m.scale = down, up, scale
+        return m(x, index)
+
+    assert torch.autograd.gradcheck(call, given)
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_the_index_is_checked(device):
     m, x, index = layer(device=device)
