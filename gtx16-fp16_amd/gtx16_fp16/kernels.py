@@ -244,10 +244,15 @@ def _grown(table: dict, key, nbytes: int, floor: int, device, zero: bool) -> tor
             buf = table.get(key)
             if buf is None or buf.numel() < nbytes:
                 size = max(nbytes, floor, 0 if buf is None else 2 * buf.numel())
-                if buf is not None:
-                    _retired.append(buf)
                 # Allocated (and zero-filled) on the current stream, so ordered before the kernels.
                 make = torch.zeros if zero else torch.empty
+                if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+                    # The graph's own: its memory is the graph's, and the zero-fill runs with its replays only, so
+                    # an eager call must not find it (nor another capture).
+                    _retired.append(make(size, dtype=torch.uint8, device=device))
+                    return _retired[-1]
+                if buf is not None:
+                    _retired.append(buf)
                 buf = make(size, dtype=torch.uint8, device=device)
                 table[key] = buf
     return buf
@@ -265,7 +270,8 @@ def split_buffers(device: torch.device, stream: int, partial_bytes: int, counter
     part = _grown(_partials, key, partial_bytes, _MIN_PARTIAL_BYTES, device, zero=False)
     cnt = _grown(_counters, key, counter_bytes, _MIN_COUNTER_BYTES, device, zero=True)
     ptrs = (part.data_ptr(), part.numel(), cnt.data_ptr(), cnt.numel())
-    _current[key] = (part.numel(), cnt.numel(), ptrs)
+    if _partials.get(key) is part and _counters.get(key) is cnt:
+        _current[key] = (part.numel(), cnt.numel(), ptrs)
     return ptrs
 
 

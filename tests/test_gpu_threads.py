@@ -51,3 +51,33 @@ def test_threads_share_a_stream(cuda):
     for t in threads:
         t.join()
     assert not wrong, f"calls {sorted(set(wrong))} differed"
+
+
+def test_a_capture_by_a_thread_without_buffers(cuda):
+    # The thread that warmed the stream up is not the one that captures: the graph takes buffers of its own, which eager
+    # calls of that thread, before and after replays, do not use.
+    fns = calls(cuda)[:5]
+    with torch.no_grad():
+        want = [fn() for fn in fns]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def body():
+        s, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        with torch.no_grad(), torch.cuda.stream(s):
+            with torch.cuda.graph(graph, stream=s):
+                captured = [fn() for fn in fns]
+            for r in range(4):
+                eager = [fn() for fn in fns]
+                torch.cuda.synchronize()
+                wrong.extend(("eager", r, j) for j, y in enumerate(eager) if not torch.equal(y, want[j]))
+                for y in captured:
+                    y.zero_()
+                graph.replay()
+                torch.cuda.synchronize()
+                wrong.extend(("replay", r, j) for j, y in enumerate(captured) if not torch.equal(y, want[j]))
+
+    t = threading.Thread(target=body)
+    t.start()
+    t.join()
+    assert not wrong, wrong
