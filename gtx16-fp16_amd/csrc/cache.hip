@@ -1,0 +1,230 @@
+// A cache of keys and values in 8 bits: written as tokens arrive (g16_cache_write) and read back as rows
+// (g16_cache_read). The formats stand in g16.h.
+//
+// Both pass over their data once and are bound by memory. A run is the d values of one token's head; LP lanes have it, 8
+// values each, and find its largest magnitude by exchanges within a row of 16 lanes.
+#include <type_traits>
+
+#include "code8.hpp"
+
+namespace g16 {
+namespace {
+
+constexpr int kThreads = 256;
+
+struct Params {
+  char* rows[2];  // k, v
+  uint8_t* codes[2];
+  float* scales[2];
+  const int32_t* slots;
+  int64_t token[2], head[2];                                                        // bytes, of the rows
+  int64_t c_page[2], c_token[2], c_head[2], s_page[2], s_token[2], s_head[2];       // elements: bytes of the codes
+  uint32_t n, page, hkv, d, capacity;                                               // capacity: slots
+  uint32_t block_rows;
+};
+
+// The largest of LP lanes' values.
+template <int LP>
+__device__ inline uint32_t largest(uint32_t v) {
+  auto with = [&](auto ctrl) {
+    v = max(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), decltype(ctrl)::value, 0xf, 0xf, true)));
+  };
+  if constexpr (LP >= 2) with(std::integral_constant<int, 0xb1>{});    // lane ^ 1
+  if constexpr (LP >= 4) with(std::integral_constant<int, 0x4e>{});    // lane ^ 2
+  if constexpr (LP >= 8) with(std::integral_constant<int, 0x141>{});   // 7 - lane, of 8
+  if constexpr (LP >= 16) with(std::integral_constant<int, 0x140>{});  // 15 - lane, of 16
+  return v;
+}
+
+template <typename T>
+struct alignas(16) Eight {
+  T v[8];
+};
+
+// The largest magnitude's bits, as a float's, of eight values. Bits in place of values: NaN is above infinity then, so
+// nothing that is not finite is passed over.
+__device__ inline uint32_t top_of(const Eight<float>& x) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(x.v[j]) & 0x7fffffffu);
+  return m;
+}
+typedef unsigned short ushort2v __attribute__((ext_vector_type(2)));
+__device__ inline uint32_t top_of(const Eight<_Float16>& x) {
+  const u32x4 w = __builtin_bit_cast(u32x4, x);
+  ushort2v m = {0, 0};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) m = __builtin_elementwise_max(m, __builtin_bit_cast(ushort2v, w[j] & 0x7fff7fffu));
+  const unsigned short h = max(m[0], m[1]);
+  return __float_as_uint(static_cast<float>(__builtin_bit_cast(_Float16, h)));
+}
+
+// A workgroup: block_rows rows, all runs of them. Of rows with one slot the last is written, so every workgroup looks
+// through the later rows' slots: a map of its own slots' last 12 bits passes over nearly all of the others (n rows
+// are n^2 / 2 / block_rows looks in all).
+constexpr uint32_t kMapBits = 4096, kMostRows = 32;
+
+template <typename T, int CODE, int LP>
+__global__ __launch_bounds__(kThreads) void write_kernel(Params p) {
+  __shared__ uint32_t slot_of[kMostRows], live[kMostRows], map[kMapBits / 32];
+  const uint32_t tid = threadIdx.x, first = blockIdx.x * p.block_rows, here = min(p.block_rows, p.n - first);
+  const uint32_t lane = tid % LP, runs = here * 2 * p.hkv;
+  const bool inside = lane * 8 < p.d;
+  Eight<T> x = {};
+  auto load = [&](uint32_t run) {
+    const uint32_t r = run / (2 * p.hkv), of = run % (2 * p.hkv), kv = of >= p.hkv, h = of - (kv ? p.hkv : 0);
+    if (run < runs && inside)
+      x = *reinterpret_cast<const Eight<T>*>(p.rows[kv] + (first + r) * p.token[kv] + h * p.head[kv] + lane * 8 * sizeof(T));
+  };
+  uint32_t run = tid / LP;
+  load(run);
+  if (tid < here) {
+    const uint32_t s = static_cast<uint32_t>(p.slots[first + tid]);  // (negative ones: past every capacity)
+    slot_of[tid] = s;
+    live[tid] = s < p.capacity;
+  }
+  if (tid < kMapBits / 32) map[tid] = 0;
+  __syncthreads();
+  if (tid < here) atomicOr(&map[(slot_of[tid] % kMapBits) / 32], 1u << (slot_of[tid] % 32));
+  __syncthreads();
+  for (uint32_t i = first + 1 + tid; i < p.n; i += kThreads) {
+    const uint32_t s = static_cast<uint32_t>(p.slots[i]);
+    if (map[(s % kMapBits) / 32] >> (s % 32) & 1) {
+      for (uint32_t r = 0; r < here && first + r < i; ++r)
+        if (slot_of[r] == s) live[r] = 0;
+    }
+  }
+  __syncthreads();
+  for (; run < runs; run += kThreads / LP) {
+    const uint32_t r = run / (2 * p.hkv), of = run % (2 * p.hkv), kv = of >= p.hkv, h = of - (kv ? p.hkv : 0);
+    const Scaling s = scaling_of<CODE>(__uint_as_float(largest<LP>(top_of(x))));
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = to_f(x.v[j]);
+    const u32x2 codes = encode8<CODE>(v, s);
+    load(run + kThreads / LP);
+    if (live[r] != 0 && inside) {
+      const uint32_t page = slot_of[r] / p.page, at = slot_of[r] - page * p.page;
+      *reinterpret_cast<u32x2*>(p.codes[kv] + page * p.c_page[kv] + at * p.c_token[kv] + h * p.c_head[kv] + lane * 8) = codes;
+      if (lane == 0) p.scales[kv][page * p.s_page[kv] + at * p.s_token[kv] + h * p.s_head[kv]] = s.scale;
+    }
+  }
+}
+
+// A thread: eight values of kRuns runs.
+constexpr int kRuns = 4;
+
+template <typename T, int CODE, int LP>
+__global__ __launch_bounds__(kThreads) void read_kernel(Params p) {
+  const uint32_t lane = threadIdx.x % LP;
+  if (lane * 8 >= p.d) return;
+  const uint64_t first = static_cast<uint64_t>(blockIdx.x) * (kRuns * kThreads / LP) + threadIdx.x / LP;
+  const uint64_t runs = static_cast<uint64_t>(p.n) * 2 * p.hkv;
+  u32x2 codes[kRuns];
+  float scale[kRuns];
+  char* to[kRuns];
+#pragma unroll
+  for (int i = 0; i < kRuns; ++i) {
+    const uint64_t run = first + i * (kThreads / LP);
+    codes[i] = u32x2{0, 0};
+    scale[i] = 0.f;
+    to[i] = nullptr;
+    if (run >= runs) continue;
+    const uint32_t r = static_cast<uint32_t>(run / (2 * p.hkv)), of = static_cast<uint32_t>(run % (2 * p.hkv)), kv = of >= p.hkv;
+    const uint32_t h = of - (kv ? p.hkv : 0), slot = static_cast<uint32_t>(p.slots[r]);
+    to[i] = p.rows[kv] + ((static_cast<uint64_t>(r) * p.hkv + h) * p.d + lane * 8) * sizeof(T);
+    if (slot >= p.capacity) continue;
+    const uint32_t page = slot / p.page, at = slot - page * p.page;
+    codes[i] = *reinterpret_cast<const u32x2*>(p.codes[kv] + page * p.c_page[kv] + at * p.c_token[kv] + h * p.c_head[kv] + lane * 8);
+    scale[i] = p.scales[kv][page * p.s_page[kv] + at * p.s_token[kv] + h * p.s_head[kv]];
+  }
+#pragma unroll
+  for (int i = 0; i < kRuns; ++i) {
+    if (to[i] == nullptr) continue;
+    float v[8];
+    decode8<CODE>(codes[i], v);
+    Eight<T> x;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x.v[j] = static_cast<T>(v[j] * scale[i]);
+    *reinterpret_cast<Eight<T>*>(to[i]) = x;
+  }
+}
+
+template <typename T, int CODE, int LP>
+int run(Params p, bool write, hipStream_t stream) {
+  if (!write) {
+    const uint64_t runs = static_cast<uint64_t>(p.n) * 2 * p.hkv, blocks = (runs + kRuns * kThreads / LP - 1) / (kRuns * kThreads / LP);
+    if (blocks > (1u << 24) - 1) return G16_E_SHAPE;  // (2^32 threads a launch)
+    return launch(read_kernel<T, CODE, LP>, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), stream, p);
+  }
+  // Rows of a workgroup: enough for every lane, and more where there are many workgroups, which all look through the
+  // later rows' slots.
+  uint32_t rows = kThreads / LP / (2 * p.hkv);
+  rows = max(rows, p.n / 1024);
+  p.block_rows = min(max(rows, 1u), kMostRows);
+  const uint32_t blocks = (p.n + p.block_rows - 1) / p.block_rows;
+  if (blocks > (1u << 24) - 1) return G16_E_SHAPE;  // (2^32 threads a launch)
+  return launch(write_kernel<T, CODE, LP>, dim3(blocks), dim3(kThreads), stream, p);
+}
+template <typename T, int CODE>
+int run(const Params& p, bool write, hipStream_t stream) {
+  return p.d <= 8 ? run<T, CODE, 1>(p, write, stream) : p.d <= 16 ? run<T, CODE, 2>(p, write, stream) : p.d <= 32 ? run<T, CODE, 4>(p, write, stream)
+         : p.d <= 64 ? run<T, CODE, 8>(p, write, stream) : run<T, CODE, 16>(p, write, stream);
+}
+
+// (what the Python binding packs)
+static_assert(sizeof(g16_cache_args) == 7 * 8 + 16 * 8 + 8 * 4, "no padding");
+
+int cache(const g16_cache_args* args, bool write, void* stream) {
+  if (args == nullptr) return G16_E_NULL;
+  const g16_cache_args& a = *args;
+  if ((a.is_f32 != 0 && a.is_f32 != 1) || (a.code != G16_CODE_INT8 && a.code != G16_CODE_E4M3)) return G16_E_DTYPE;
+  if (a.rows < 0 || a.pages < 0 || a.page < 0 || a.hkv < 0 || a.hkv > (1 << 20) || a.d <= 0 || a.d % 8 != 0 || a.d > G16_ATTENTION_MAX_D) return G16_E_SHAPE;
+  if (static_cast<int64_t>(a.pages) * a.page > (1LL << 31) - 1) return G16_E_SHAPE;
+  if (a.rows == 0 || a.hkv == 0) return G16_OK;
+  const int64_t size = a.is_f32 ? 4 : 2;
+  if (a.k == nullptr || a.v == nullptr || a.slots == nullptr) return G16_E_NULL;
+  if (!aligned16(a.k) || !aligned16(a.v)) return G16_E_ALIGN;
+  const int64_t capacity = static_cast<int64_t>(a.pages) * a.page;
+  if (capacity > 0) {
+    if (a.k_cache == nullptr || a.v_cache == nullptr || a.k_scale == nullptr || a.v_scale == nullptr) return G16_E_NULL;
+    const int64_t all = a.kc_page | a.kc_token | a.kc_head | a.vc_page | a.vc_token | a.vc_head | static_cast<int64_t>(reinterpret_cast<uintptr_t>(a.k_cache)) |
+                        static_cast<int64_t>(reinterpret_cast<uintptr_t>(a.v_cache));
+    if (all % 8 != 0) return G16_E_ALIGN;
+  }
+  if (write && (a.k_token * size % 16 != 0 || a.k_head * size % 16 != 0 || a.v_token * size % 16 != 0 || a.v_head * size % 16 != 0)) return G16_E_ALIGN;
+  Params p = {};
+  p.rows[0] = static_cast<char*>(a.k);
+  p.rows[1] = static_cast<char*>(a.v);
+  p.codes[0] = static_cast<uint8_t*>(a.k_cache);
+  p.codes[1] = static_cast<uint8_t*>(a.v_cache);
+  p.scales[0] = a.k_scale;
+  p.scales[1] = a.v_scale;
+  p.slots = a.slots;
+  const int64_t strides[2][8] = {{a.k_token, a.k_head, a.kc_page, a.kc_token, a.kc_head, a.ks_page, a.ks_token, a.ks_head},
+                                 {a.v_token, a.v_head, a.vc_page, a.vc_token, a.vc_head, a.vs_page, a.vs_token, a.vs_head}};
+  for (int i = 0; i < 2; ++i) {
+    p.token[i] = strides[i][0] * size;
+    p.head[i] = strides[i][1] * size;
+    p.c_page[i] = strides[i][2];
+    p.c_token[i] = strides[i][3];
+    p.c_head[i] = strides[i][4];
+    p.s_page[i] = strides[i][5];
+    p.s_token[i] = strides[i][6];
+    p.s_head[i] = strides[i][7];
+  }
+  p.n = static_cast<uint32_t>(a.rows);
+  p.page = static_cast<uint32_t>(a.page > 0 ? a.page : 1);
+  p.hkv = static_cast<uint32_t>(a.hkv);
+  p.d = static_cast<uint32_t>(a.d);
+  p.capacity = static_cast<uint32_t>(capacity);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (a.code == G16_CODE_INT8) return a.is_f32 ? run<float, G16_CODE_INT8>(p, write, s) : run<_Float16, G16_CODE_INT8>(p, write, s);
+  return a.is_f32 ? run<float, G16_CODE_E4M3>(p, write, s) : run<_Float16, G16_CODE_E4M3>(p, write, s);
+}
+
+}  // namespace
+}  // namespace g16
+
+extern "C" int g16_cache_write(const g16_cache_args* args, void* stream) { return g16::cache(args, true, stream); }
+extern "C" int g16_cache_read(const g16_cache_args* args, void* stream) { return g16::cache(args, false, stream); }

@@ -234,6 +234,28 @@ static PyObject* fast_args_call(PyObject* self, PyObject* const* args, Py_ssize_
   return PyLong_FromLong(st);
 }
 
+/* struct_call(fn_addr, args, stream) -> status of int fn(const args*, stream) */
+static PyObject* fast_struct_call(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  void *fn, *stream;
+  char* data;
+  Py_ssize_t n;
+  int st;
+  _Alignas(16) unsigned char buf[kMaxArgs];
+  if (check_nargs("struct_call", nargs, 3) || as_ptr(args[0], &fn) || check_bound(fn) || as_ptr(args[2], &stream) ||
+      PyBytes_AsStringAndSize(args[1], &data, &n))
+    return NULL;
+  if (n % 8 != 0 || n > kMaxArgs) {
+    PyErr_SetString(PyExc_ValueError, "argument struct of an unexpected size");
+    return NULL;
+  }
+  memcpy(buf, data, (size_t)n);
+  Py_BEGIN_ALLOW_THREADS
+  st = ((args_call_fn)fn)(buf, stream);
+  Py_END_ALLOW_THREADS
+  return PyLong_FromLong(st);
+}
+
 /* ---- the usual calls of attention, attention_decode and lora_mm_t, checked and packed here -------------
  * Each takes what its Python function takes and returns the output, or None for anything but a call that
  * could go straight to the kernels: operands of another type, shape, layout or device, a gradient wanted,
@@ -704,6 +726,8 @@ static PyMethodDef fast_methods[] = {
      "a *_workspace_bytes entry point, by address, on a struct of arguments; returns its size"},
     {"args_call", (PyCFunction)(void (*)(void))fast_args_call, METH_FASTCALL,
      "an entry point, by address, on a struct of arguments; returns its status"},
+    {"struct_call", (PyCFunction)(void (*)(void))fast_struct_call, METH_FASTCALL,
+     "an entry point without workspace, by address, on a struct of arguments; returns its status"},
     {NULL, NULL, 0, NULL},
 };
 

@@ -16,7 +16,7 @@ from pathlib import Path
 import torch  # noqa: F401  (loads torch's HIP runtime before libg16.so)
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libg16.so"
-ABI_VERSION = 18
+ABI_VERSION = 19
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
@@ -73,6 +73,9 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "g16_attention": (_I, [_P, _P]),
     "g16_attention_decode_workspace_bytes": (_SZ, [_P]),
     "g16_attention_decode": (_I, [_P, _P]),
+    "g16_rotary": (_I, [_P, _P]),
+    "g16_cache_write": (_I, [_P, _P]),
+    "g16_cache_read": (_I, [_P, _P]),
     "g16_lora_workspace_bytes": (_SZ, [_P]),
     "g16_lora_shrink": (_I, [_P, _P]),
     "g16_lora_expand": (_I, [_P, _P]),

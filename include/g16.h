@@ -50,7 +50,7 @@
 extern "C" {
 #endif
 
-#define G16_ABI_VERSION 18
+#define G16_ABI_VERSION 19
 
 /* Status codes (negative: rejected by the library before any launch). */
 #define G16_OK 0
@@ -409,6 +409,61 @@ int g16_attention(const g16_attention_args* args, void* stream);
 int g16_attention_plan(const g16_attention_args* args, int* row_tile, int* splits);
 size_t g16_attention_decode_workspace_bytes(const g16_attention_args* args);
 int g16_attention_decode(const g16_attention_args* args, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Rotary positions. For row r, head h and pair i < pairs, by a = positions[axis(i) * rows + r] * freqs[i] radians,
+ *     (x0, x1) -> (x0 cos a - x1 sin a, x1 cos a + x0 sin a),
+ * (x0, x1) = values i and i + pairs of the head, or (interleaved) 2 i and 2 i + 1; values from 2 * pairs on are
+ * copied. rows = seqs * tokens, x [seqs, tokens, heads, d] by its strides, out contiguous; fp16 or fp32 (is_f32).
+ * Pairs sections[0] .. go by the first axis, the next sections[1] by the second, and so on: up to
+ * G16_ROTARY_MAX_AXES of them, pairs in all. The angle is the product of the two numbers as they are, reduced in
+ * 64 bits; cosine, sine and the rotation are fp32.
+ *   d a multiple of 8, 2 * pairs <= d; strides in elements, multiples of 16 bytes. One launch.
+ */
+#define G16_ROTARY_MAX_AXES 4
+#define G16_ROTARY_MAX_D 4096
+typedef struct {
+  const void* x;
+  void* out;
+  const int32_t* positions;
+  const float* freqs;
+  int64_t x_seq, x_token, x_head;
+  int32_t seqs, tokens, heads, d, pairs, axes;
+  int32_t sections[G16_ROTARY_MAX_AXES];
+  int32_t interleaved, is_f32;
+} g16_rotary_args;
+int g16_rotary(const g16_rotary_args* args, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * A cache of keys and values in 8 bits. For a token's head with values x and m = max |x|,
+ *     G16_CODE_INT8: scale = m / 127, code = x * (127 / m) rounded to the nearest integer, ties to even (the two
+ *       quotients in fp32, the product exact);
+ *     G16_CODE_E4M3: scale = 2^e with the smallest e that has m <= 448 * 2^e, code = x / scale rounded to the nearest
+ *       e4m3 value, ties to even (OCP: 4 bits of exponent, no infinities, largest value 448);
+ * the value that a code stands for is code * scale. m below G16_CODE_LEAST: scale and codes 0. An x that is not
+ * finite: scale NaN, codes 0, so that all of the head's values read as NaN.
+ *   Slot s of a cache [pages, page, hkv, d] is token s % page of page s / page; the codes are one byte each and contiguous
+ * along d, the scales are fp32, [pages, page, hkv]; strides in elements, those of the codes multiples of 8 bytes.
+ * k, v (rows; out rows for a read) [rows, hkv, d], fp16 or fp32 (is_f32).
+ * g16_cache_write: row r goes to slots[r]; a slot below 0 or past the cache's end is not written, and of several rows
+ * with one slot the last is. rows strides in elements, multiples of 16 bytes. One launch.
+ * g16_cache_read: row r is what slots[r] holds, zeros for a slot outside; k and v contiguous. One launch.
+ */
+#define G16_CODE_INT8 1
+#define G16_CODE_E4M3 2
+#define G16_CODE_LEAST 0x1p-96f
+typedef struct {
+  void *k, *v; /* rows: read by g16_cache_write, written by g16_cache_read */
+  void *k_cache, *v_cache;
+  float *k_scale, *v_scale;
+  const int32_t* slots;
+  int64_t k_token, k_head, v_token, v_head;
+  int64_t kc_page, kc_token, kc_head, vc_page, vc_token, vc_head;
+  int64_t ks_page, ks_token, ks_head, vs_page, vs_token, vs_head;
+  int32_t rows, pages, page, hkv, d, code, is_f32, reserved;
+} g16_cache_args;
+int g16_cache_write(const g16_cache_args* args, void* stream);
+int g16_cache_read(const g16_cache_args* args, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
  * Low-rank adapters beside a shared projection: with y [M,N] (fp32) the projection's result,
