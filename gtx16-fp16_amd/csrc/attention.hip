@@ -39,13 +39,12 @@
 #include <cfloat>
 #include <type_traits>
 
-#include "g16_common.hpp"
+#include "code8.hpp"
 
 namespace g16 {
 namespace {
 
 typedef float float8v __attribute__((ext_vector_type(8)));
-typedef float float2v __attribute__((ext_vector_type(2)));
 
 constexpr float kLag = 7.f;
 // fp16 weights are 2^kShift above their value, by way of the exponent. fp32 ones would lose bits of the exponent by that
@@ -1459,6 +1458,8 @@ __global__ __launch_bounds__(kThreads) void decode_join_kernel(Params p, int srt
                   });
 }
 
+#include "attention8.hpp"
+
 // ---- host ------------------------------------------------------------------------------------------------
 
 // (what the Python binding packs)
@@ -1471,8 +1472,9 @@ int cus_of(const g16_attention_args& a) {
   return n > 0 ? n : 256;
 }
 
-// What both entry points check; the strides of operands without elements are not looked at.
-int check(const g16_attention_args& a, bool decode) {
+// What the entry points check; the strides of operands without elements are not looked at. codes: the cache is in 8 bits,
+// whose rows are read by addresses of their own.
+int check(const g16_attention_args& a, bool decode, bool codes = false) {
   const int size = a.is_f32 ? 4 : 2;
   if (a.is_f32 != 0 && a.is_f32 != 1) return G16_E_DTYPE;
   if (a.seqs < 0 || a.q_len < 0 || a.k_len < 0 || a.hq < 0 || a.hkv < 0 || a.shared < 0 || a.d <= 0 || a.d % 8 != 0 ||
@@ -1491,8 +1493,15 @@ int check(const g16_attention_args& a, bool decode) {
   if (!aligned16(a.q) || !aligned16(a.out) || !row(decode ? 0 : a.q_token, a.q_head, false) || a.q_seq * size % 16 != 0) return G16_E_ALIGN;
   if (a.k_len > 0) {
     if (a.k == nullptr || a.v == nullptr) return G16_E_NULL;
-    if (!aligned16(a.k) || !aligned16(a.v) || a.k_seq * size % 16 != 0 || a.v_seq * size % 16 != 0) return G16_E_ALIGN;
-    if (!row(a.k_token, a.k_head, true) || !row(a.v_token, a.v_head, true)) return G16_E_SHAPE;
+    if (codes) {
+      const int64_t all = a.k_seq | a.k_token | a.k_head | a.v_seq | a.v_token | a.v_head | static_cast<int64_t>(reinterpret_cast<uintptr_t>(a.k)) |
+                          static_cast<int64_t>(reinterpret_cast<uintptr_t>(a.v));
+      if (all % 8 != 0) return G16_E_ALIGN;
+    } else if (!aligned16(a.k) || !aligned16(a.v) || a.k_seq * size % 16 != 0 || a.v_seq * size % 16 != 0) {
+      return G16_E_ALIGN;
+    } else if (!row(a.k_token, a.k_head, true) || !row(a.v_token, a.v_head, true)) {
+      return G16_E_SHAPE;
+    }
   }
   if (a.shared > 0) {
     if (a.shared_k == nullptr || a.shared_v == nullptr) return G16_E_NULL;
@@ -1708,6 +1717,37 @@ int run_decode(const Params& p, const DecodePlan& plan, hipStream_t stream) {
   return rc;
 }
 
+int check8(const g16_attention8_args& e) {
+  const int st = check(e.a, true, true);
+  if (e.code != G16_CODE_INT8 && e.code != G16_CODE_E4M3) return G16_E_DTYPE;
+  if (st != G16_OK || e.a.seqs == 0 || e.a.hq == 0) return st;
+  return e.a.k_len > 0 && (e.k_scale == nullptr || e.v_scale == nullptr) ? G16_E_NULL : G16_OK;
+}
+
+template <typename T, int DP, int CODE, int NR>
+int run_own8(const Params& p, const Params8& e, dim3 grid, hipStream_t stream) {
+  return p.d == DP ? launch(decode8_kernel<T, DP, CODE, NR, true>, grid, dim3(kThreads), stream, p, e)
+                   : launch(decode8_kernel<T, DP, CODE, NR, false>, grid, dim3(kThreads), stream, p, e);
+}
+template <typename T, int DP>
+int run_decode8(const Params& p, Params8 e, int code, const DecodePlan& plan, hipStream_t stream) {
+  const int srt = plan.skeys ? kKeyTile : kRowTile;
+  const unsigned nshared = static_cast<unsigned>(p.stiles) * p.ssplits * p.hkv;
+  e.first = nshared * slot_floats(srt, DP);
+  int rc = 0;
+  if (nshared > 0)
+    rc = plan.skeys ? launch(decode_kernel<T, DP, true>, dim3(nshared), dim3(kThreads), stream, p)
+                    : launch(decode_kernel<T, DP, false>, dim3(nshared), dim3(kThreads), stream, p);
+  const dim3 grid(static_cast<unsigned>(plan.own) * p.hkv);
+  if (rc == 0) {
+    if (code == G16_CODE_INT8) rc = p.group <= 16 ? run_own8<T, DP, G16_CODE_INT8, 1>(p, e, grid, stream) : run_own8<T, DP, G16_CODE_INT8, 2>(p, e, grid, stream);
+    else rc = p.group <= 16 ? run_own8<T, DP, G16_CODE_E4M3, 1>(p, e, grid, stream) : run_own8<T, DP, G16_CODE_E4M3, 2>(p, e, grid, stream);
+  }
+  if (rc == 0 && plan.join)
+    rc = launch(decode_join_kernel<T, DP>, dim3(static_cast<unsigned>((static_cast<int64_t>(p.seqs) * p.hq + 3) / 4)), dim3(kThreads), stream, p, srt);
+  return rc;
+}
+
 }  // namespace
 }  // namespace g16
 
@@ -1752,25 +1792,59 @@ extern "C" size_t g16_attention_decode_workspace_bytes(const g16_attention_args*
   return plan_decode(*args).bytes;
 }
 
-extern "C" int g16_attention_decode(const g16_attention_args* args, void* stream) {
-  if (args == nullptr) return G16_E_NULL;
-  const g16_attention_args& a = *args;
-  const int st = check(a, true);
-  if (st != G16_OK || a.seqs == 0 || a.hq == 0) return st;
-  const DecodePlan plan = plan_decode(a);
+// The plan of a call with checked arguments, and its parameters
+static int begin_decode(const g16_attention_args& a, DecodePlan& plan, Params& p) {
+  plan = plan_decode(a);
   if (plan.bytes > 0 && (a.workspace == nullptr || static_cast<size_t>(a.workspace_bytes) < plan.bytes)) return G16_E_WORKSPACE;
   if (!aligned16(a.workspace)) return G16_E_ALIGN;
   if (!fits_grid((static_cast<int64_t>(plan.stiles) * plan.ssplits + plan.own) * a.hkv) ||
       !fits_grid((static_cast<int64_t>(a.seqs) * a.hq + 3) / 4))
     return G16_E_SHAPE;
-  Params p = params(a);
+  p = params(a);
   p.causal = 0;
   p.stiles = plan.stiles;
   p.ssplits = plan.ssplits;
   p.otiles = plan.otiles;
   p.oitems = plan.oitems;
   p.least = plan.least;
+  return G16_OK;
+}
+
+extern "C" int g16_attention_decode(const g16_attention_args* args, void* stream) {
+  if (args == nullptr) return G16_E_NULL;
+  const g16_attention_args& a = *args;
+  int st = check(a, true);
+  if (st != G16_OK || a.seqs == 0 || a.hq == 0) return st;
+  DecodePlan plan;
+  Params p;
+  st = begin_decode(a, plan, p);
+  if (st != G16_OK) return st;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (a.is_f32) return a.d <= 64 ? run_decode<float, 64>(p, plan, s) : run_decode<float, 128>(p, plan, s);
   return a.d <= 64 ? run_decode<_Float16, 64>(p, plan, s) : run_decode<_Float16, 128>(p, plan, s);
+}
+
+extern "C" size_t g16_attention_decode8_workspace_bytes(const g16_attention8_args* args) {
+  if (args == nullptr || check8(*args) != G16_OK || args->a.seqs == 0 || args->a.hq == 0) return 0;
+  return plan_decode(args->a).bytes;
+}
+
+extern "C" int g16_attention_decode8(const g16_attention8_args* args, void* stream) {
+  if (args == nullptr) return G16_E_NULL;
+  const g16_attention8_args& e = *args;
+  const g16_attention_args& a = e.a;
+  int st = check8(e);
+  if (st != G16_OK || a.seqs == 0 || a.hq == 0) return st;
+  DecodePlan plan;
+  Params p;
+  st = begin_decode(a, plan, p);
+  if (st != G16_OK) return st;
+  p.k_seq = a.k_seq;
+  p.k_head = a.k_head;
+  p.v_seq = a.v_seq;
+  p.v_head = a.v_head;
+  const Params8 own = {e.k_scale, e.v_scale, e.ks_seq, e.ks_head, e.ks_token, e.vs_seq, e.vs_head, e.vs_token, a.k_token, a.v_token, 0};
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (a.is_f32) return a.d <= 64 ? run_decode8<float, 64>(p, own, e.code, plan, s) : run_decode8<float, 128>(p, own, e.code, plan, s);
+  return a.d <= 64 ? run_decode8<_Float16, 64>(p, own, e.code, plan, s) : run_decode8<_Float16, 128>(p, own, e.code, plan, s);
 }

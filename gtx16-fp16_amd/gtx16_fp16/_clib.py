@@ -76,6 +76,8 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "g16_rotary": (_I, [_P, _P]),
     "g16_cache_write": (_I, [_P, _P]),
     "g16_cache_read": (_I, [_P, _P]),
+    "g16_attention_decode8_workspace_bytes": (_SZ, [_P]),
+    "g16_attention_decode8": (_I, [_P, _P]),
     "g16_lora_workspace_bytes": (_SZ, [_P]),
     "g16_lora_shrink": (_I, [_P, _P]),
     "g16_lora_expand": (_I, [_P, _P]),

@@ -25,6 +25,10 @@ _FLT_MAX = torch.finfo(torch.float32).max
 _ARGS = struct.Struct("@12P13q13i2fi")
 assert _ARGS.size == 12 * 8 + 13 * 8 + 16 * 4
 
+# g16_attention8_args before its g16_attention_args
+_ARGS8 = struct.Struct("@2P6q2i")
+assert _ARGS8.size == 2 * 8 + 6 * 8 + 2 * 4
+
 _entry: dict[str, tuple[int, int]] = {}
 
 
@@ -183,10 +187,24 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_offsets: t
     return out
 
 
+def _pages(pages, k_cache: torch.Tensor, seqs: int):
+    """(page table or None, keys of a page, pages and keys of a request)"""
+    page = k_cache.shape[1]
+    if pages is None:
+        if k_cache.shape[0] != seqs:
+            raise ValueError("attention_decode: without pages, the caches' first dimension is the requests")
+        return None, page, 0, page
+    if pages.dim() != 2:
+        raise ValueError("attention_decode: pages must be [requests, pages of each]")
+    most = pages.shape[1]
+    return _ints("attention_decode", pages, (seqs, most), k_cache.device, "pages"), page, most, page * most
+
+
 def attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor, *,
                      pages: torch.Tensor | None = None, shared_k: torch.Tensor | None = None,
                      shared_v: torch.Tensor | None = None, scale: float | None = None, softcap: float = 0.0,
-                     slopes: torch.Tensor | None = None) -> torch.Tensor:
+                     slopes: torch.Tensor | None = None, k_scale: torch.Tensor | None = None,
+                     v_scale: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of one token per request: q [requests, heads, d] over each request's cached keys, its own
     token's among them, and a prefix that all requests share (read once for all of them).
 
@@ -195,9 +213,16 @@ def attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     request has ``lengths[b]`` (int32) keys, held to 0 .. its capacity; what lies behind them is not used, whatever
     it holds, and a page number outside the cache reads as zeros. ``shared_k`` and ``shared_v`` [prefix, key heads, d]
     come before every request's own keys. The token stands at its last key's position. Types, heads, scores
-    and the result are ``attention``'s; a request without any key gives zeros."""
+    and the result are ``attention``'s; a request without any key gives zeros.
+
+    With ``k_scale`` and ``v_scale`` the caches are in 8 bits, as ``cache_write`` leaves them: int8 or float8_e4m3fn, the scales fp32
+    of the caches' shape without d. Keys and values are then the codes' exact products with their scales; a shared
+    prefix stays in q's type. Such a cache is never copied: a head's codes are contiguous and start at a multiple of 8
+    bytes, all other strides are free."""
     if forward_ad._current_level >= 0:
-        refuse_tangents("attention_decode", q, k_cache, v_cache, shared_k, shared_v, slopes)
+        refuse_tangents("attention_decode", q, k_cache, v_cache, shared_k, shared_v, slopes, k_scale, v_scale)
+    if k_scale is not None or v_scale is not None:
+        return _decode8(q, k_cache, v_cache, lengths, pages, shared_k, shared_v, scale, softcap, slopes, k_scale, v_scale)
     out = direct().attention_decode(q, k_cache, v_cache, lengths, pages, shared_k, shared_v, scale, softcap, slopes)
     if out is not None:
         return out
@@ -209,17 +234,7 @@ def attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     refuse_gradients("attention_decode", q, k_cache, v_cache, shared_k, shared_v, slopes)
     dev, size = q.device, q.element_size()
     lengths = _ints("attention_decode", lengths, (seqs,), dev, "lengths")
-    page, max_pages = k_cache.shape[1], 0
-    if pages is not None:
-        if pages.dim() != 2:
-            raise ValueError("attention_decode: pages must be [requests, pages of each]")
-        max_pages = pages.shape[1]
-        pages = _ints("attention_decode", pages, (seqs, max_pages), dev, "pages")
-        capacity = page * max_pages
-    else:
-        if k_cache.shape[0] != seqs:
-            raise ValueError("attention_decode: without pages, the caches' first dimension is the requests")
-        capacity = page
+    pages, page, max_pages, capacity = _pages(pages, k_cache, seqs)
     scale, softcap = _numbers("attention_decode", scale, softcap, d)
     slopes = _slopes("attention_decode", slopes, hq, dev)
     q, k, v = _rows(q, size, d, False), _rows(k_cache, size, d, True), _rows(v_cache, size, d, True)
@@ -232,4 +247,41 @@ def attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
                      lengths.data_ptr(), _ptr(pages) if capacity else 0, _ptr(slopes), q.stride(0), 0, q.stride(1), *k.stride()[:3], *v.stride()[:3],
                      *shared_strides, seqs, 1, capacity, hq, hkv, d, shared, 0, page, max_pages, k.shape[0],
                      1 if size == 4 else 0, _sm_count(dev), scale, softcap, 0), dev)
+    return out
+
+
+def _decode8(q, k_cache, v_cache, lengths, pages, shared_k, shared_v, scale, softcap, slopes, k_scale, v_scale) -> torch.Tensor:
+    # attention_decode over a cache in 8 bits
+    from .cache import check_cache  # (which has its checks from here)
+
+    name = "attention_decode"
+    if k_scale is None or v_scale is None:
+        raise ValueError(f"{name}: k_scale and v_scale come together")
+    dev, dt = q.device, q.dtype
+    if not (q.is_cuda and (dt == _F16 or dt == _F32) and _is_target(dev.index or 0)):
+        raise ValueError(f"{name}: q must be an fp16 or fp32 tensor on a gfx950 device")
+    code = check_cache(name, k_cache, v_cache, k_scale, v_scale)
+    hkv, d = k_cache.shape[2:]
+    if q.dim() != 3 or q.shape[2] != d or k_cache.device != dev:
+        raise ValueError(f"{name}: q {tuple(q.shape)} must be [requests, heads, {d}] on the cache's device")
+    seqs, hq = q.shape[:2]
+    if hq and (not hkv or hq % hkv):
+        raise ValueError(f"{name}: {hq} query heads do not share {hkv} key heads evenly")
+    refuse_gradients(name, q, shared_k, shared_v, slopes, k_scale, v_scale)
+    lengths = _ints(name, lengths, (seqs,), dev, "lengths")
+    pages, page, max_pages, capacity = _pages(pages, k_cache, seqs)
+    scale, softcap = _numbers(name, scale, softcap, d)
+    slopes = _slopes(name, slopes, hq, dev)
+    size = q.element_size()
+    q = _rows(q, size, d, False)
+    sk, sv, shared, shared_strides = _shared(name, shared_k, shared_v, q, hkv, d, size)
+    out = torch.empty(q.shape, dtype=dt, device=dev)
+    if out.numel() == 0:
+        return out
+    _call("g16_attention_decode8",
+          _ARGS8.pack(k_scale.data_ptr(), v_scale.data_ptr(), *k_scale.stride(), *v_scale.stride(), code, 0)
+          + _ARGS.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _ptr(sk), _ptr(sv), out.data_ptr(), 0, 0, 0, lengths.data_ptr(),
+                       _ptr(pages) if capacity else 0, _ptr(slopes), q.stride(0), 0, q.stride(1), *k_cache.stride()[:3], *v_cache.stride()[:3],
+                       *shared_strides, seqs, 1, capacity, hq, hkv, d, shared, 0, page, max_pages, k_cache.shape[0],
+                       1 if size == 4 else 0, _sm_count(dev), scale, softcap, 0), dev)
     return out

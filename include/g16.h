@@ -465,6 +465,19 @@ typedef struct {
 int g16_cache_write(const g16_cache_args* args, void* stream);
 int g16_cache_read(const g16_cache_args* args, void* stream);
 
+/* g16_attention_decode over such a cache: `a` as there, k and v the codes, whose strides are in bytes and, like their
+ * pointers, multiples of 8 (no other limits); scales by strides in elements, ks_seq a request's or a page's. q, out and the
+ * shared prefix have a's type. A score is scale * k_scale * (q . code), a value v_scale * code; codes are multiplied exactly,
+ * with fp16 weights to 2^-17. A page outside the cache reads as zeros. One launch, one more for shared keys, one more where keys are split. */
+typedef struct {
+  const float *k_scale, *v_scale;
+  int64_t ks_seq, ks_token, ks_head, vs_seq, vs_token, vs_head;
+  int32_t code, reserved; /* G16_CODE_*; 0 */
+  g16_attention_args a;
+} g16_attention8_args;
+size_t g16_attention_decode8_workspace_bytes(const g16_attention8_args* args);
+int g16_attention_decode8(const g16_attention8_args* args, void* stream);
+
 /* ---------------------------------------------------------------------------------------------
  * Low-rank adapters beside a shared projection: with y [M,N] (fp32) the projection's result,
  *     out[m,:] = y[m,:] + scale[a] * (x[m,:] @ down[a]^T) @ up[a]^T,   a = index[m],
