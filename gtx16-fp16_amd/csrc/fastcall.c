@@ -256,7 +256,7 @@ static PyObject* fast_struct_call(PyObject* self, PyObject* const* args, Py_ssiz
   return PyLong_FromLong(st);
 }
 
-/* ---- the usual calls of attention, attention_decode and lora_mm_t, checked and packed here -------------
+/* ---- the usual calls of attention, attention_decode, lora_mm_t and others, checked and packed here -------------
  * Each takes what its Python function takes and returns the output, or None for anything but a call that
  * could go straight to the kernels: operands of another type, shape, layout or device, a gradient wanted,
  * a scratch buffer that has to grow. The Python function then looks at the arguments one by one, copies
@@ -670,15 +670,262 @@ no:
   return none_clear();
 }
 
+/* ---- rotary positions and caches in 8 bits --------------------------------------------------------------- */
+static PyObject *g_i8 = NULL, *g_e4m3 = NULL;
+typedef int (*rotary_fn)(const g16_rotary_args*, void*);
+typedef int (*cache_fn)(const g16_cache_args*, void*);
+typedef size_t (*attention8_size_fn)(const g16_attention8_args*);
+typedef int (*attention8_fn)(const g16_attention8_args*, void*);
+static rotary_fn g_rotary;
+static cache_fn g_cache_write, g_cache_read;
+static attention8_size_fn g_attention8_size;
+static attention8_fn g_attention8;
+
+static int contiguous(const tensor_t* t) {
+  int64_t step = 1;
+  for (int i = t->nd - 1; i >= 0; --i) {
+    if (t->shape[i] > 1 && t->stride[i] != step) return 0;
+    step *= t->shape[i];
+  }
+  return 1;
+}
+
+/* rotary(x, positions, freqs, sections, interleaved) */
+static const int kGradRotary[2] = {0, 2};
+static PyObject* fast_rotary(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  tensor_t x, at, f, t;
+  g16_rotary_args a;
+  void* stream;
+  PyObject* out;
+  int st;
+  if (check_nargs("rotary", nargs, 5)) return NULL;
+  if (g_ready == NULL) Py_RETURN_NONE;
+  memset(&a, 0, sizeof(a));
+  if (read_tensor(args[0], &x) || (x.nd != 3 && x.nd != 4) || (x.dtype != g_f16 && x.dtype != g_f32) || device_cus(x.device) <= 0 ||
+      !rows_ok(&x, x.dtype == g_f32 ? 4 : 2, 0, 0) || read_tensor(args[1], &at) || at.dtype != g_i32 || at.device != x.device || !contiguous(&at) ||
+      read_tensor(args[2], &f) || f.dtype != g_f32 || f.nd != 1 || f.device != x.device || !contiguous(&f) || wants_grad(args, kGradRotary, 2))
+    return none_clear();
+  const int64_t d = x.shape[x.nd - 1], pairs = f.shape[0];
+  if (d % 8 != 0 || d <= 0 || d > G16_ROTARY_MAX_D || 2 * pairs > d) return none_clear();
+  const int lead = x.nd - 2;
+  int skip = 0;
+  if (args[3] == Py_None) {
+    a.axes = 1;
+    a.sections[0] = (int)pairs;
+  } else {
+    int64_t parts[4], sum = 0;
+    Py_INCREF(args[3]);
+    if (int_tuple(args[3], parts, &a.axes) || a.axes < 1 || a.axes > G16_ROTARY_MAX_AXES) return none_clear();
+    for (int i = 0; i < a.axes; ++i) {
+      if (parts[i] < 0 || parts[i] > pairs) return none_clear();
+      a.sections[i] = (int)parts[i];
+      sum += parts[i];
+    }
+    if (sum != pairs) return none_clear();
+    skip = 1;
+  }
+  if (at.nd != lead + skip || (skip && at.shape[0] != a.axes)) return none_clear();
+  for (int i = 0; i < lead; ++i)
+    if (at.shape[skip + i] != x.shape[i]) return none_clear();
+  for (int i = 0; i < x.nd; ++i)
+    if (x.shape[i] <= 0 || !fits(x.shape[i])) return none_clear();
+  const int interleaved = PyObject_IsTrue(args[4]);
+  if (interleaved < 0 || raw_stream(x.device, &stream)) return none_clear();
+  out = empty_like(args[0]);
+  if (out == NULL || read_tensor(out, &t)) {
+    Py_XDECREF(out);
+    return none_clear();
+  }
+  a.x = x.ptr, a.out = t.ptr, a.positions = at.ptr, a.freqs = f.ptr;
+  a.x_seq = lead == 2 ? x.stride[0] : 0, a.x_token = x.stride[lead - 1], a.x_head = x.stride[lead];
+  a.seqs = lead == 2 ? (int)x.shape[0] : 1, a.tokens = (int)x.shape[lead - 1], a.heads = (int)x.shape[lead];
+  a.d = (int)d, a.pairs = (int)pairs, a.interleaved = interleaved, a.is_f32 = x.dtype == g_f32;
+  Py_BEGIN_ALLOW_THREADS
+  st = g_rotary(&a, stream);
+  Py_END_ALLOW_THREADS
+  if (st != 0) {
+    Py_DECREF(out);
+    Py_RETURN_NONE;
+  }
+  return out;
+}
+
+/* A cache that the kernels read in place: args k_cache, v_cache, k_scale, v_scale (check_cache in cache.py); its code, 0 else */
+static int cache_ok(PyObject* const* args, tensor_t* kc, tensor_t* vc, tensor_t* ks, tensor_t* vs) {
+  if (read_tensor(args[0], kc) || read_tensor(args[1], vc) || read_tensor(args[2], ks) || read_tensor(args[3], vs)) return 0;
+  const int code = kc->dtype == g_i8 ? G16_CODE_INT8 : kc->dtype == g_e4m3 ? G16_CODE_E4M3 : 0;
+  if (code == 0 || vc->dtype != kc->dtype || kc->nd != 4 || vc->nd != 4 || ks->nd != 3 || vs->nd != 3 || ks->dtype != g_f32 || vs->dtype != g_f32 ||
+      vc->device != kc->device || ks->device != kc->device || vs->device != kc->device || device_cus(kc->device) <= 0)
+    return 0;
+  for (int i = 0; i < 4; ++i)
+    if (kc->shape[i] <= 0 || !fits(kc->shape[i]) || vc->shape[i] != kc->shape[i] || (i < 3 && (ks->shape[i] != kc->shape[i] || vs->shape[i] != kc->shape[i])))
+      return 0;
+  if (kc->shape[3] % 8 != 0 || kc->shape[3] > G16_ATTENTION_MAX_D || kc->stride[3] != 1 || vc->stride[3] != 1 ||
+      ((kc->stride[0] | kc->stride[1] | kc->stride[2] | vc->stride[0] | vc->stride[1] | vc->stride[2]) & 7) != 0 ||
+      (((uintptr_t)kc->ptr | (uintptr_t)vc->ptr) & 7) != 0 || kc->shape[0] * kc->shape[1] > INT32_MAX)
+    return 0;
+  return code;
+}
+
+static void cache_args(g16_cache_args* a, const tensor_t* kc, const tensor_t* vc, const tensor_t* ks, const tensor_t* vs, const tensor_t* slots,
+                       int code, int is_f32) {
+  memset(a, 0, sizeof(*a));
+  a->k_cache = kc->ptr, a->v_cache = vc->ptr, a->k_scale = ks->ptr, a->v_scale = vs->ptr, a->slots = slots->ptr;
+  a->kc_page = kc->stride[0], a->kc_token = kc->stride[1], a->kc_head = kc->stride[2];
+  a->vc_page = vc->stride[0], a->vc_token = vc->stride[1], a->vc_head = vc->stride[2];
+  a->ks_page = ks->stride[0], a->ks_token = ks->stride[1], a->ks_head = ks->stride[2];
+  a->vs_page = vs->stride[0], a->vs_token = vs->stride[1], a->vs_head = vs->stride[2];
+  a->rows = (int)slots->shape[0], a->pages = (int)kc->shape[0], a->page = (int)kc->shape[1], a->hkv = (int)kc->shape[2], a->d = (int)kc->shape[3];
+  a->code = code, a->is_f32 = is_f32;
+}
+
+/* A vector of slots on a device */
+static int slots_ok(PyObject* o, int device, tensor_t* t) {
+  return !read_tensor(o, t) && t->dtype == g_i32 && t->nd == 1 && t->device == device && contiguous(t) && t->shape[0] > 0 && fits(t->shape[0]);
+}
+
+/* cache_write(k, v, k_cache, v_cache, k_scale, v_scale, slots): true where it is done */
+static const int kGradWrite[4] = {0, 1, 4, 5};
+static PyObject* fast_cache_write(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  tensor_t k, v, kc, vc, ks, vs, slots;
+  g16_cache_args a;
+  void* stream;
+  int st;
+  if (check_nargs("cache_write", nargs, 7)) return NULL;
+  if (g_ready == NULL) Py_RETURN_NONE;
+  const int code = cache_ok(args + 2, &kc, &vc, &ks, &vs);
+  if (code == 0 || read_tensor(args[0], &k) || read_tensor(args[1], &v) || k.nd != 3 || v.nd != 3 || (k.dtype != g_f16 && k.dtype != g_f32) ||
+      v.dtype != k.dtype || k.device != kc.device || v.device != kc.device || !slots_ok(args[6], kc.device, &slots) || wants_grad(args, kGradWrite, 4))
+    return none_clear();
+  const int size = k.dtype == g_f32 ? 4 : 2;
+  if (k.shape[0] != slots.shape[0] || k.shape[1] != kc.shape[2] || k.shape[2] != kc.shape[3] || memcmp(k.shape, v.shape, sizeof(int64_t) * 3) != 0 ||
+      !rows_ok(&k, size, 0, 0) || !rows_ok(&v, size, 0, 0))
+    return none_clear();
+  const tensor_t* own[4] = {&kc, &vc, &ks, &vs};
+  for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < 3; ++j)
+      if (own[i]->shape[j] > 1 && own[i]->stride[j] == 0) return none_clear();
+  if (raw_stream(kc.device, &stream)) return none_clear();
+  cache_args(&a, &kc, &vc, &ks, &vs, &slots, code, size == 4);
+  a.k = k.ptr, a.v = v.ptr;
+  a.k_token = k.stride[0], a.k_head = k.stride[1], a.v_token = v.stride[0], a.v_head = v.stride[1];
+  Py_BEGIN_ALLOW_THREADS
+  st = g_cache_write(&a, stream);
+  Py_END_ALLOW_THREADS
+  if (st != 0) Py_RETURN_NONE;
+  Py_RETURN_TRUE;
+}
+
+/* cache_read(k_cache, v_cache, k_scale, v_scale, slots, out_dtype) -> (k, v) */
+static const int kGradRead[2] = {2, 3};
+static PyObject* fast_cache_read(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  tensor_t kc, vc, ks, vs, slots, t;
+  g16_cache_args a;
+  void* stream;
+  PyObject *k = NULL, *v = NULL, *shape = NULL, *both = NULL;
+  int st = -1;
+  if (check_nargs("cache_read", nargs, 6)) return NULL;
+  if (g_ready == NULL) Py_RETURN_NONE;
+  const int code = cache_ok(args, &kc, &vc, &ks, &vs);
+  if (code == 0 || !slots_ok(args[4], kc.device, &slots) || (args[5] != g_f16 && args[5] != g_f32) || wants_grad(args, kGradRead, 2) ||
+      raw_stream(kc.device, &stream))
+    return none_clear();
+  cache_args(&a, &kc, &vc, &ks, &vs, &slots, code, args[5] == g_f32);
+  shape = Py_BuildValue("(LLL)", (long long)slots.shape[0], (long long)kc.shape[2], (long long)kc.shape[3]);
+  PyObject* argv[3] = {args[2], shape, args[5]};
+  if (shape != NULL) k = PyObject_VectorcallMethod(s_new_empty, argv, 2, s_dtype_names);
+  if (k != NULL) v = PyObject_VectorcallMethod(s_new_empty, argv, 2, s_dtype_names);
+  if (v != NULL && !read_tensor(k, &t)) {
+    a.k = t.ptr;
+    if (!read_tensor(v, &t)) {
+      a.v = t.ptr;
+      Py_BEGIN_ALLOW_THREADS
+      st = g_cache_read(&a, stream);
+      Py_END_ALLOW_THREADS
+    }
+  }
+  if (st == 0) both = PyTuple_Pack(2, k, v);
+  Py_XDECREF(shape);
+  Py_XDECREF(k);
+  Py_XDECREF(v);
+  return both != NULL ? both : none_clear();
+}
+
+/* attention_decode8(q, k_cache, v_cache, lengths, pages, shared_k, shared_v, scale, softcap, slopes, k_scale, v_scale) */
+static const int kGradDecode8[6] = {0, 5, 6, 9, 10, 11};
+static PyObject* fast_attention_decode8(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  tensor_t q, kc, vc, ks, vs, t;
+  g16_attention8_args e;
+  void* stream;
+  PyObject* out;
+  int st;
+  if (check_nargs("attention_decode8", nargs, 12)) return NULL;
+  if (g_ready == NULL) Py_RETURN_NONE;
+  memset(&e, 0, sizeof(e));
+  g16_attention_args* a = &e.a;
+  PyObject* const cache[4] = {args[1], args[2], args[10], args[11]};
+  e.code = cache_ok(cache, &kc, &vc, &ks, &vs);
+  if (e.code == 0 || read_tensor(args[0], &q) || q.nd != 3 || (q.dtype != g_f16 && q.dtype != g_f32) || q.device != kc.device || q.shape[0] <= 0 ||
+      !fits(q.shape[0]) || q.shape[1] <= 0 || !fits(q.shape[1]) || q.shape[1] % kc.shape[2] != 0 || q.shape[2] != kc.shape[3] ||
+      !rows_ok(&q, q.dtype == g_f32 ? 4 : 2, 0, 0) || wants_grad(args, kGradDecode8, 6) ||
+      vector(args[3], g_i32, q.shape[0], q.device, (const void**)&a->lengths) || a->lengths == NULL)
+    return none_clear();
+  a->is_f32 = q.dtype == g_f32, a->num_cus = device_cus(q.device);
+  a->seqs = (int)q.shape[0], a->q_len = 1, a->hq = (int)q.shape[1], a->hkv = (int)kc.shape[2], a->d = (int)q.shape[2];
+  a->page = (int)kc.shape[1], a->num_pages = (int)kc.shape[0], a->k_len = a->page;
+  if (args[4] != Py_None) {
+    if (read_tensor(args[4], &t) || t.dtype != g_i32 || t.nd != 2 || t.shape[0] != a->seqs || t.device != q.device || !contiguous(&t) || t.shape[1] == 0 ||
+        !fits(t.shape[1] * a->page))
+      return none_clear();
+    a->pages = t.ptr;
+    a->max_pages = (int)t.shape[1];
+    a->k_len = a->max_pages * a->page;
+  } else if (kc.shape[0] != a->seqs) {
+    return none_clear();
+  }
+  if (!rest_ok(args[7], args[8], args[5], args[6], args[9], q.device, q.dtype, a)) return none_clear();
+  a->q = q.ptr, a->k = kc.ptr, a->v = vc.ptr;
+  a->q_seq = q.stride[0], a->q_head = q.stride[1];
+  a->k_seq = kc.stride[0], a->k_token = kc.stride[1], a->k_head = kc.stride[2];
+  a->v_seq = vc.stride[0], a->v_token = vc.stride[1], a->v_head = vc.stride[2];
+  e.k_scale = ks.ptr, e.v_scale = vs.ptr;
+  e.ks_seq = ks.stride[0], e.ks_token = ks.stride[1], e.ks_head = ks.stride[2];
+  e.vs_seq = vs.stride[0], e.vs_token = vs.stride[1], e.vs_head = vs.stride[2];
+  const size_t bytes = g_attention8_size(&e);
+  if (raw_stream(q.device, &stream) || (bytes > 0 && scratch(q.device, stream, bytes, &a->workspace))) return none_clear();
+  if (bytes > 0 && a->workspace == NULL) Py_RETURN_NONE;
+  a->workspace_bytes = (int64_t)bytes;
+  out = empty_like(args[0]);
+  if (out == NULL || read_tensor(out, &t)) {
+    Py_XDECREF(out);
+    return none_clear();
+  }
+  a->out = t.ptr;
+  Py_BEGIN_ALLOW_THREADS
+  st = g_attention8(&e, stream);
+  Py_END_ALLOW_THREADS
+  if (st != 0) {
+    Py_DECREF(out);
+    Py_RETURN_NONE;
+  }
+  return out;
+}
+
 /* bind_torch(float16, float32, int32, raw_stream(device), is_grad_enabled(), ready(device) -> compute units or
  * -1, scratch(device, stream, bytes) -> pointer, route (see product_route), [addresses of
  * g16_attention_workspace_bytes, g16_attention, g16_attention_decode_workspace_bytes, g16_attention_decode,
- * g16_mm_t_raw, g16_mm_t_direct, g16_lora_workspace_bytes, g16_lora_shrink, g16_lora_expand]) */
+ * g16_mm_t_raw, g16_mm_t_direct, g16_lora_workspace_bytes, g16_lora_shrink, g16_lora_expand, g16_rotary, g16_cache_write,
+ * g16_cache_read, g16_attention_decode8_workspace_bytes, g16_attention_decode8], int8, float8_e4m3fn) */
+enum { kEntryPoints = 14 };
 static PyObject* fast_bind_torch(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
   (void)self;
-  void* fn[9];
-  if (check_nargs("bind_torch", nargs, 9)) return NULL;
-  for (int i = 0; i < 9; ++i) {
+  void* fn[kEntryPoints];
+  if (check_nargs("bind_torch", nargs, 11)) return NULL;
+  for (int i = 0; i < kEntryPoints; ++i) {
     PyObject* o = PySequence_GetItem(args[8], i);
     const int bad = o == NULL || as_ptr(o, &fn[i]) || check_bound(fn[i]);
     Py_XDECREF(o);
@@ -693,8 +940,14 @@ static PyObject* fast_bind_torch(PyObject* self, PyObject* const* args, Py_ssize
   g_lora_size = (lora_size_fn)fn[6];
   g_lora_shrink = (lora_fn)fn[7];
   g_lora_expand = (lora_fn)fn[8];
-  PyObject** to[8] = {&g_f16, &g_f32, &g_i32, &g_raw_stream, &g_grad_enabled, &g_ready, &g_scratch, &g_route};
-  for (int i = 0; i < 8; ++i) {
+  g_rotary = (rotary_fn)fn[9];
+  g_cache_write = (cache_fn)fn[10];
+  g_cache_read = (cache_fn)fn[11];
+  g_attention8_size = (attention8_size_fn)fn[12];
+  g_attention8 = (attention8_fn)fn[13];
+  PyObject** to[11] = {&g_f16, &g_f32, &g_i32, &g_raw_stream, &g_grad_enabled, &g_ready, &g_scratch, &g_route, NULL, &g_i8, &g_e4m3};
+  for (int i = 0; i < 11; ++i) {
+    if (to[i] == NULL) continue;
     Py_INCREF(args[i]);
     Py_XSETREF(*to[i], args[i]);
   }
@@ -722,6 +975,13 @@ static PyMethodDef fast_methods[] = {
      "attention_decode for arguments that need no copy; None for any others"},
     {"lora_mm_t", (PyCFunction)(void (*)(void))fast_lora_mm_t, METH_FASTCALL,
      "lora_mm_t for arguments that need no copy; None for any others"},
+    {"rotary", (PyCFunction)(void (*)(void))fast_rotary, METH_FASTCALL, "rotary for arguments that need no copy; None for any others"},
+    {"cache_write", (PyCFunction)(void (*)(void))fast_cache_write, METH_FASTCALL,
+     "cache_write for arguments that need no copy; None for any others"},
+    {"cache_read", (PyCFunction)(void (*)(void))fast_cache_read, METH_FASTCALL,
+     "cache_read for arguments that need no copy; None for any others"},
+    {"attention_decode8", (PyCFunction)(void (*)(void))fast_attention_decode8, METH_FASTCALL,
+     "attention_decode over a cache in 8 bits for arguments that need no copy; None for any others"},
     {"args_size", (PyCFunction)(void (*)(void))fast_args_size, METH_FASTCALL,
      "a *_workspace_bytes entry point, by address, on a struct of arguments; returns its size"},
     {"args_call", (PyCFunction)(void (*)(void))fast_args_call, METH_FASTCALL,

@@ -252,6 +252,9 @@ def attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
 
 def _decode8(q, k_cache, v_cache, lengths, pages, shared_k, shared_v, scale, softcap, slopes, k_scale, v_scale) -> torch.Tensor:
     # attention_decode over a cache in 8 bits
+    out = direct().attention_decode8(q, k_cache, v_cache, lengths, pages, shared_k, shared_v, scale, softcap, slopes, k_scale, v_scale)
+    if out is not None:
+        return out
     from .cache import check_cache  # (which has its checks from here)
 
     name = "attention_decode"

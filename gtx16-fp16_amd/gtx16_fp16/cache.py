@@ -13,7 +13,7 @@ from torch.autograd import forward_ad
 
 from . import _clib
 from .attn import MAX_HEAD_DIM, _ints, _rows
-from .direct import refuse_gradients, refuse_tangents
+from .direct import direct, refuse_gradients, refuse_tangents
 from .kernels import stream_handle
 from .ops import _is_target
 
@@ -74,6 +74,8 @@ def cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache
     name = "cache_write"
     if forward_ad._current_level >= 0:
         refuse_tangents(name, k, v, k_scale, v_scale)
+    if direct().cache_write(k, v, k_cache, v_cache, k_scale, v_scale, slots):
+        return
     dev = k.device
     if not (k.is_cuda and k.dtype in (torch.float16, torch.float32) and v.dtype == k.dtype and v.device == dev and _is_target(dev.index or 0)):
         raise ValueError(f"{name}: k and v must be fp16 or fp32 tensors of one type on one gfx950 device")
@@ -101,6 +103,9 @@ def cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tens
     name = "cache_read"
     if forward_ad._current_level >= 0:
         refuse_tangents(name, k_scale, v_scale)
+    both = direct().cache_read(k_cache, v_cache, k_scale, v_scale, slots, out_dtype)
+    if both is not None:
+        return both
     if out_dtype not in (torch.float32, torch.float16):
         raise ValueError(f"out_dtype must be float32 or float16, got {out_dtype}")
     dev = k_cache.device

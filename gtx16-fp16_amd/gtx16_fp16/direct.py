@@ -1,4 +1,5 @@
-"""The usual calls of ``attention``, ``attention_decode`` and ``lora_mm_t``, made by the extension.
+"""The usual calls of ``attention``, ``attention_decode``, ``lora_mm_t``, ``rotary`` and the caches in 8 bits, made by the
+extension.
 
 A small call is bound by the host: checked and packed in Python, one costs 8 us besides its launches, about
 as long as its kernels run. ``_g16fast`` does the same for arguments that need no copy, and returns None for
@@ -15,7 +16,8 @@ from .kernels import _MAX_CACHED_SCRATCH, SKINNY_MAX_M, scratch_buffer, split_bu
 from .ops import _is_target, _sm_count
 
 _ENTRY_POINTS = ("g16_attention_workspace_bytes", "g16_attention", "g16_attention_decode_workspace_bytes", "g16_attention_decode",
-                 "g16_mm_t_raw", "g16_mm_t_direct", "g16_lora_workspace_bytes", "g16_lora_shrink", "g16_lora_expand")
+                 "g16_mm_t_raw", "g16_mm_t_direct", "g16_lora_workspace_bytes", "g16_lora_shrink", "g16_lora_expand", "g16_rotary",
+                 "g16_cache_write", "g16_cache_read", "g16_attention_decode8_workspace_bytes", "g16_attention_decode8")
 
 
 def _ready(device: int) -> int:
@@ -71,6 +73,6 @@ def direct():
     if _bound is None:
         fast = _clib.fast()
         fast.bind_torch(torch.float16, torch.float32, torch.int32, torch._C._cuda_getCurrentRawStream, torch.is_grad_enabled, _ready,
-                        _scratch_ptr, _route, [_clib.address(n) for n in _ENTRY_POINTS])
+                        _scratch_ptr, _route, [_clib.address(n) for n in _ENTRY_POINTS], torch.int8, torch.float8_e4m3fn)
         _bound = fast
     return _bound

@@ -12,7 +12,7 @@ from torch.autograd import forward_ad
 
 from . import _clib
 from .attn import _ints, _rows
-from .direct import refuse_gradients, refuse_tangents
+from .direct import direct, refuse_gradients, refuse_tangents
 from .kernels import stream_handle
 from .ops import _is_target
 
@@ -41,6 +41,9 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, *, sec
     their places); its cosine and sine, to 1e-7, and the rotation are fp32."""
     if forward_ad._current_level >= 0:
         refuse_tangents("rotary", x, freqs)
+    out = direct().rotary(x, positions, freqs, sections, interleaved)
+    if out is not None:
+        return out
     dev, dt = x.device, x.dtype
     if not (x.is_cuda and (dt == torch.float16 or dt == torch.float32) and _is_target(dev.index or 0)):
         raise ValueError("rotary: x must be an fp16 or fp32 tensor on a gfx950 device")
