@@ -36,108 +36,12 @@
 // With too few tiles to fill the card, the keys are split over workgroups as well, which leave (O, maximum,
 // sum) in the workspace (prompt_time weighs shapes and splits); a second launch joins them in split order (no
 // atomics: repeated calls agree).
-#include <cfloat>
-#include <type_traits>
-
-#include "code8.hpp"
+#include "attention8.hpp"
 
 namespace g16 {
 namespace {
 
-typedef float float8v __attribute__((ext_vector_type(8)));
-
-constexpr float kLag = 7.f;
-// fp16 weights are 2^kShift above their value, by way of the exponent. fp32 ones would lose bits of the exponent by that
-// (2^-20 of a weight at 23), and are multiplied by kScale: at most 2^-16, so that the sums over 65536
-// keys of the largest weight stay within the values' range.
-template <typename T>
-constexpr float kShift = sizeof(T) == 2 ? 8.f : 0.f;
-template <typename T>
-constexpr float kScale = sizeof(T) == 2 ? 1.f : 0x1p-23f;
-constexpr float kLog2e = 1.44269504088896341f;
-constexpr float kPlainCap = 256.f;  // largest tanh cap that fp16 inputs take the plain form for (tanh_of)
-constexpr float kNoCap = 0x1p100f;  // a cap from here on changes no fp32 score below 2^88, and would not fit in log2 units
-constexpr int kRowTile = 128, kKeyTile = 32;  // query rows of the two workgroup shapes
-constexpr int kThreads = 256;
-
-__device__ __attribute__((aligned(16))) const uint32_t g_zero_row[G16_ATTENTION_MAX_D] = {};
-
-template <typename T>
-struct Vec8 {
-  using V = half8;
-};
-template <>
-struct Vec8<float> {
-  using V = float8v;
-};
-
-__device__ inline float16v mma(half8 a, half8 b, float16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
-__device__ inline float16v mma(float8v a, float8v b, float16v c) {
-#pragma unroll
-  for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
-  return c;
-}
-
-// fp32 as three bf16 parts, hi + mid + lo.
-typedef __bf16 bhalf8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bhalf2 __attribute__((ext_vector_type(2)));
-struct Split8 {
-  bhalf8 hi, mid, lo;
-};
-__device__ inline float16v mma(bhalf8 a, bhalf8 b, float16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
-__device__ inline float8v widen(bhalf8 v) { return __builtin_convertvector(v, float8v); }
-__device__ inline float8v whole(const Split8& s) { return widen(s.hi) + widen(s.mid) + widen(s.lo); }  // (no part rounds)
-// ... all products of parts but the largest
-__device__ inline float16v mma_small(const Split8& a, const Split8& b, float16v c) {
-  c = mma(a.lo, b.hi, c);
-  c = mma(a.mid, b.mid, c);
-  c = mma(a.hi, b.lo, c);
-  c = mma(a.mid, b.hi, c);
-  return mma(a.hi, b.mid, c);
-}
-__device__ inline float16v mma(const Split8& a, const Split8& b, float16v c) { return mma(a.hi, b.hi, mma_small(a, b, c)); }
-// What becomes of 8 values that are multiplied: fp16 as it is, fp32 in parts.
-__device__ inline half8 operand(half8 v) { return v; }
-// Values rounded to bf16, taken off them: 20 instructions for 8. (A dot product with (-1, 0) would save the unpacking,
-// but v_dot2_f32_bf16 does not give the difference exactly, and takes as long.)
-__device__ inline bhalf8 take_part(float8v& v) {
-  bhalf8 part;
-#pragma unroll
-  for (int j = 0; j < 8; j += 2) {
-    const bhalf2 two = __builtin_convertvector((float2v{v[j], v[j + 1]}), bhalf2);
-    const uint32_t bits = __builtin_bit_cast(uint32_t, two);
-    part[j] = two[0];
-    part[j + 1] = two[1];
-    v[j] -= __uint_as_float(bits << 16);
-    v[j + 1] -= __uint_as_float(bits & 0xffff0000u);
-  }
-  return part;
-}
-__device__ inline Split8 operand(float8v v) {
-  Split8 s;
-  s.hi = take_part(v);
-  s.mid = take_part(v);
-  s.lo = __builtin_convertvector(v, bhalf8);
-  return s;
-}
-// The same for any fp32 value: whole() gives it back, NaN, infinities and those that round to one included.
-__device__ inline Split8 operand_of_any(float8v v) {
-  bhalf8 hi = __builtin_convertvector(v, bhalf8);
-  float8v rest;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    if (fabsf(static_cast<float>(hi[j])) <= FLT_MAX || v[j] != v[j]) {
-      rest[j] = v[j] - static_cast<float>(hi[j]);
-    } else {  // its first 8 bits, cut off
-      const float cut = __uint_as_float(__float_as_uint(v[j]) & 0xffff0000u);
-      hi[j] = static_cast<__bf16>(cut);
-      rest[j] = fabsf(cut) <= FLT_MAX ? v[j] - cut : 0.f;
-    }
-  }
-  Split8 s = operand(rest);
-  // (at most 16 bits are left: two parts)
-  return Split8{hi, s.hi, s.mid};
-}
+using g16::uniform;
 
 // Whether what a lane has seen is to be split: not where a value is 2^64 or more or not a number (or, which does no
 // harm, where a sum of large ones is).
@@ -155,40 +59,6 @@ __device__ inline float other_half(float v) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
 }
-
-template <typename P>
-__device__ inline P* uniform(P* p) {
-  const uint64_t v = reinterpret_cast<uint64_t>(p);
-  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
-  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32));
-  return reinterpret_cast<P*>((static_cast<uint64_t>(hi) << 32) | lo);
-}
-__device__ inline int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-
-// Where part `i` of `parts` about equal ones of n things begins (32 bits throughout: n * i / parts in 64 would be
-// 150 scalar instructions).
-__device__ inline int share_begin(int n, int i, int parts) {
-  const uint32_t each = static_cast<uint32_t>(n) / static_cast<uint32_t>(parts), more = static_cast<uint32_t>(n) % static_cast<uint32_t>(parts);
-  return static_cast<int>(each * i + min(more, static_cast<uint32_t>(i)));
-}
-
-struct Params {
-  const char *q, *k, *v, *sk, *sv;
-  char* out;
-  const int32_t *q_off, *k_off, *visible, *lengths, *pages;
-  const float* slopes;
-  float* part;
-  int64_t q_seq, q_tok, q_head, k_seq, k_head, v_seq, v_head, sk_head, sv_head;  // bytes
-  uint32_t k_tok, v_tok, sk_tok, sv_tok;                                        // bytes
-  int seqs, q_len, k_len, hq, hkv, group, d, shared, causal;
-  int page, max_pages, num_pages;
-  int tiles, splits;              // prompts: row tiles (an upper bound where packed), key splits
-  int stiles, ssplits;            // single tokens: row tiles and splits of the shared keys
-  int otiles, oitems, least;      // ... row tiles of a request's `group` rows; parts of the own keys, of all
-                                  // requests together: about `oitems`, of at least `least` tiles (0: one each)
-  float scale, softcap;  // scale > 0, with its sign (0 for 0) in `sign`, which the queries take on
-  float sign;
-};
 
 // One run of keys: the shared ones, or a sequence's own.
 struct Keys {
@@ -357,28 +227,6 @@ struct Row {
   float slope;     // slope * log2(e)
 };
 
-// Scores (products q.k) -> t = log2(e) * f(scale * s) - slope * distance, for keys pos0 + {0 .. } of a
-// block whose lane half h holds keys 8 (r / 4) + 4 h + r % 4 in register r.
-struct Scoring {
-  float c;         // scale * log2(e)
-  float cap;       // softcap * log2(e)
-  float inv, inv2; // scale / softcap, and that times 2 log2(e)
-  bool capped, fine, biased;  // fine: the cap needs tanh's relative precision near 0 (below)
-};
-
-__device__ inline Scoring scoring(const Params& p) {
-  Scoring s;
-  s.c = p.scale * kLog2e;
-  s.capped = p.softcap != 0.f && p.softcap < kNoCap;
-  s.fine = p.softcap > kPlainCap;
-  s.biased = p.slopes != nullptr;
-  s.cap = p.softcap * kLog2e;
-  // (held to where no score's product with it is 0 times infinity; past that every score is at a cap of nearly 0)
-  s.inv = s.capped ? fminf(p.scale / p.softcap, 1e37f) : 0.f;
-  s.inv2 = s.inv * (2.f * kLog2e);
-  return s;
-}
-
 // What a workgroup needs to know besides its rows and keys.
 struct What {
   Scoring sc;
@@ -386,22 +234,6 @@ struct What {
   int d, causal;
 };
 __device__ inline What what_of(const Params& p) { return What{scoring(p), p.sign, p.d, p.causal}; }
-
-// tanh to fp32's last bits near 0, where a cap leaves most scores (an odd polynomial fitted by least
-// squares to (tanh(y) / y - 1) / y^2 on [0, 0.625], largest relative error 4e-9), and 1 - 2 / (e^2y + 1)
-// past it. With fp16 inputs and a cap up to kPlainCap the second form's absolute error, 1e-7 of the cap, is
-// enough throughout.
-__device__ inline float tanh_of(float y) {
-  const float e = __builtin_amdgcn_exp2f(y * (2.f * kLog2e));
-  const float big = 1.f - 2.f * __builtin_amdgcn_rcpf(e + 1.f);
-  const float u = y * y;
-  float r = fmaf(u, -0.00571705f, 0.02065059f);
-  r = fmaf(u, r, -0.0537435f);
-  r = fmaf(u, r, 0.13331491f);
-  r = fmaf(u, r, -0.33333284f);
-  r = fmaf(y * u, r, y);
-  return fabsf(y) < 0.625f ? r : big;
-}
 
 __device__ inline float score_of(const Scoring& s, float x, float slope, float distance) {
   const float t = s.capped ? s.cap * tanh_of(x * s.inv) : x * s.c;
@@ -676,37 +508,6 @@ struct Wave {
     }
   }
 };
-
-// Where a tile's rows go: the output, or a slot of the workspace with rows x DP sums, then the rows'
-// reference maxima and sums of weights (and a gap, so that every slot starts on 16 bytes).
-__host__ __device__ constexpr size_t slot_floats(int rows, int dp) { return static_cast<size_t>(rows) * (dp + 4); }
-struct Slot {
-  float* at;  // NULL: the output
-  int rows;
-};
-template <int DP>
-__device__ inline float* slot_m(const Slot& s) { return s.at + static_cast<size_t>(s.rows) * DP; }
-
-template <typename T, int N>
-__device__ inline void store_out(char* out, int d0, const float (&v)[N]) {
-  if constexpr (sizeof(T) == 2) {
-    if constexpr (N == 4) {
-      const half4 h = {static_cast<_Float16>(v[0]), static_cast<_Float16>(v[1]), static_cast<_Float16>(v[2]), static_cast<_Float16>(v[3])};
-      *reinterpret_cast<half4*>(out + d0 * 2) = h;
-    } else {
-      half8 h;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) h[i] = static_cast<_Float16>(v[i]);
-      *reinterpret_cast<half8*>(out + d0 * 2) = h;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; i += 4) *reinterpret_cast<float4v*>(out + (d0 + i) * 4) = float4v{v[i], v[i + 1], v[i + 2], v[i + 3]};
-  }
-}
-
-// 1 / l, with 0 for a row that saw no key (a NaN stays one)
-__device__ inline float inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
 
 // The rows of wavefront `wave` of a workgroup of 128 to their places.
 template <typename T, int DP, int DU>
@@ -1318,55 +1119,6 @@ __global__ __launch_bounds__(kThreads) void prompt_join_kernel(Params p, int rt)
 // requests at once. Then the requests' own keys, 32 rows a tile, in parts of about equal length over all
 // requests: the device knows their lengths, so every wavefront adds them up and finds its part (see Part).
 // Slots in the same order. A request's only part writes the output itself.
-__host__ __device__ inline int own_rows(int group) { return group < kKeyTile ? group : kKeyTile; }
-
-struct Part {
-  int seq, len, split, splits;  // the request and its length; which of its parts this is, and of how many
-  int first;                    // number of the request's first part
-};
-__device__ inline int length_of(const Params& p, int b) { return min(max(p.lengths[b], 0), p.k_len); }
-
-// Tiles of 32 keys a part gets: the requests' tiles over the parts that there should be.
-__device__ inline int part_tiles(const Params& p) {
-  const int lane = threadIdx.x & 63;
-  int64_t total = 0;
-  for (int b = lane; b < p.seqs; b += kWave) total += ceil_div(length_of(p, b), 32);
-#pragma unroll
-  for (int i = 1; i < kWave; i *= 2) total += __shfl_xor(static_cast<long long>(total), i);
-  return max(p.least, uniform(static_cast<int>((total + p.oitems - 1) / p.oitems)));
-}
-// Part `item` of all (by_item), or the first part of request `item`. false: past the last one.
-__device__ inline bool find_part(const Params& p, int item, bool by_item, Part& r) {
-  if (p.least == 0) {
-    r = Part{item, item < p.seqs ? uniform(length_of(p, item)) : 0, 0, 1, item};
-    return item < p.seqs;
-  }
-  const int lane = threadIdx.x & 63, chunk = part_tiles(p);
-  int before = 0;
-  for (int b0 = 0; b0 < p.seqs; b0 += kWave) {
-    const int b = b0 + lane, len = b < p.seqs ? length_of(p, b) : 0;
-    const int n = b < p.seqs ? max(1, ceil_div(ceil_div(len, 32), chunk)) : 0;
-    int upto = n;
-#pragma unroll
-    for (int i = 1; i < kWave; i *= 2) {
-      const int x = __shfl_up(upto, i);
-      if (lane >= i) upto += x;
-    }
-    const uint64_t hit = __ballot(by_item ? item < before + upto : b == item);
-    if (hit != 0) {
-      const int l = __builtin_ctzll(hit);
-      r.seq = b0 + l;
-      r.len = __builtin_amdgcn_readlane(len, l);
-      r.splits = __builtin_amdgcn_readlane(n, l);
-      r.first = before + __builtin_amdgcn_readlane(upto, l) - r.splits;
-      r.split = by_item ? item - r.first : 0;
-      return true;
-    }
-    before += __builtin_amdgcn_readlane(upto, kWave - 1);
-  }
-  return false;
-}
-
 template <typename T, int DP, bool SKEYS>
 __global__ __launch_bounds__(kThreads, 2) void decode_kernel(Params p) {
   constexpr int SRT = SKEYS ? kKeyTile : kRowTile, SBN = SKEYS ? 32 : (sizeof(T) == 2 ? 64 : 32);
@@ -1457,8 +1209,6 @@ __global__ __launch_bounds__(kThreads) void decode_join_kernel(Params p, int srt
                     m = slot + static_cast<size_t>(rows) * DP + r;
                   });
 }
-
-#include "attention8.hpp"
 
 // ---- host ------------------------------------------------------------------------------------------------
 
@@ -1724,11 +1474,6 @@ int check8(const g16_attention8_args& e) {
   return e.a.k_len > 0 && (e.k_scale == nullptr || e.v_scale == nullptr) ? G16_E_NULL : G16_OK;
 }
 
-template <typename T, int DP, int CODE, int NR>
-int run_own8(const Params& p, const Params8& e, dim3 grid, hipStream_t stream) {
-  return p.d == DP ? launch(decode8_kernel<T, DP, CODE, NR, true>, grid, dim3(kThreads), stream, p, e)
-                   : launch(decode8_kernel<T, DP, CODE, NR, false>, grid, dim3(kThreads), stream, p, e);
-}
 template <typename T, int DP>
 int run_decode8(const Params& p, Params8 e, int code, const DecodePlan& plan, hipStream_t stream) {
   const int srt = plan.skeys ? kKeyTile : kRowTile;
@@ -1738,11 +1483,8 @@ int run_decode8(const Params& p, Params8 e, int code, const DecodePlan& plan, hi
   if (nshared > 0)
     rc = plan.skeys ? launch(decode_kernel<T, DP, true>, dim3(nshared), dim3(kThreads), stream, p)
                     : launch(decode_kernel<T, DP, false>, dim3(nshared), dim3(kThreads), stream, p);
-  const dim3 grid(static_cast<unsigned>(plan.own) * p.hkv);
-  if (rc == 0) {
-    if (code == G16_CODE_INT8) rc = p.group <= 16 ? run_own8<T, DP, G16_CODE_INT8, 1>(p, e, grid, stream) : run_own8<T, DP, G16_CODE_INT8, 2>(p, e, grid, stream);
-    else rc = p.group <= 16 ? run_own8<T, DP, G16_CODE_E4M3, 1>(p, e, grid, stream) : run_own8<T, DP, G16_CODE_E4M3, 2>(p, e, grid, stream);
-  }
+  e.parts = static_cast<int>(plan.own / plan.otiles);
+  if (rc == 0) rc = run_own8(p, e, code, sizeof(T) == 4, stream);
   if (rc == 0 && plan.join)
     rc = launch(decode_join_kernel<T, DP>, dim3(static_cast<unsigned>((static_cast<int64_t>(p.seqs) * p.hq + 3) / 4)), dim3(kThreads), stream, p, srt);
   return rc;
@@ -1843,7 +1585,8 @@ extern "C" int g16_attention_decode8(const g16_attention8_args* args, void* stre
   p.k_head = a.k_head;
   p.v_seq = a.v_seq;
   p.v_head = a.v_head;
-  const Params8 own = {e.k_scale, e.v_scale, e.ks_seq, e.ks_head, e.ks_token, e.vs_seq, e.vs_head, e.vs_token, a.k_token, a.v_token, 0};
+  const Params8 own = {e.k_scale, e.v_scale, e.ks_seq, e.ks_head, e.ks_token, e.vs_seq, e.vs_head, e.vs_token, a.k_token, a.v_token,
+                       divide_by(a.page > 0 ? static_cast<uint32_t>(a.page) : 1u), 0, 0};
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (a.is_f32) return a.d <= 64 ? run_decode8<float, 64>(p, own, e.code, plan, s) : run_decode8<float, 128>(p, own, e.code, plan, s);
   return a.d <= 64 ? run_decode8<_Float16, 64>(p, own, e.code, plan, s) : run_decode8<_Float16, 128>(p, own, e.code, plan, s);
