@@ -1027,69 +1027,6 @@ __global__ __launch_bounds__(kThreads, DP == 64 && (!KEYS || sizeof(T) == 2) ? 3
   }
 }
 
-// One row from its partial sums: `of(i)` gives part i's sums, reference maximum and, `rows` floats behind it,
-// sum of weights. A wavefront a row: a lane holds 4 values of every kP-th part, whose weight the lane of
-// that number has. The sums' loads do not wait for the weights.
-template <typename T, int DP, typename F>
-__device__ inline void join_row(char* out, int d, int parts, const F& of) {
-  constexpr int L = DP / 4, kP = kWave / L, kB = 8;  // lanes of a part, parts at a time, loads at a time
-  const int lane = threadIdx.x & 63, d0 = (lane % L) * 4, mine = lane / L;
-  const float *s, *m;
-  int rows;
-  float top = -__builtin_huge_valf(), first_m = top, first_l = 0.f;
-  if (lane < parts) {
-    of(lane, s, m, rows);
-    first_m = *m;
-    first_l = m[rows];
-  }
-  float4v v[kB];
-  auto load = [&](int b) {
-#pragma unroll
-    for (int i = 0; i < kB; ++i) {
-      of(min(b + i * kP + mine, parts - 1), s, m, rows);
-      v[i] = *reinterpret_cast<const float4v*>(s + d0);
-    }
-  };
-  load(0);
-  top = first_m;
-  for (int i = lane + kWave; i < parts; i += kWave) {
-    of(i, s, m, rows);
-    top = fmaxf(top, *m);
-  }
-#pragma unroll
-  for (int i = 1; i < kWave; i *= 2) top = fmaxf(top, __shfl_xor(top, i));
-  float l = 0.f, f = 0.f;  // f: the weight of part (64 n + lane)
-  float4v o = {};
-  for (int b = 0; b < parts; b += kB * kP) {
-    if (b % kWave == 0) {
-      float pm = first_m, pl = first_l;
-      if (b > 0 && b + lane < parts) {
-        of(b + lane, s, m, rows);
-        pm = *m;
-        pl = m[rows];
-      }
-      f = b + lane >= parts ? 0.f : (pm == top ? 1.f : __builtin_amdgcn_exp2f(pm - top));
-      l = fmaf(f, b + lane < parts ? pl : 0.f, l);
-    }
-    if (b > 0) load(b);
-#pragma unroll
-    for (int i = 0; i < kB; ++i) {
-      const int part = b + i * kP + mine;
-      const float fi = __shfl(f, part & (kWave - 1));
-      if (part < parts) o += fi * v[i];
-    }
-  }
-#pragma unroll
-  for (int i = 1; i < kWave; i *= 2) l += __shfl_xor(l, i);
-#pragma unroll
-  for (int i = L; i < kWave; i *= 2)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], i);
-  const float inv = inverse(l);
-  const float r[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
-  if (lane < L && d0 < d) store_out<T, 4>(out, d0, r);
-}
-
 constexpr int kJoinRows = 8;  // rows of a workgroup of the joining kernels: two a wavefront
 
 template <typename T, int DP>
@@ -1474,20 +1411,35 @@ int check8(const g16_attention8_args& e) {
   return e.a.k_len > 0 && (e.k_scale == nullptr || e.v_scale == nullptr) ? G16_E_NULL : G16_OK;
 }
 
+// The own keys' part of the plan for a cache in 8 bits (see attention8.hip), and what the workspace has to hold.
+struct Plan8 {
+  DecodePlan shared;
+  int shares;
+  bool split;
+  size_t first, bytes;  // floats of the shared keys' slots; bytes in all
+};
+Plan8 plan_decode8(const g16_attention_args& a) {
+  Plan8 r = {};
+  r.shared = plan_decode(a);
+  const int group = a.hq / a.hkv, dp = a.d <= 64 ? 64 : 128, srt = r.shared.skeys ? kKeyTile : kRowTile;
+  const int64_t heads = static_cast<int64_t>(r.shared.otiles) * a.hkv;
+  r.split = a.k_len > kWhole8 * kTile8;
+  r.shares = a.seqs;
+  if (r.split) {
+    // as many as run at once, the same number for every XCD
+    const int64_t each = static_cast<int64_t>(cus_of(a)) / kXcds * waves_of8(a.is_f32 != 0, dp, rows_of8(group), a.d == dp) / heads;
+    r.shares = static_cast<int>(each < 1 ? kXcds : each * kXcds);
+  }
+  r.first = static_cast<size_t>(r.shared.stiles) * r.shared.ssplits * a.hkv * slot_floats(srt, dp);
+  if (r.shared.stiles > 0 || r.split)
+    r.bytes = (r.first + (static_cast<size_t>(r.shares) + (r.split ? a.seqs : 0)) * heads * slot_floats(own_rows(group), dp)) * sizeof(float);
+  return r;
+}
+
 template <typename T, int DP>
-int run_decode8(const Params& p, Params8 e, int code, const DecodePlan& plan, hipStream_t stream) {
-  const int srt = plan.skeys ? kKeyTile : kRowTile;
-  const unsigned nshared = static_cast<unsigned>(p.stiles) * p.ssplits * p.hkv;
-  e.first = nshared * slot_floats(srt, DP);
-  int rc = 0;
-  if (nshared > 0)
-    rc = plan.skeys ? launch(decode_kernel<T, DP, true>, dim3(nshared), dim3(kThreads), stream, p)
-                    : launch(decode_kernel<T, DP, false>, dim3(nshared), dim3(kThreads), stream, p);
-  e.parts = static_cast<int>(plan.own / plan.otiles);
-  if (rc == 0) rc = run_own8(p, e, code, sizeof(T) == 4, stream);
-  if (rc == 0 && plan.join)
-    rc = launch(decode_join_kernel<T, DP>, dim3(static_cast<unsigned>((static_cast<int64_t>(p.seqs) * p.hq + 3) / 4)), dim3(kThreads), stream, p, srt);
-  return rc;
+int run_shared8(const Params& p, bool skeys, hipStream_t stream) {
+  const dim3 grid(static_cast<unsigned>(p.stiles) * p.ssplits * p.hkv);
+  return skeys ? launch(decode_kernel<T, DP, true>, grid, dim3(kThreads), stream, p) : launch(decode_kernel<T, DP, false>, grid, dim3(kThreads), stream, p);
 }
 
 }  // namespace
@@ -1534,33 +1486,24 @@ extern "C" size_t g16_attention_decode_workspace_bytes(const g16_attention_args*
   return plan_decode(*args).bytes;
 }
 
-// The plan of a call with checked arguments, and its parameters
-static int begin_decode(const g16_attention_args& a, DecodePlan& plan, Params& p) {
-  plan = plan_decode(a);
+extern "C" int g16_attention_decode(const g16_attention_args* args, void* stream) {
+  if (args == nullptr) return G16_E_NULL;
+  const g16_attention_args& a = *args;
+  const int st = check(a, true);
+  if (st != G16_OK || a.seqs == 0 || a.hq == 0) return st;
+  const DecodePlan plan = plan_decode(a);
   if (plan.bytes > 0 && (a.workspace == nullptr || static_cast<size_t>(a.workspace_bytes) < plan.bytes)) return G16_E_WORKSPACE;
   if (!aligned16(a.workspace)) return G16_E_ALIGN;
   if (!fits_grid((static_cast<int64_t>(plan.stiles) * plan.ssplits + plan.own) * a.hkv) ||
       !fits_grid((static_cast<int64_t>(a.seqs) * a.hq + 3) / 4))
     return G16_E_SHAPE;
-  p = params(a);
+  Params p = params(a);
   p.causal = 0;
   p.stiles = plan.stiles;
   p.ssplits = plan.ssplits;
   p.otiles = plan.otiles;
   p.oitems = plan.oitems;
   p.least = plan.least;
-  return G16_OK;
-}
-
-extern "C" int g16_attention_decode(const g16_attention_args* args, void* stream) {
-  if (args == nullptr) return G16_E_NULL;
-  const g16_attention_args& a = *args;
-  int st = check(a, true);
-  if (st != G16_OK || a.seqs == 0 || a.hq == 0) return st;
-  DecodePlan plan;
-  Params p;
-  st = begin_decode(a, plan, p);
-  if (st != G16_OK) return st;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (a.is_f32) return a.d <= 64 ? run_decode<float, 64>(p, plan, s) : run_decode<float, 128>(p, plan, s);
   return a.d <= 64 ? run_decode<_Float16, 64>(p, plan, s) : run_decode<_Float16, 128>(p, plan, s);
@@ -1568,26 +1511,38 @@ extern "C" int g16_attention_decode(const g16_attention_args* args, void* stream
 
 extern "C" size_t g16_attention_decode8_workspace_bytes(const g16_attention8_args* args) {
   if (args == nullptr || check8(*args) != G16_OK || args->a.seqs == 0 || args->a.hq == 0) return 0;
-  return plan_decode(args->a).bytes;
+  return plan_decode8(args->a).bytes;
 }
 
 extern "C" int g16_attention_decode8(const g16_attention8_args* args, void* stream) {
   if (args == nullptr) return G16_E_NULL;
   const g16_attention8_args& e = *args;
   const g16_attention_args& a = e.a;
-  int st = check8(e);
+  const int st = check8(e);
   if (st != G16_OK || a.seqs == 0 || a.hq == 0) return st;
-  DecodePlan plan;
-  Params p;
-  st = begin_decode(a, plan, p);
-  if (st != G16_OK) return st;
+  if (static_cast<int64_t>(a.seqs) * (a.k_len / kTile8 + 1) > (1LL << 31) - 1) return G16_E_SHAPE;  // (tiles are counted in 32 bits)
+  const Plan8 plan = plan_decode8(a);
+  if (plan.bytes > 0 && (a.workspace == nullptr || static_cast<size_t>(a.workspace_bytes) < plan.bytes)) return G16_E_WORKSPACE;
+  if (!aligned16(a.workspace)) return G16_E_ALIGN;
+  if (!fits_grid(static_cast<int64_t>(plan.shared.stiles) * plan.shared.ssplits * a.hkv) ||
+      !fits_grid((static_cast<int64_t>(plan.shares) + kXcds) * plan.shared.otiles * a.hkv) || !fits_grid((static_cast<int64_t>(a.seqs) * a.hq + 3) / 4))
+    return G16_E_SHAPE;
+  Params p = params(a);
+  p.causal = 0;
+  p.stiles = plan.shared.stiles;
+  p.ssplits = plan.shared.ssplits;
+  p.otiles = plan.shared.otiles;
   p.k_seq = a.k_seq;
   p.k_head = a.k_head;
   p.v_seq = a.v_seq;
   p.v_head = a.v_head;
   const Params8 own = {e.k_scale, e.v_scale, e.ks_seq, e.ks_head, e.ks_token, e.vs_seq, e.vs_head, e.vs_token, a.k_token, a.v_token,
-                       divide_by(a.page > 0 ? static_cast<uint32_t>(a.page) : 1u), 0, 0};
+                       divide_by(a.page > 0 ? static_cast<uint32_t>(a.page) : 1u), plan.shares, plan.split, plan.shared.skeys ? kKeyTile : kRowTile, plan.first};
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (a.is_f32) return a.d <= 64 ? run_decode8<float, 64>(p, own, e.code, plan, s) : run_decode8<float, 128>(p, own, e.code, plan, s);
-  return a.d <= 64 ? run_decode8<_Float16, 64>(p, own, e.code, plan, s) : run_decode8<_Float16, 128>(p, own, e.code, plan, s);
+  int rc = 0;
+  if (p.stiles > 0) {
+    if (a.is_f32) rc = a.d <= 64 ? run_shared8<float, 64>(p, plan.shared.skeys, s) : run_shared8<float, 128>(p, plan.shared.skeys, s);
+    else rc = a.d <= 64 ? run_shared8<_Float16, 64>(p, plan.shared.skeys, s) : run_shared8<_Float16, 128>(p, plan.shared.skeys, s);
+  }
+  return rc == 0 ? run_own8(p, own, e.code, a.is_f32 != 0, s) : rc;
 }

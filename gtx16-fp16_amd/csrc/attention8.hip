@@ -1,10 +1,11 @@
 // Single tokens over a cache of 8 bits (g16_attention_decode8; its formulas stand in g16.h): the products of the requests' own
 // keys. A shared prefix is not in 8 bits and decode_kernel's, the joins are decode_join_kernel's (attention.hip).
 //
-// A workgroup has the query rows of one key head and a part of one request's keys; each of its four wavefronts takes
-// tiles of 64 keys of its own, straight from memory into registers:
-//   * S = Q K^T in 16x16x32 blocks of 16 keys: lane l's key is l % 16, and its values come in 16-byte loads, 64 bytes of a key
-//     an instruction: a step's values are bytes 8 of such a piece, in another order than in memory, the queries' too.
+// All requests' keys, in tiles of 64 one request after another, are dealt in shares of equal length, as many as run on the card at
+// once: whatever the lengths, all workgroups end together (see Deal for few keys). A workgroup has the query rows of one key head and a
+// share's tiles, a request's after another's; its four wavefronts take a tile in turn, straight from memory into registers:
+//   * S = Q K^T in 16x16x32 blocks of 16 keys, lane l's key l % 16, by way of LDS. A step's values of a lane are half of a 16-byte
+//     piece, in another order than in memory, the queries' too.
 //   * With few query rows the blocks' 16 rows are as many copies of them, and the lanes of row group l / 16 keep those of
 //     another block of keys: up to four rows, lane l has the scores of key l of the tile, and a row's 64 weights are one
 //     register; up to eight, two blocks share a register set. What a score costs (an exponential, the parts of its
@@ -111,8 +112,125 @@ __device__ inline void wave_order() {
   __builtin_amdgcn_wave_barrier();
 }
 
-constexpr int kTile8 = 64;
 constexpr int kRun8 = kTile8 + 8;  // weights of a row in LDS: rows on different banks
+
+// ---- shares ----------------------------------------------------------------------------------------------
+// A request without keys has one tile, too: somebody has to write its zeros. (The host sees to it that 32 bits hold all tiles.)
+__device__ inline int tiles_of(int len) { return max(1, ceil_div(len, kTile8)); }
+
+// A run of 64 requests in a wavefront: lane i has the length of request b0 + i and how many of what is counted (tiles, or pieces
+// of `chunk` tiles) there are up to and with its own.
+struct Run64 {
+  int len, count, upto;
+  __device__ Run64(const Params& p, int b0, int chunk = 1) {
+    const int lane = threadIdx.x & 63;
+    len = b0 + lane < p.seqs ? length_of(p, b0 + lane) : 0;
+    set(b0 + lane < p.seqs, chunk);
+  }
+  __device__ void set(bool some, int chunk) {
+    const int lane = threadIdx.x & 63;
+    count = some ? tiles_of(len) : 0;
+    if (chunk > 1) count = static_cast<int>(static_cast<uint32_t>(count + chunk - 1) / static_cast<uint32_t>(chunk));
+    upto = count;
+#pragma unroll
+    for (int i = 1; i < kWave; i *= 2) {
+      const int x = __shfl_up(upto, i);
+      if (lane >= i) upto += x;
+    }
+  }
+  __device__ int all() const { return __builtin_amdgcn_readlane(upto, kWave - 1); }
+};
+__device__ inline int all_tiles(const Params& p, const Run64& head) {
+  int total = head.all();
+  for (int b0 = kWave; b0 < p.seqs; b0 += kWave) total += Run64(p, b0).all();
+  return total;
+}
+
+// How all requests' tiles are dealt. Long ones in shares of equal length, whatever the requests: the first `more` shares
+// have each + 1, the others each. Where a share would have few tiles, its time is that of the waits for one after another, not of its bytes,
+// and a second request's would come on top: every request then has its own pieces, of `chunk` tiles, one for each
+// wavefront or two (16 requests of up to 1500 after 2048, 8 heads of 128: PIECES).
+struct Deal {
+  int shares, each, more, chunk;
+  __device__ Deal(const Params& p, const Params8& e, int total) {
+    const int four = static_cast<int>((static_cast<uint32_t>(total) + 2u * p.seqs) / (4u * e.shares)) + 1;
+    chunk = four <= 2 ? 4 * four : 0;
+    shares = e.shares;
+    each = static_cast<int>(static_cast<uint32_t>(total) / static_cast<uint32_t>(shares));
+    more = total - each * shares;
+  }
+  __device__ int begin(int share) const { return each * share + min(more, share); }
+  __device__ int share_of(int tile) const {
+    const int ahead = more * (each + 1);
+    return tile < ahead ? static_cast<int>(static_cast<uint32_t>(tile) / static_cast<uint32_t>(each + 1))
+                        : more + static_cast<int>(static_cast<uint32_t>(tile - ahead) / static_cast<uint32_t>(each));
+  }
+};
+
+// What a workgroup has: `tiles` tiles from one of request `seq` on, over the requests behind it as well; then, of pieces, the one
+// `shares` further on.
+struct Share {
+  int seq, len, tile, tiles, slot;  // the first request, its length, the first tile of it; the first slot
+  bool pieces;
+};
+// Piece number `piece` (a share is one).
+__device__ inline bool find_share(const Params& p, const Params8& e, int piece, Share& r) {
+  r.pieces = false;
+  if (!e.split) {
+    if (piece >= p.seqs) return false;
+    r.seq = r.slot = piece;
+    r.len = uniform(length_of(p, piece));
+    r.tile = 0;
+    r.tiles = tiles_of(r.len);
+    return true;
+  }
+  Run64 head(p, 0);
+  const Deal deal(p, e, all_tiles(p, head));
+  r.pieces = deal.chunk > 0;
+  const int from = r.pieces ? piece : deal.begin(piece);
+  if (!r.pieces) r.tiles = deal.begin(piece + 1) - from;
+  if (r.pieces ? false : piece >= deal.shares || r.tiles == 0) return false;
+  if (r.pieces) head.set(static_cast<int>(threadIdx.x & 63) < p.seqs, deal.chunk);
+  int before = 0;
+  for (int b0 = 0; b0 < p.seqs; b0 += kWave) {
+    const Run64 run = b0 == 0 ? head : Run64(p, b0, r.pieces ? deal.chunk : 1);
+    const uint64_t hit = __ballot(from < before + run.upto);
+    if (hit != 0) {
+      const int at = __builtin_ctzll(hit), behind = from - before - __builtin_amdgcn_readlane(run.upto - run.count, at);
+      r.seq = b0 + at;
+      r.len = __builtin_amdgcn_readlane(run.len, at);
+      r.tile = r.pieces ? behind * deal.chunk : behind;
+      if (r.pieces) r.tiles = min(deal.chunk, tiles_of(r.len) - r.tile);
+      r.slot = r.pieces ? piece : piece + r.seq;
+      return true;
+    }
+    before += run.all();
+  }
+  return false;
+}
+// The slots of request b.
+__device__ inline void find_request(const Params& p, const Params8& e, int b, int& first, int& parts) {
+  first = b;
+  parts = 1;
+  if (!e.split) return;
+  const Run64 head(p, 0);
+  const Deal deal(p, e, all_tiles(p, head));
+  int before = 0;
+  for (int b0 = 0;; b0 += kWave) {
+    const Run64 run(p, b0, deal.chunk > 0 ? deal.chunk : 1);
+    if (b < b0 + kWave) {
+      parts = __builtin_amdgcn_readlane(run.count, b - b0);
+      first = before + __builtin_amdgcn_readlane(run.upto, b - b0) - parts;
+      break;
+    }
+    before += run.all();
+  }
+  if (deal.chunk == 0) {
+    const int tile = first, last = first + parts - 1;
+    first = deal.share_of(tile) + b;
+    parts = deal.share_of(last) + b - first + 1;
+  }
+}
 
 // RQ: query rows that there is room for, 1, 4, 8, 16 or 32. FULL: heads of DP values.
 template <typename T, int DP, int RQ>
@@ -123,39 +241,39 @@ struct Shape8 {
   static constexpr int NS = QP / 4;             // register sets of scores a block of rows has
   static constexpr int RI = RQ < 4 ? RQ : 4;    // registers of a set in use
   static constexpr int PARTS = sizeof(T) == 4 ? 3 : 2;
-  // wavefronts a SIMD that the registers are held to
-  static constexpr int WAVES = NR == 2 ? (DP == 64 ? 2 : 1) : sizeof(T) == 4 ? 2 : DP == 64 ? (QP == 4 ? 4 : 3) : 2;
 };
 
 template <typename T, int DP, int CODE, int RQ, bool FULL>
-__global__ __launch_bounds__(kThreads, (Shape8<T, DP, RQ>::WAVES)) void decode8_kernel(Params p, Params8 e) {
+__global__ __launch_bounds__(kThreads, waves_of8(sizeof(T) == 4, DP, RQ, FULL)) void decode8_kernel(Params p, Params8 e) {
   using S = Shape8<T, DP, RQ>;
-  constexpr int VB = DP / 16, KW = DP / 16, VW = DP / 64;  // values of a lane (and blocks of the second product); dwords of a key's, a value's piece
+  constexpr int VB = DP / 16, VW = DP / 64;  // values of a lane (and blocks of the second product), in dwords
   constexpr int R = S::R, NR = S::NR, NS = S::NS, RI = S::RI, PARTS = S::PARTS;
-  constexpr int kWeights = 4 * PARTS * R * kRun8 * 2, kSums = 4 * R * DP * 4;
-  __shared__ __attribute__((aligned(16))) char lds[kWeights > kSums ? kWeights : kSums];
+  constexpr int kKeys = kTile8 * DP, kWeights = PARTS * R * kRun8 * 2, kSums = R * DP * 4;  // bytes of a wavefront
+  __shared__ __attribute__((aligned(16))) char lds[4 * (kKeys + kWeights > kSums ? kKeys + kWeights : kSums)];
   __shared__ __attribute__((aligned(16))) uint64_t places[4][2][kTile8];
   __shared__ float joint[2][4][R];
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), col = lane & 15, g = lane >> 4;
-  // Workgroups go to the XCDs in turn, and every XCD has an L2 of its own. The heads of a part share cache lines (of codes
-  // where a head's are less than a line, of scales always), so they are all given to one XCD where there are parts for all
+  // Workgroups go to the XCDs in turn, and every XCD has an L2 of its own. The heads of a share read the same cache lines (of
+  // codes where a head's are less than a line, of scales always), so they are all given to one XCD where there are shares for all
   // (96 requests of up to 2048, 12 heads of 64: 76 us, so 63).
   int lin = blockIdx.x;
-  if (e.parts >= kXcds) {
-    const int per = p.otiles * p.hkv, i = lin / kXcds, part = i / per * kXcds + lin % kXcds;
-    if (part >= e.parts) return;
-    lin = part * per + i % per;
+  if (e.shares >= kXcds) {
+    const int per = p.otiles * p.hkv, i = lin / kXcds, share = i / per * kXcds + lin % kXcds;
+    if (share >= e.shares) return;
+    lin = share * per + i % per;
   }
-  const int own = lin;
   const int kv = lin % p.hkv;
   lin /= p.hkv;
-  const int rt = lin % p.otiles;
-  Part part;
-  if (!find_part(p, lin / p.otiles, true, part)) return;
-  const int b = part.seq, len = part.len, orows = own_rows(p.group);
+  const int rt = lin % p.otiles, share = lin / p.otiles;
+  Share has;
+  if (!find_share(p, e, share, has)) return;
+  const int orows = own_rows(p.group);
   const Scoring sc = scoring(p);
-  const int n = ceil_div(len, 32);
-  const int begin = 32 * share_begin(n, part.split, part.splits), end = min(len, 32 * share_begin(n, part.split + 1, part.splits));
+  int b = has.seq, len = has.len, u0 = has.tile, todo = has.tiles, at_slot = has.slot;  // request, its first tile here, tiles to do
+
+  for (int piece = share;;) {
+  const int tiles = tiles_of(len), u1 = min(u0 + todo, tiles);
+  const int begin = kTile8 * u0, end = min(len, kTile8 * u1);
 
   // ---- places of a tile's rows, this lane's key ----
   const int32_t* table = p.pages == nullptr ? nullptr : p.pages + static_cast<size_t>(b) * p.max_pages;
@@ -183,29 +301,30 @@ __global__ __launch_bounds__(kThreads, (Shape8<T, DP, RQ>::WAVES)) void decode8_
     vs = pg < 0 ? 0.f : vsbase[pg * e.vs_seq + at * e.vs_tok];
     wave_order();
   };
-  uint32_t k[4][KW], v[2][8][VW];
-  // Bytes 64 c + 16 g .. of a key, and what is to be done with them where a row ends inside: rows end at a multiple of 8, and
-  // nothing behind them is read.
+  // A key is CH pieces of 16 bytes. A load takes whole keys, in the order in which they lie in memory; LDS turns them
+  // into the product's order, where lane l has piece 4 c + l / 16 of key l % 16: pieces are at places that put those of 8 keys on
+  // different banks. (Loaded in that order, a lane's piece next to another key's, 40 requests of 8192 e4m3 keys of 8 heads of 128
+  // take KLOADS.)
+  constexpr int CH = DP / 16, PER = 64 / CH, NK = CH;  // pieces of a key; keys of a load; loads of a tile
+  auto place_of = [](int key, int piece) { return key * DP + ((piece ^ (CH == 8 ? key & 7 : (key >> 1) & 3)) << 4); };
+  char* keys = lds + wave * (kKeys + kWeights);
+  u32x4 k[NK];
+  uint32_t v[2][8][VW];
   auto load_k = [&]() {
     typedef uint32_t piece __attribute__((ext_vector_type(4), aligned(8)));
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      const uint64_t row = places[wave][0][16 * s + col];
+    for (int n = 0; n < NK; ++n) {
+      const uint64_t row = places[wave][0][n * PER + lane / CH];
+      const int at0 = lane % CH * 16;
+      if constexpr (FULL) {
+        k[n] = load_at<piece>(row + at0);
+      } else {  // (rows end at a multiple of 8, and nothing behind them is read)
 #pragma unroll
-      for (int c = 0; c < DP / 64; ++c) {
-        const int at0 = 64 * c + 16 * g;
-        if constexpr (FULL) {
-          const piece x = load_at<piece>(row + at0);
-#pragma unroll
-          for (int w = 0; w < 4; ++w) k[s][4 * c + w] = x[w];
-        } else {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const bool some = at0 + 8 * h < p.d;
-            const u32x2 x = load_at<u32x2>(row + (some ? at0 + 8 * h : 0));
-            k[s][4 * c + 2 * h] = some ? x[0] : 0;
-            k[s][4 * c + 2 * h + 1] = some ? x[1] : 0;
-          }
+        for (int h = 0; h < 2; ++h) {
+          const bool some = at0 + 8 * h < p.d;
+          const u32x2 x = load_at<u32x2>(row + (some ? at0 + 8 * h : 0));
+          k[n][2 * h] = some ? x[0] : 0;
+          k[n][2 * h + 1] = some ? x[1] : 0;
         }
       }
     }
@@ -279,30 +398,42 @@ __global__ __launch_bounds__(kThreads, (Shape8<T, DP, RQ>::WAVES)) void decode8_
     return x;
   };
 
-  __bf16* weights = reinterpret_cast<__bf16*>(lds) + wave * (PARTS * R * kRun8);
+  __bf16* weights = reinterpret_cast<__bf16*>(keys + kKeys);
   float* factors = joint[0][wave];
   for (; j0 < end; j0 += kStep) {
     // ---- scores ----
+#pragma unroll
+    for (int n = 0; n < NK; ++n) *reinterpret_cast<u32x4*>(keys + place_of(n * PER + lane / CH, lane % CH)) = k[n];
+    wave_order();
     float w[NR][NS][4];
+    float4v x[NR][4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+#pragma unroll
+      for (int r = 0; r < NR; ++r) x[r][s] = float4v{};
+#pragma unroll
+      for (int c = 0; c < DP / 64; ++c) {
+        const u32x4 piece = *reinterpret_cast<const u32x4*>(keys + place_of(16 * s + col, 4 * c + g));
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+          x[r][s] = q[r][2 * c].template times<CODE>(u32x2{piece[0], piece[1]}, x[r][s]);
+          x[r][s] = q[r][2 * c + 1].template times<CODE>(u32x2{piece[2], piece[3]}, x[r][s]);
+        }
+      }
+    }
+    wave_order();
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
-      float4v x[4];
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        x[s] = float4v{};
-#pragma unroll
-        for (int c = 0; c < DP / 32; ++c) x[s] = q[r][c].template times<CODE>(u32x2{k[s][2 * c], k[s][2 * c + 1]}, x[s]);
-      }
 #pragma unroll
       for (int i = 0; i < RI; ++i) {
         if constexpr (S::QP == 4) {
-          w[r][0][i] = g < 2 ? (g == 0 ? x[0][i] : x[1][i]) : (g == 2 ? x[2][i] : x[3][i]);
+          w[r][0][i] = g < 2 ? (g == 0 ? x[r][0][i] : x[r][1][i]) : (g == 2 ? x[r][2][i] : x[r][3][i]);
         } else if constexpr (S::QP == 8) {
-          w[r][0][i] = g < 2 ? x[0][i] : x[1][i];
-          w[r][1][i] = g < 2 ? x[2][i] : x[3][i];
+          w[r][0][i] = g < 2 ? x[r][0][i] : x[r][1][i];
+          w[r][1][i] = g < 2 ? x[r][2][i] : x[r][3][i];
         } else {
 #pragma unroll
-          for (int s = 0; s < 4; ++s) w[r][s][i] = x[s][i];
+          for (int s = 0; s < 4; ++s) w[r][s][i] = x[r][s][i];
         }
       }
     }
@@ -328,11 +459,9 @@ __global__ __launch_bounds__(kThreads, (Shape8<T, DP, RQ>::WAVES)) void decode8_
       for (int s = 0; s < NS; ++s) vscale[s] *= unit;
     }
     // ---- the next keys ----
-    const bool more = j0 + kStep < end;
-    if (more) {
-      find(j0 + kStep, next);
-      load_k();
-    }
+    // (behind the last tile the rows of zeros again: under a condition all of the registers would be copied)
+    find(j0 + kStep, next);
+    load_k();
     next = page_of(j0 + 2 * kStep);
     // ---- weights ----
     const int left = end - j0;
@@ -445,7 +574,7 @@ __global__ __launch_bounds__(kThreads, (Shape8<T, DP, RQ>::WAVES)) void decode8_
       }
     }
     wave_order();
-    if (more) load_v();
+    load_v();
   }
 
   // ---- join the four wavefronts: sums [wave][row][value] in LDS, then eight values a thread ----
@@ -471,7 +600,8 @@ __global__ __launch_bounds__(kThreads, (Shape8<T, DP, RQ>::WAVES)) void decode8_
   }
   __syncthreads();
   Slot slot = {nullptr, orows};
-  if (p.stiles > 0 || part.splits > 1) slot.at = p.part + e.first + static_cast<size_t>(own) * slot_floats(orows, DP);
+  if (p.stiles > 0 || u0 > 0 || u1 < tiles)
+    slot.at = p.part + e.first + ((static_cast<size_t>(at_slot) * p.otiles + rt) * p.hkv + kv) * slot_floats(orows, DP);
   for (int item = tid; item < R * (DP / 8); item += kThreads) {
     const int r = item / (DP / 8), d0 = item % (DP / 8) * 8, row = rt * kKeyTile + r;
     if (row >= p.group) break;
@@ -505,6 +635,82 @@ __global__ __launch_bounds__(kThreads, (Shape8<T, DP, RQ>::WAVES)) void decode8_
       store_out<T, 8>(p.out + (static_cast<int64_t>(b) * p.hq + kv * p.group + row) * p.d * static_cast<int>(sizeof(T)), d0, x);
     }
   }
+  todo -= u1 - u0;
+  if (todo > 0) {
+    len = uniform(length_of(p, ++b));
+    u0 = 0;
+    ++at_slot;
+  } else {
+    piece += e.shares;
+    if (!has.pieces || !find_share(p, e, piece, has)) break;
+    b = has.seq;
+    len = has.len;
+    u0 = has.tile;
+    todo = has.tiles;
+    at_slot = has.slot;
+  }
+  __syncthreads();  // (the sums in LDS have been read)
+  }
+}
+
+// A row's slots: of the shared keys, then of its request's pieces in shares one after another. W wavefronts have a row's slots
+// among them: four where there are few rows, whose time is that of the longest (64 slots of one of 32 rows of 128 values: JOINS).
+template <typename T, int DP, int W>
+__global__ __launch_bounds__(kThreads) void decode8_join_kernel(Params p, Params8 e) {
+  __shared__ __attribute__((aligned(16))) float sums[W == 1 ? 1 : 4][DP + 4];
+  const int wave = uniform(static_cast<int>(threadIdx.x >> 6));
+  const int row = W == 1 ? static_cast<int>(blockIdx.x) * 4 + wave : static_cast<int>(blockIdx.x);
+  if (row >= p.seqs * p.hq) return;
+  const int b = row / p.hq, head = row % p.hq, kv = head / p.group, g = head % p.group;
+  const int ns = p.stiles > 0 ? p.ssplits : 0, orows = own_rows(p.group), sr = b * p.group + g;
+  int first, parts;
+  find_request(p, e, b, first, parts);
+  parts += ns;
+  if (parts == 1) return;
+  auto slot_of = [&](int i, const float*& o, const float*& m, int& rows) {
+    const float* slot;
+    int r;
+    if (i < ns) {
+      slot = p.part + (static_cast<size_t>((sr / e.srt) * p.ssplits + i) * p.hkv + kv) * slot_floats(e.srt, DP);
+      r = sr % e.srt;
+      rows = e.srt;
+    } else {
+      const size_t at = (static_cast<size_t>(first) + (i - ns)) * p.otiles + g / kKeyTile;
+      slot = p.part + e.first + (at * p.hkv + kv) * slot_floats(orows, DP);
+      r = g % kKeyTile;
+      rows = orows;
+    }
+    o = slot + static_cast<size_t>(r) * DP;
+    m = slot + static_cast<size_t>(rows) * DP + r;
+  };
+  char* out = p.out + static_cast<int64_t>(row) * p.d * static_cast<int>(sizeof(T));
+  if constexpr (W == 1) {
+    join_row<T, DP>(out, p.d, parts, slot_of);
+  } else {
+    const int from = share_begin(parts, wave, 4), mine = share_begin(parts, wave + 1, 4) - from;
+    float top = -__builtin_huge_valf(), l = 0.f;
+    float4v o = {};
+    if (mine > 0) join_sums<DP>(mine, [&](int i, const float*& s, const float*& m, int& rows) { slot_of(from + i, s, m, rows); }, top, l, o);
+    const int lane = threadIdx.x & 63, d0 = lane % (DP / 4) * 4;
+    if (lane < DP / 4) *reinterpret_cast<float4v*>(&sums[wave][d0]) = o;
+    if (lane == 0) {
+      sums[wave][DP] = top;
+      sums[wave][DP + 1] = l;
+    }
+    __syncthreads();
+    if (wave != 0 || lane >= DP / 4 || d0 >= p.d) return;
+    top = fmaxf(fmaxf(sums[0][DP], sums[1][DP]), fmaxf(sums[2][DP], sums[3][DP]));
+    l = 0.f;
+    o = float4v{};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float f = sums[i][DP] == top ? 1.f : __builtin_amdgcn_exp2f(sums[i][DP] - top);
+      l = fmaf(f, sums[i][DP + 1], l);
+      o += f * *reinterpret_cast<const float4v*>(&sums[i][d0]);
+    }
+    const float inv = inverse(l), r[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+    store_out<T, 4>(out, d0, r);
+  }
 }
 
 template <typename T, int DP, int CODE, int RQ>
@@ -514,13 +720,22 @@ int run(const Params& p, const Params8& e, dim3 grid, hipStream_t stream) {
 }
 template <typename T, int DP, int CODE>
 int run(const Params& p, const Params8& e, hipStream_t stream) {
-  const unsigned parts = static_cast<unsigned>(e.parts >= kXcds ? ceil_div(e.parts, kXcds) * kXcds : e.parts);
-  const dim3 grid(parts * p.otiles * p.hkv);
-  return p.group == 1    ? run<T, DP, CODE, 1>(p, e, grid, stream)
-         : p.group <= 4  ? run<T, DP, CODE, 4>(p, e, grid, stream)
-         : p.group <= 8  ? run<T, DP, CODE, 8>(p, e, grid, stream)
-         : p.group <= 16 ? run<T, DP, CODE, 16>(p, e, grid, stream)
-                         : run<T, DP, CODE, 32>(p, e, grid, stream);
+  const unsigned shares = static_cast<unsigned>(e.shares >= kXcds ? ceil_div(e.shares, kXcds) * kXcds : e.shares);
+  const dim3 grid(shares * p.otiles * p.hkv);
+  int rc = 0;
+  switch (rows_of8(p.group)) {
+    case 1: rc = run<T, DP, CODE, 1>(p, e, grid, stream); break;
+    case 4: rc = run<T, DP, CODE, 4>(p, e, grid, stream); break;
+    case 8: rc = run<T, DP, CODE, 8>(p, e, grid, stream); break;
+    case 16: rc = run<T, DP, CODE, 16>(p, e, grid, stream); break;
+    default: rc = run<T, DP, CODE, 32>(p, e, grid, stream);
+  }
+  if (rc == 0 && (p.stiles > 0 || e.split)) {
+    const unsigned rows = static_cast<unsigned>(p.seqs) * p.hq;
+    rc = rows <= 512 ? launch(decode8_join_kernel<T, DP, 4>, dim3(rows), dim3(kThreads), stream, p, e)
+                     : launch(decode8_join_kernel<T, DP, 1>, dim3((rows + 3) / 4), dim3(kThreads), stream, p, e);
+  }
+  return rc;
 }
 template <typename T>
 int run(const Params& p, const Params8& e, int code, hipStream_t stream) {

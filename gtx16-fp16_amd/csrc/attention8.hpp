@@ -6,6 +6,8 @@
 namespace g16 {
 
 constexpr int kXcds = 8;
+constexpr int kTile8 = 64;  // keys of a tile
+constexpr int kWhole8 = 8;  // tiles of a request whose keys are never split
 
 // n / by without a division: (2 n magic >> 32) >> shift, for n below 2^31.
 struct Divide {
@@ -23,11 +25,21 @@ struct Params8 {
   int64_t ks_seq, ks_head, ks_tok, vs_seq, vs_head, vs_tok;  // elements
   int64_t k_tok, v_tok;                                      // bytes
   Divide page;
-  int parts;     // of all requests, at most
-  size_t first;  // floats of the shared keys' slots, before these parts'
+  int shares;    // at most
+  bool split;    // shares of equal length; else one for each request
+  int srt;       // rows of the shared keys' slots
+  size_t first;  // floats of the shared keys' slots, before the own keys'
 };
 
-// Enqueues the products of the requests' own keys.
+// Query rows that a workgroup has room for.
+constexpr int rows_of8(int group) { return group == 1 ? 1 : group <= 4 ? 4 : group <= 8 ? 8 : group <= 16 ? 16 : 32; }
+// Workgroups on a CU that the registers are held to.
+constexpr int waves_of8(bool f32, int dp, int rows, bool full) {
+  if (rows == 32) return dp == 64 ? 2 : 1;
+  return f32 || dp == 128 || rows == 16 ? 2 : rows == 1 && full ? 4 : 3;
+}
+
+// Enqueues the products of the requests' own keys and the joins.
 int run_own8(const Params& p, const Params8& e, int code, bool f32, hipStream_t stream);
 
 }  // namespace g16

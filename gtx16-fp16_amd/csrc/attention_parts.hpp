@@ -208,6 +208,78 @@ __device__ inline void store_out(char* out, int d0, const float (&v)[N]) {
 // 1 / l, with 0 for a row that saw no key (a NaN stays one)
 __device__ inline float inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
 
+// One row from its partial sums: `of(i)` gives part i's sums, reference maximum and, `rows` floats behind it,
+// sum of weights. A wavefront a row: a lane holds 4 values of every kP-th part, whose weight the lane of
+// that number has. The sums' loads do not wait for the weights.
+// (join_sums: the same without the division, o being values 4 (lane % (DP / 4)) ..)
+template <int DP, typename F>
+__device__ inline void join_sums(int parts, const F& of, float& top, float& l, float4v& o) {
+  constexpr int L = DP / 4, kP = kWave / L, kB = 8;  // lanes of a part, parts at a time, loads at a time
+  const int lane = threadIdx.x & 63, d0 = (lane % L) * 4, mine = lane / L;
+  const float *s, *m;
+  int rows;
+  float first_m = -__builtin_huge_valf(), first_l = 0.f;
+  if (lane < parts) {
+    of(lane, s, m, rows);
+    first_m = *m;
+    first_l = m[rows];
+  }
+  float4v v[kB];
+  auto load = [&](int b) {
+#pragma unroll
+    for (int i = 0; i < kB; ++i) {
+      of(min(b + i * kP + mine, parts - 1), s, m, rows);
+      v[i] = *reinterpret_cast<const float4v*>(s + d0);
+    }
+  };
+  load(0);
+  top = first_m;
+  for (int i = lane + kWave; i < parts; i += kWave) {
+    of(i, s, m, rows);
+    top = fmaxf(top, *m);
+  }
+#pragma unroll
+  for (int i = 1; i < kWave; i *= 2) top = fmaxf(top, __shfl_xor(top, i));
+  float f = 0.f;  // the weight of part (64 n + lane)
+  l = 0.f;
+  o = float4v{};
+  for (int b = 0; b < parts; b += kB * kP) {
+    if (b % kWave == 0) {
+      float pm = first_m, pl = first_l;
+      if (b > 0 && b + lane < parts) {
+        of(b + lane, s, m, rows);
+        pm = *m;
+        pl = m[rows];
+      }
+      f = b + lane >= parts ? 0.f : (pm == top ? 1.f : __builtin_amdgcn_exp2f(pm - top));
+      l = fmaf(f, b + lane < parts ? pl : 0.f, l);
+    }
+    if (b > 0) load(b);
+#pragma unroll
+    for (int i = 0; i < kB; ++i) {
+      const int part = b + i * kP + mine;
+      const float fi = __shfl(f, part & (kWave - 1));
+      if (part < parts) o += fi * v[i];
+    }
+  }
+#pragma unroll
+  for (int i = 1; i < kWave; i *= 2) l += __shfl_xor(l, i);
+#pragma unroll
+  for (int i = L; i < kWave; i *= 2)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], i);
+}
+template <typename T, int DP, typename F>
+__device__ inline void join_row(char* out, int d, int parts, const F& of) {
+  const int lane = threadIdx.x & 63, d0 = lane % (DP / 4) * 4;
+  float top, l;
+  float4v o;
+  join_sums<DP>(parts, of, top, l, o);
+  const float inv = inverse(l);
+  const float r[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+  if (lane < DP / 4 && d0 < d) store_out<T, 4>(out, d0, r);
+}
+
 // ---- the parts of single tokens' keys ----------------------------------------------------------------------
 __host__ __device__ inline int own_rows(int group) { return group < kKeyTile ? group : kKeyTile; }
 
