@@ -36,7 +36,7 @@
 // With too few tiles to fill the card, the keys are split over workgroups as well, which leave (O, maximum,
 // sum) in the workspace (prompt_time weighs shapes and splits); a second launch joins them in split order (no
 // atomics: repeated calls agree).
-#include "attention8.hpp"
+#include "attention8_own.hpp"
 
 namespace g16 {
 namespace {
@@ -1056,43 +1056,52 @@ __global__ __launch_bounds__(kThreads) void prompt_join_kernel(Params p, int rt)
 // requests at once. Then the requests' own keys, 32 rows a tile, in parts of about equal length over all
 // requests: the device knows their lengths, so every wavefront adds them up and finds its part (see Part).
 // Slots in the same order. A request's only part writes the output itself.
+__device__ inline Row token_row(const Params& p, int b, int head, bool ok, int size) {
+  Row row;
+  row.q = ok ? p.q + b * p.q_seq + head * p.q_head : nullptr;
+  row.out = ok ? p.out + (static_cast<int64_t>(b) * p.hq + head) * p.d * size : nullptr;
+  const int len = ok ? length_of(p, b) : 0;
+  row.pos = p.shared + len - 1;
+  row.limit = 0x7fffffff;
+  row.slope = ok && p.slopes != nullptr ? p.slopes[head] * kLog2e : 0.f;
+  return row;
+}
+
+// Workgroup `block` of those for the shared keys. ranges: 8 values in LDS, where workgroups have 128 rows.
+template <typename T, int DP, bool SKEYS>
+__device__ inline void shared_workgroup(const Params& p, int block, char* lds, float* joint, int* ranges) {
+  constexpr int SRT = SKEYS ? kKeyTile : kRowTile, SBN = SKEYS ? 32 : (sizeof(T) == 2 ? 64 : 32);
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  int lin = block;
+  const int kv = lin % p.hkv;
+  lin /= p.hkv;
+  // (a split's row tiles next to each other: they read the same keys)
+  const int t = lin % p.stiles, split = lin / p.stiles;
+  const int r = t * SRT + (SKEYS ? 0 : 32 * wave) + (lane & 31);
+  const int b = r / p.group;
+  const Row row = token_row(p, b, kv * p.group + r % p.group, b < p.seqs, sizeof(T));
+  const KeyRuns runs = {{p.sk + kv * p.sk_head, p.sv + kv * p.sv_head, p.sk_tok, p.sv_tok, p.shared, 0}, {}};
+  const int n = ceil_div(p.shared, SBN);
+  const int tbeg = share_begin(n, split, p.ssplits), tend = share_begin(n, split + 1, p.ssplits);
+  Slot slot = {p.part + (static_cast<size_t>(t * p.ssplits + split) * p.hkv + kv) * slot_floats(SRT, DP), SRT};
+  if constexpr (SKEYS) {
+    keys_workgroup<T, DP, false, false>(what_of(p), lds, joint, row, runs, Pages{}, n, tbeg, tend, 0x7fffffff, slot);
+  } else {
+    const bool some = t * SRT + 32 * wave < p.seqs * p.group;  // a wavefront without rows computes nothing
+    rows_workgroup<T, DP, DP, false>(p, lds, ranges, row, runs, n, tbeg, tend, 0x7fffffff, some ? 0x7fffffff : -1, slot, [&]() { return row; });
+  }
+}
+
 template <typename T, int DP, bool SKEYS>
 __global__ __launch_bounds__(kThreads, 2) void decode_kernel(Params p) {
-  constexpr int SRT = SKEYS ? kKeyTile : kRowTile, SBN = SKEYS ? 32 : (sizeof(T) == 2 ? 64 : 32);
+  constexpr int SRT = SKEYS ? kKeyTile : kRowTile;
   __shared__ __attribute__((aligned(1024))) char lds[SKEYS ? keys_lds<T, DP>() : cmax(keys_lds<T, DP>(), rows_lds<T, DP>())];
   __shared__ float joint[256];
   __shared__ int ranges[8];
-  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
   const int nshared = p.stiles * p.ssplits * p.hkv;
-  auto row_of = [&](int b, int head, bool ok) {
-    Row row;
-    row.q = ok ? p.q + b * p.q_seq + head * p.q_head : nullptr;
-    row.out = ok ? p.out + (static_cast<int64_t>(b) * p.hq + head) * p.d * static_cast<int>(sizeof(T)) : nullptr;
-    const int len = ok ? length_of(p, b) : 0;
-    row.pos = p.shared + len - 1;
-    row.limit = 0x7fffffff;
-    row.slope = ok && p.slopes != nullptr ? p.slopes[head] * kLog2e : 0.f;
-    return row;
-  };
   if (static_cast<int>(blockIdx.x) < nshared) {
-    int lin = blockIdx.x;
-    const int kv = lin % p.hkv;
-    lin /= p.hkv;
-    // (a split's row tiles next to each other: they read the same keys)
-    const int t = lin % p.stiles, split = lin / p.stiles;
-    const int r = t * SRT + (SKEYS ? 0 : 32 * wave) + (lane & 31);
-    const int b = r / p.group;
-    const Row row = row_of(b, kv * p.group + r % p.group, b < p.seqs);
-    const KeyRuns runs = {{p.sk + kv * p.sk_head, p.sv + kv * p.sv_head, p.sk_tok, p.sv_tok, p.shared, 0}, {}};
-    const int n = ceil_div(p.shared, SBN);
-    const int tbeg = share_begin(n, split, p.ssplits), tend = share_begin(n, split + 1, p.ssplits);
-    Slot slot = {p.part + (static_cast<size_t>(t * p.ssplits + split) * p.hkv + kv) * slot_floats(SRT, DP), SRT};
-    if constexpr (SKEYS) {
-      keys_workgroup<T, DP, false, false>(what_of(p), lds, joint, row, runs, Pages{}, n, tbeg, tend, 0x7fffffff, slot);
-    } else {
-      const bool some = t * SRT + 32 * wave < p.seqs * p.group;  // a wavefront without rows computes nothing
-      rows_workgroup<T, DP, DP, false>(p, lds, ranges, row, runs, n, tbeg, tend, 0x7fffffff, some ? 0x7fffffff : -1, slot, [&]() { return row; });
-    }
+    shared_workgroup<T, DP, SKEYS>(p, static_cast<int>(blockIdx.x), lds, joint, ranges);
     return;
   }
   int lin = blockIdx.x - nshared;
@@ -1104,7 +1113,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(Params p) {
   if (!find_part(p, lin / p.otiles, true, part)) return;
   const int b = part.seq, len = part.len;
   const int orows = own_rows(p.group), r = rt * kKeyTile + (lane & 31);
-  const Row row = row_of(b, kv * p.group + r, r < p.group);
+  const Row row = token_row(p, b, kv * p.group + r, r < p.group, sizeof(T));
   KeyRuns runs = {{}, {p.k + kv * p.k_head, p.v + kv * p.v_head, p.k_tok, p.v_tok, len, p.shared}};
   const Pages pages = {p.pages == nullptr ? nullptr : p.pages + static_cast<size_t>(b) * p.max_pages, p.page, p.num_pages, p.k_seq, p.v_seq};
   if (p.pages == nullptr) {
@@ -1116,6 +1125,22 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(Params p) {
   Slot slot = {nullptr, orows};
   if (p.stiles > 0 || part.splits > 1) slot.at = p.part + static_cast<size_t>(nshared) * slot_floats(SRT, DP) + static_cast<size_t>(own) * slot_floats(orows, DP);
   keys_workgroup<T, DP, true, false>(what_of(p), lds, joint, row, runs, pages, 0, tbeg, tend, 0x7fffffff, slot);
+}
+
+// The shared keys for few rows and, over a cache of 8 bits, the own ones in one launch: one after the other, each would leave the
+// card half empty (16 requests of up to 1500 in int8 after 2048, 8 heads of 128: BOTH).
+template <int DP, int CODE, int RQ>
+__global__ __launch_bounds__(kThreads, 2) void decode_both8_kernel(Params p, Params8 e) {
+  __shared__ union Lds {
+    Lds8<_Float16, DP, RQ> own;
+    struct {
+      alignas(1024) char tiles[keys_lds<_Float16, DP>()];
+      float joint[256];
+    } shared;
+  } lds;
+  const int nshared = p.stiles * p.ssplits * p.hkv;
+  if (static_cast<int>(blockIdx.x) < nshared) shared_workgroup<_Float16, DP, true>(p, static_cast<int>(blockIdx.x), lds.shared.tiles, lds.shared.joint, nullptr);
+  else own8_workgroup<_Float16, DP, CODE, RQ, true>(p, e, static_cast<int>(blockIdx.x) - nshared, lds.own);
 }
 
 template <typename T, int DP>
@@ -1436,6 +1461,18 @@ Plan8 plan_decode8(const g16_attention_args& a) {
   return r;
 }
 
+// Whether shared and own keys go into one launch: what has as many workgroups on a CU either way, and few enough kernels.
+bool both8(const g16_attention_args& a, const Plan8& plan) {
+  return plan.shared.stiles > 0 && plan.shared.skeys && !a.is_f32 && (a.d == 64 || a.d == 128) && a.hq / a.hkv <= 8;
+}
+template <int DP, int CODE>
+int run_both8(const Params& p, const Params8& e, hipStream_t stream) {
+  const dim3 grid(static_cast<unsigned>(p.stiles) * p.ssplits * p.hkv + workgroups_of8(p, e));
+  return p.group == 1   ? launch(decode_both8_kernel<DP, CODE, 1>, grid, dim3(kThreads), stream, p, e)
+         : p.group <= 4 ? launch(decode_both8_kernel<DP, CODE, 4>, grid, dim3(kThreads), stream, p, e)
+                        : launch(decode_both8_kernel<DP, CODE, 8>, grid, dim3(kThreads), stream, p, e);
+}
+
 template <typename T, int DP>
 int run_shared8(const Params& p, bool skeys, hipStream_t stream) {
   const dim3 grid(static_cast<unsigned>(p.stiles) * p.ssplits * p.hkv);
@@ -1524,8 +1561,7 @@ extern "C" int g16_attention_decode8(const g16_attention8_args* args, void* stre
   const Plan8 plan = plan_decode8(a);
   if (plan.bytes > 0 && (a.workspace == nullptr || static_cast<size_t>(a.workspace_bytes) < plan.bytes)) return G16_E_WORKSPACE;
   if (!aligned16(a.workspace)) return G16_E_ALIGN;
-  if (!fits_grid(static_cast<int64_t>(plan.shared.stiles) * plan.shared.ssplits * a.hkv) ||
-      !fits_grid((static_cast<int64_t>(plan.shares) + kXcds) * plan.shared.otiles * a.hkv) || !fits_grid((static_cast<int64_t>(a.seqs) * a.hq + 3) / 4))
+  if (!fits_grid((static_cast<int64_t>(plan.shared.stiles) * plan.shared.ssplits + (static_cast<int64_t>(plan.shares) + kXcds) * plan.shared.otiles) * a.hkv) || !fits_grid((static_cast<int64_t>(a.seqs) * a.hq + 3) / 4))
     return G16_E_SHAPE;
   Params p = params(a);
   p.causal = 0;
@@ -1537,10 +1573,13 @@ extern "C" int g16_attention_decode8(const g16_attention8_args* args, void* stre
   p.v_seq = a.v_seq;
   p.v_head = a.v_head;
   const Params8 own = {e.k_scale, e.v_scale, e.ks_seq, e.ks_head, e.ks_token, e.vs_seq, e.vs_head, e.vs_token, a.k_token, a.v_token,
-                       divide_by(a.page > 0 ? static_cast<uint32_t>(a.page) : 1u), plan.shares, plan.split, plan.shared.skeys ? kKeyTile : kRowTile, plan.first};
+                       divide_by(a.page > 0 ? static_cast<uint32_t>(a.page) : 1u), plan.shares, plan.split, plan.shared.skeys ? kKeyTile : kRowTile, !both8(a, plan), plan.first};
   hipStream_t s = static_cast<hipStream_t>(stream);
   int rc = 0;
-  if (p.stiles > 0) {
+  if (!own.apart) {
+    if (e.code == G16_CODE_INT8) rc = a.d == 64 ? run_both8<64, G16_CODE_INT8>(p, own, s) : run_both8<128, G16_CODE_INT8>(p, own, s);
+    else rc = a.d == 64 ? run_both8<64, G16_CODE_E4M3>(p, own, s) : run_both8<128, G16_CODE_E4M3>(p, own, s);
+  } else if (p.stiles > 0) {
     if (a.is_f32) rc = a.d <= 64 ? run_shared8<float, 64>(p, plan.shared.skeys, s) : run_shared8<float, 128>(p, plan.shared.skeys, s);
     else rc = a.d <= 64 ? run_shared8<_Float16, 64>(p, plan.shared.skeys, s) : run_shared8<_Float16, 128>(p, plan.shared.skeys, s);
   }

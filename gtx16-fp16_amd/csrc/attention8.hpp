@@ -9,17 +9,6 @@ constexpr int kXcds = 8;
 constexpr int kTile8 = 64;  // keys of a tile
 constexpr int kWhole8 = 8;  // tiles of a request whose keys are never split
 
-// n / by without a division: (2 n magic >> 32) >> shift, for n below 2^31.
-struct Divide {
-  uint32_t by, magic, shift;
-  __device__ uint32_t operator()(uint32_t n) const { return __umulhi(2 * n, magic) >> shift; }
-};
-inline Divide divide_by(uint32_t by) {
-  uint32_t shift = 0;
-  while ((1ull << shift) < by) ++shift;
-  return Divide{by, static_cast<uint32_t>((1ull << (31 + shift)) / by + 1), shift};
-}
-
 struct Params8 {
   const float *ks, *vs;
   int64_t ks_seq, ks_head, ks_tok, vs_seq, vs_head, vs_tok;  // elements
@@ -28,6 +17,7 @@ struct Params8 {
   int shares;    // at most
   bool split;    // shares of equal length; else one for each request
   int srt;       // rows of the shared keys' slots
+  bool apart;    // the own keys have a launch of their own
   size_t first;  // floats of the shared keys' slots, before the own keys'
 };
 
@@ -39,7 +29,11 @@ constexpr int waves_of8(bool f32, int dp, int rows, bool full) {
   return f32 || dp == 128 || rows == 16 ? 2 : rows == 1 && full ? 4 : 3;
 }
 
-// Enqueues the products of the requests' own keys and the joins.
+inline unsigned workgroups_of8(const Params& p, const Params8& e) {
+  return static_cast<unsigned>(e.shares >= kXcds ? ceil_div(e.shares, kXcds) * kXcds : e.shares) * p.otiles * p.hkv;
+}
+
+// Enqueues the products of the requests' own keys, where they are apart, and the joins.
 int run_own8(const Params& p, const Params8& e, int code, bool f32, hipStream_t stream);
 
 }  // namespace g16

@@ -12,14 +12,19 @@ namespace {
 
 constexpr int kThreads = 256;
 
+// Keys or values: workgroups are told apart by blockIdx.y, so that what is here stays in scalar registers.
+struct Side {
+  char* rows;
+  uint8_t* codes;
+  float* scales;
+  int64_t token, head;                                       // bytes, of the rows
+  int64_t c_page, c_token, c_head, s_page, s_token, s_head;  // elements: bytes of the codes
+};
 struct Params {
-  char* rows[2];  // k, v
-  uint8_t* codes[2];
-  float* scales[2];
+  Side side[2];
   const int32_t* slots;
-  int64_t token[2], head[2];                                                        // bytes, of the rows
-  int64_t c_page[2], c_token[2], c_head[2], s_page[2], s_token[2], s_head[2];       // elements: bytes of the codes
-  uint32_t n, page, hkv, d, capacity;                                               // capacity: slots
+  Divide page, hkv, block;  // by a page's tokens; by the heads; to read: by block_rows where runs go row by row within a head, else by 1
+  uint32_t n, d, capacity;  // capacity: slots
   uint32_t block_rows;
 };
 
@@ -59,22 +64,22 @@ __device__ inline uint32_t top_of(const Eight<_Float16>& x) {
   return __float_as_uint(static_cast<float>(__builtin_bit_cast(_Float16, h)));
 }
 
-// A workgroup: block_rows rows, all runs of them. Of rows with one slot the last is written, so every workgroup looks
+// A workgroup: block_rows rows, all heads of them. Of rows with one slot the last is written, so every workgroup looks
 // through the later rows' slots: a map of its own slots' last 12 bits passes over nearly all of the others (n rows
-// are n^2 / 2 / block_rows looks in all).
+// are n^2 / block_rows looks in all).
 constexpr uint32_t kMapBits = 4096, kMostRows = 32;
 
 template <typename T, int CODE, int LP>
 __global__ __launch_bounds__(kThreads) void write_kernel(Params p) {
   __shared__ uint32_t slot_of[kMostRows], live[kMostRows], map[kMapBits / 32];
+  const Side& side = p.side[blockIdx.y];
   const uint32_t tid = threadIdx.x, first = blockIdx.x * p.block_rows, here = min(p.block_rows, p.n - first);
-  const uint32_t lane = tid % LP, runs = here * 2 * p.hkv;
+  const uint32_t lane = tid % LP, runs = here * p.hkv.by;
   const bool inside = lane * 8 < p.d;
   Eight<T> x = {};
   auto load = [&](uint32_t run) {
-    const uint32_t r = run / (2 * p.hkv), of = run % (2 * p.hkv), kv = of >= p.hkv, h = of - (kv ? p.hkv : 0);
-    if (run < runs && inside)
-      x = *reinterpret_cast<const Eight<T>*>(p.rows[kv] + (first + r) * p.token[kv] + h * p.head[kv] + lane * 8 * sizeof(T));
+    const uint32_t r = p.hkv(run), h = run - r * p.hkv.by;
+    if (run < runs && inside) x = *reinterpret_cast<const Eight<T>*>(side.rows + (first + r) * side.token + h * side.head + lane * 8 * sizeof(T));
   };
   uint32_t run = tid / LP;
   load(run);
@@ -87,16 +92,23 @@ __global__ __launch_bounds__(kThreads) void write_kernel(Params p) {
   __syncthreads();
   if (tid < here) atomicOr(&map[(slot_of[tid] % kMapBits) / 32], 1u << (slot_of[tid] % 32));
   __syncthreads();
-  for (uint32_t i = first + 1 + tid; i < p.n; i += kThreads) {
-    const uint32_t s = static_cast<uint32_t>(p.slots[i]);
-    if (map[(s % kMapBits) / 32] >> (s % 32) & 1) {
-      for (uint32_t r = 0; r < here && first + r < i; ++r)
-        if (slot_of[r] == s) live[r] = 0;
+  constexpr int kLooks = 8;  // under way together
+  for (uint32_t i0 = first + 1 + tid; i0 < p.n; i0 += kLooks * kThreads) {
+    uint32_t s[kLooks];
+#pragma unroll
+    for (int j = 0; j < kLooks; ++j) s[j] = static_cast<uint32_t>(p.slots[min(i0 + j * kThreads, p.n - 1)]);
+#pragma unroll
+    for (int j = 0; j < kLooks; ++j) {  // (behind the end the last one again)
+      const uint32_t i = min(i0 + j * kThreads, p.n - 1);
+      if (map[(s[j] % kMapBits) / 32] >> (s[j] % 32) & 1) {
+        for (uint32_t r = 0; r < here && first + r < i; ++r)
+          if (slot_of[r] == s[j]) live[r] = 0;
+      }
     }
   }
   __syncthreads();
   for (; run < runs; run += kThreads / LP) {
-    const uint32_t r = run / (2 * p.hkv), of = run % (2 * p.hkv), kv = of >= p.hkv, h = of - (kv ? p.hkv : 0);
+    const uint32_t r = p.hkv(run), h = run - r * p.hkv.by;
     const Scaling s = scaling_of<CODE>(__uint_as_float(largest<LP>(top_of(x))));
     float v[8];
 #pragma unroll
@@ -104,67 +116,79 @@ __global__ __launch_bounds__(kThreads) void write_kernel(Params p) {
     const u32x2 codes = encode8<CODE>(v, s);
     load(run + kThreads / LP);
     if (live[r] != 0 && inside) {
-      const uint32_t page = slot_of[r] / p.page, at = slot_of[r] - page * p.page;
-      *reinterpret_cast<u32x2*>(p.codes[kv] + page * p.c_page[kv] + at * p.c_token[kv] + h * p.c_head[kv] + lane * 8) = codes;
-      if (lane == 0) p.scales[kv][page * p.s_page[kv] + at * p.s_token[kv] + h * p.s_head[kv]] = s.scale;
+      const uint32_t page = p.page(slot_of[r]), at = slot_of[r] - page * p.page.by;
+      *reinterpret_cast<u32x2*>(side.codes + page * side.c_page + at * side.c_token + h * side.c_head + lane * 8) = codes;
+      if (lane == 0) side.scales[page * side.s_page + at * side.s_token + h * side.s_head] = s.scale;
     }
   }
 }
 
-// A thread: eight values of kRuns runs.
+// A workgroup: block_rows rows, all heads of them; a thread: eight values of kRuns runs at a time.
 constexpr int kRuns = 4;
 
 template <typename T, int CODE, int LP>
 __global__ __launch_bounds__(kThreads) void read_kernel(Params p) {
-  const uint32_t lane = threadIdx.x % LP;
+  constexpr uint32_t kStep = kThreads / LP;
+  const Side& side = p.side[blockIdx.y];
+  const uint32_t lane = threadIdx.x % LP, first = blockIdx.x * p.block_rows, here = min(p.block_rows, p.n - first);
+  const bool by_head = p.block.by > 1;
+  const uint32_t runs = (by_head ? p.block_rows : here) * p.hkv.by;
   if (lane * 8 >= p.d) return;
-  const uint64_t first = static_cast<uint64_t>(blockIdx.x) * (kRuns * kThreads / LP) + threadIdx.x / LP;
-  const uint64_t runs = static_cast<uint64_t>(p.n) * 2 * p.hkv;
-  u32x2 codes[kRuns];
-  float scale[kRuns];
-  char* to[kRuns];
+  for (uint32_t run0 = threadIdx.x / LP; run0 < runs; run0 += kRuns * kStep) {
+    u32x2 codes[kRuns];
+    float scale[kRuns];
+    uint32_t row[kRuns], h[kRuns], slot[kRuns];
+    bool some[kRuns];
 #pragma unroll
-  for (int i = 0; i < kRuns; ++i) {
-    const uint64_t run = first + i * (kThreads / LP);
-    codes[i] = u32x2{0, 0};
-    scale[i] = 0.f;
-    to[i] = nullptr;
-    if (run >= runs) continue;
-    const uint32_t r = static_cast<uint32_t>(run / (2 * p.hkv)), of = static_cast<uint32_t>(run % (2 * p.hkv)), kv = of >= p.hkv;
-    const uint32_t h = of - (kv ? p.hkv : 0), slot = static_cast<uint32_t>(p.slots[r]);
-    to[i] = p.rows[kv] + ((static_cast<uint64_t>(r) * p.hkv + h) * p.d + lane * 8) * sizeof(T);
-    if (slot >= p.capacity) continue;
-    const uint32_t page = slot / p.page, at = slot - page * p.page;
-    codes[i] = *reinterpret_cast<const u32x2*>(p.codes[kv] + page * p.c_page[kv] + at * p.c_token[kv] + h * p.c_head[kv] + lane * 8);
-    scale[i] = p.scales[kv][page * p.s_page[kv] + at * p.s_token[kv] + h * p.s_head[kv]];
-  }
+    for (int i = 0; i < kRuns; ++i) {
+      const uint32_t run = min(run0 + i * kStep, runs - 1);
+      uint32_t r;
+      if (by_head) {
+        h[i] = p.block(run);
+        r = run - h[i] * p.block.by;
+      } else {
+        r = p.hkv(run);
+        h[i] = run - r * p.hkv.by;
+      }
+      some[i] = r < here && run0 + i * kStep < runs;
+      row[i] = first + min(r, here - 1);
+      slot[i] = static_cast<uint32_t>(p.slots[row[i]]);  // (negative ones: past every capacity)
+    }
 #pragma unroll
-  for (int i = 0; i < kRuns; ++i) {
-    if (to[i] == nullptr) continue;
-    float v[8];
-    decode8<CODE>(codes[i], v);
-    Eight<T> x;
+    for (int i = 0; i < kRuns; ++i) {
+      codes[i] = u32x2{0, 0};
+      scale[i] = 0.f;
+      if (slot[i] >= p.capacity) continue;
+      const uint32_t page = p.page(slot[i]), at = slot[i] - page * p.page.by;
+      codes[i] = *reinterpret_cast<const u32x2*>(side.codes + page * side.c_page + at * side.c_token + h[i] * side.c_head + lane * 8);
+      scale[i] = side.scales[page * side.s_page + at * side.s_token + h[i] * side.s_head];
+    }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x.v[j] = static_cast<T>(v[j] * scale[i]);
-    *reinterpret_cast<Eight<T>*>(to[i]) = x;
+    for (int i = 0; i < kRuns; ++i) {
+      if (!some[i]) continue;
+      float v[8];
+      decode8<CODE>(codes[i], v);
+      Eight<T> x;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x.v[j] = static_cast<T>(v[j] * scale[i]);
+      *reinterpret_cast<Eight<T>*>(side.rows + ((static_cast<uint64_t>(row[i]) * p.hkv.by + h[i]) * p.d + lane * 8) * sizeof(T)) = x;
+    }
   }
 }
 
 template <typename T, int CODE, int LP>
 int run(Params p, bool write, hipStream_t stream) {
-  if (!write) {
-    const uint64_t runs = static_cast<uint64_t>(p.n) * 2 * p.hkv, blocks = (runs + kRuns * kThreads / LP - 1) / (kRuns * kThreads / LP);
-    if (blocks > (1u << 24) - 1) return G16_E_SHAPE;  // (2^32 threads a launch)
-    return launch(read_kernel<T, CODE, LP>, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), stream, p);
-  }
-  // Rows of a workgroup: enough for every lane, and more where there are many workgroups, which all look through the
-  // later rows' slots.
-  uint32_t rows = kThreads / LP / (2 * p.hkv);
-  rows = max(rows, p.n / 1024);
-  p.block_rows = min(max(rows, 1u), kMostRows);
+  // Rows of a workgroup: enough for every lane (to read, four times), and, to write, more where there are many
+  // workgroups, which all look through the later rows' slots.
+  const uint32_t full = kThreads / LP / p.hkv.by;
+  p.block_rows = write ? min(max(max(full, p.n / 1024), 1u), kMostRows) : max(full * kRuns, 1u);
+  // A cache whose memory is ordered by heads is read head by head.
+  const bool by_head = !write && p.side[0].c_token < p.side[0].c_head && p.n > 64;
+  if (by_head) p.block_rows = max(p.block_rows, 16u);
+  p.block = divide_by(by_head ? p.block_rows : 1);
   const uint32_t blocks = (p.n + p.block_rows - 1) / p.block_rows;
-  if (blocks > (1u << 24) - 1) return G16_E_SHAPE;  // (2^32 threads a launch)
-  return launch(write_kernel<T, CODE, LP>, dim3(blocks), dim3(kThreads), stream, p);
+  if (blocks > (1u << 23) - 1) return G16_E_SHAPE;  // (2^32 threads a launch)
+  return launch(write ? write_kernel<T, CODE, LP> : read_kernel<T, CODE, LP>, dim3(blocks, 2), dim3(kThreads), stream, p);
 }
 template <typename T, int CODE>
 int run(const Params& p, bool write, hipStream_t stream) {
@@ -194,28 +218,14 @@ int cache(const g16_cache_args* args, bool write, void* stream) {
   }
   if (write && (a.k_token * size % 16 != 0 || a.k_head * size % 16 != 0 || a.v_token * size % 16 != 0 || a.v_head * size % 16 != 0)) return G16_E_ALIGN;
   Params p = {};
-  p.rows[0] = static_cast<char*>(a.k);
-  p.rows[1] = static_cast<char*>(a.v);
-  p.codes[0] = static_cast<uint8_t*>(a.k_cache);
-  p.codes[1] = static_cast<uint8_t*>(a.v_cache);
-  p.scales[0] = a.k_scale;
-  p.scales[1] = a.v_scale;
+  p.side[0] = {static_cast<char*>(a.k), static_cast<uint8_t*>(a.k_cache), a.k_scale, a.k_token * size, a.k_head * size,
+               a.kc_page, a.kc_token, a.kc_head, a.ks_page, a.ks_token, a.ks_head};
+  p.side[1] = {static_cast<char*>(a.v), static_cast<uint8_t*>(a.v_cache), a.v_scale, a.v_token * size, a.v_head * size,
+               a.vc_page, a.vc_token, a.vc_head, a.vs_page, a.vs_token, a.vs_head};
   p.slots = a.slots;
-  const int64_t strides[2][8] = {{a.k_token, a.k_head, a.kc_page, a.kc_token, a.kc_head, a.ks_page, a.ks_token, a.ks_head},
-                                 {a.v_token, a.v_head, a.vc_page, a.vc_token, a.vc_head, a.vs_page, a.vs_token, a.vs_head}};
-  for (int i = 0; i < 2; ++i) {
-    p.token[i] = strides[i][0] * size;
-    p.head[i] = strides[i][1] * size;
-    p.c_page[i] = strides[i][2];
-    p.c_token[i] = strides[i][3];
-    p.c_head[i] = strides[i][4];
-    p.s_page[i] = strides[i][5];
-    p.s_token[i] = strides[i][6];
-    p.s_head[i] = strides[i][7];
-  }
   p.n = static_cast<uint32_t>(a.rows);
-  p.page = static_cast<uint32_t>(a.page > 0 ? a.page : 1);
-  p.hkv = static_cast<uint32_t>(a.hkv);
+  p.page = divide_by(static_cast<uint32_t>(a.page > 0 ? a.page : 1));
+  p.hkv = divide_by(static_cast<uint32_t>(a.hkv));
   p.d = static_cast<uint32_t>(a.d);
   p.capacity = static_cast<uint32_t>(capacity);
   hipStream_t s = static_cast<hipStream_t>(stream);

@@ -7,6 +7,17 @@ namespace g16 {
 
 typedef float float2v __attribute__((ext_vector_type(2)));
 
+// n / by without a division: (2 n magic >> 32) >> shift, for n below 2^31.
+struct Divide {
+  uint32_t by, magic, shift;
+  __device__ uint32_t operator()(uint32_t n) const { return __umulhi(2 * n, magic) >> shift; }
+};
+inline Divide divide_by(uint32_t by) {
+  uint32_t shift = 0;
+  while ((1ull << shift) < by) ++shift;
+  return Divide{by, static_cast<uint32_t>((1ull << (31 + shift)) / by + 1), shift};
+}
+
 // The eight numbers of two dwords of codes, exactly.
 template <int CODE>
 __device__ inline void decode8(u32x2 codes, float (&x)[8]) {

@@ -80,39 +80,31 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(Params p) {
     const double position = p.positions[static_cast<uint64_t>(axis) * p.rows + row];
     turn(position * (p.freqs[i] * 0.63661977236758134308), c[j], s[j]);  // 2 / pi
   }
-  const uint32_t at0 = (NEIGHBOURS ? 2 * first : first) * sizeof(T), at1 = NEIGHBOURS ? at0 + V * sizeof(T) : at0 + p.pairs * sizeof(T);
+  // Halves: V values from each of them; neighbours: 2 V values in a row.
+  constexpr int L = NEIGHBOURS ? 1 : 2, N = 2 * V / L;
+  const uint32_t at[2] = {static_cast<uint32_t>((NEIGHBOURS ? 2 * first : first) * sizeof(T)), static_cast<uint32_t>((p.pairs + first) * sizeof(T))};
   for (uint32_t h0 = slice; h0 < p.heads; h0 += kAhead * p.slices) {
-    Run<T, V> a[kAhead], b[kAhead];
+    Run<T, N> v[kAhead][L];
 #pragma unroll
     for (int n = 0; n < kAhead; ++n) {
       const uint32_t h = min(h0 + n * p.slices, p.heads - 1);
-      a[n] = *reinterpret_cast<const Run<T, V>*>(x + h * p.x_head + at0);
-      b[n] = *reinterpret_cast<const Run<T, V>*>(x + h * p.x_head + at1);
+#pragma unroll
+      for (int i = 0; i < L; ++i) v[n][i] = *reinterpret_cast<const Run<T, N>*>(x + h * p.x_head + at[i]);
     }
 #pragma unroll
     for (int n = 0; n < kAhead; ++n) {
       const uint32_t h = h0 + n * p.slices;
       if (h >= p.heads) break;
-      T in[2 * V], res[2 * V];
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        in[j] = a[n].v[j];
-        in[V + j] = b[n].v[j];
+        T& a = NEIGHBOURS ? v[n][0].v[2 * j] : v[n][0].v[j];
+        T& b = NEIGHBOURS ? v[n][0].v[2 * j + 1] : v[n][L - 1].v[j];
+        const float x0 = to_f(a), x1 = to_f(b);
+        a = static_cast<T>(fmaf(x0, c[j], -(x1 * s[j])));
+        b = static_cast<T>(fmaf(x1, c[j], x0 * s[j]));
       }
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const int i0 = NEIGHBOURS ? 2 * j : j, i1 = NEIGHBOURS ? 2 * j + 1 : V + j;
-        const float x0 = to_f(in[i0]), x1 = to_f(in[i1]);
-        res[i0] = static_cast<T>(fmaf(x0, c[j], -(x1 * s[j])));
-        res[i1] = static_cast<T>(fmaf(x1, c[j], x0 * s[j]));
-      }
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        a[n].v[j] = res[j];
-        b[n].v[j] = res[V + j];
-      }
-      *reinterpret_cast<Run<T, V>*>(out + h * out_head + at0) = a[n];
-      *reinterpret_cast<Run<T, V>*>(out + h * out_head + at1) = b[n];
+      for (int i = 0; i < L; ++i) *reinterpret_cast<Run<T, N>*>(out + h * out_head + at[i]) = v[n][i];
     }
   }
 }
@@ -131,19 +123,19 @@ int run(Params p, hipStream_t stream) {
   if (blocks > (1u << 24) - 1) return G16_E_SHAPE;  // (2^32 threads a launch)
   return launch(rotary_kernel<T, V, NEIGHBOURS>, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), stream, p);
 }
-template <typename T, int V>
-int run(const Params& p, bool neighbours, hipStream_t stream) {
-  return neighbours ? run<T, V, true>(p, stream) : run<T, V, false>(p, stream);
-}
-// Pairs of a thread: 16 bytes of each load where their number allows that (fp32: 4; neighbours: both of a pair in
-// one load would be half as many, but 32 bytes a thread read as fast).
+// Pairs of a thread: 16 bytes a load where their number allows that (neighbours: 12291 patches, 32 heads of 128 fp16, 40 pairs:
+// CLIPS with 32 bytes a thread).
 template <typename T>
 int run(const Params& p, bool neighbours, hipStream_t stream) {
-  if constexpr (sizeof(T) == 2) {
-    if (p.pairs % 8 == 0) return run<T, 8>(p, neighbours, stream);
+  constexpr uint32_t kMost = 16 / sizeof(T);
+  if (!neighbours) {
+    if (p.pairs % kMost == 0) return run<T, kMost, false>(p, stream);
+    if (sizeof(T) == 2 && p.pairs % 4 == 0) return run<T, 4, false>(p, stream);
+    return p.pairs % 2 == 0 ? run<T, 2, false>(p, stream) : run<T, 1, false>(p, stream);
   }
-  if (p.pairs % 4 == 0) return run<T, 4>(p, neighbours, stream);
-  return p.pairs % 2 == 0 ? run<T, 2>(p, neighbours, stream) : run<T, 1>(p, neighbours, stream);
+  if (p.pairs % (kMost / 2) == 0) return run<T, kMost / 2, true>(p, stream);
+  if (sizeof(T) == 2 && p.pairs % 2 == 0) return run<T, 2, true>(p, stream);
+  return run<T, 1, true>(p, stream);
 }
 
 // (what the Python binding packs)
