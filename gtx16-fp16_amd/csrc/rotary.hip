@@ -63,26 +63,26 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(Params p) {
   const char* x = p.x + seq * p.x_seq + (row - seq * p.tokens) * p.x_token;
   char* out = p.out + static_cast<uint64_t>(row) * p.heads * p.d * sizeof(T);
   const uint64_t out_head = p.d * sizeof(T);
-  if (item >= p.turned) {
-    const uint32_t at = (2 * p.pairs + (item - p.turned) * W) * sizeof(T);
-    for (uint32_t h = slice; h < p.heads; h += p.slices)
-      *reinterpret_cast<Run<T, W>*>(out + h * out_head + at) = *reinterpret_cast<const Run<T, W>*>(x + h * p.x_head + at);
-    return;
-  }
+  const bool turns = item < p.turned;  // else values that stay as they are
   const uint32_t first = item * V;
   float c[V], s[V];
+  if (turns) {
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const uint32_t i = first + j;
-    uint32_t axis = 0;
+    for (int j = 0; j < V; ++j) {
+      const uint32_t i = first + j;
+      uint32_t axis = 0;
 #pragma unroll
-    for (int a = 0; a < G16_ROTARY_MAX_AXES - 1; ++a) axis += i >= p.ends[a];
-    const double position = p.positions[static_cast<uint64_t>(axis) * p.rows + row];
-    turn(position * (p.freqs[i] * 0.63661977236758134308), c[j], s[j]);  // 2 / pi
+      for (int a = 0; a < G16_ROTARY_MAX_AXES - 1; ++a) axis += i >= p.ends[a];
+      const double position = p.positions[static_cast<uint64_t>(axis) * p.rows + row];
+      turn(position * (p.freqs[i] * 0.63661977236758134308), c[j], s[j]);  // 2 / pi
+    }
   }
-  // Halves: V values from each of them; neighbours: 2 V values in a row.
+  // Halves: V values from each of them; neighbours: 2 V values in a row. Those that stay are W in a row, as one such run or as two
+  // (or as the same one twice).
   constexpr int L = NEIGHBOURS ? 1 : 2, N = 2 * V / L;
-  const uint32_t at[2] = {static_cast<uint32_t>((NEIGHBOURS ? 2 * first : first) * sizeof(T)), static_cast<uint32_t>((p.pairs + first) * sizeof(T))};
+  const uint32_t stay = 2 * p.pairs + (item - p.turned) * W;
+  const uint32_t at[2] = {static_cast<uint32_t>((turns ? (NEIGHBOURS ? 2 * first : first) : stay) * sizeof(T)),
+                          static_cast<uint32_t>((turns ? p.pairs + first : stay + W - N) * sizeof(T))};
   for (uint32_t h0 = slice; h0 < p.heads; h0 += kAhead * p.slices) {
     Run<T, N> v[kAhead][L];
 #pragma unroll
@@ -95,13 +95,15 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(Params p) {
     for (int n = 0; n < kAhead; ++n) {
       const uint32_t h = h0 + n * p.slices;
       if (h >= p.heads) break;
+      if (turns) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        T& a = NEIGHBOURS ? v[n][0].v[2 * j] : v[n][0].v[j];
-        T& b = NEIGHBOURS ? v[n][0].v[2 * j + 1] : v[n][L - 1].v[j];
-        const float x0 = to_f(a), x1 = to_f(b);
-        a = static_cast<T>(fmaf(x0, c[j], -(x1 * s[j])));
-        b = static_cast<T>(fmaf(x1, c[j], x0 * s[j]));
+        for (int j = 0; j < V; ++j) {
+          T& a = NEIGHBOURS ? v[n][0].v[2 * j] : v[n][0].v[j];
+          T& b = NEIGHBOURS ? v[n][0].v[2 * j + 1] : v[n][L - 1].v[j];
+          const float x0 = to_f(a), x1 = to_f(b);
+          a = static_cast<T>(fmaf(x0, c[j], -(x1 * s[j])));
+          b = static_cast<T>(fmaf(x1, c[j], x0 * s[j]));
+        }
       }
 #pragma unroll
       for (int i = 0; i < L; ++i) *reinterpret_cast<Run<T, N>*>(out + h * out_head + at[i]) = v[n][i];
