@@ -1,13 +1,14 @@
 """Serve requests with adapters of their own after a shared system prompt.
 
-    python examples/serve_adapters.py [--layers 4 --requests 12 --tokens 32 --check]
+    python examples/serve_adapters.py [--layers 4 --requests 12 --tokens 32 --rotary --cache int8 --check]
 
 A small half-precision decoder with random weights: its projections are ``AdapterLinear`` layers (one
 fp16 weight for all requests, a low-rank adapter for each), its attention has grouped heads, a bias that
-grows with the distance in place of positions, and capped scores. The system prompt's keys and values are
-computed once; every request's own prompt follows it (``attention`` with ``shared_k``), and the tokens after
-that are generated for all requests together (``attention_decode`` over pages of 16 keys). ``--check``
-computes every request again by itself, in fp32 and in plain torch, and compares the logits.
+grows with the distance in place of positions (or, with ``--rotary``, rotary positions), and capped scores. The system
+prompt's keys and values are computed once; every request's own prompt follows it (``attention`` with ``shared_k``),
+and the tokens after that are generated for all requests together (``attention_decode`` over pages of 16 keys, in
+fp16 or, with ``--cache int8`` or ``e4m3``, written by ``cache_write``). ``--check`` computes every request again by itself, in
+fp32 and in plain torch, and compares the logits.
 """
 from __future__ import annotations
 
@@ -24,6 +25,7 @@ import gtx16_fp16 as g  # noqa: E402
 
 PAGE = 16
 SOFTCAP = 30.0
+CACHES = {"fp16": torch.float16, "int8": torch.int8, "e4m3": torch.float8_e4m3fn}
 
 
 def layer(n_in: int, n_out: int, adapters: int, rank: int, gen: torch.Generator, device) -> g.AdapterLinear:
@@ -43,10 +45,13 @@ class Block(nn.Module):
         self.qkv = make(width, (heads + 2 * key_heads) * self.d)
         self.out, self.up, self.down = make(width, width), make(width, 4 * width), make(4 * width, width)
 
-    def split(self, x, index):
-        """Views of the fused projection's output: q, k, v [rows, heads, d]."""
+    def split(self, x, index, at, freqs):
+        """q, k, v [rows, heads, d], views of the fused projection's output; rotated (freqs) where rows stand ``at``."""
         y = self.qkv(self.norm1(x), index).unflatten(-1, (-1, self.d))
-        return y.split((self.heads, self.key_heads, self.key_heads), dim=-2)
+        if freqs is None:
+            return y.split((self.heads, self.key_heads, self.key_heads), dim=-2)
+        qk = g.rotary(y[:, :self.heads + self.key_heads], at, freqs)
+        return *qk.split((self.heads, self.key_heads), dim=-2), y[:, self.heads + self.key_heads:]
 
     def rest(self, x, attended, index):
         x = x + self.out(attended.flatten(-2), index)
@@ -56,24 +61,28 @@ class Block(nn.Module):
 class Server(nn.Module):
     """``requests`` slots, each with an adapter and pages for its own keys in every layer."""
 
-    def __init__(self, width=512, heads=8, key_heads=2, layers=4, vocab=1024, adapters=5, rank=16, seed=0, device="cuda"):
+    def __init__(self, width=512, heads=8, key_heads=2, layers=4, vocab=1024, adapters=5, rank=16, seed=0, device="cuda",
+                 rotary=False, cache="fp16"):
         super().__init__()
         gen = torch.Generator().manual_seed(seed)
         self.blocks = nn.ModuleList(Block(width, heads, key_heads, adapters, rank, gen, device) for _ in range(layers))
         self.embed = (0.7 * torch.randn(vocab, width, generator=gen)).half().to(device)
         self.head = g.FastLinear(width, vocab, bias=False, device=device)
         self.head.weight_t.copy_(self.embed.t())
-        self.slopes = torch.tensor([2.0 ** (-8.0 * (h + 1) / heads) for h in range(heads)], device=device)
-        self.device = device
+        d = width // heads
+        self.slopes = None if rotary else torch.tensor([2.0 ** (-8.0 * (h + 1) / heads) for h in range(heads)], device=device)
+        self.freqs = torch.tensor([10000.0 ** (-2 * i / d) for i in range(d // 2)], device=device) if rotary else None
+        self.device, self.coded = device, CACHES[cache]
         self.shared: list = []
 
     def prefix(self, ids: torch.Tensor) -> None:
         """The system prompt, which has no adapter: its keys and values are kept for all requests."""
         x, index = self.embed[ids], torch.full((len(ids),), -1, dtype=torch.int32, device=self.device)
         whole = torch.tensor([0, len(ids)], dtype=torch.int32, device=self.device)
+        at = torch.arange(len(ids), dtype=torch.int32, device=self.device)
         self.shared = []
         for b in self.blocks:
-            q, k, v = b.split(x, index)
+            q, k, v = b.split(x, index, at, self.freqs)
             self.shared.append((k.contiguous(), v.contiguous()))
             x = b.rest(x, g.attention(q, k, v, q_offsets=whole, causal=True, slopes=self.slopes, softcap=SOFTCAP), index)
 
@@ -85,31 +94,46 @@ class Server(nn.Module):
         self.adapter, self.lengths = adapter, lens.to(torch.int32).to(self.device)
         self.pages = torch.randperm(n * per).view(n, per).to(torch.int32).to(self.device)
         b0 = self.blocks[0]
-        self.cache = [tuple(torch.empty(n * per, PAGE, b0.key_heads, b0.d, dtype=torch.float16, device=self.device) for _ in "kv")
-                      for _ in self.blocks]
+        shape = (n * per, PAGE, b0.key_heads, b0.d)
+        scaled = self.coded != torch.float16
+        self.cache = [(*(torch.empty(shape, dtype=self.coded, device=self.device) for _ in "kv"),
+                       *(torch.empty(shape[:3], device=self.device) if scaled else None for _ in "kv")) for _ in self.blocks]
         index = adapter.repeat_interleave(lens.to(self.device), output_size=int(lens.sum()))
         seq = torch.repeat_interleave(torch.arange(n, device=self.device), lens.to(self.device), output_size=int(lens.sum()))
         at = torch.arange(int(lens.sum()), device=self.device) - offsets[seq]
-        page, slot = self.pages[seq, at // PAGE].long(), at % PAGE
+        slots = self.slots(seq, at)
+        at = (at + len(self.shared[0][0])).to(torch.int32)
         x = self.embed[torch.cat(prompts).to(self.device)]
-        for b, (sk, sv), (kc, vc) in zip(self.blocks, self.shared, self.cache):
-            q, k, v = b.split(x, index)
-            kc[page, slot], vc[page, slot] = k, v
+        for b, (sk, sv), cache in zip(self.blocks, self.shared, self.cache):
+            q, k, v = b.split(x, index, at, self.freqs)
+            self.keep(k, v, cache, slots)
             x = b.rest(x, g.attention(q, k, v, q_offsets=offsets, causal=True, shared_k=sk, shared_v=sv, slopes=self.slopes,
                                       softcap=SOFTCAP), index)
         return self.head(x[offsets[1:].long() - 1])
 
+    def slots(self, seq: torch.Tensor, at: torch.Tensor) -> torch.Tensor:
+        """Where the cache has token ``at`` of request ``seq``: tokens counted through all pages."""
+        return (self.pages[seq, (at // PAGE).long()] * PAGE + at % PAGE).to(torch.int32)
+
+    def keep(self, k, v, cache, slots) -> None:
+        kc, vc, ks, vs = cache
+        if ks is not None:
+            g.cache_write(k, v, kc, vc, ks, vs, slots)
+        else:
+            kc.view(-1, *kc.shape[2:])[slots.long()], vc.view(-1, *vc.shape[2:])[slots.long()] = k, v
+
     def step(self, ids: torch.Tensor) -> torch.Tensor:
         """One more token of every request; the logits of the next."""
-        rows = torch.arange(len(ids), device=self.device)
-        page, slot = self.pages[rows, (self.lengths // PAGE).long()].long(), (self.lengths % PAGE).long()
+        slots = self.slots(torch.arange(len(ids), device=self.device), self.lengths)
+        at = self.lengths + len(self.shared[0][0])
         self.lengths += 1
         x = self.embed[ids]
-        for b, (sk, sv), (kc, vc) in zip(self.blocks, self.shared, self.cache):
-            q, k, v = b.split(x, self.adapter)
-            kc[page, slot], vc[page, slot] = k, v
+        for b, (sk, sv), cache in zip(self.blocks, self.shared, self.cache):
+            q, k, v = b.split(x, self.adapter, at, self.freqs)
+            self.keep(k, v, cache, slots)
+            kc, vc, ks, vs = cache
             x = b.rest(x, g.attention_decode(q, kc, vc, self.lengths, pages=self.pages, shared_k=sk, shared_v=sv, slopes=self.slopes,
-                                             softcap=SOFTCAP), self.adapter)
+                                             softcap=SOFTCAP, k_scale=ks, v_scale=vs), self.adapter)
         return self.head(x)
 
 
@@ -130,8 +154,13 @@ def plain(server: Server, system: torch.Tensor, ids: torch.Tensor, adapter: int)
         norm = lambda w, x: torch.nn.functional.rms_norm(x, x.shape[-1:], w.weight.float())  # noqa: E731
         q, k, v = (t.transpose(0, 1) for t in product(b.qkv, norm(b.norm1, x)).unflatten(-1, (-1, b.d)).split(
             (b.heads, b.key_heads, b.key_heads), dim=-2))
+        if server.freqs is not None:
+            angle = pos[:, None] * server.freqs.double()
+            z = torch.polar(torch.ones_like(angle), angle).to(torch.complex64)
+            q, k = (torch.cat(((y := z * torch.complex(*t.chunk(2, -1))).real, y.imag), -1) for t in (q, k))
         k, v = (t.repeat_interleave(b.heads // b.key_heads, 0) for t in (k, v))
-        s = SOFTCAP * torch.tanh((q @ k.transpose(1, 2)) * b.d ** -0.5 / SOFTCAP) - server.slopes[:, None, None] * away
+        s = SOFTCAP * torch.tanh((q @ k.transpose(1, 2)) * b.d ** -0.5 / SOFTCAP)
+        s = s if server.slopes is None else s - server.slopes[:, None, None] * away
         a = torch.softmax(s.masked_fill(away < 0, float("-inf")), -1) @ v
         x = x + product(b.out, a.transpose(0, 1).flatten(1))
         x = x + product(b.down, torch.nn.functional.gelu(product(b.up, norm(b.norm2, x))))
@@ -145,9 +174,11 @@ def main(argv: list[str] | None = None) -> float:
     for name, value in (("--width", 512), ("--heads", 8), ("--key-heads", 2), ("--layers", 4), ("--requests", 12), ("--system", 300),
                         ("--prompt", 60), ("--tokens", 32)):
         ap.add_argument(name, type=int, default=value)
+    ap.add_argument("--rotary", action="store_true", help="rotary positions in place of the distance bias")
+    ap.add_argument("--cache", choices=CACHES, default="fp16", help="what the requests' own keys and values are kept in")
     ap.add_argument("--check", action="store_true", help="compare with plain torch in fp32")
     a = ap.parse_args(argv)
-    server = Server(a.width, a.heads, a.key_heads, a.layers)
+    server = Server(a.width, a.heads, a.key_heads, a.layers, rotary=a.rotary, cache=a.cache)
     dev, gen = server.device, torch.Generator().manual_seed(1)
     vocab = server.embed.shape[0]
     system = torch.randint(0, vocab, (a.system,), generator=gen).to(dev)

@@ -1,5 +1,5 @@
 // Single tokens over a cache of 8 bits (g16_attention_decode8; its formulas stand in g16.h): the products of the requests' own
-// keys, by one workgroup. A shared prefix is not in 8 bits and decode_kernel's, the joins are decode_join_kernel's (attention.hip).
+// keys, by one workgroup. A shared prefix is not in 8 bits and shared_workgroup's (attention.hip), the joins are attention8.hip's.
 //
 // All requests' keys, in tiles of 64 one request after another, are dealt in shares of equal length, as many as run on the card at
 // once: whatever the lengths, all workgroups end together (see Deal for few keys). A workgroup has the query rows of one key head and a
@@ -151,7 +151,8 @@ __device__ inline int all_tiles(const Params& p, const Run64& head) {
 // How all requests' tiles are dealt. Long ones in shares of equal length, whatever the requests: the first `more` shares
 // have each + 1, the others each. Where a share would have few tiles, its time is that of the waits for one after another, not of its bytes,
 // and a second request's would come on top: every request then has its own pieces, of `chunk` tiles, one for each
-// wavefront or two (16 requests of up to 1500 after 2048, 8 heads of 128: PIECES).
+// wavefront or two (16 requests of up to 1500 after 2048, 8 heads of 128: 42 us by shares,
+// 36 so).
 struct Deal {
   int shares, each, more, chunk;
   __device__ Deal(const Params& p, const Params8& e, int total) {
@@ -260,7 +261,7 @@ struct Lds8 {
 template <typename T, int DP, int CODE, int RQ, bool FULL>
 __device__ inline void own8_workgroup(const Params& p, const Params8& e, int block, Lds8<T, DP, RQ>& shared) {
   using S = Shape8<T, DP, RQ>;
-  constexpr int VB = DP / 16, VW = DP / 64;  // values of a lane (and blocks of the second product), in dwords
+  constexpr int VB = DP / 16, VW = DP / 64;  // values of a lane, and blocks of the second product; dwords of a lane's values
   constexpr int R = S::R, NR = S::NR, NS = S::NS, RI = S::RI, PARTS = S::PARTS;
   constexpr int kKeys = Lds8<T, DP, RQ>::kKeys, kWeights = Lds8<T, DP, RQ>::kWeights;
   char* lds = shared.data;
@@ -269,7 +270,7 @@ __device__ inline void own8_workgroup(const Params& p, const Params8& e, int blo
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), col = lane & 15, g = lane >> 4;
   // Workgroups go to the XCDs in turn, and every XCD has an L2 of its own. The heads of a share read the same cache lines (of
   // codes where a head's are less than a line, of scales always), so they are all given to one XCD where there are shares for all
-  // (96 requests of up to 2048, 12 heads of 64: 76 us, so 63).
+  // (96 requests of up to 2048, 12 heads of 64: 76 us, and by this alone 63).
   int lin = block;
   if (e.shares >= kXcds) {
     const int per = p.otiles * p.hkv, i = lin / kXcds, share = i / per * kXcds + lin % kXcds;
@@ -318,7 +319,7 @@ __device__ inline void own8_workgroup(const Params& p, const Params8& e, int blo
     // A key is CH pieces of 16 bytes. A load takes whole keys, in the order in which they lie in memory; LDS turns them
     // into the product's order, where lane l has piece 4 c + l / 16 of key l % 16: pieces are at places that put those of 8 keys on
     // different banks. (Loaded in that order, a lane's piece next to another key's, 40 requests of 8192 e4m3 keys of 8 heads of 128
-    // take KLOADS.)
+    // take 166 us, so 161; ordered by heads 143 and 146.)
     constexpr int CH = DP / 16, PER = 64 / CH, NK = CH;  // pieces of a key; keys of a load; loads of a tile
     auto place_of = [](int key, int piece) { return key * DP + ((piece ^ (CH == 8 ? key & 7 : (key >> 1) & 3)) << 4); };
     char* keys = lds + wave * (kKeys + kWeights);

@@ -13,7 +13,7 @@ from .cache import cache_read, cache_write
 from .linear import FastLinear, patch
 from .lora import AdapterLinear, lora_mm_t
 from .ops import is_affected, matmul, mm_t, supported
-from .rotary import rotary
+from .positions import rotary
 
 __all__ = ["FastLinear", "patch", "is_affected", "matmul", "mm_t", "supported"]
 __version__ = "0.1.0"

@@ -93,10 +93,22 @@ def test_keys_split_over_workgroups(cuda, dtype, code, lengths, hq, hkv, d, kw):
     assert torch.equal(y, g.attention_decode(*args, **more))
 
 
+@pytest.mark.parametrize("lengths,kw", [
+    ([(37 * i) % 190 for i in range(150)], dict(capacity=600, page=16)),  # dealt in shares over more requests than a wavefront has lanes
+    ([(7 * i) % 65 for i in range(40)], dict(capacity=600)),               # in more pieces than there are workgroups
+    ([(7 * i) % 65 for i in range(140)], dict(capacity=600, page=24)),
+    ([0] * 70 + [300] + [0] * 70, dict(capacity=600)),
+], ids=lambda v: str(len(v)))
+def test_many_requests(cuda, lengths, kw):
+    args, more, ref = case(cuda, F16, "int8", lengths, 32, 32, 8, seed=len(lengths), **kw)
+    check(g.attention_decode(*args, **more), ref)
+
+
 @pytest.mark.parametrize("code", ["int8", "e4m3"])
 @pytest.mark.parametrize("dtype", [F16, F32])
 @pytest.mark.parametrize("lengths,hq,hkv,d,kw", [
-    ([0, 1, 40], 4, 2, 64, dict(shared=1)), ([10, 0], 8, 1, 128, dict(shared=300, page=16)), ([5] * 40, 4, 2, 72, dict(shared=70)),
+    ([0, 1, 40], 4, 2, 64, dict(shared=1)), ([10, 0], 8, 1, 128, dict(shared=300, page=16)), ([5] * 40, 4, 2, 72, dict(shared=70)), ([3, 70], 2, 2, 64, dict(shared=40)),
+    ([900, 0, 64], 16, 2, 128, dict(shared=65, page=16, by_head=True)), ([7] * 3, 12, 2, 64, dict(shared=200)),
     ([600, 30], 20, 1, 64, dict(shared=900, page=16, softcap=30.0, biased=True)), ([1200] * 2, 4, 2, 96, dict(shared=33, page=24, by_head=True)),
 ], ids=str)
 def test_after_a_shared_prefix(cuda, dtype, code, lengths, hq, hkv, d, kw):
