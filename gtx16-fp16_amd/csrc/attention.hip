@@ -1441,7 +1441,8 @@ struct Plan8 {
   DecodePlan shared;
   int shares;
   bool split;
-  size_t first, bytes;  // floats of the shared keys' slots; bytes in all
+  size_t table;         // floats of the requests' table, before the slots
+  size_t first, bytes;  // floats before the own keys' slots; bytes in all
 };
 Plan8 plan_decode8(const g16_attention_args& a) {
   Plan8 r = {};
@@ -1455,8 +1456,10 @@ Plan8 plan_decode8(const g16_attention_args& a) {
     const int64_t each = static_cast<int64_t>(cus_of(a)) / kXcds * waves_of8(a.is_f32 != 0, dp, rows_of8(group), a.d == dp) / heads;
     r.shares = static_cast<int>(each < 1 ? kXcds : each * kXcds);
   }
-  r.first = static_cast<size_t>(r.shared.stiles) * r.shared.ssplits * a.hkv * slot_floats(srt, dp);
-  if (r.shared.stiles > 0 || r.split)
+  const bool join = r.shared.stiles > 0 || r.split;
+  r.table = join ? (static_cast<size_t>(a.seqs) * sizeof(Slots) + 15) / 16 * 4 : 0;
+  r.first = r.table + static_cast<size_t>(r.shared.stiles) * r.shared.ssplits * a.hkv * slot_floats(srt, dp);
+  if (join)
     r.bytes = (r.first + (static_cast<size_t>(r.shares) + (r.split ? a.seqs : 0)) * heads * slot_floats(own_rows(group), dp)) * sizeof(float);
   return r;
 }
@@ -1568,12 +1571,14 @@ extern "C" int g16_attention_decode8(const g16_attention8_args* args, void* stre
   p.stiles = plan.shared.stiles;
   p.ssplits = plan.shared.ssplits;
   p.otiles = plan.shared.otiles;
+  p.part += plan.table;
   p.k_seq = a.k_seq;
   p.k_head = a.k_head;
   p.v_seq = a.v_seq;
   p.v_head = a.v_head;
   const Params8 own = {e.k_scale, e.v_scale, e.ks_seq, e.ks_head, e.ks_token, e.vs_seq, e.vs_head, e.vs_token, a.k_token, a.v_token,
-                       divide_by(a.page > 0 ? static_cast<uint32_t>(a.page) : 1u), plan.shares, plan.split, plan.shared.skeys ? kKeyTile : kRowTile, !both8(a, plan), plan.first};
+                       divide_by(a.page > 0 ? static_cast<uint32_t>(a.page) : 1u), plan.shares, plan.split, plan.shared.skeys ? kKeyTile : kRowTile, !both8(a, plan), plan.first - plan.table,
+                       plan.bytes > 0 ? static_cast<Slots*>(a.workspace) : nullptr};
   hipStream_t s = static_cast<hipStream_t>(stream);
   int rc = 0;
   if (!own.apart) {

@@ -15,9 +15,8 @@ __global__ __launch_bounds__(kThreads) void decode8_join_kernel(Params p, Params
   if (row >= p.seqs * p.hq) return;
   const int b = row / p.hq, head = row % p.hq, kv = head / p.group, g = head % p.group;
   const int ns = p.stiles > 0 ? p.ssplits : 0, orows = own_rows(p.group), sr = b * p.group + g;
-  int first, parts;
-  find_request(p, e, b, first, parts);
-  parts += ns;
+  const Slots own = e.table[b];
+  const int parts = ns + own.count;
   if (parts == 1) return;
   auto slot_of = [&](int i, const float*& o, const float*& m, int& rows) {
     const float* slot;
@@ -27,7 +26,7 @@ __global__ __launch_bounds__(kThreads) void decode8_join_kernel(Params p, Params
       r = sr % e.srt;
       rows = e.srt;
     } else {
-      const size_t at = (static_cast<size_t>(first) + (i - ns)) * p.otiles + g / kKeyTile;
+      const size_t at = (static_cast<size_t>(own.first) + (i - ns)) * p.otiles + g / kKeyTile;
       slot = p.part + e.first + (at * p.hkv + kv) * slot_floats(orows, DP);
       r = g % kKeyTile;
       rows = orows;

@@ -9,6 +9,11 @@ constexpr int kXcds = 8;
 constexpr int kTile8 = 64;  // keys of a tile
 constexpr int kWhole8 = 8;  // tiles of a request whose keys are never split
 
+// A request's slots: the first one's number, and how many there are.
+struct Slots {
+  int first, count;
+};
+
 struct Params8 {
   const float *ks, *vs;
   int64_t ks_seq, ks_head, ks_tok, vs_seq, vs_head, vs_tok;  // elements
@@ -19,6 +24,7 @@ struct Params8 {
   int srt;       // rows of the shared keys' slots
   bool apart;    // the own keys have a launch of their own
   size_t first;  // floats of the shared keys' slots, before the own keys'
+  Slots* table;  // of all requests, for the join (NULL: there is none), before the slots
 };
 
 // Query rows that a workgroup has room for.

@@ -120,6 +120,17 @@ constexpr int kRun8 = kTile8 + 8;  // weights of a row in LDS: rows on different
 // A request without keys has one tile, too: somebody has to write its zeros. (The host sees to it that 32 bits hold all tiles.)
 __device__ inline int tiles_of(int len) { return max(1, ceil_div(len, kTile8)); }
 
+// The sum of a value over the lanes up to and with this one.
+__device__ inline int sum_up(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // within rows of 16 lanes: from 1, 2, 4 and 8 before
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // rows 1 and 3: the last lane's of the row before
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // rows 2 and 3: lane 31's
+  return v;
+}
+
 // A run of 64 requests in a wavefront: lane i has the length of request b0 + i and how many of what is counted (tiles, or pieces
 // of `chunk` tiles) there are up to and with its own.
 struct Run64 {
@@ -130,15 +141,9 @@ struct Run64 {
     set(b0 + lane < p.seqs, chunk);
   }
   __device__ void set(bool some, int chunk) {
-    const int lane = threadIdx.x & 63;
     count = some ? tiles_of(len) : 0;
     if (chunk > 1) count = static_cast<int>(static_cast<uint32_t>(count + chunk - 1) / static_cast<uint32_t>(chunk));
-    upto = count;
-#pragma unroll
-    for (int i = 1; i < kWave; i *= 2) {
-      const int x = __shfl_up(upto, i);
-      if (lane >= i) upto += x;
-    }
+    upto = sum_up(count);
   }
   __device__ int all() const { return __builtin_amdgcn_readlane(upto, kWave - 1); }
 };
@@ -154,7 +159,8 @@ __device__ inline int all_tiles(const Params& p, const Run64& head) {
 // wavefront or two (16 requests of up to 1500 after 2048, 8 heads of 128: 42 us by shares,
 // 36 so).
 struct Deal {
-  int shares, each, more, chunk;
+  int shares = 1, each = 1, more = 0, chunk = 0;
+  __device__ Deal() {}
   __device__ Deal(const Params& p, const Params8& e, int total) {
     const int four = static_cast<int>((static_cast<uint32_t>(total) + 2u * p.seqs) / (4u * e.shares)) + 1;
     chunk = four <= 2 ? 4 * four : 0;
@@ -174,11 +180,13 @@ struct Deal {
 // `shares` further on.
 struct Share {
   int seq, len, tile, tiles, slot;  // the first request, its length, the first tile of it; the first slot
+  int ahead;                        // tiles of the requests before that one
   bool pieces;
 };
 // Piece number `piece` (a share is one).
-__device__ inline bool find_share(const Params& p, const Params8& e, int piece, Share& r) {
+__device__ inline bool find_share(const Params& p, const Params8& e, int piece, Share& r, Deal& deal) {
   r.pieces = false;
+  r.ahead = 0;
   if (!e.split) {
     if (piece >= p.seqs) return false;
     r.seq = r.slot = piece;
@@ -188,7 +196,7 @@ __device__ inline bool find_share(const Params& p, const Params8& e, int piece, 
     return true;
   }
   Run64 head(p, 0);
-  const Deal deal(p, e, all_tiles(p, head));
+  deal = Deal(p, e, all_tiles(p, head));
   r.pieces = deal.chunk > 0;
   const int from = r.pieces ? piece : deal.begin(piece);
   if (!r.pieces) r.tiles = deal.begin(piece + 1) - from;
@@ -205,36 +213,13 @@ __device__ inline bool find_share(const Params& p, const Params8& e, int piece, 
       r.tile = r.pieces ? behind * deal.chunk : behind;
       if (r.pieces) r.tiles = min(deal.chunk, tiles_of(r.len) - r.tile);
       r.slot = r.pieces ? piece : piece + r.seq;
+      r.ahead = from - r.tile;
       return true;
     }
     before += run.all();
   }
   return false;
 }
-// The slots of request b.
-__device__ inline void find_request(const Params& p, const Params8& e, int b, int& first, int& parts) {
-  first = b;
-  parts = 1;
-  if (!e.split) return;
-  const Run64 head(p, 0);
-  const Deal deal(p, e, all_tiles(p, head));
-  int before = 0;
-  for (int b0 = 0;; b0 += kWave) {
-    const Run64 run(p, b0, deal.chunk > 0 ? deal.chunk : 1);
-    if (b < b0 + kWave) {
-      parts = __builtin_amdgcn_readlane(run.count, b - b0);
-      first = before + __builtin_amdgcn_readlane(run.upto, b - b0) - parts;
-      break;
-    }
-    before += run.all();
-  }
-  if (deal.chunk == 0) {
-    const int tile = first, last = first + parts - 1;
-    first = deal.share_of(tile) + b;
-    parts = deal.share_of(last) + b - first + 1;
-  }
-}
-
 // RQ: query rows that there is room for, 1, 4, 8, 16 or 32. FULL: heads of DP values.
 template <typename T, int DP, int RQ>
 struct Shape8 {
@@ -281,10 +266,12 @@ __device__ inline void own8_workgroup(const Params& p, const Params8& e, int blo
   lin /= p.hkv;
   const int rt = lin % p.otiles, share = lin / p.otiles;
   Share has;
-  if (!find_share(p, e, share, has)) return;
+  Deal deal;
+  if (!find_share(p, e, share, has, deal)) return;
   const int orows = own_rows(p.group);
   const Scoring sc = scoring(p);
-  int b = has.seq, len = has.len, u0 = has.tile, todo = has.tiles, at_slot = has.slot;  // request, its first tile here, tiles to do
+  int b = has.seq, len = has.len, u0 = has.tile, todo = has.tiles;  // request, its first tile here, tiles to do
+  int at_slot = has.slot, ahead = has.ahead;
 
   for (int piece = share;;) {
     const int tiles = tiles_of(len), u1 = min(u0 + todo, tiles);
@@ -361,6 +348,13 @@ __device__ inline void own8_workgroup(const Params& p, const Params8& e, int blo
           }
         }
     };
+
+    if (u0 == 0 && kv == 0 && rt == 0 && e.table != nullptr && tid == 0) {
+      Slots s = {at_slot, 1};
+      if (has.pieces) s.count = static_cast<int>(static_cast<uint32_t>(tiles + deal.chunk - 1) / static_cast<uint32_t>(deal.chunk));
+      else if (e.split) s.count = deal.share_of(ahead + tiles - 1) - share + 1;
+      e.table[b] = s;
+    }
 
     int j0 = begin + kTile8 * wave;
     constexpr int kStep = 4 * kTile8;
@@ -655,14 +649,16 @@ __device__ inline void own8_workgroup(const Params& p, const Params8& e, int blo
       len = uniform(length_of(p, ++b));
       u0 = 0;
       ++at_slot;
+      ahead += tiles;
     } else {
       piece += e.shares;
-      if (!has.pieces || !find_share(p, e, piece, has)) break;
+      if (!has.pieces || !find_share(p, e, piece, has, deal)) break;
       b = has.seq;
       len = has.len;
       u0 = has.tile;
       todo = has.tiles;
       at_slot = has.slot;
+      ahead = has.ahead;
     }
     __syncthreads();  // (the sums in LDS have been read)
   }
