@@ -315,6 +315,15 @@ no:
   return -1;
 }
 
+/* Where a tensor that was made here lies; NULL where that cannot be told */
+static void* pointer_of(PyObject* o) {
+  PyObject* x = PyObject_CallMethodNoArgs(o, s_data_ptr);
+  void* ptr = x == NULL ? NULL : PyLong_AsVoidPtr(x);
+  Py_XDECREF(x);
+  PyErr_Clear();
+  return ptr;
+}
+
 /* Compute units of a device these kernels run on; -1 else */
 static int device_cus(int device) {
   if (device < 0 || device >= MAX_DEVICES) return -1;
@@ -694,7 +703,7 @@ static int contiguous(const tensor_t* t) {
 static const int kGradRotary[2] = {0, 2};
 static PyObject* fast_rotary(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
   (void)self;
-  tensor_t x, at, f, t;
+  tensor_t x, at, f;
   g16_rotary_args a;
   void* stream;
   PyObject* out;
@@ -733,11 +742,11 @@ static PyObject* fast_rotary(PyObject* self, PyObject* const* args, Py_ssize_t n
   const int interleaved = PyObject_IsTrue(args[4]);
   if (interleaved < 0 || raw_stream(x.device, &stream)) return none_clear();
   out = empty_like(args[0]);
-  if (out == NULL || read_tensor(out, &t)) {
+  if (out == NULL || (a.out = pointer_of(out)) == NULL) {
     Py_XDECREF(out);
     return none_clear();
   }
-  a.x = x.ptr, a.out = t.ptr, a.positions = at.ptr, a.freqs = f.ptr;
+  a.x = x.ptr, a.positions = at.ptr, a.freqs = f.ptr;
   a.x_seq = lead == 2 ? x.stride[0] : 0, a.x_token = x.stride[lead - 1], a.x_head = x.stride[lead];
   a.seqs = lead == 2 ? (int)x.shape[0] : 1, a.tokens = (int)x.shape[lead - 1], a.heads = (int)x.shape[lead];
   a.d = (int)d, a.pairs = (int)pairs, a.interleaved = interleaved, a.is_f32 = x.dtype == g_f32;
@@ -822,7 +831,7 @@ static PyObject* fast_cache_write(PyObject* self, PyObject* const* args, Py_ssiz
 static const int kGradRead[2] = {2, 3};
 static PyObject* fast_cache_read(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
   (void)self;
-  tensor_t kc, vc, ks, vs, slots, t;
+  tensor_t kc, vc, ks, vs, slots;
   g16_cache_args a;
   void* stream;
   PyObject *k = NULL, *v = NULL, *shape = NULL, *both = NULL;
@@ -838,14 +847,10 @@ static PyObject* fast_cache_read(PyObject* self, PyObject* const* args, Py_ssize
   PyObject* argv[3] = {args[2], shape, args[5]};
   if (shape != NULL) k = PyObject_VectorcallMethod(s_new_empty, argv, 2, s_dtype_names);
   if (k != NULL) v = PyObject_VectorcallMethod(s_new_empty, argv, 2, s_dtype_names);
-  if (v != NULL && !read_tensor(k, &t)) {
-    a.k = t.ptr;
-    if (!read_tensor(v, &t)) {
-      a.v = t.ptr;
-      Py_BEGIN_ALLOW_THREADS
-      st = g_cache_read(&a, stream);
-      Py_END_ALLOW_THREADS
-    }
+  if (v != NULL && (a.k = pointer_of(k)) != NULL && (a.v = pointer_of(v)) != NULL) {
+    Py_BEGIN_ALLOW_THREADS
+    st = g_cache_read(&a, stream);
+    Py_END_ALLOW_THREADS
   }
   if (st == 0) both = PyTuple_Pack(2, k, v);
   Py_XDECREF(shape);
@@ -900,11 +905,10 @@ static PyObject* fast_attention_decode8(PyObject* self, PyObject* const* args, P
   if (bytes > 0 && a->workspace == NULL) Py_RETURN_NONE;
   a->workspace_bytes = (int64_t)bytes;
   out = empty_like(args[0]);
-  if (out == NULL || read_tensor(out, &t)) {
+  if (out == NULL || (a->out = pointer_of(out)) == NULL) {
     Py_XDECREF(out);
     return none_clear();
   }
-  a->out = t.ptr;
   Py_BEGIN_ALLOW_THREADS
   st = g_attention8(&e, stream);
   Py_END_ALLOW_THREADS
