@@ -65,13 +65,15 @@ __device__ inline uint32_t top_of(const Eight<_Float16>& x) {
 }
 
 // A workgroup: block_rows rows, all heads of them. Of rows with one slot the last is written, so every workgroup looks
-// through the later rows' slots: a map of its own slots' last 12 bits passes over nearly all of the others (n rows
-// are n^2 / block_rows looks in all).
-constexpr uint32_t kMapBits = 4096, kMostRows = 32;
+// through the later rows' slots, n^2 / block_rows looks in all: a map of its own slots' last bits passes over nearly all of the
+// others, and the lanes together, a row each, compare one that it does not. (32768 rows of 8 heads of 128, fp16: 210 us where every lane
+// compared its own with all rows, 46.5 so.) A launch has at most kLaunchRows: the next one's rows are later ones anyway
+// (2^20 rows of one head of 64: 0.85 ms, 0.96 by 16384).
+constexpr uint32_t kMapBits = 32 * kThreads, kMostRows = 32, kLaunchRows = 32768;
 
 template <typename T, int CODE, int LP>
 __global__ __launch_bounds__(kThreads) void write_kernel(Params p) {
-  __shared__ uint32_t slot_of[kMostRows], live[kMostRows], map[kMapBits / 32];
+  __shared__ uint32_t slot_of[kMostRows], live[kMostRows], map[kThreads];
   const Side& side = p.side[blockIdx.y];
   const uint32_t tid = threadIdx.x, first = blockIdx.x * p.block_rows, here = min(p.block_rows, p.n - first);
   const uint32_t lane = tid % LP, runs = here * p.hkv.by;
@@ -88,21 +90,25 @@ __global__ __launch_bounds__(kThreads) void write_kernel(Params p) {
     slot_of[tid] = s;
     live[tid] = s < p.capacity;
   }
-  if (tid < kMapBits / 32) map[tid] = 0;
+  map[tid] = 0;
   __syncthreads();
-  if (tid < here) atomicOr(&map[(slot_of[tid] % kMapBits) / 32], 1u << (slot_of[tid] % 32));
+  if (tid < here && live[tid] != 0) atomicOr(&map[(slot_of[tid] % kMapBits) / 32], 1u << (slot_of[tid] % 32));
   __syncthreads();
   constexpr int kLooks = 8;  // under way together
-  for (uint32_t i0 = first + 1 + tid; i0 < p.n; i0 += kLooks * kThreads) {
+  const uint32_t row = tid % 64, own = row < here && live[row] != 0 ? slot_of[row] : ~0u;
+  for (uint32_t i0 = first + 1; i0 < p.n; i0 += kLooks * kThreads) {
     uint32_t s[kLooks];
 #pragma unroll
-    for (int j = 0; j < kLooks; ++j) s[j] = static_cast<uint32_t>(p.slots[min(i0 + j * kThreads, p.n - 1)]);
+    for (int j = 0; j < kLooks; ++j) s[j] = static_cast<uint32_t>(p.slots[min(i0 + tid + j * kThreads, p.n - 1)]);
 #pragma unroll
-    for (int j = 0; j < kLooks; ++j) {  // (behind the end the last one again)
-      const uint32_t i = min(i0 + j * kThreads, p.n - 1);
-      if (map[(s[j] % kMapBits) / 32] >> (s[j] % 32) & 1) {
-        for (uint32_t r = 0; r < here && first + r < i; ++r)
-          if (slot_of[r] == s[j]) live[r] = 0;
+    for (int j = 0; j < kLooks; ++j) {
+      const uint32_t i = i0 + tid + j * kThreads;
+      const bool maybe = i < p.n && s[j] < p.capacity && (map[(s[j] % kMapBits) / 32] >> (s[j] % 32) & 1) != 0;
+      for (uint64_t hits = __ballot(maybe); hits != 0; hits &= hits - 1) {
+        const int at = __builtin_ctzll(hits);
+        if (own == static_cast<uint32_t>(__builtin_amdgcn_readlane(s[j], at)) &&
+            first + row < static_cast<uint32_t>(__builtin_amdgcn_readlane(i, at)))
+          live[row] = 0;
       }
     }
   }
@@ -177,29 +183,44 @@ __global__ __launch_bounds__(kThreads) void read_kernel(Params p) {
 }
 
 template <typename T, int CODE, int LP>
-int run(Params p, bool write, hipStream_t stream) {
-  // Rows of a workgroup: enough for every lane (to read, four times), and, to write, more where there are many
-  // workgroups, which all look through the later rows' slots.
-  const uint32_t full = kThreads / LP / p.hkv.by;
-  p.block_rows = write ? min(max(max(full, p.n / 1024), 1u), kMostRows) : max(full * kRuns, 1u);
+int write(Params p, hipStream_t stream) {
+  const uint32_t full = kThreads / LP / p.hkv.by, rows = p.n;
+  for (uint32_t done = 0; done < rows; done += p.n) {
+    p.n = min(rows - done, kLaunchRows);
+    // Rows of a workgroup: enough for every lane, and more where there are many workgroups, which all look through the later rows' slots.
+    p.block_rows = min(max(max(full, p.n / 1024), 1u), kMostRows);
+    const int rc = launch(write_kernel<T, CODE, LP>, dim3((p.n + p.block_rows - 1) / p.block_rows, 2), dim3(kThreads), stream, p);
+    if (rc != 0) return rc;
+    for (Side& side : p.side) side.rows += p.n * side.token;
+    p.slots += p.n;
+  }
+  return G16_OK;
+}
+template <typename T, int CODE, int LP>
+int read(Params p, hipStream_t stream) {
+  p.block_rows = max(kThreads / LP / p.hkv.by * kRuns, 1u);  // enough for every lane, four times
   // A cache whose memory is ordered by heads is read head by head.
-  const bool by_head = !write && p.side[0].c_token < p.side[0].c_head && p.n > 64;
+  const bool by_head = p.side[0].c_token < p.side[0].c_head && p.n > 64;
   if (by_head) p.block_rows = max(p.block_rows, 16u);
   p.block = divide_by(by_head ? p.block_rows : 1);
   const uint32_t blocks = (p.n + p.block_rows - 1) / p.block_rows;
   if (blocks > (1u << 23) - 1) return G16_E_SHAPE;  // (2^32 threads a launch)
-  return launch(write ? write_kernel<T, CODE, LP> : read_kernel<T, CODE, LP>, dim3(blocks, 2), dim3(kThreads), stream, p);
+  return launch(read_kernel<T, CODE, LP>, dim3(blocks, 2), dim3(kThreads), stream, p);
+}
+template <typename T, int CODE, int LP>
+int run(const Params& p, bool to_cache, hipStream_t stream) {
+  return to_cache ? write<T, CODE, LP>(p, stream) : read<T, CODE, LP>(p, stream);
 }
 template <typename T, int CODE>
-int run(const Params& p, bool write, hipStream_t stream) {
-  return p.d <= 8 ? run<T, CODE, 1>(p, write, stream) : p.d <= 16 ? run<T, CODE, 2>(p, write, stream) : p.d <= 32 ? run<T, CODE, 4>(p, write, stream)
-         : p.d <= 64 ? run<T, CODE, 8>(p, write, stream) : run<T, CODE, 16>(p, write, stream);
+int run(const Params& p, bool to_cache, hipStream_t stream) {
+  return p.d <= 8 ? run<T, CODE, 1>(p, to_cache, stream) : p.d <= 16 ? run<T, CODE, 2>(p, to_cache, stream) : p.d <= 32 ? run<T, CODE, 4>(p, to_cache, stream)
+         : p.d <= 64 ? run<T, CODE, 8>(p, to_cache, stream) : run<T, CODE, 16>(p, to_cache, stream);
 }
 
 // (what the Python binding packs)
 static_assert(sizeof(g16_cache_args) == 7 * 8 + 16 * 8 + 8 * 4, "no padding");
 
-int cache(const g16_cache_args* args, bool write, void* stream) {
+int cache(const g16_cache_args* args, bool to_cache, void* stream) {
   if (args == nullptr) return G16_E_NULL;
   const g16_cache_args& a = *args;
   if ((a.is_f32 != 0 && a.is_f32 != 1) || (a.code != G16_CODE_INT8 && a.code != G16_CODE_E4M3)) return G16_E_DTYPE;
@@ -216,7 +237,7 @@ int cache(const g16_cache_args* args, bool write, void* stream) {
                         static_cast<int64_t>(reinterpret_cast<uintptr_t>(a.v_cache));
     if (all % 8 != 0) return G16_E_ALIGN;
   }
-  if (write && (a.k_token * size % 16 != 0 || a.k_head * size % 16 != 0 || a.v_token * size % 16 != 0 || a.v_head * size % 16 != 0)) return G16_E_ALIGN;
+  if (to_cache && (a.k_token * size % 16 != 0 || a.k_head * size % 16 != 0 || a.v_token * size % 16 != 0 || a.v_head * size % 16 != 0)) return G16_E_ALIGN;
   Params p = {};
   p.side[0] = {static_cast<char*>(a.k), static_cast<uint8_t*>(a.k_cache), a.k_scale, a.k_token * size, a.k_head * size,
                a.kc_page, a.kc_token, a.kc_head, a.ks_page, a.ks_token, a.ks_head};
@@ -229,8 +250,8 @@ int cache(const g16_cache_args* args, bool write, void* stream) {
   p.d = static_cast<uint32_t>(a.d);
   p.capacity = static_cast<uint32_t>(capacity);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (a.code == G16_CODE_INT8) return a.is_f32 ? run<float, G16_CODE_INT8>(p, write, s) : run<_Float16, G16_CODE_INT8>(p, write, s);
-  return a.is_f32 ? run<float, G16_CODE_E4M3>(p, write, s) : run<_Float16, G16_CODE_E4M3>(p, write, s);
+  if (a.code == G16_CODE_INT8) return a.is_f32 ? run<float, G16_CODE_INT8>(p, to_cache, s) : run<_Float16, G16_CODE_INT8>(p, to_cache, s);
+  return a.is_f32 ? run<float, G16_CODE_E4M3>(p, to_cache, s) : run<_Float16, G16_CODE_E4M3>(p, to_cache, s);
 }
 
 }  // namespace

@@ -446,7 +446,7 @@ int g16_rotary(const g16_rotary_args* args, void* stream);
  * along d, the scales are fp32, [pages, page, hkv]; strides in elements, those of the codes multiples of 8 bytes.
  * k, v (rows; out rows for a read) [rows, hkv, d], fp16 or fp32 (is_f32).
  * g16_cache_write: row r goes to slots[r]; a slot below 0 or past the cache's end is not written, and of several rows
- * with one slot the last is. rows strides in elements, multiples of 16 bytes. One launch.
+ * with one slot the last is. rows strides in elements, multiples of 16 bytes. One launch for every 32768 rows.
  * g16_cache_read: row r is what slots[r] holds, zeros for a slot outside; k and v contiguous. One launch.
  */
 #define G16_CODE_INT8 1
@@ -468,7 +468,9 @@ int g16_cache_read(const g16_cache_args* args, void* stream);
 /* g16_attention_decode over such a cache: `a` as there, k and v the codes, whose strides are in bytes and, like their
  * pointers, multiples of 8 (no other limits); scales by strides in elements, ks_seq a request's or a page's. q, out and the
  * shared prefix have a's type. A score is scale * k_scale * (q . code), a value v_scale * code; codes are multiplied exactly,
- * with fp16 weights to 2^-17. A page outside the cache reads as zeros. One launch, one more for shared keys, one more where keys are split. */
+ * with fp16 weights to 2^-17. A page outside the cache reads as zeros. One launch, one more where keys are split or shared, and
+ * one for the shared keys unless d is 64 or 128, q fp16, hq / hkv up to 8 and seqs * hq / hkv up to 64.
+ * seqs * (k_len / 64 + 1) up to 2^31 - 1. */
 typedef struct {
   const float *k_scale, *v_scale;
   int64_t ks_seq, ks_token, ks_head, vs_seq, vs_token, vs_head;

@@ -158,6 +158,20 @@ def test_slots_past_32_bits_of_bytes(cuda):
         assert torch.equal(y.cpu()[:3], (c * s[..., None]).float()[:3]) and not y[3].any()
 
 
+def test_many_rows(cuda):
+    # more rows than a launch has, slots that come again in a later one, and rows that are not written
+    n, pages, page = 70000, 9, 5000
+    gen = torch.Generator().manual_seed(3)
+    slots = torch.randint(-9000, pages * page, (n,), generator=gen, dtype=torch.int32)
+    slots[[5, 40000, 69999]] = 17
+    slots[[6, 32767, 32768]] = 18
+    k, v = (torch.randn(n, 2, 8, generator=gen).half() for _ in "kv")
+    cache = empty(pages, page, 2, 8, "int8", cuda)
+    before = [t.clone() for t in cache]
+    g.cache_write(k.to(cuda), v.to(cuda), *cache, slots.to(cuda))
+    check(cache, before, k, v, slots, "int8")
+
+
 def test_graphs(cuda):
     cache = empty(4, 16, 2, 64, "e4m3", cuda)
     k, v = (torch.randn(9, 2, 64, device=cuda).half() for _ in "kv")
