@@ -680,7 +680,7 @@ no:
 }
 
 /* ---- rotary positions and caches in 8 bits --------------------------------------------------------------- */
-static PyObject *g_i8 = NULL, *g_e4m3 = NULL;
+static PyObject *g_i8 = NULL, *g_e4m3 = NULL, *g_capturing = NULL;
 typedef int (*rotary_fn)(const g16_rotary_args*, void*);
 typedef int (*cache_fn)(const g16_cache_args*, void*);
 typedef size_t (*attention8_size_fn)(const g16_attention8_args*);
@@ -901,6 +901,12 @@ static PyObject* fast_attention_decode8(PyObject* self, PyObject* const* args, P
   e.ks_seq = ks.stride[0], e.ks_token = ks.stride[1], e.ks_head = ks.stride[2];
   e.vs_seq = vs.stride[0], e.vs_token = vs.stride[1], e.vs_head = vs.stride[2];
   const size_t bytes = g_attention8_size(&e);
+  if (bytes > 0) {  /* (a graph has a workspace of its own) */
+    PyObject* capturing = PyObject_CallNoArgs(g_capturing);
+    const int plain = capturing == Py_False;
+    Py_XDECREF(capturing);
+    if (!plain) return none_clear();
+  }
   if (raw_stream(q.device, &stream) || (bytes > 0 && scratch(q.device, stream, bytes, &a->workspace))) return none_clear();
   if (bytes > 0 && a->workspace == NULL) Py_RETURN_NONE;
   a->workspace_bytes = (int64_t)bytes;
@@ -923,12 +929,12 @@ static PyObject* fast_attention_decode8(PyObject* self, PyObject* const* args, P
  * -1, scratch(device, stream, bytes) -> pointer, route (see product_route), [addresses of
  * g16_attention_workspace_bytes, g16_attention, g16_attention_decode_workspace_bytes, g16_attention_decode,
  * g16_mm_t_raw, g16_mm_t_direct, g16_lora_workspace_bytes, g16_lora_shrink, g16_lora_expand, g16_rotary, g16_cache_write,
- * g16_cache_read, g16_attention_decode8_workspace_bytes, g16_attention_decode8], int8, float8_e4m3fn) */
+ * g16_cache_read, g16_attention_decode8_workspace_bytes, g16_attention_decode8], int8, float8_e4m3fn, capturing()) */
 enum { kEntryPoints = 14 };
 static PyObject* fast_bind_torch(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
   (void)self;
   void* fn[kEntryPoints];
-  if (check_nargs("bind_torch", nargs, 11)) return NULL;
+  if (check_nargs("bind_torch", nargs, 12)) return NULL;
   for (int i = 0; i < kEntryPoints; ++i) {
     PyObject* o = PySequence_GetItem(args[8], i);
     const int bad = o == NULL || as_ptr(o, &fn[i]) || check_bound(fn[i]);
@@ -949,8 +955,8 @@ static PyObject* fast_bind_torch(PyObject* self, PyObject* const* args, Py_ssize
   g_cache_read = (cache_fn)fn[11];
   g_attention8_size = (attention8_size_fn)fn[12];
   g_attention8 = (attention8_fn)fn[13];
-  PyObject** to[11] = {&g_f16, &g_f32, &g_i32, &g_raw_stream, &g_grad_enabled, &g_ready, &g_scratch, &g_route, NULL, &g_i8, &g_e4m3};
-  for (int i = 0; i < 11; ++i) {
+  PyObject** to[12] = {&g_f16, &g_f32, &g_i32, &g_raw_stream, &g_grad_enabled, &g_ready, &g_scratch, &g_route, NULL, &g_i8, &g_e4m3, &g_capturing};
+  for (int i = 0; i < 12; ++i) {
     if (to[i] == NULL) continue;
     Py_INCREF(args[i]);
     Py_XSETREF(*to[i], args[i]);

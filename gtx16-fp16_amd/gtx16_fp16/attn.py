@@ -39,12 +39,16 @@ def _entry_points(name: str) -> tuple[int, int]:
     return e
 
 
-def _call(name: str, head: bytes, dev: torch.device) -> None:
+def _call(name: str, head: bytes, dev: torch.device, apart: bool = False) -> None:
+    # apart: a graph's call has a workspace of the graph's own memory, and so graphs captured on one stream may run at once
     fast = _clib.fast()
     size, fn = _entry_points(name)
     stream = stream_handle(dev.index or 0)
     nbytes = fast.args_size(size, head)
-    ws = scratch_buffer(dev, stream, nbytes) if nbytes else None
+    if apart and nbytes and torch.cuda.is_current_stream_capturing():
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    else:
+        ws = scratch_buffer(dev, stream, nbytes) if nbytes else None
     status = fast.args_call(fn, head, None if ws is None else ws.data_ptr(), nbytes, stream)
     if status != 0:
         _clib.check(status, name)
@@ -286,5 +290,5 @@ def _decode8(q, k_cache, v_cache, lengths, pages, shared_k, shared_v, scale, sof
           + _ARGS.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _ptr(sk), _ptr(sv), out.data_ptr(), 0, 0, 0, lengths.data_ptr(),
                        _ptr(pages) if capacity else 0, _ptr(slopes), q.stride(0), 0, q.stride(1), *k_cache.stride()[:3], *v_cache.stride()[:3],
                        *shared_strides, seqs, 1, capacity, hq, hkv, d, shared, 0, page, max_pages, k_cache.shape[0],
-                       1 if size == 4 else 0, _sm_count(dev), scale, softcap, 0), dev)
+                       1 if size == 4 else 0, _sm_count(dev), scale, softcap, 0), dev, True)
     return out

@@ -73,6 +73,7 @@ def direct():
     if _bound is None:
         fast = _clib.fast()
         fast.bind_torch(torch.float16, torch.float32, torch.int32, torch._C._cuda_getCurrentRawStream, torch.is_grad_enabled, _ready,
-                        _scratch_ptr, _route, [_clib.address(n) for n in _ENTRY_POINTS], torch.int8, torch.float8_e4m3fn)
+                        _scratch_ptr, _route, [_clib.address(n) for n in _ENTRY_POINTS], torch.int8, torch.float8_e4m3fn,
+                        torch.cuda.is_current_stream_capturing)
         _bound = fast
     return _bound

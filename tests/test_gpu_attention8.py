@@ -227,6 +227,27 @@ def test_two_streams_and_graphs(cuda):
             assert torch.equal(y, eager)
 
 
+def test_graphs_of_one_stream_at_once(cuda):
+    # two graphs captured on one stream, replayed on two: neither uses the other's workspace
+    cases = [case(cuda, F16, "int8", [3000, 1500, 40 + i], 8, 2, 128, page=16, shared=200, spoil=False) for i in range(2)]
+    expect = [g.attention_decode(*args, **kw) for args, kw, _ in cases]
+    streams, graphs, outs = [torch.cuda.Stream() for _ in range(2)], [], []
+    torch.cuda.synchronize()
+    for args, kw, _ in cases:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=streams[0]):
+            outs.append([g.attention_decode(*args, **kw) for _ in range(8)])
+    for _ in range(5):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for ys, y in zip(outs, expect):
+            assert all(torch.equal(x, y) for x in ys)
+            for x in ys:
+                x.zero_()
+
+
 def test_refusals(cuda):
     (q, kc, vc, lengths), kw, _ = case(cuda, F16, "int8", [20, 30], 4, 2, 64, page=16, shared=5)
     args = dict(q=q, k=kc, v=vc, lengths=lengths)
