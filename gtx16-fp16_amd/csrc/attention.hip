@@ -1453,7 +1453,7 @@ Plan8 plan_decode8(const g16_attention_args& a) {
   r.shares = a.seqs;
   if (r.split) {
     // as many as run at once, the same number for every XCD
-    const int64_t each = static_cast<int64_t>(cus_of(a)) / kXcds * waves_of8(a.is_f32 != 0, dp, rows_of8(group), a.d == dp) / heads;
+    const int64_t each = static_cast<int64_t>(cus_of(a)) / kXcds * waves_of8(a.is_f32 != 0, dp, rows_of8(group)) / heads;
     r.shares = static_cast<int>(each < 1 ? kXcds : each * kXcds);
   }
   const bool join = r.shared.stiles > 0 || r.split;

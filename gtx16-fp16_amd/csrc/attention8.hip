@@ -65,7 +65,7 @@ __global__ __launch_bounds__(kThreads) void decode8_join_kernel(Params p, Params
 }
 
 template <typename T, int DP, int CODE, int RQ, bool FULL>
-__global__ __launch_bounds__(kThreads, waves_of8(sizeof(T) == 4, DP, RQ, FULL)) void decode8_kernel(Params p, Params8 e) {
+__global__ __launch_bounds__(kThreads, waves_of8(sizeof(T) == 4, DP, RQ)) void decode8_kernel(Params p, Params8 e) {
   __shared__ Lds8<T, DP, RQ> lds;
   own8_workgroup<T, DP, CODE, RQ, FULL>(p, e, static_cast<int>(blockIdx.x), lds);
 }

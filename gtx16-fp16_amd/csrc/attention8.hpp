@@ -29,10 +29,12 @@ struct Params8 {
 
 // Query rows that a workgroup has room for.
 constexpr int rows_of8(int group) { return group == 1 ? 1 : group <= 4 ? 4 : group <= 8 ? 8 : group <= 16 ? 16 : 32; }
-// Workgroups on a CU that the registers are held to.
-constexpr int waves_of8(bool f32, int dp, int rows, bool full) {
+// Workgroups on a CU that the registers are held to: as many as leave a tile's keys and values in registers. (One more for heads of
+// 128, and some are in scratch memory: 106 us where two take 87, 40 requests of up to 8192 e4m3 keys. For 12 heads of 64 and one
+// query row four take 57.7 us, three 56.6, five 88.6: 96 requests of up to 2048.)
+constexpr int waves_of8(bool f32, int dp, int rows) {
   if (rows == 32) return dp == 64 ? 2 : 1;
-  return f32 || dp == 128 || rows == 16 ? 2 : rows == 1 && full ? 4 : 3;
+  return f32 || dp == 128 || rows == 16 ? 2 : 3;
 }
 
 inline unsigned workgroups_of8(const Params& p, const Params8& e) {
