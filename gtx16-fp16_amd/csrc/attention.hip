@@ -1129,7 +1129,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(Params p) {
 
 // The shared keys for few rows and, over a cache of 8 bits, the own ones in one launch: one after the other, each would leave the
 // card half empty (16 requests of up to 1500 in int8 after 2048, 8 heads of 128: 36 us, so 31).
-template <int DP, int CODE, int RQ>
+template <int DP, int CODE, int RQ, int HEADS>
 __global__ __launch_bounds__(kThreads, 2) void decode_both8_kernel(Params p, Params8 e) {
   __shared__ union Lds {
     Lds8<_Float16, DP, RQ> own;
@@ -1140,7 +1140,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_both8_kernel(Params p, Par
   } lds;
   const int nshared = p.stiles * p.ssplits * p.hkv;
   if (static_cast<int>(blockIdx.x) < nshared) shared_workgroup<_Float16, DP, true>(p, static_cast<int>(blockIdx.x), lds.shared.tiles, lds.shared.joint, nullptr);
-  else own8_workgroup<_Float16, DP, CODE, RQ, true>(p, e, static_cast<int>(blockIdx.x) - nshared, lds.own);
+  else own8_workgroup<_Float16, DP, CODE, RQ, true, HEADS>(p, e, static_cast<int>(blockIdx.x) - nshared, lds.own);
 }
 
 template <typename T, int DP>
@@ -1439,7 +1439,7 @@ int check8(const g16_attention8_args& e) {
 // The own keys' part of the plan for a cache in 8 bits (see attention8.hip), and what the workspace has to hold.
 struct Plan8 {
   DecodePlan shared;
-  int shares;
+  int heads, shares;
   bool split;
   size_t table;         // floats of the requests' table, before the slots
   size_t first, bytes;  // floats before the own keys' slots; bytes in all
@@ -1451,10 +1451,18 @@ Plan8 plan_decode8(const g16_attention_args& a) {
   const int64_t heads = static_cast<int64_t>(r.shared.otiles) * a.hkv;
   r.split = a.k_len > kWhole8 * kTile8;
   r.shares = a.seqs;
+  r.heads = 1;
   if (r.split) {
     // as many as run at once, the same number for every XCD
-    const int64_t each = static_cast<int64_t>(cus_of(a)) / kXcds * waves_of8(a.is_f32 != 0, dp, rows_of8(group)) / heads;
-    r.shares = static_cast<int>(each < 1 ? kXcds : each * kXcds);
+    auto shares = [&](int together) {
+      const int64_t each = static_cast<int64_t>(cus_of(a)) / kXcds * waves_of8(a.is_f32 != 0, dp, rows_of8(group)) * together / heads;
+      return static_cast<int>(each < 1 ? kXcds : each * kXcds);
+    };
+    // Where a token's heads lie next to each other in memory, a workgroup takes four of them together (see own8_workgroup), unless
+    // there are so few requests that their joins would take longer (one request of 8192 keys, 32 heads on 8, d 128, 256 parts of a row:
+    // 19.2 us, 17.3 by single heads; on 16 heads, 128 parts: 18.4 and 19.0; 64 of up to 700: 24.4 and 30.9).
+    if (a.hkv % kHeads8 == 0 && rows_of8(group) <= kRowsOfHeads8 && a.d == dp && a.k_token > a.k_head && shares(kHeads8) <= 128LL * a.seqs) r.heads = kHeads8;
+    r.shares = shares(r.heads);
   }
   const bool join = r.shared.stiles > 0 || r.split;
   r.table = join ? (static_cast<size_t>(a.seqs) * sizeof(Slots) + 15) / 16 * 4 : 0;
@@ -1468,12 +1476,16 @@ Plan8 plan_decode8(const g16_attention_args& a) {
 bool both8(const g16_attention_args& a, const Plan8& plan) {
   return plan.shared.stiles > 0 && plan.shared.skeys && !a.is_f32 && (a.d == 64 || a.d == 128) && a.hq / a.hkv <= 8;
 }
-template <int DP, int CODE>
+template <int DP, int CODE, int HEADS>
 int run_both8(const Params& p, const Params8& e, hipStream_t stream) {
   const dim3 grid(static_cast<unsigned>(p.stiles) * p.ssplits * p.hkv + workgroups_of8(p, e));
-  return p.group == 1   ? launch(decode_both8_kernel<DP, CODE, 1>, grid, dim3(kThreads), stream, p, e)
-         : p.group <= 4 ? launch(decode_both8_kernel<DP, CODE, 4>, grid, dim3(kThreads), stream, p, e)
-                        : launch(decode_both8_kernel<DP, CODE, 8>, grid, dim3(kThreads), stream, p, e);
+  return p.group == 1   ? launch(decode_both8_kernel<DP, CODE, 1, HEADS>, grid, dim3(kThreads), stream, p, e)
+         : p.group <= 4 ? launch(decode_both8_kernel<DP, CODE, 4, HEADS>, grid, dim3(kThreads), stream, p, e)
+                        : launch(decode_both8_kernel<DP, CODE, 8, HEADS>, grid, dim3(kThreads), stream, p, e);
+}
+template <int DP, int CODE>
+int run_both8(const Params& p, const Params8& e, hipStream_t stream) {
+  return e.heads == 1 ? run_both8<DP, CODE, 1>(p, e, stream) : run_both8<DP, CODE, kHeads8>(p, e, stream);
 }
 
 template <typename T, int DP>
@@ -1577,7 +1589,7 @@ extern "C" int g16_attention_decode8(const g16_attention8_args* args, void* stre
   p.v_seq = a.v_seq;
   p.v_head = a.v_head;
   const Params8 own = {e.k_scale, e.v_scale, e.ks_seq, e.ks_head, e.ks_token, e.vs_seq, e.vs_head, e.vs_token, a.k_token, a.v_token,
-                       divide_by(a.page > 0 ? static_cast<uint32_t>(a.page) : 1u), plan.shares, plan.split, plan.shared.skeys ? kKeyTile : kRowTile, !both8(a, plan), plan.first - plan.table,
+                       divide_by(a.page > 0 ? static_cast<uint32_t>(a.page) : 1u), plan.heads, plan.shares, plan.split, plan.shared.skeys ? kKeyTile : kRowTile, !both8(a, plan), plan.first - plan.table,
                        plan.bytes > 0 ? static_cast<Slots*>(a.workspace) : nullptr};
   hipStream_t s = static_cast<hipStream_t>(stream);
   int rc = 0;

@@ -64,16 +64,19 @@ __global__ __launch_bounds__(kThreads) void decode8_join_kernel(Params p, Params
   }
 }
 
-template <typename T, int DP, int CODE, int RQ, bool FULL>
+template <typename T, int DP, int CODE, int RQ, bool FULL, int HEADS>
 __global__ __launch_bounds__(kThreads, waves_of8(sizeof(T) == 4, DP, RQ)) void decode8_kernel(Params p, Params8 e) {
   __shared__ Lds8<T, DP, RQ> lds;
-  own8_workgroup<T, DP, CODE, RQ, FULL>(p, e, static_cast<int>(blockIdx.x), lds);
+  own8_workgroup<T, DP, CODE, RQ, FULL, HEADS>(p, e, static_cast<int>(blockIdx.x), lds);
 }
 
 template <typename T, int DP, int CODE, int RQ>
 int run(const Params& p, const Params8& e, dim3 grid, hipStream_t stream) {
-  return p.d == DP ? launch(decode8_kernel<T, DP, CODE, RQ, true>, grid, dim3(kThreads), stream, p, e)
-                   : launch(decode8_kernel<T, DP, CODE, RQ, false>, grid, dim3(kThreads), stream, p, e);
+  if constexpr (RQ <= kRowsOfHeads8) {
+    if (e.heads == kHeads8) return launch(decode8_kernel<T, DP, CODE, RQ, true, kHeads8>, grid, dim3(kThreads), stream, p, e);
+  }
+  return p.d == DP ? launch(decode8_kernel<T, DP, CODE, RQ, true, 1>, grid, dim3(kThreads), stream, p, e)
+                   : launch(decode8_kernel<T, DP, CODE, RQ, false, 1>, grid, dim3(kThreads), stream, p, e);
 }
 template <typename T, int DP>
 int join(const Params& p, const Params8& e, hipStream_t stream) {

@@ -8,6 +8,8 @@ namespace g16 {
 constexpr int kXcds = 8;
 constexpr int kTile8 = 64;  // keys of a tile
 constexpr int kWhole8 = 8;  // tiles of a request whose keys are never split
+constexpr int kHeads8 = 4;        // key heads that a workgroup may take together,
+constexpr int kRowsOfHeads8 = 8;  // of how many query rows at most
 
 // A request's slots: the first one's number, and how many there are.
 struct Slots {
@@ -19,6 +21,7 @@ struct Params8 {
   int64_t ks_seq, ks_head, ks_tok, vs_seq, vs_head, vs_tok;  // elements
   int64_t k_tok, v_tok;                                      // bytes
   Divide page;
+  int heads;     // key heads of a workgroup, 1 or kHeads8
   int shares;    // at most
   bool split;    // shares of equal length; else one for each request
   int srt;       // rows of the shared keys' slots
@@ -38,7 +41,7 @@ constexpr int waves_of8(bool f32, int dp, int rows) {
 }
 
 inline unsigned workgroups_of8(const Params& p, const Params8& e) {
-  return static_cast<unsigned>(e.shares >= kXcds ? ceil_div(e.shares, kXcds) * kXcds : e.shares) * p.otiles * p.hkv;
+  return static_cast<unsigned>(e.shares >= kXcds ? ceil_div(e.shares, kXcds) * kXcds : e.shares) * p.otiles * (p.hkv / e.heads);
 }
 
 // Enqueues the products of the requests' own keys, where they are apart, and the joins.

@@ -3,7 +3,8 @@
 //
 // All requests' keys, in tiles of 64 one request after another, are dealt in shares of equal length, as many as run on the card at
 // once: whatever the lengths, all workgroups end together (see Deal for few keys). A workgroup has the query rows of one key head and a
-// share's tiles, a request's after another's; its four wavefronts take a tile in turn, straight from memory into registers:
+// share's tiles, a request's after another's; its four wavefronts take a tile in turn (or a head each, see own8_workgroup),
+// straight from memory into registers:
 //   * S = Q K^T in 16x16x32 blocks of 16 keys, lane l's key l % 16, by way of LDS. A step's values of a lane are half of a 16-byte
 //     piece, in another order than in memory, the queries' too.
 //   * With few query rows the blocks' 16 rows are as many copies of them, and the lanes of row group l / 16 keep those of
@@ -156,14 +157,14 @@ __device__ inline int all_tiles(const Params& p, const Run64& head) {
 // How all requests' tiles are dealt. Long ones in shares of equal length, whatever the requests: the first `more` shares
 // have each + 1, the others each. Where a share would have few tiles, its time is that of the waits for one after another, not of its bytes,
 // and a second request's would come on top: every request then has its own pieces, of `chunk` tiles, one for each
-// wavefront or two (16 requests of up to 1500 after 2048, 8 heads of 128: 42 us by shares,
-// 36 so).
+// wavefront or two (16 requests of up to 1500 after 2048, 8 heads of 128, HEADS = 1: 42 us by shares, 36 so).
 struct Deal {
   int shares = 1, each = 1, more = 0, chunk = 0;
   __device__ Deal() {}
   __device__ Deal(const Params& p, const Params8& e, int total) {
-    const int four = static_cast<int>((static_cast<uint32_t>(total) + 2u * p.seqs) / (4u * e.shares)) + 1;
-    chunk = four <= 2 ? 4 * four : 0;
+    const uint32_t waves = 4 / e.heads;  // wavefronts that a head has
+    const int each_one = static_cast<int>((static_cast<uint32_t>(total) + 2u * p.seqs) / (waves * e.shares)) + 1;
+    chunk = each_one <= 2 ? static_cast<int>(waves) * each_one : 0;
     shares = e.shares;
     each = static_cast<int>(static_cast<uint32_t>(total) / static_cast<uint32_t>(shares));
     more = total - each * shares;
@@ -242,8 +243,12 @@ struct Lds8 {
   float joint[2][4][S::R];
 };
 
-// Workgroup `block` of those for the requests' own keys.
-template <typename T, int DP, int CODE, int RQ, bool FULL>
+// Workgroup `block` of those for the requests' own keys. HEADS: 1, a key head, whose tiles the wavefronts take in turn; or 4, one for
+// each wavefront, which has all of the share's tiles. What a workgroup reads of a token is then four heads' codes in
+// a row, and their scales: 40 requests of 8192 e4m3 keys of 8 heads of 128 take 138 us (5.0 TB/s), so 160 with HEADS = 1;
+// 96 of up to 2048 of 12 heads of 64 51.5 and 59.2. No wavefront waits for another, there is nothing to join in LDS, and a
+// row has four times as many parts. A cache that is ordered by heads has a head's codes in a row, and HEADS = 1.
+template <typename T, int DP, int CODE, int RQ, bool FULL, int HEADS>
 __device__ inline void own8_workgroup(const Params& p, const Params8& e, int block, Lds8<T, DP, RQ>& shared) {
   using S = Shape8<T, DP, RQ>;
   constexpr int VB = DP / 16, VW = DP / 64;  // values of a lane, and blocks of the second product; dwords of a lane's values
@@ -258,12 +263,12 @@ __device__ inline void own8_workgroup(const Params& p, const Params8& e, int blo
   // (96 requests of up to 2048, 12 heads of 64: 76 us, and by this alone 63).
   int lin = block;
   if (e.shares >= kXcds) {
-    const int per = p.otiles * p.hkv, i = lin / kXcds, share = i / per * kXcds + lin % kXcds;
+    const int per = p.otiles * (p.hkv / HEADS), i = lin / kXcds, share = i / per * kXcds + lin % kXcds;
     if (share >= e.shares) return;
     lin = share * per + i % per;
   }
-  const int kv = lin % p.hkv;
-  lin /= p.hkv;
+  const int kv = HEADS == 1 ? lin % p.hkv : lin % (p.hkv / HEADS) * HEADS + wave;
+  lin /= p.hkv / HEADS;
   const int rt = lin % p.otiles, share = lin / p.otiles;
   Share has;
   Deal deal;
@@ -306,7 +311,7 @@ __device__ inline void own8_workgroup(const Params& p, const Params8& e, int blo
     // A key is CH pieces of 16 bytes. A load takes whole keys, in the order in which they lie in memory; LDS turns them
     // into the product's order, where lane l has piece 4 c + l / 16 of key l % 16: pieces are at places that put those of 8 keys on
     // different banks. (Loaded in that order, a lane's piece next to another key's, 40 requests of 8192 e4m3 keys of 8 heads of 128
-    // take 166 us, so 161; ordered by heads 143 and 146.)
+    // take 166 us, so 161 (HEADS = 1); ordered by heads 143 and 146.)
     constexpr int CH = DP / 16, PER = 64 / CH, NK = CH;  // pieces of a key; keys of a load; loads of a tile
     auto place_of = [](int key, int piece) { return key * DP + ((piece ^ (CH == 8 ? key & 7 : (key >> 1) & 3)) << 4); };
     char* keys = lds + wave * (kKeys + kWeights);
@@ -356,8 +361,8 @@ __device__ inline void own8_workgroup(const Params& p, const Params8& e, int blo
       e.table[b] = s;
     }
 
-    int j0 = begin + kTile8 * wave;
-    constexpr int kStep = 4 * kTile8;
+    int j0 = begin + (HEADS == 1 ? kTile8 * wave : 0);
+    constexpr int kStep = 4 / HEADS * kTile8;
     if (j0 < end) {
       find(j0, page_of(j0));
       load_k();
@@ -587,8 +592,10 @@ __device__ inline void own8_workgroup(const Params& p, const Params8& e, int blo
     }
 
     // ---- join the four wavefronts: sums [wave][row][value] in LDS, then eight values a thread ----
-    __syncthreads();  // (other wavefronts' weights have been read)
-    float* so = reinterpret_cast<float*>(lds);
+    if constexpr (HEADS == 1) __syncthreads();  // (other wavefronts' weights have been read)
+    float* so = reinterpret_cast<float*>(HEADS == 1 ? lds : keys);
+    constexpr int kJoined = 4 / HEADS;
+    const int part0 = HEADS == 1 ? 0 : wave, so_wave = HEADS == 1 ? wave : 0;
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
 #pragma unroll
@@ -603,25 +610,26 @@ __device__ inline void own8_workgroup(const Params& p, const Params8& e, int blo
         for (int n4 = 0; n4 < 4; ++n4)  // row 4 g + n4 of every block: values (4 g + n4) VB + {0 .. VB - 1}
 #pragma unroll
           for (int i = 0; i < VB; i += 4)
-            *reinterpret_cast<float4v*>(&so[(wave * R + 16 * r + col) * DP + (4 * g + n4) * VB + i]) =
+            *reinterpret_cast<float4v*>(&so[(so_wave * R + 16 * r + col) * DP + (4 * g + n4) * VB + i]) =
                 float4v{o[r][i][n4], o[r][i + 1][n4], o[r][i + 2][n4], o[r][i + 3][n4]} * back;
       }
     }
-    __syncthreads();
+    if constexpr (HEADS == 1) __syncthreads();
+    else wave_order();
     Slot slot = {nullptr, orows};
     if (p.stiles > 0 || u0 > 0 || u1 < tiles)
       slot.at = p.part + e.first + ((static_cast<size_t>(at_slot) * p.otiles + rt) * p.hkv + kv) * slot_floats(orows, DP);
-    for (int item = tid; item < R * (DP / 8); item += kThreads) {
+    for (int item = HEADS == 1 ? tid : lane; item < R * (DP / 8); item += kThreads / HEADS) {
       const int r = item / (DP / 8), d0 = item % (DP / 8) * 8, row = rt * kKeyTile + r;
       if (row >= p.group) break;
-      float top = -__builtin_huge_valf(), f[4], total = 0.f;
+      float top = -__builtin_huge_valf(), f[kJoined], total = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) top = fmaxf(top, joint[0][i][r]);
+      for (int i = 0; i < kJoined; ++i) top = fmaxf(top, joint[0][part0 + i][r]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float mi = joint[0][i][r];
+      for (int i = 0; i < kJoined; ++i) {
+        const float mi = joint[0][part0 + i][r];
         f[i] = mi == top ? 1.f : __builtin_amdgcn_exp2f(mi - top);
-        total = fmaf(f[i], joint[1][i][r], total);
+        total = fmaf(f[i], joint[1][part0 + i][r], total);
       }
       const float inv = slot.at != nullptr ? 1.f : inverse(total);
       float x[8];
@@ -629,7 +637,7 @@ __device__ inline void own8_workgroup(const Params& p, const Params8& e, int blo
       for (int j = 0; j < 8; ++j) {
         x[j] = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[j] = fmaf(f[i], so[(i * R + r) * DP + d0 + j], x[j]);
+        for (int i = 0; i < kJoined; ++i) x[j] = fmaf(f[i], so[(i * R + r) * DP + d0 + j], x[j]);
         x[j] *= inv;
       }
       if (slot.at != nullptr) {
@@ -660,7 +668,8 @@ __device__ inline void own8_workgroup(const Params& p, const Params8& e, int blo
       at_slot = has.slot;
       ahead = has.ahead;
     }
-    __syncthreads();  // (the sums in LDS have been read)
+    if constexpr (HEADS == 1) __syncthreads();  // (the sums in LDS have been read)
+    else wave_order();
   }
 }
 

@@ -227,6 +227,20 @@ def test_two_streams_and_graphs(cuda):
             assert torch.equal(y, eager)
 
 
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("lengths,hq,hkv,d,kw", [
+    ([700, 0, 64, 1, 513, 65], 4, 4, 64, dict(page=16)), ([600, 1300, 63, 2], 32, 8, 128, dict(page=24, shared=70)),
+    ([1100, 0, 0, 5], 24, 12, 64, dict(softcap=20.0, biased=True)), ([900, 40], 64, 8, 128, dict(page=64, biased=True)),
+    ([640, 129, 31], 20, 4, 64, dict(shared=33, softcap=30.0)),
+    ([1500 - 31 * i for i in range(48)], 16, 16, 64, dict(page=16)), ([1200] * 23 + [0, 7], 8, 8, 128, {}),
+])
+def test_heads_next_to_each_other(cuda, dtype, code, lengths, hq, hkv, d, kw):
+    # past 512 keys four heads of a token go together, by pieces of few tiles or (many keys) by equal shares
+    args, kw, expect = case(cuda, dtype, code, lengths, hq, hkv, d, **kw)
+    check(g.attention_decode(*args, **kw), expect)
+
+
 def test_graphs_of_one_stream_at_once(cuda):
     # two graphs captured on one stream, replayed on two: neither uses the other's workspace
     cases = [case(cuda, F16, "int8", [3000, 1500, 40 + i], 8, 2, 128, page=16, shared=200, spoil=False) for i in range(2)]
