@@ -1460,7 +1460,8 @@ Plan8 plan_decode8(const g16_attention_args& a) {
     };
     // Where a token's heads lie next to each other in memory, a workgroup takes four of them together (see own8_workgroup), unless
     // there are so few requests that their joins would take longer (one request of 8192 keys, 32 heads on 8, d 128, 256 parts of a row:
-    // 19.2 us, 17.3 by single heads; on 16 heads, 128 parts: 18.4 and 19.0; 64 of up to 700: 24.4 and 30.9).
+    // 19.2 us, 17.3 by single heads; 16 heads on 16, 128 parts: 18.4 and 19.0, of 65536 70.0 and 77.1; two requests of 8192, 64 heads on 8,
+    // 128 parts: 23.8 and 21.3; 64 of up to 700, 32 heads on 8: 24.2 and 30.6).
     if (a.hkv % kHeads8 == 0 && rows_of8(group) <= kRowsOfHeads8 && a.d == dp && a.k_token > a.k_head && shares(kHeads8) <= 128LL * a.seqs) r.heads = kHeads8;
     r.shares = shares(r.heads);
   }

@@ -245,8 +245,8 @@ struct Lds8 {
 
 // Workgroup `block` of those for the requests' own keys. HEADS: 1, a key head, whose tiles the wavefronts take in turn; or 4, one for
 // each wavefront, which has all of the share's tiles. What a workgroup reads of a token is then four heads' codes in
-// a row, and their scales: 40 requests of 8192 e4m3 keys of 8 heads of 128 take 138 us (5.0 TB/s), so 160 with HEADS = 1;
-// 96 of up to 2048 of 12 heads of 64 51.5 and 59.2. No wavefront waits for another, there is nothing to join in LDS, and a
+// a row, and their scales: 40 requests of 8192 e4m3 keys, 32 heads on 8 of 128, take 138 us (5.0 TB/s), with HEADS = 1 160;
+// 96 of up to 2048, 12 heads of 64, 51.5 and 59.2. No wavefront waits for another, there is nothing to join in LDS, and a
 // row has four times as many parts. A cache that is ordered by heads has a head's codes in a row, and HEADS = 1.
 template <typename T, int DP, int CODE, int RQ, bool FULL, int HEADS>
 __device__ inline void own8_workgroup(const Params& p, const Params8& e, int block, Lds8<T, DP, RQ>& shared) {
