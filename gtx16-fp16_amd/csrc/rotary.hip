@@ -1,7 +1,7 @@
 // Rotary positions by one axis or several (g16_rotary; the formulas stand in g16.h).
 //
 // The pass reads and writes every value once and is bound by memory. A thread has V pairs of one row, takes their angles once
-// and turns the pairs of several of the row's heads by them: an angle costs about 25 instructions, of which seven in
+// and turns the pairs of several of the row's heads by them: an angle costs about 30 instructions, of which eleven in
 // 64 bits, a rotated pair four.
 #include "g16_common.hpp"
 
@@ -27,14 +27,21 @@ struct alignas(sizeof(T) * N > 16 ? 16 : sizeof(T) * N) Run {
   T v[N];
 };
 
-// cos and sin of pi / 2 times a number of quarter turns. Of the nearest whole number of them only the last two bits
-// matter; what is left, at most half of one, goes through polynomials fitted to sin(f pi / 2) / f and (cos(f pi / 2) - 1) / f^2
-// in f^2 by least squares, reweighted to even errors (largest 4e-9 and 7e-11; in fp32 1e-7 and 6e-8).
-__device__ inline void turn(double quarters, float& c, float& s) {
+// cos and sin of position * freq radians. Quarter turns for each position, freq * 2 / pi, are held as the sum of two doubles, and what the
+// position times the first has over a whole number of them is one fma's, without a product rounded before: 2^-54 of a quarter and
+// 2^-104 of the angle are lost, whatever the angle (with one double and a rounded product 2^-52 of it: 1e-7 radians from 2^29
+// on). Of the whole quarters only the last two bits matter; what is left, at most half of one, goes through polynomials
+// fitted to sin(f pi / 2) / f and (cos(f pi / 2) - 1) / f^2 in f^2 by least squares, reweighted to even errors (largest 4e-9 and 7e-11;
+// in fp32 1e-7 and 6e-8).
+__device__ inline void turn(double position, double freq, float& c, float& s) {
+  constexpr double k2OverPi = 0.63661977236758134308, k2OverPiRest = -3.935735335036497e-17;
+  const double rate = freq * k2OverPi, rate_rest = fma(freq, k2OverPiRest, fma(freq, k2OverPi, -rate));
   const double magic = 6755399441055744.0;  // 1.5 * 2^52: a sum with it has whole numbers' bits at its end
-  const double shifted = quarters + magic;
-  const uint32_t q = static_cast<uint32_t>(__double_as_longlong(shifted));
-  const float f = static_cast<float>(quarters - (shifted - magic)), u = f * f;
+  const double shifted = fma(position, rate, magic);
+  const double left = fma(position, rate_rest, fma(position, rate, -(shifted - magic)));
+  const double more = __builtin_rint(left);  // (the second double's part may add to a half: an eighth at 2^51)
+  const uint32_t q = static_cast<uint32_t>(__double_as_longlong(shifted)) + static_cast<uint32_t>(static_cast<int>(more));
+  const float f = static_cast<float>(left - more), u = f * f;
   float a = fmaf(u, -0.00460165785625577f, 0.07968003302812576f);
   a = fmaf(u, a, -0.6459634900093079f);
   a = fmaf(u, a, 1.5707963705062866f) * f;
@@ -74,7 +81,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(Params p) {
 #pragma unroll
       for (int a = 0; a < G16_ROTARY_MAX_AXES - 1; ++a) axis += i >= p.ends[a];
       const double position = p.positions[static_cast<uint64_t>(axis) * p.rows + row];
-      turn(position * (p.freqs[i] * 0.63661977236758134308), c[j], s[j]);  // 2 / pi
+      turn(position, p.freqs[i], c[j], s[j]);
     }
   }
   // Halves: V values from each of them; neighbours: 2 V values in a row. Those that stay are W in a row, as one such run or as two

@@ -37,8 +37,8 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, *, sec
     pairs in all) positions are [axes, ..one a row..]: pairs 0 .. sections[0] - 1 go by the first axis, the next
     sections[1] by the second, and so on (time, height and width of images and video).
 
-    Returns x's shape and type, contiguous. The angle is the exact product, reduced in 64 bits (far positions keep
-    their places; angles stay below 2^51); its cosine and sine, to 1e-7, and the rotation are fp32."""
+    Returns x's shape and type, contiguous. The angle is the exact product less whole turns (far positions keep their
+    places; angles stay below 2^51); its cosine and sine, to 1e-7, and the rotation are fp32."""
     if forward_ad._current_level >= 0:
         refuse_tangents("rotary", x, freqs)
     out = direct().rotary(x, positions, freqs, sections, interleaved)

@@ -416,8 +416,8 @@ int g16_attention_decode(const g16_attention_args* args, void* stream);
  * (x0, x1) = values i and i + pairs of the head, or (interleaved) 2 i and 2 i + 1; values from 2 * pairs on are
  * copied. rows = seqs * tokens, x [seqs, tokens, heads, d] by its strides, out contiguous; fp16 or fp32 (is_f32).
  * Pairs sections[0] .. go by the first axis, the next sections[1] by the second, and so on: up to
- * G16_ROTARY_MAX_AXES of them, pairs in all. The angle is the product of the two numbers as they are, below 2^51, reduced
- * in 64 bits; cosine, sine and the rotation are fp32.
+ * G16_ROTARY_MAX_AXES of them, pairs in all. The angle is the exact product of the two numbers, below 2^51, less whole turns;
+ * its cosine and sine (to 1e-7) and the rotation are fp32.
  *   d a multiple of 8, 2 * pairs <= d; strides in elements, multiples of 16 bytes. One launch.
  */
 #define G16_ROTARY_MAX_AXES 4
