@@ -795,7 +795,7 @@ static int slots_ok(PyObject* o, int device, tensor_t* t) {
 }
 
 /* cache_write(k, v, k_cache, v_cache, k_scale, v_scale, slots): true where it is done */
-static const int kGradWrite[4] = {0, 1, 4, 5};
+static const int kGradWrite[6] = {0, 1, 2, 3, 4, 5};
 static PyObject* fast_cache_write(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
   (void)self;
   tensor_t k, v, kc, vc, ks, vs, slots;
@@ -806,7 +806,7 @@ static PyObject* fast_cache_write(PyObject* self, PyObject* const* args, Py_ssiz
   if (g_ready == NULL) Py_RETURN_NONE;
   const int code = cache_ok(args + 2, &kc, &vc, &ks, &vs);
   if (code == 0 || read_tensor(args[0], &k) || read_tensor(args[1], &v) || k.nd != 3 || v.nd != 3 || (k.dtype != g_f16 && k.dtype != g_f32) ||
-      v.dtype != k.dtype || k.device != kc.device || v.device != kc.device || !slots_ok(args[6], kc.device, &slots) || wants_grad(args, kGradWrite, 4))
+      v.dtype != k.dtype || k.device != kc.device || v.device != kc.device || !slots_ok(args[6], kc.device, &slots) || wants_grad(args, kGradWrite, 6))
     return none_clear();
   const int size = k.dtype == g_f32 ? 4 : 2;
   if (k.shape[0] != slots.shape[0] || k.shape[1] != kc.shape[2] || k.shape[2] != kc.shape[3] || memcmp(k.shape, v.shape, sizeof(int64_t) * 3) != 0 ||
@@ -828,7 +828,7 @@ static PyObject* fast_cache_write(PyObject* self, PyObject* const* args, Py_ssiz
 }
 
 /* cache_read(k_cache, v_cache, k_scale, v_scale, slots, out_dtype) -> (k, v) */
-static const int kGradRead[2] = {2, 3};
+static const int kGradRead[4] = {0, 1, 2, 3};
 static PyObject* fast_cache_read(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
   (void)self;
   tensor_t kc, vc, ks, vs, slots;
@@ -839,7 +839,7 @@ static PyObject* fast_cache_read(PyObject* self, PyObject* const* args, Py_ssize
   if (check_nargs("cache_read", nargs, 6)) return NULL;
   if (g_ready == NULL) Py_RETURN_NONE;
   const int code = cache_ok(args, &kc, &vc, &ks, &vs);
-  if (code == 0 || !slots_ok(args[4], kc.device, &slots) || (args[5] != g_f16 && args[5] != g_f32) || wants_grad(args, kGradRead, 2) ||
+  if (code == 0 || !slots_ok(args[4], kc.device, &slots) || (args[5] != g_f16 && args[5] != g_f32) || wants_grad(args, kGradRead, 4) ||
       raw_stream(kc.device, &stream))
     return none_clear();
   cache_args(&a, &kc, &vc, &ks, &vs, &slots, code, args[5] == g_f32);
@@ -860,7 +860,7 @@ static PyObject* fast_cache_read(PyObject* self, PyObject* const* args, Py_ssize
 }
 
 /* attention_decode8(q, k_cache, v_cache, lengths, pages, shared_k, shared_v, scale, softcap, slopes, k_scale, v_scale) */
-static const int kGradDecode8[6] = {0, 5, 6, 9, 10, 11};
+static const int kGradDecode8[8] = {0, 1, 2, 5, 6, 9, 10, 11};
 static PyObject* fast_attention_decode8(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
   (void)self;
   tensor_t q, kc, vc, ks, vs, t;
@@ -876,7 +876,7 @@ static PyObject* fast_attention_decode8(PyObject* self, PyObject* const* args, P
   e.code = cache_ok(cache, &kc, &vc, &ks, &vs);
   if (e.code == 0 || read_tensor(args[0], &q) || q.nd != 3 || (q.dtype != g_f16 && q.dtype != g_f32) || q.device != kc.device || q.shape[0] <= 0 ||
       !fits(q.shape[0]) || q.shape[1] <= 0 || !fits(q.shape[1]) || q.shape[1] % kc.shape[2] != 0 || q.shape[2] != kc.shape[3] ||
-      !rows_ok(&q, q.dtype == g_f32 ? 4 : 2, 0, 0) || wants_grad(args, kGradDecode8, 6) ||
+      !rows_ok(&q, q.dtype == g_f32 ? 4 : 2, 0, 0) || wants_grad(args, kGradDecode8, 8) ||
       vector(args[3], g_i32, q.shape[0], q.device, (const void**)&a->lengths) || a->lengths == NULL)
     return none_clear();
   a->is_f32 = q.dtype == g_f32, a->num_cus = device_cus(q.device);

@@ -274,7 +274,7 @@ def _decode8(q, k_cache, v_cache, lengths, pages, shared_k, shared_v, scale, sof
     seqs, hq = q.shape[:2]
     if hq and (not hkv or hq % hkv):
         raise ValueError(f"{name}: {hq} query heads do not share {hkv} key heads evenly")
-    refuse_gradients(name, q, shared_k, shared_v, slopes, k_scale, v_scale)
+    refuse_gradients(name, q, k_cache, v_cache, shared_k, shared_v, slopes, k_scale, v_scale)
     lengths = _ints(name, lengths, (seqs,), dev, "lengths")
     pages, page, max_pages, capacity = _pages(pages, k_cache, seqs)
     scale, softcap = _numbers(name, scale, softcap, d)

@@ -73,7 +73,7 @@ def cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache
     2^-96 are written as zeros; a head with a value that is not finite reads as NaN throughout."""
     name = "cache_write"
     if forward_ad._current_level >= 0:
-        refuse_tangents(name, k, v, k_scale, v_scale)
+        refuse_tangents(name, k, v, k_cache, v_cache, k_scale, v_scale)
     if direct().cache_write(k, v, k_cache, v_cache, k_scale, v_scale, slots):
         return
     dev = k.device
@@ -87,7 +87,7 @@ def cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache
         if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
             raise ValueError(f"{name}: the cache's tokens must have memory of their own")
     slots = _ints(name, slots, k.shape[:-2], dev, "slots").reshape(-1)
-    refuse_gradients(name, k, v, k_scale, v_scale)
+    refuse_gradients(name, k, v, k_cache, v_cache, k_scale, v_scale)
     if k.numel() == 0 or k_cache.numel() == 0:
         return
     size = k.element_size()
@@ -102,7 +102,7 @@ def cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tens
     as zeros. ``attention`` takes them as the keys of a prompt's earlier chunks."""
     name = "cache_read"
     if forward_ad._current_level >= 0:
-        refuse_tangents(name, k_scale, v_scale)
+        refuse_tangents(name, k_cache, v_cache, k_scale, v_scale)
     both = direct().cache_read(k_cache, v_cache, k_scale, v_scale, slots, out_dtype)
     if both is not None:
         return both
@@ -113,7 +113,7 @@ def cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tens
         raise ValueError(f"{name}: the cache must be on a gfx950 device")
     code = check_cache(name, k_cache, v_cache, k_scale, v_scale)
     slots = _ints(name, slots, slots.shape, dev, "slots")
-    refuse_gradients(name, k_scale, v_scale)
+    refuse_gradients(name, k_cache, v_cache, k_scale, v_scale)
     k, v = (torch.empty(*slots.shape, *k_cache.shape[2:], dtype=out_dtype, device=dev) for _ in "kv")
     if k.numel() != 0:
         hkv, d = k_cache.shape[2:]

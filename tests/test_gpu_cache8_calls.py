@@ -1,0 +1,36 @@
+"""A cache of 8 bits on the GPU as autograd sees it."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import gtx16_fp16 as g
+from _cache8 import empty
+
+pytestmark = pytest.mark.gpu
+
+
+def rows(n, heads, d, cuda):
+    return [torch.randn(n, heads, d, device=cuda).half() for _ in "kv"]
+
+
+@pytest.mark.parametrize("which", range(4))
+@pytest.mark.parametrize("usual", [True, False])
+def test_a_gradient_wanted_of_the_cache_is_refused(cuda, which, usual):
+    # e4m3 codes are floating numbers, of which autograd takes a gradient; `usual`: what the extension looks at, else the Python functions
+    cache = empty(3, 16, 2, 64, "e4m3", cuda)
+    k, v = rows(3, 2, 64, cuda)
+    slots, lengths = torch.arange(3, dtype=torch.int32, device=cuda), torch.ones(3, dtype=torch.int32, device=cuda)
+    q = torch.randn(3, 4, 64, device=cuda).half()
+    if not usual:
+        k, v, slots, lengths = k[None], v[None], slots[None], lengths.repeat(2)[::2]
+    calls = (lambda: g.cache_write(k, v, *cache, slots), lambda: g.cache_read(*cache, slots),
+             lambda: g.attention_decode(q, cache[0], cache[1], lengths, k_scale=cache[2], v_scale=cache[3]))
+    g.cache_write(k, v, *cache, slots)
+    cache[which].requires_grad_()
+    for call in calls:
+        with pytest.raises(RuntimeError, match="no gradient"):
+            call()
+    with torch.no_grad():
+        for call in calls:
+            call()
