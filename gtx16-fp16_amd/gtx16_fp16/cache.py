@@ -10,6 +10,7 @@ import struct
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from . import _clib
 from .attn import MAX_HEAD_DIM, _ints, _rows
@@ -65,7 +66,8 @@ def cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache
     [pages, page, heads] (a padded cache is [requests, capacity, heads, d]); slots int32, one a token, k's shape without
     the last two dimensions: token t of page p is slot p * page + t. A token whose slot is negative or past the cache is not
     written; of several with one slot the last one is. d a multiple of 8 up to 128; strides are free, but a head's codes
-    are contiguous and start at a multiple of 8 bytes. Nothing else of the cache changes.
+    are contiguous and start at a multiple of 8 bytes. Nothing else of the cache changes. To autograd all four tensors are
+    changed in place.
 
     Every token's head has a scale of its own. int8: scale = max|x| / 127, codes nearest to x * (127 / max|x|), ties to
     even. e4m3: the smallest power of two that brings the values to at most 448 (another scale would gain a
@@ -75,6 +77,7 @@ def cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache
     if forward_ad._current_level >= 0:
         refuse_tangents(name, k, v, k_cache, v_cache, k_scale, v_scale)
     if direct().cache_write(k, v, k_cache, v_cache, k_scale, v_scale, slots):
+        increment_version((k_cache, v_cache, k_scale, v_scale))  # (written in place, as autograd has to know)
         return
     dev = k.device
     if not (k.is_cuda and k.dtype in (torch.float16, torch.float32) and v.dtype == k.dtype and v.device == dev and _is_target(dev.index or 0)):
@@ -93,6 +96,7 @@ def cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache
     size = k.element_size()
     k, v = (_rows(t.reshape(-1, hkv, d), size, d, False) for t in (k, v))
     _call(name, k, v, k_cache, v_cache, k_scale, v_scale, slots, code)
+    increment_version((k_cache, v_cache, k_scale, v_scale))
 
 
 def cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, slots: torch.Tensor, *,

@@ -34,3 +34,38 @@ def test_a_gradient_wanted_of_the_cache_is_refused(cuda, which, usual):
     with torch.no_grad():
         for call in calls:
             call()
+
+
+@pytest.mark.parametrize("usual", [True, False])
+def test_a_write_is_seen_by_autograd(cuda, usual):
+    # what torch's own operations in place do: a tensor that backward needs as it was is missed
+    cache = empty(2, 16, 2, 64, "int8", cuda, fill=0)
+    k, v = rows(3, 2, 64, cuda)
+    slots = torch.arange(3, dtype=torch.int32, device=cuda)
+    if not usual:
+        k, v, slots = k[None], v[None], slots[None]
+    before = [t._version for t in cache]
+    w = torch.ones_like(cache[2], requires_grad=True)
+    loss = (w * cache[2]).sum()
+    view = cache[3][0]
+    g.cache_write(k, v, *cache, slots)
+    assert all(t._version > n for t, n in zip(cache, before)) and view._version == cache[3]._version
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    g.cache_read(*cache, slots)
+    after = [t._version for t in cache]
+    g.attention_decode(torch.randn(2, 4, 64, device=cuda).half(), cache[0], cache[1], torch.ones(2, dtype=torch.int32, device=cuda), k_scale=cache[2],
+                       v_scale=cache[3])
+    assert [t._version for t in cache] == after  # (nobody else changes them)
+
+
+def test_a_cache_made_in_inference_mode(cuda):
+    with torch.inference_mode():
+        cache = empty(2, 16, 2, 64, "int8", cuda, fill=0)
+    k, v = rows(3, 2, 64, cuda)
+    slots = torch.arange(3, dtype=torch.int32, device=cuda)
+    g.cache_write(k, v, *cache, slots)
+    with torch.inference_mode():
+        g.cache_write(k, v, *cache, slots + 3)
+    a, b = (g.cache_read(*cache, s)[0] for s in (slots, slots + 3))
+    assert a.any() and torch.equal(a, b)
