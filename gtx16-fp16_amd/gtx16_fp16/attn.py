@@ -39,19 +39,28 @@ def _entry_points(name: str) -> tuple[int, int]:
     return e
 
 
-def _call(name: str, head: bytes, dev: torch.device, apart: bool = False) -> None:
-    # apart: a graph's call has a workspace of the graph's own memory, and so graphs captured on one stream may run at once
+def _call(name: str, head: bytes, dev: torch.device, ws: int | None = None) -> None:
+    # ws: the workspace, where the caller has one
     fast = _clib.fast()
     size, fn = _entry_points(name)
     stream = stream_handle(dev.index or 0)
     nbytes = fast.args_size(size, head)
-    if apart and nbytes and torch.cuda.is_current_stream_capturing():
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    else:
-        ws = scratch_buffer(dev, stream, nbytes) if nbytes else None
-    status = fast.args_call(fn, head, None if ws is None else ws.data_ptr(), nbytes, stream)
+    if nbytes and ws is None:
+        buf = scratch_buffer(dev, stream, nbytes)
+        ws = buf.data_ptr()
+    status = fast.args_call(fn, head, ws, nbytes, stream)
     if status != 0:
         _clib.check(status, name)
+
+
+def _with_workspace(like: torch.Tensor, nbytes: int) -> tuple[torch.Tensor, int]:
+    # (a tensor like `like`, contiguous; `nbytes` of workspace behind it in the same allocation). For a captured call, whose replays
+    # use the workspace: nothing else is placed there as long as the result has memory, whoever captures and wherever the memory is from.
+    at = -(-like.numel() * like.element_size() // 256) * 256
+    both = torch.empty(at + nbytes, dtype=torch.uint8, device=like.device)
+    out = torch.empty(0, dtype=like.dtype, device=like.device)
+    out.set_(both.untyped_storage(), 0, like.shape, torch.empty(like.shape, device="meta").stride())
+    return out, both.data_ptr() + at
 
 
 def _rows(t: torch.Tensor, size: int, d: int, keys: bool) -> torch.Tensor:
@@ -282,13 +291,21 @@ def _decode8(q, k_cache, v_cache, lengths, pages, shared_k, shared_v, scale, sof
     size = q.element_size()
     q = _rows(q, size, d, False)
     sk, sv, shared, shared_strides = _shared(name, shared_k, shared_v, q, hkv, d, size)
-    out = torch.empty(q.shape, dtype=dt, device=dev)
-    if out.numel() == 0:
-        return out
-    _call("g16_attention_decode8",
-          _ARGS8.pack(k_scale.data_ptr(), v_scale.data_ptr(), *k_scale.stride(), *v_scale.stride(), code, 0)
-          + _ARGS.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _ptr(sk), _ptr(sv), out.data_ptr(), 0, 0, 0, lengths.data_ptr(),
-                       _ptr(pages) if capacity else 0, _ptr(slopes), q.stride(0), 0, q.stride(1), *k_cache.stride()[:3], *v_cache.stride()[:3],
-                       *shared_strides, seqs, 1, capacity, hq, hkv, d, shared, 0, page, max_pages, k_cache.shape[0],
-                       1 if size == 4 else 0, _sm_count(dev), scale, softcap, 0), dev, True)
+    if q.numel() == 0:
+        return torch.empty(q.shape, dtype=dt, device=dev)
+
+    def packed(out: int) -> bytes:
+        return (_ARGS8.pack(k_scale.data_ptr(), v_scale.data_ptr(), *k_scale.stride(), *v_scale.stride(), code, 0)
+                + _ARGS.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _ptr(sk), _ptr(sv), out, 0, 0, 0, lengths.data_ptr(),
+                             _ptr(pages) if capacity else 0, _ptr(slopes), q.stride(0), 0, q.stride(1), *k_cache.stride()[:3], *v_cache.stride()[:3],
+                             *shared_strides, seqs, 1, capacity, hq, hkv, d, shared, 0, page, max_pages, k_cache.shape[0],
+                             1 if size == 4 else 0, _sm_count(dev), scale, softcap, 0))
+
+    entry, ws = "g16_attention_decode8", None
+    if torch.cuda.is_current_stream_capturing():  # a workspace of the call's own, so that graphs captured on one stream may run at once
+        # (its size does not depend on where the result goes)
+        out, ws = _with_workspace(q, _clib.fast().args_size(_entry_points(entry)[0], packed(q.data_ptr())))
+    else:
+        out = torch.empty(q.shape, dtype=dt, device=dev)
+    _call(entry, packed(out.data_ptr()), dev, ws)
     return out
