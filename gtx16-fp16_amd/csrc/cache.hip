@@ -66,9 +66,10 @@ __device__ inline uint32_t top_of(const Eight<_Float16>& x) {
 
 // A workgroup: block_rows rows, all heads of them. Of rows with one slot the last is written, so every workgroup looks
 // through the later rows' slots, n^2 / block_rows looks in all: a map of its own slots' last bits passes over nearly all of the
-// others, and the lanes together, a row each, compare one that it does not. (32768 rows of 8 heads of 128, fp16: 210 us where every lane
-// compared its own with all rows, 46.5 so.) A launch has at most kLaunchRows: the next one's rows are later ones anyway
-// (2^20 rows of one head of 64: 0.85 ms, 0.96 by 16384).
+// others, and the lanes together, a row each, compare one that it does not, of the same slot in 64 rows only the last. A
+// wavefront whose rows have all been found looks no further. (32768 rows of 8 heads of 128, fp16: 210 us where every lane
+// compared its own with all rows, 46.5 so; all of one slot: 23 us, where each was compared 756.) A launch has at most kLaunchRows: the next one's rows are
+// later ones anyway (2^20 rows of one head of 64: 0.85 ms, 0.96 by 16384).
 constexpr uint32_t kMapBits = 32 * kThreads, kMostRows = 32, kLaunchRows = 32768;
 
 template <typename T, int CODE, int LP>
@@ -95,8 +96,9 @@ __global__ __launch_bounds__(kThreads) void write_kernel(Params p) {
   if (tid < here && live[tid] != 0) atomicOr(&map[(slot_of[tid] % kMapBits) / 32], 1u << (slot_of[tid] % 32));
   __syncthreads();
   constexpr int kLooks = 8;  // under way together
-  const uint32_t row = tid % 64, own = row < here && live[row] != 0 ? slot_of[row] : ~0u;
-  for (uint32_t i0 = first + 1; i0 < p.n; i0 += kLooks * kThreads) {
+  const uint32_t row = tid % 64, end = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(tid & ~63u))) + 63;  // (lane 63's row)
+  uint32_t own = row < here && live[row] != 0 ? slot_of[row] : ~0u;  // ~0: nothing to look for
+  for (uint32_t i0 = first + 1; i0 < p.n && __ballot(own != ~0u) != 0; i0 += kLooks * kThreads) {
     uint32_t s[kLooks];
 #pragma unroll
     for (int j = 0; j < kLooks; ++j) s[j] = static_cast<uint32_t>(p.slots[min(i0 + tid + j * kThreads, p.n - 1)]);
@@ -104,11 +106,14 @@ __global__ __launch_bounds__(kThreads) void write_kernel(Params p) {
     for (int j = 0; j < kLooks; ++j) {
       const uint32_t i = i0 + tid + j * kThreads;
       const bool maybe = i < p.n && s[j] < p.capacity && (map[(s[j] % kMapBits) / 32] >> (s[j] % 32) & 1) != 0;
-      for (uint64_t hits = __ballot(maybe); hits != 0; hits &= hits - 1) {
-        const int at = __builtin_ctzll(hits);
-        if (own == static_cast<uint32_t>(__builtin_amdgcn_readlane(s[j], at)) &&
-            first + row < static_cast<uint32_t>(__builtin_amdgcn_readlane(i, at)))
+      for (uint64_t hits = __ballot(maybe); hits != 0;) {
+        const uint32_t slot = static_cast<uint32_t>(__builtin_amdgcn_readlane(s[j], __builtin_ctzll(hits)));
+        const uint64_t same = hits & __ballot(s[j] == slot);
+        if (own == slot && first + row < i0 + j * kThreads + end - static_cast<uint32_t>(__builtin_clzll(same))) {
           live[row] = 0;
+          own = ~0u;
+        }
+        hits &= ~same;
       }
     }
   }
