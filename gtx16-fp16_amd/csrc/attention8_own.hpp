@@ -17,7 +17,8 @@
 //     nothing but the choice of bytes, and block b's row m is value m DP / 16 + b.
 //   * Codes are exact in fp16 and bf16. K is multiplied as fp16 where the queries are, else as bf16 with the queries in three
 //     parts. A key's scale joins its score; a value's joins its weight, whose range then is fp32's, so weights are multiplied as
-//     bf16 parts: two for fp16 (to 2^-17; results are 2.1e-4 from the exact ones, all of it their own rounding), three for fp32.
+//     bf16 parts: two for fp16 (to 2^-17; results are 2.1e-4 from the exact ones, all of it their own rounding, and 2.6e-4 after a
+//     shared prefix, whose weights shared_workgroup rounds to fp16, as for 16 bits), three for fp32.
 //     So that the last of three is no subnormal, which the products take for 0, fp32's sums are kept in a unit: the power of
 //     two of the largest scale so far, within 2^40.
 //   * The keys' registers are loaded again as soon as the first product has read them, the values' after the second;

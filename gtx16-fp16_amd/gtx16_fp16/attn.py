@@ -229,9 +229,9 @@ def attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     and the result are ``attention``'s; a request without any key gives zeros.
 
     With ``k_scale`` and ``v_scale`` the caches are in 8 bits, as ``cache_write`` leaves them: int8 or float8_e4m3fn, the scales fp32
-    of the caches' shape without d. Keys and values are then the codes' exact products with their scales; a shared
-    prefix stays in q's type. Such a cache is never copied: a head's codes are contiguous and start at a multiple of 8
-    bytes, all other strides are free."""
+    of the caches' shape without d. Keys and values are then the codes' exact products with their scales, and fp16 queries'
+    weights are held to 2^-17 for them; a shared prefix stays in q's type, its weights are ``attention``'s. Such a cache is never
+    copied: a head's codes are contiguous and start at a multiple of 8 bytes, all other strides are free."""
     if forward_ad._current_level >= 0:
         refuse_tangents("attention_decode", q, k_cache, v_cache, shared_k, shared_v, slopes, k_scale, v_scale)
     if k_scale is not None or v_scale is not None:

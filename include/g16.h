@@ -468,7 +468,8 @@ int g16_cache_read(const g16_cache_args* args, void* stream);
 /* g16_attention_decode over such a cache: `a` as there, k and v the codes, whose strides are in bytes and, like their
  * pointers, multiples of 8 (no other limits); scales by strides in elements, ks_seq a request's or a page's. q, out and the
  * shared prefix have a's type. A score is scale * k_scale * (q . code), a value v_scale * code; codes are multiplied exactly,
- * with fp16 weights to 2^-17. A page outside the cache reads as zeros. One launch, one more where keys are split or shared, and
+ * with weights to 2^-17 of each where q is fp16 (those of a shared prefix are rounded to fp16, 2^-12, as in
+ * g16_attention_decode). A page outside the cache reads as zeros. One launch, one more where keys are split or shared, and
  * one for the shared keys unless d is 64 or 128, q fp16, hq / hkv up to 8 and seqs * hq / hkv up to 64.
  * seqs * (k_len / 64 + 1) up to 2^31 - 1. */
 typedef struct {
