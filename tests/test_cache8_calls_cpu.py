@@ -6,6 +6,7 @@ import torch
 from torch.autograd import forward_ad
 
 import gtx16_fp16 as g
+from test_cache8_cpu import ALIGN, SHAPE, WORKSPACE, decode_call, decode_size
 
 
 def test_tangents_of_e4m3_codes_are_refused():
@@ -22,3 +23,17 @@ def test_tangents_of_e4m3_codes_are_refused():
                     call(*given)
                 with pytest.raises(ValueError):  # (these tensors are on the CPU)
                     call(c, c)
+
+
+@pytest.mark.parametrize("step", [1 << 30, 1 << 24, 0, 8])
+def test_tokens_far_apart_and_on_top_of_each_other_are_taken(step):
+    # without a workspace the call ends where everything else has been looked at, before a launch
+    long = dict(k_len=8000, page=8000, k_token=step, v_token=step)
+    assert decode_size(**long) > 0 and decode_call(**long) == WORKSPACE
+
+
+def test_a_workspace_does_not_lift_the_other_checks():
+    long = dict(k_len=8000, page=8000)
+    assert decode_call(**long, k_token=(1 << 30) + 4) == ALIGN and decode_call(**long, v_head=4) == ALIGN
+    # keys are counted in 32 bits with room: up to 2^30 in all
+    assert decode_call(k_len=(1 << 30) + 1, page=(1 << 30) + 1) == SHAPE and decode_size(k_len=(1 << 30) + 1, page=(1 << 30) + 1) == 0
