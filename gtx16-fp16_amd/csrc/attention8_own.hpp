@@ -19,8 +19,10 @@
 //     parts. A key's scale joins its score; a value's joins its weight, whose range then is fp32's, so weights are multiplied as
 //     bf16 parts: two for fp16 (to 2^-17; results are 2.1e-4 from the exact ones, all of it their own rounding, and 2.6e-4 after a
 //     shared prefix, whose weights shared_workgroup rounds to fp16, as for 16 bits), three for fp32.
-//     So that the last of three is no subnormal, which the products take for 0, fp32's sums are kept in a unit: the power of
-//     two of the largest scale so far, within 2^40.
+//     So that the last of three is no subnormal, which the products take for 0, a row's fp32 sums are kept in a unit of its own, a
+//     power of two that brings its largest product of weight and scale to 2^60 or so, and all down to 2^-170 of it have
+//     their bits: it falls where a product is past 2^80, and rises as far as a new maximum makes the sums fall. (With one unit
+//     for all rows, by the largest scale, rows that gave a value 2^60 times the others' no weight lost their result.)
 //   * The keys' registers are loaded again as soon as the first product has read them, the values' after the second;
 //     other wavefronts fill the gaps. The places of a tile's rows are found one key a lane and passed on through LDS.
 // A key behind its part's end, or on a page outside the cache, is read from a row of zeros; the former get no weight.
@@ -376,7 +378,9 @@ __device__ inline void own8_workgroup(const Params& p, const Params8& e, int blo
     const int mine = S::QP == 4 ? 0 : S::QP == 8 ? 4 * (g & 1) : 4 * g;
     auto key_of = [&](int s) { return S::QP == 4 ? lane : S::QP == 8 ? 32 * s + 16 * (g >> 1) + col : 16 * s + col; };
     Query8<T> q[NR][DP / 32];
-    float slope[NR][RI], m[NR][RI], l[NR][RI], unit = 0x1p100f;
+    constexpr bool kUnits = sizeof(T) == 4;
+    constexpr float kMostUnit = 0x1p100f;
+    float slope[NR][RI], m[NR][RI], l[NR][RI], unit[NR][RI];
     float4v o[NR][VB];
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
@@ -398,6 +402,7 @@ __device__ inline void own8_workgroup(const Params& p, const Params8& e, int blo
         slope[r][i] = p.slopes != nullptr && head < p.group ? p.slopes[kv * p.group + head] * kLog2e : 0.f;
         m[r][i] = -__builtin_huge_valf();
         l[r][i] = 0.f;
+        unit[r][i] = kMostUnit;
       }
 #pragma unroll
       for (int i = 0; i < VB; ++i) o[r][i] = float4v{};
@@ -415,6 +420,13 @@ __device__ inline void own8_workgroup(const Params& p, const Params8& e, int blo
 
     __bf16* weights = reinterpret_cast<__bf16*>(keys + kKeys);
     float* factors = joint[0][wave];
+    auto scale_sums = [&](int r) {  // by the rows' factors
+      wave_order();
+      const float f = factors[col % (RQ < 16 ? RQ : 16)];
+      wave_order();
+#pragma unroll
+      for (int i = 0; i < VB; ++i) o[r][i] *= f;
+    };
     for (; j0 < end; j0 += kStep) {
       // ---- scores ----
 #pragma unroll
@@ -457,21 +469,6 @@ __device__ inline void own8_workgroup(const Params& p, const Params8& e, int blo
       for (int s = 0; s < NS; ++s) {
         kscale[s] = S::QP == 4 ? ks : __shfl(ks, key_of(s));
         vscale[s] = S::QP == 4 ? vs : __shfl(vs, key_of(s));
-      }
-      if constexpr (sizeof(T) == 4) {
-        if (__any(fabsf(vs) * unit > 0x1p40f)) {
-          float most = fabsf(vs);
-#pragma unroll
-          for (int i = 1; i < 64; i *= 2) most = fmaxf(most, __shfl_xor(most, i));
-          const float was = unit;
-          unit = __uint_as_float((254u << 23) - (min(__float_as_uint(most), 0x7e800000u) & 0x7f800000u));
-#pragma unroll
-          for (int r = 0; r < NR; ++r)
-#pragma unroll
-            for (int i = 0; i < VB; ++i) o[r][i] *= unit / was;
-        }
-#pragma unroll
-        for (int s = 0; s < NS; ++s) vscale[s] *= unit;
       }
       // ---- the next keys ----
       // (behind the last tile the rows of zeros again: under a condition all of the registers would be copied)
@@ -535,17 +532,30 @@ __device__ inline void own8_workgroup(const Params& p, const Params8& e, int blo
 #pragma unroll
           for (int i = 0; i < RI; ++i) {
             const float to = fmaxf(m[r][i], across(top[i], [](float x, float y) { return fmaxf(x, y); }));
-            const float f = to == m[r][i] ? 1.f : __builtin_amdgcn_exp2f(m[r][i] - to);
+            float f = to == m[r][i] ? 1.f : __builtin_amdgcn_exp2f(m[r][i] - to);
             m[r][i] = to;
             l[r][i] *= f;
+            if constexpr (kUnits) {  // by the power of two that brings f to between 1/2 and 1
+              const float by = fminf(__uint_as_float((253u - min(__float_as_uint(f) >> 23, 126u)) << 23), kMostUnit / unit[r][i]);
+              unit[r][i] *= by;
+              f *= by;
+            }
             factors[mine + i] = f;  // (the same from all lanes of a row)
           }
-          wave_order();
-          const float f = factors[col % (RQ < 16 ? RQ : 16)];
-          wave_order();
-#pragma unroll
-          for (int i = 0; i < VB; ++i) o[r][i] *= f;
+          scale_sums(r);
         }
+        auto leave = [&](int s, int i, float rest) {  // the parts of a weight
+          __bf16* to = weights + (16 * r + mine + i) * kRun8 + key_of(s);
+          if (RQ >= 4 || mine == 0) {
+#pragma unroll
+            for (int part = 0; part < PARTS; ++part) {
+              const __bf16 h = static_cast<__bf16>(rest);
+              to[part * (R * kRun8)] = h;
+              rest -= static_cast<float>(h);
+            }
+          }
+        };
+        bool far = false;
 #pragma unroll
         for (int i = 0; i < RI; ++i) {
           const float ref = (m[r][i] == -__builtin_huge_valf() ? 0.f : m[r][i]) - kShift<T> - off;
@@ -553,17 +563,36 @@ __device__ inline void own8_workgroup(const Params& p, const Params8& e, int blo
           for (int s = 0; s < NS; ++s) {
             const float x = __builtin_amdgcn_exp2f(fmaf(w[r][s][i], c, -ref)) * kScale<T>;
             l[r][i] += x;
-            float rest = x * vscale[s];
-            __bf16* to = weights + (16 * r + mine + i) * kRun8 + key_of(s);
-            if (RQ >= 4 || mine == 0) {
-#pragma unroll
-              for (int part = 0; part < PARTS; ++part) {
-                const __bf16 h = static_cast<__bf16>(rest);
-                to[part * (R * kRun8)] = h;
-                rest -= static_cast<float>(h);
-              }
+            if constexpr (kUnits) {
+              w[r][s][i] = x;
+              far = far || fabsf(x * unit[r][i] * vscale[s]) > 0x1p80f;
+            } else {
+              leave(s, i, x * vscale[s]);
             }
           }
+        }
+        if constexpr (kUnits) {
+          if (__any(far)) {
+#pragma unroll
+            for (int i = 0; i < RI; ++i) {
+              float most = 0.f;
+#pragma unroll
+              for (int s = 0; s < NS; ++s) most = fmaxf(most, w[r][s][i] * fabsf(vscale[s]));
+              most = across(most, [](float x, float y) { return fmaxf(x, y); });
+              float f = 1.f;
+              if (most * unit[r][i] > 0x1p80f) {  // to 2^60 .. 2^61 (weights are at most 2^-16)
+                const float to = __uint_as_float((314u - min(__float_as_uint(most) >> 23, 239u)) << 23);
+                f = to / unit[r][i];
+                unit[r][i] = to;
+              }
+              factors[mine + i] = f;
+            }
+            scale_sums(r);
+          }
+#pragma unroll
+          for (int i = 0; i < RI; ++i)
+#pragma unroll
+            for (int s = 0; s < NS; ++s) leave(s, i, w[r][s][i] * unit[r][i] * vscale[s]);
         }
       }
       wave_order();
@@ -597,6 +626,14 @@ __device__ inline void own8_workgroup(const Params& p, const Params8& e, int blo
     float* so = reinterpret_cast<float*>(HEADS == 1 ? lds : keys);
     constexpr int kJoined = 4 / HEADS;
     const int part0 = HEADS == 1 ? 0 : wave, so_wave = HEADS == 1 ? wave : 0;
+    if constexpr (kUnits) {  // out of their units
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+#pragma unroll
+        for (int i = 0; i < RI; ++i) factors[mine + i] = 1.f / unit[r][i];
+        scale_sums(r);
+      }
+    }
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
 #pragma unroll
@@ -605,14 +642,13 @@ __device__ inline void own8_workgroup(const Params& p, const Params8& e, int blo
         joint[0][wave][16 * r + mine + i] = m[r][i];
         joint[1][wave][16 * r + mine + i] = l[r][i];
       }
-      const float back = sizeof(T) == 4 ? 1.f / unit : 1.f;
       if (col < RQ) {
 #pragma unroll
         for (int n4 = 0; n4 < 4; ++n4)  // row 4 g + n4 of every block: values (4 g + n4) VB + {0 .. VB - 1}
 #pragma unroll
           for (int i = 0; i < VB; i += 4)
             *reinterpret_cast<float4v*>(&so[(so_wave * R + 16 * r + col) * DP + (4 * g + n4) * VB + i]) =
-                float4v{o[r][i][n4], o[r][i + 1][n4], o[r][i + 2][n4], o[r][i + 3][n4]} * back;
+                float4v{o[r][i][n4], o[r][i + 1][n4], o[r][i + 2][n4], o[r][i + 3][n4]};
       }
     }
     if constexpr (HEADS == 1) __syncthreads();
