@@ -519,7 +519,7 @@ __device__ inline void own8_workgroup(const Params& p, const Params8& e, int blo
               if (key_of(s) >= left) w[r][s][i] = -__builtin_huge_valf();
         }
         float top[RI];
-        bool up = false;
+        bool up = false, wide = false;
 #pragma unroll
         for (int i = 0; i < RI; ++i) {
           top[i] = w[r][0][i];
@@ -527,6 +527,15 @@ __device__ inline void own8_workgroup(const Params& p, const Params8& e, int blo
           for (int s = 1; s < NS; ++s) top[i] = fmaxf(top[i], w[r][s][i]);
           top[i] = fmaf(top[i], c, off);
           up = up || top[i] > m[r][i] + kLag;
+          wide = wide || fabsf(top[i]) > kWide;
+        }
+        if (__any(wide)) {
+#pragma unroll
+          for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int i = 0; i < RI; ++i) w[r][s][i] = fmaf(w[r][s][i], c, off);
+          c = 1.f;
+          off = 0.f;
         }
         if (__any(up)) {
 #pragma unroll

@@ -12,6 +12,9 @@ namespace g16 {
 typedef float float8v __attribute__((ext_vector_type(8)));
 
 constexpr float kLag = 7.f;
+// Where the largest score is more than this, the scores are rounded, like the maximum, before it is taken off them: the product with
+// the scale within the difference, which is exact, would leave the best key's weight at 2 to the maximum's rounding.
+constexpr float kWide = 0x1p22f;
 // fp16 weights are 2^kShift above their value, by way of the exponent. fp32 ones would lose bits of the exponent by that
 // (2^-20 of a weight at 23), and are multiplied by kScale: at most 2^-16, so that the sums over 65536
 // keys of the largest weight stay within the values' range.
