@@ -265,6 +265,7 @@ struct Wave {
   float16v o[DP / 32];
   float m, l;  // the reference maximum (log2 units) and this lane's part of the sum of weights
   bool exact;  // fp32: whether a row of the wavefront is not to be split
+  bool wide;   // whether a row's maximum is past kWide
 
   __device__ void start(const Row& row, float sign, int d, int lane) {
     const int h = lane >> 5;
@@ -298,6 +299,7 @@ struct Wave {
     for (int i = 0; i < DP / 32; ++i) o[i] = float16v{};
     m = -__builtin_huge_valf();
     l = 0.f;
+    wide = false;
   }
 
   // Keeps the sums whole up to here: taken apart for the stores below, they would be copied in every
@@ -404,10 +406,11 @@ struct Wave {
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[kb][r]);
     top = fmaf(fmaxf(top, other_half(top)), c, off);
     // (-inf times c stays -inf: c > 0.) A lane whose maximum moves takes the whole wavefront along.
-    if (__any(top > m + kLag)) {
+    if (__any(top > m + (wide ? 0.f : kLag))) {
       const float next = fmaxf(m, top);
       const float f = next == m ? 1.f : __builtin_amdgcn_exp2f(m - next);
       m = next;
+      wide = __any(fabsf(next) > kWide && next != -__builtin_huge_valf()) != 0;
       l *= f;
 #pragma unroll
       for (int i = 0; i < DP / 32; ++i)
@@ -415,7 +418,16 @@ struct Wave {
         for (int r = 0; r < 16; ++r) o[i][r] *= f;
     }
     // a row that has seen no key yet (m = -inf): every score is -inf, every weight 0
-    const float ref = (m == -__builtin_huge_valf() ? 0.f : m) - kShift<T> - off;
+    const float from = m == -__builtin_huge_valf() ? 0.f : m;
+    float ref = from - kShift<T> - off;
+    if (wide) {  // (nor would such a maximum hold kShift, or a lag of kLag: fp16 weights would be infinite)
+#pragma unroll
+      for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[kb][r] = fmaf(s[kb][r], c, off) - from;
+      c = 1.f;
+      ref = -kShift<T>;
+    }
     float sum = 0.f;
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb)
