@@ -237,8 +237,14 @@ struct Shape8 {
 
 // What a workgroup keeps in LDS: its wavefronts' keys and weights, which the sums that are joined take the place of; the places of
 // a tile's rows, of keys and of values; maxima and sums.
+template <typename T, int NR>
+struct Lifts {};
+template <int NR>
+struct Lifts<float, NR> {
+  float lifts[4][16 * NR];  // of a wavefront's rows: what large queries have been divided by
+};
 template <typename T, int DP, int RQ>
-struct Lds8 {
+struct Lds8 : Lifts<T, Shape8<T, DP, RQ>::NR> {
   using S = Shape8<T, DP, RQ>;
   static constexpr int kKeys = kTile8 * DP, kWeights = S::PARTS * S::R * kRun8 * 2, kSums = S::R * DP * 4;  // bytes of a wavefront
   alignas(16) char data[4 * (kKeys + kWeights > kSums ? kKeys + kWeights : kSums)];
@@ -379,14 +385,16 @@ __device__ inline void own8_workgroup(const Params& p, const Params8& e, int blo
     auto key_of = [&](int s) { return S::QP == 4 ? lane : S::QP == 8 ? 32 * s + 16 * (g >> 1) + col : 16 * s + col; };
     Query8<T> q[NR][DP / 32];
     constexpr bool kUnits = sizeof(T) == 4;
-    constexpr float kMostUnit = 0x1p100f;
+    constexpr float kMostUnit = 0x1p100f, kLarge = 0x1p64f;
     float slope[NR][RI], m[NR][RI], l[NR][RI], unit[NR][RI];
     float4v o[NR][VB];
+    bool lifted = false;
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
       const int row = rt * kKeyTile + 16 * r + col % S::QP;
       const bool some = row < p.group;
       const char* at = p.q + b * p.q_seq + (kv * p.group + (some ? row : 0)) * p.q_head;
+      bool large = false;
 #pragma unroll
       for (int s = 0; s < DP / 32; ++s) {
         using V8 = typename Vec8<T>::V;
@@ -394,7 +402,29 @@ __device__ inline void own8_workgroup(const Params& p, const Params8& e, int blo
         V8 x = {};
         if (some && d0 < p.d) x = *reinterpret_cast<const V8*>(at + d0 * sizeof(T));
         if (p.sign != 1.f) x *= static_cast<T>(p.sign);
+        if constexpr (kUnits) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) large = large || fabsf(x[j]) >= kLarge;
+        }
         q[r][s].set(x);
+      }
+      if constexpr (kUnits) {
+        // The sums of a large query's products with codes, which the keys' scales may well bring back, could be past fp32's
+        // range: it is divided, and its scores multiplied once they have their scales.
+        const uint64_t lanes = __ballot(large);
+        if (lanes != 0) {
+          const bool divided = ((lanes | lanes >> 16 | lanes >> 32 | lanes >> 48) >> col & 1) != 0;
+#pragma unroll
+          for (int s = 0; s < DP / 32; ++s) {
+            const int d0 = 64 * (s >> 1) + 16 * g + 8 * (s & 1);
+            float8v x = {};
+            if (some && d0 < p.d) x = *reinterpret_cast<const float8v*>(at + d0 * 4);
+            q[r][s].set(x * (divided ? p.sign / kLarge : p.sign));
+          }
+          if (NR > 1 && !lifted) shared.lifts[wave][16 * (1 - r) + col] = 1.f;
+          shared.lifts[wave][16 * r + col] = divided ? kLarge : 1.f;
+          lifted = true;
+        }
       }
 #pragma unroll
       for (int i = 0; i < RI; ++i) {
@@ -485,6 +515,14 @@ __device__ inline void own8_workgroup(const Params& p, const Params8& e, int blo
         for (int s = 0; s < NS; ++s)
 #pragma unroll
           for (int i = 0; i < RI; ++i) w[r][s][i] *= kscale[s];
+        if constexpr (kUnits) {
+          if (lifted) {
+#pragma unroll
+            for (int i = 0; i < RI; ++i)
+#pragma unroll
+              for (int s = 0; s < NS; ++s) w[r][s][i] *= shared.lifts[wave][16 * r + mine + i];
+          }
+        }
         if (sc.capped) {
           if (sizeof(T) == 2 && !sc.fine) {
 #pragma unroll
