@@ -1140,7 +1140,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(Params p) {
 }
 
 // The shared keys for few rows and, over a cache of 8 bits, the own ones in one launch: one after the other, each would leave the
-// card half empty (16 requests of up to 1500 in int8 after 2048, 8 heads of 128: 36 us, so 31).
+// card half empty (16 requests of up to 1500 in int8 after 2048, 32 heads on 8 of 128, in a graph: 31.6 us, so 22.4).
 template <int DP, int CODE, int RQ, int HEADS>
 __global__ __launch_bounds__(kThreads, 2) void decode_both8_kernel(Params p, Params8 e) {
   __shared__ union Lds {
@@ -1472,8 +1472,8 @@ Plan8 plan_decode8(const g16_attention_args& a) {
     };
     // Where a token's heads lie next to each other in memory, a workgroup takes four of them together (see own8_workgroup), unless
     // there are so few requests that their joins would take longer (one request of 8192 keys, 32 heads on 8, d 128, 256 parts of a row:
-    // 19.2 us, 17.3 by single heads; 16 heads on 16, 128 parts: 18.4 and 19.0, of 65536 70.0 and 77.1; two requests of 8192, 64 heads on 8,
-    // 128 parts: 23.8 and 21.3; 64 of up to 700, 32 heads on 8: 24.2 and 30.6).
+    // 19.9 us, 18.5 by single heads; 16 heads on 16, 128 parts: 18.8 and 19.6, of 65536 69.2 and 76.7; two requests of 8192, 64 heads on 8,
+    // 128 parts: 23.9 and 21.8; 64 of up to 700, 32 heads on 8: 24.7 and 30.8; all in graphs).
     if (a.hkv % kHeads8 == 0 && rows_of8(group) <= kRowsOfHeads8 && a.d == dp && a.k_token > a.k_head && shares(kHeads8) <= 128LL * a.seqs) r.heads = kHeads8;
     r.shares = shares(r.heads);
   }
@@ -1485,7 +1485,9 @@ Plan8 plan_decode8(const g16_attention_args& a) {
   return r;
 }
 
-// Whether shared and own keys go into one launch: what has as many workgroups on a CU either way, and few enough kernels.
+// Whether shared and own keys go into one launch: few enough kernels, and with two workgroups on a CU as many as either would
+// have by itself, or nearly: for heads of 64 the own keys' shares are counted for three (counting two: 16.4 us for 16.3, 16 requests
+// of up to 1500 after 2048, 12 heads of 64).
 bool both8(const g16_attention_args& a, const Plan8& plan) {
   return plan.shared.stiles > 0 && plan.shared.skeys && !a.is_f32 && (a.d == 64 || a.d == 128) && a.hq / a.hkv <= 8;
 }

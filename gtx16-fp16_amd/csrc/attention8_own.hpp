@@ -160,7 +160,8 @@ __device__ inline int all_tiles(const Params& p, const Run64& head) {
 // How all requests' tiles are dealt. Long ones in shares of equal length, whatever the requests: the first `more` shares
 // have each + 1, the others each. Where a share would have few tiles, its time is that of the waits for one after another, not of its bytes,
 // and a second request's would come on top: every request then has its own pieces, of `chunk` tiles, one for each
-// wavefront or two (16 requests of up to 1500 after 2048, 8 heads of 128, HEADS = 1: 42 us by shares, 36 so).
+// wavefront or two (16 requests of up to 1500, 32 heads on 8 of 128, HEADS = 1: 24.0 us by shares, 20.9 so; HEADS = 4: 20.1 and 20.9,
+// but 64 of up to 700 25.3 and 24.5).
 struct Deal {
   int shares = 1, each = 1, more = 0, chunk = 0;
   __device__ Deal() {}
@@ -254,8 +255,8 @@ struct Lds8 : Lifts<T, Shape8<T, DP, RQ>::NR> {
 
 // Workgroup `block` of those for the requests' own keys. HEADS: 1, a key head, whose tiles the wavefronts take in turn; or 4, one for
 // each wavefront, which has all of the share's tiles. What a workgroup reads of a token is then four heads' codes in
-// a row, and their scales: 40 requests of 8192 e4m3 keys, 32 heads on 8 of 128, take 138 us (5.0 TB/s), with HEADS = 1 160;
-// 96 of up to 2048, 12 heads of 64, 51.5 and 59.2. No wavefront waits for another, there is nothing to join in LDS, and a
+// a row, and their scales: 40 requests of up to 8192 e4m3 keys, 32 heads on 8 of 128, take 72.7 us, with HEADS = 1 85.8;
+// 96 of up to 2048, 12 heads of 64, 46.6 and 54.7. No wavefront waits for another, there is nothing to join in LDS, and a
 // row has four times as many parts. A cache that is ordered by heads has a head's codes in a row, and HEADS = 1.
 template <typename T, int DP, int CODE, int RQ, bool FULL, int HEADS>
 __device__ inline void own8_workgroup(const Params& p, const Params8& e, int block, Lds8<T, DP, RQ>& shared) {
@@ -269,7 +270,7 @@ __device__ inline void own8_workgroup(const Params& p, const Params8& e, int blo
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), col = lane & 15, g = lane >> 4;
   // Workgroups go to the XCDs in turn, and every XCD has an L2 of its own. The heads of a share read the same cache lines (of
   // codes where a head's are less than a line, of scales always), so they are all given to one XCD where there are shares for all
-  // (96 requests of up to 2048, 12 heads of 64: 76 us, and by this alone 63).
+  // (96 requests of up to 2048, 12 heads of 64, by single heads: 76 us, and by this alone 63; four heads together take as long without).
   int lin = block;
   if (e.shares >= kXcds) {
     const int per = p.otiles * (p.hkv / HEADS), i = lin / kXcds, share = i / per * kXcds + lin % kXcds;

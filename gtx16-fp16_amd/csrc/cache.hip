@@ -67,9 +67,10 @@ __device__ inline uint32_t top_of(const Eight<_Float16>& x) {
 // A workgroup: block_rows rows, all heads of them. Of rows with one slot the last is written, so every workgroup looks
 // through the later rows' slots, n^2 / block_rows looks in all: a map of its own slots' last bits passes over nearly all of the
 // others, and the lanes together, a row each, compare one that it does not, of the same slot in 64 rows only the last. A
-// wavefront whose rows have all been found looks no further. (32768 rows of 8 heads of 128, fp16: 210 us where every lane
-// compared its own with all rows, 46.5 so; all of one slot: 23 us, where each was compared 756.) A launch has at most kLaunchRows: the next one's rows are
-// later ones anyway (2^20 rows of one head of 64: 0.85 ms, 0.96 by 16384).
+// wavefront whose rows have all been found looks no further. (32768 rows of 8 heads of 128, fp16, the same ones again and again:
+// 210 us where every lane compared its own with all rows, 46.5 so, 58 for other rows every time; all of one slot: 23 us, where
+// each was compared 756.) A launch has at most kLaunchRows: the next one's rows are later ones anyway (2^20 rows of one
+// head of 64: 0.90 ms, 1.01 by 16384).
 constexpr uint32_t kMapBits = 32 * kThreads, kMostRows = 32, kLaunchRows = 32768;
 
 template <typename T, int CODE, int LP>

@@ -133,7 +133,7 @@ int run(Params p, hipStream_t stream) {
   return launch(rotary_kernel<T, V, NEIGHBOURS>, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), stream, p);
 }
 // Pairs of a thread: 16 bytes a load where their number allows that (neighbours: 12291 patches, 32 heads of 128 fp16, 40 pairs:
-// 66 us with 32 bytes a thread, 60 so, and 40.5 with the values that stay in the same loop).
+// 66 us with 32 bytes a thread, 60 so, and 40.8 with the values that stay in the same loop).
 template <typename T>
 int run(const Params& p, bool neighbours, hipStream_t stream) {
   constexpr uint32_t kMost = 16 / sizeof(T);
