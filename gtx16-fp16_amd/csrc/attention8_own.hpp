@@ -568,14 +568,6 @@ __device__ inline void own8_workgroup(const Params& p, const Params8& e, int blo
           up = up || top[i] > m[r][i] + kLag;
           wide = wide || fabsf(top[i]) > kWide;
         }
-        if (__any(wide)) {
-#pragma unroll
-          for (int s = 0; s < NS; ++s)
-#pragma unroll
-            for (int i = 0; i < RI; ++i) w[r][s][i] = fmaf(w[r][s][i], c, off);
-          c = 1.f;
-          off = 0.f;
-        }
         if (__any(up)) {
 #pragma unroll
           for (int i = 0; i < RI; ++i) {
@@ -592,6 +584,14 @@ __device__ inline void own8_workgroup(const Params& p, const Params8& e, int blo
           }
           scale_sums(r);
         }
+        const bool flat = __any(wide) != 0;  // (see kWide; nor would such a maximum hold kShift)
+        if (flat) {
+#pragma unroll
+          for (int i = 0; i < RI; ++i)
+#pragma unroll
+            for (int s = 0; s < NS; ++s) w[r][s][i] = fmaf(w[r][s][i], c, off) - (m[r][i] == -__builtin_huge_valf() ? 0.f : m[r][i]);
+          c = 1.f;
+        }
         auto leave = [&](int s, int i, float rest) {  // the parts of a weight
           __bf16* to = weights + (16 * r + mine + i) * kRun8 + key_of(s);
           if (RQ >= 4 || mine == 0) {
@@ -606,7 +606,7 @@ __device__ inline void own8_workgroup(const Params& p, const Params8& e, int blo
         bool far = false;
 #pragma unroll
         for (int i = 0; i < RI; ++i) {
-          const float ref = (m[r][i] == -__builtin_huge_valf() ? 0.f : m[r][i]) - kShift<T> - off;
+          const float ref = flat ? -kShift<T> : (m[r][i] == -__builtin_huge_valf() ? 0.f : m[r][i]) - kShift<T> - off;
 #pragma unroll
           for (int s = 0; s < NS; ++s) {
             const float x = __builtin_amdgcn_exp2f(fmaf(w[r][s][i], c, -ref)) * kScale<T>;

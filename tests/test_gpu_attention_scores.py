@@ -68,3 +68,27 @@ def test_a_prefix_before_a_cache_in_8_bits(cuda, keys, shared, hq, hkv, d, dtype
     y = g.attention_decode(q, cache[0].to(cuda), cache[1].to(cuda), n, shared_k=k, shared_v=v, k_scale=cache[2].to(cuda), v_scale=cache[3].to(cuda), **kw)
     both = torch.cat((k.cpu().double(), k8[0] * 2.0 ** ek)), torch.cat((v.cpu().double(), v8[0]))
     check(y, q, *both, kw.get("scale", d ** -0.5))
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("hq", [2, 12])
+def test_a_key_of_the_prefix_and_its_like_in_8_bits(cuda, dtype, hq):
+    # the same key before and in the cache, exactly: half of the weight each, however large the score
+    d, gen = 64, torch.Generator().manual_seed(0)
+    cache, _, v8 = random_cache(1, 5, 1, d, "int8", gen)
+    cache[0].zero_()
+    cache[0][0, 2, 0, 0], cache[2][0] = 64, 2.0 ** -4
+    k, v = torch.zeros(7, 1, d), torch.randn(7, 1, d, generator=gen).to(dtype)
+    k[4, 0, 0] = 4.0
+    q = torch.zeros(1, hq, d)
+    q[:, :, 0] = 2.0 ** 10 * (1 + torch.arange(hq) / 16)
+    want = (v[4].double() + v8[0, 2]) / 2
+    n = torch.tensor([5], dtype=torch.int32, device=cuda)
+    u = 2.0 ** -11 if dtype == F16 else 2.0 ** -24
+    for step in range(50):  # scores from 2^23 on, which are rounded alike on both sides
+        scale = 2.0 ** (step / 3 + 11) * 1.07
+        y = g.attention_decode(q.to(dtype).to(cuda), cache[0].to(cuda), cache[1].to(cuda), n, shared_k=k.to(dtype).to(cuda), shared_v=v.to(cuda),
+                               k_scale=cache[2].to(cuda), v_scale=cache[3].to(cuda), scale=scale).cpu()
+        # (the other keys, of score 0, get nothing) the weights are 1 and exact; their sums' products and the result are rounded
+        off = (y[0].double() - want).abs() - (u * want.abs() + (2.0 ** -16 if dtype == F16 else 2.0 ** -21) * (v[4].double().abs() + v8[0, 2].abs()))
+        assert (off <= 0).all(), scale
