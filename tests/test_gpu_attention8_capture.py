@@ -70,3 +70,18 @@ def test_a_capture_that_torch_does_not_know(cuda):
             assert torch.equal(y, want) and all(bool((t == 0x5a).all()) for t in others)
         ok(hip.hipGraphExecDestroy(run))
         ok(hip.hipGraphDestroy(graph))
+
+
+def test_in_inference_mode(cuda):
+    args, kw, _ = case(cuda, F16, "e4m3", [900, 3000], 8, 2, 64, page=16, spoil=False)
+    want = g.attention_decode(*args, **kw)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.inference_mode(), torch.cuda.stream(side):
+        with torch.cuda.graph(graph, stream=side):
+            y = g.attention_decode(*args, **kw)
+        for _ in range(2):
+            y.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, want)
